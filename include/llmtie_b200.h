@@ -509,6 +509,144 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
                                     size_t head_dim, float theta, float scale, float *out,
                                     size_t out_len);
 
+/* ---- the 8-bit KV cache ------------------------------------------------------- */
+
+/* A cache of one layer that holds its keys and values in 8 bits (the reference
+ * has none): half the memory of the f16 caches, and half the bytes that a
+ * decode step reads.
+ *
+ * Tokens lie in blocks of 32. A complete block of one KV head is int8 codes
+ * with one f32 scale for its keys and one for its values: code =
+ * rint(x / scale), scale = max|x| / 127 over the block, x the row rounded to
+ * f16. The tokens of the last, incomplete block are f16 rows (the tail) until
+ * the block is complete, so the codes do not depend on how the tokens arrived,
+ * one by one or in prompts cut anywhere. A block that holds an infinity or a
+ * NaN reads back as NaN throughout.
+ *
+ * A cache is ONE buffer of llmtie_kv_q8_bytes bytes, 16-byte aligned, for a
+ * capacity of a multiple of 32 tokens. With nb = capacity / 32 it holds, each
+ * section starting at the next multiple of 128 bytes:
+ *   key codes    int8 [kv_heads][nb][head_dim/64][32 tokens][64]
+ *   value codes  int8 [kv_heads][nb][head_dim][32 tokens]
+ *   key scales   f32  [kv_heads][nb]
+ *   value scales f32  [kv_heads][nb]
+ *   weights      f32  [kv_heads][nb]  accumulated attention weight of a block
+ *   key tail     f16  [kv_heads][32][head_dim]
+ *   value tail   f16  [kv_heads][32][head_dim]
+ * How many tokens it holds is the caller's to know (its `live` or `past`).
+ * head_dim is 64 or 128. The entries take HOST tables with a cache, a capacity
+ * and lengths for each sequence, any number of sequences a call; caches that
+ * one call writes must not share memory. A capacity that is not a multiple of
+ * 32 is refused with LLMTIE_ERR_RAGGED_BLOCK.
+ *
+ * Calls may be captured into a CUDA graph once the same call has been made
+ * before the capture: workspaces grow on the first call, which a capture
+ * refuses, and a workspace that was outgrown is kept until the handle (or the
+ * decode scratch) is freed, so that a captured call may be replayed. Graphs
+ * that share a handle or a scratch must not be replayed at the same time. */
+
+/* Bytes of a cache; 0 for a shape that there is none of. Host only. */
+size_t llmtie_kv_q8_bytes(size_t kv_heads, size_t head_dim, size_t cap);
+/* A zeroed cache, freed with llmtie_free. */
+llmtie_status llmtie_kv_alloc_q8(llmtie_gpu *g, size_t kv_heads, size_t head_dim, size_t cap,
+                                 void **cache);
+
+/* The inverse frequencies theta^(-2j/head_dim), over freq_div[j] where that is
+ * not NULL, that llmtie_rope_scaled works out in every call: out f32
+ * [head_dim/2], to be kept and given to llmtie_rope_append_q8. */
+llmtie_status llmtie_rope_inv_freq(llmtie_gpu *g, const float *freq_div, size_t head_dim,
+                                   float theta, float *out, size_t out_len);
+
+/* New rows into 8-bit caches, rotated on the way: what llmtie_rope_cache_batched
+ * is for a decode step over f16 caches and the pre-pass of llmtie_prefill_varlen
+ * for a prompt. Sequence b brings the rows cu_seqlens[b] .. cu_seqlens[b+1] of
+ * k and v f32 [rows][kv_heads*head_dim] and of q f32 [rows][heads*head_dim],
+ * as many as it likes or none; its cache holds past[b] tokens before, and
+ * past[b] + its rows after. inv_freq f32 [head_dim/2] turns pair (j, j +
+ * head_dim/2) of q and k at row i by (pos[b] + i) * inv_freq[j] (the product in
+ * 64 bits, so that far positions keep their angle; pos is apart from past
+ * because an eviction leaves a cache shorter than its conversation); rotated
+ * rows of q go to q_out, which may be q. With inv_freq NULL nothing is turned
+ * and q and q_out are not looked at; with q NULL only the keys are turned. A
+ * block that the rows complete is quantised, and its weight set to zero. */
+llmtie_status llmtie_rope_append_q8(llmtie_gpu *g, const float *q, size_t q_len, float *q_out,
+                                    size_t q_out_len, const float *k, size_t k_len, const float *v,
+                                    size_t v_len, const int32_t *cu_seqlens, size_t batch,
+                                    void *const *caches, const int32_t *past, const int32_t *pos,
+                                    const int32_t *cap, const float *inv_freq, size_t inv_len,
+                                    size_t heads, size_t kv_heads, size_t head_dim);
+
+/* Tokens first[b] .. first[b] + (cu_seqlens[b+1] - cu_seqlens[b]) of each cache
+ * as the values they stand for, f16 rows [kv_heads*head_dim] packed from row
+ * cu_seqlens[b] of k_out and v_out on. */
+llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *caches, const int32_t *cap,
+                                   const int32_t *live, const int32_t *first,
+                                   const int32_t *cu_seqlens, size_t batch, size_t kv_heads,
+                                   size_t head_dim, uint16_t *k_out, size_t k_len, uint16_t *v_out,
+                                   size_t v_len);
+
+/* Cuts caches that hold live[b] tokens back to to[b] <= live[b], as a prompt
+ * that shares only its opening with the last one asks for: where the cut falls
+ * inside a complete block, the block's first tokens go back into the tail. (They
+ * are rounded to f16 from their 8-bit values, and to 8 bits once more when the
+ * block is complete again. A cut at a multiple of 32 costs nothing.) */
+llmtie_status llmtie_cache_rewind_q8(llmtie_gpu *g, void *const *caches, const int32_t *cap,
+                                     const int32_t *live, const int32_t *to, size_t batch,
+                                     size_t kv_heads, size_t head_dim);
+
+/* llmtie_cache_grow_f16 for an 8-bit cache: `live` tokens (their codes, scales,
+ * weights and tail) from a cache of old_cap into one of new_cap >= old_cap. */
+llmtie_status llmtie_cache_grow_q8(llmtie_gpu *g, const void *src, size_t src_len, void *dst,
+                                   size_t dst_len, size_t kv_heads, size_t head_dim,
+                                   size_t old_cap, size_t new_cap, size_t live);
+
+/* llmtie_decode_batched over 8-bit caches: q f32 [batch][heads*head_dim], one
+ * query a head over live[b] tokens; out [batch][heads*head_dim], f16 (rounded
+ * once) or f32. heads/kv_heads at most 8. A sequence that holds no token gets
+ * zeros. With `weigh`, every complete block's weight gains the attention that
+ * its tokens got, summed over the heads of the group (the tail's tokens have
+ * none yet): what llmtie_cache_evict_q8 goes by. The query and the
+ * probabilities are held to 16 bits, relative to a row's and a block's largest
+ * value; sums are exact or f32. The result does not depend on what ran before
+ * or beside the call. */
+llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q, size_t q_len,
+                                       void *const *caches, const int32_t *live,
+                                       const int32_t *cap, size_t batch, size_t heads,
+                                       size_t kv_heads, size_t head_dim, float scale,
+                                       int32_t weigh, llmtie_decode_scratch *scratch, void *out,
+                                       size_t out_len, int32_t out_f16);
+
+/* llmtie_flash_attn_f16 over 8-bit caches, for a packed ragged batch: sequence
+ * b's rows cu_seqlens[b] .. cu_seqlens[b+1] of q f32 [rows][heads*head_dim]
+ * (already rotated) attend to its cache, which holds past[b] tokens before
+ * theirs and theirs (llmtie_rope_append_q8 puts them there): causal, or all to
+ * all. out [rows][heads*head_dim], f16 or f32. The live keys are unpacked to
+ * f16 once, into memory that the handle keeps for the purpose, for at most
+ * eight sequences at a time. */
+llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len,
+                                   const int32_t *cu_seqlens, size_t batch,
+                                   const void *const *caches, const int32_t *past,
+                                   const int32_t *cap, size_t heads, size_t kv_heads,
+                                   size_t head_dim, float scale, int32_t causal, void *out,
+                                   size_t out_len, int32_t out_f16);
+
+/* Shortens caches by the blocks that attention cared least for. Of the live[b]
+ * / 32 complete blocks of src[b], keep[b] stay (all, where there are no more),
+ * each KV head its own: the first keep_first, the last keep_recent, and of the
+ * others those of the largest weight, the lower block where two weigh the same
+ * (a weight that is negative or NaN counts as zero). They keep their order,
+ * codes, scales and weights, and go to dst[b], which may be src[b] (with its
+ * capacity) or a cache of its own; the tail follows them. Afterwards the cache
+ * holds min(live / 32, keep) * 32 + live % 32 tokens; the keys keep the
+ * rotation of the positions they were appended at. `index` (or NULL) gets the
+ * number in src of each block kept, int32 [batch][kv_heads][K], K the most that
+ * a sequence of the call keeps; entries past a sequence's own are left alone. */
+llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const *src, const int32_t *src_cap,
+                                    void *const *dst, const int32_t *dst_cap, const int32_t *live,
+                                    const int32_t *keep, size_t batch, size_t keep_first,
+                                    size_t keep_recent, size_t kv_heads, size_t head_dim,
+                                    int32_t *index, size_t index_len);
+
 /* ---- profiling ---------------------------------------------------------------- */
 
 /* kprof (device.rs:1490-1565): with it on, every launch is bracketed by

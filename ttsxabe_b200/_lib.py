@@ -94,6 +94,21 @@ PROTOTYPES = {
         [vp, vp, sz, vp, sz, vp, sz, pi32, sz, pvp, pvp, pi32, pi32, vp, sz, sz, sz, f32, f32,
          vp, sz],
     ),
+    "llmtie_kv_q8_bytes": (sz, [sz, sz, sz]),
+    "llmtie_kv_alloc_q8": (i32, [vp, sz, sz, sz, pvp]),
+    "llmtie_rope_inv_freq": (i32, [vp, vp, sz, f32, vp, sz]),
+    "llmtie_rope_append_q8": (
+        i32, [vp, vp, sz, vp, sz, vp, sz, vp, sz, pi32, sz, pvp, pi32, pi32, pi32, vp, sz, sz, sz, sz]),
+    "llmtie_cache_read_q8": (
+        i32, [vp, pvp, pi32, pi32, pi32, pi32, sz, sz, sz, vp, sz, vp, sz]),
+    "llmtie_cache_rewind_q8": (i32, [vp, pvp, pi32, pi32, pi32, sz, sz, sz]),
+    "llmtie_cache_grow_q8": (i32, [vp, vp, sz, vp, sz, sz, sz, sz, sz, sz]),
+    "llmtie_decode_batched_q8": (
+        i32, [vp, vp, sz, pvp, pi32, pi32, sz, sz, sz, sz, f32, i32, vp, vp, sz, i32]),
+    "llmtie_flash_attn_q8": (
+        i32, [vp, vp, sz, pi32, sz, pvp, pi32, pi32, sz, sz, sz, f32, i32, vp, sz, i32]),
+    "llmtie_cache_evict_q8": (
+        i32, [vp, pvp, pi32, pvp, pi32, pi32, pi32, sz, sz, sz, sz, sz, vp, sz]),
     "llmtie_kprof_enable": (None, [vp, i32]),
     "llmtie_kprof_reset": (None, [vp]),
     "llmtie_kprof_report": (sz, [vp, C.c_char_p, sz]),

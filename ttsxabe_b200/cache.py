@@ -10,7 +10,7 @@ lowering the live length.
 from __future__ import annotations
 
 from . import _lib
-from .gpu import Gpu
+from .gpu import Gpu, InvalidArgument, evicted_len
 
 
 def want_capacity(cap: int, past: int, n: int, max_positions: int) -> int:
@@ -64,6 +64,76 @@ class KvCache:
 
     def clear(self) -> None:
         self.len = 0
+
+
+class KvCacheQ8:
+    """The 8-bit KV cache of one layer, with the growth policy of `KvCache`
+    (capacities rounded up to whole blocks of 32 tokens). `len` counts the tokens
+    it holds, `pos` those of the conversation: an eviction makes it the shorter
+    of the two, and new tokens go on at `pos`."""
+
+    def __init__(self, gpu: Gpu, kv_heads: int, head_dim: int, max_positions: int) -> None:
+        self.gpu = gpu
+        self.kv_heads = kv_heads
+        self.head_dim = head_dim
+        self.max_positions = max_positions
+        self.cap = 0
+        self.len = 0
+        self.pos = 0
+        self.newest = 0     # this many of the last tokens lie as they came, no block gone among them
+        self.data = None
+
+    def reserve(self, n: int) -> None:
+        """Makes room for n more positions."""
+        want = want_capacity(self.cap, self.len, n, self.max_positions)
+        if want == 0:
+            return
+        want = (want + 31) // 32 * 32
+        g = self.gpu
+        data = g.kv_alloc_q8(self.kv_heads, self.head_dim, want)
+        if self.len > 0:
+            g.cache_grow_q8(self.data, data, self.kv_heads, self.head_dim, self.cap, want,
+                            self.len)
+        self.data, self.cap = data, want
+
+    def append(self, q, k, v, n: int, inv_freq, heads: int, q_out=None) -> None:
+        """Rotates n projected rows of q, k and v and appends those of k and v."""
+        self.reserve(n)
+        self.gpu.rope_append_q8(q, k, v, [0, n], [self.data], [self.cap], [self.len], [self.pos],
+                                inv_freq, heads, self.kv_heads, self.head_dim, q_out=q_out)
+        self.len += n
+        self.pos += n
+        self.newest += n
+
+    def evict(self, keep: int, keep_first: int = 1, keep_recent: int = 1) -> None:
+        """Keeps `keep` complete blocks, in place: the first, the most recent, and
+        those that decode steps with `weigh` gave the most weight."""
+        if self.len // 32 <= keep:
+            return
+        self.gpu.cache_evict_q8([self.data], [self.cap], [self.data], [self.cap], [self.len],
+                                [keep], keep_first, keep_recent, self.kv_heads, self.head_dim)
+        self.newest = min(self.newest, 32 * keep_recent + self.len % 32)
+        self.len = evicted_len(self.len, keep)
+
+    def truncate(self, length: int) -> None:
+        """Forgets every position of the conversation from `length` on."""
+        gone = self.pos - length
+        if gone <= 0:
+            return
+        if length == 0:
+            self.clear()
+            return
+        if gone > self.newest:
+            raise InvalidArgument(f"cutting a conversation of {self.pos} positions to {length}: "
+                                  f"blocks before the last {self.newest} have been evicted")
+        self.gpu.cache_rewind_q8([self.data], [self.cap], [self.len], [self.len - gone],
+                                 self.kv_heads, self.head_dim)
+        self.len -= gone
+        self.newest -= gone
+        self.pos = length
+
+    def clear(self) -> None:
+        self.len = self.pos = self.newest = 0
 
 
 def shared_prefix(held, ids) -> int:

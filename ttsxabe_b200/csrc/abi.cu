@@ -63,7 +63,17 @@ void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t
 {
     *err = cudaSuccess;
     if (bytes <= w.bytes) return w.ptr;
-    if (w.ptr) cudaFreeAsync(w.ptr, st);
+    if (w.keep) {
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        *err = cudaStreamIsCapturing(st, &capture);
+        if (*err == cudaSuccess && capture != cudaStreamCaptureStatusNone) {
+            *err = cudaErrorStreamCaptureUnsupported;   // make the call once before capturing it
+        }
+        if (*err != cudaSuccess) return nullptr;
+        if (w.ptr) w.outgrown.push_back(w.ptr);
+    } else if (w.ptr) {
+        cudaFreeAsync(w.ptr, st);
+    }
     w.ptr = nullptr;
     w.bytes = 0;
     size_t want = 1 << 20;
@@ -75,6 +85,15 @@ void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t
     }
     w.bytes = want;
     return w.ptr;
+}
+
+void workspace_free(Workspace &w, cudaStream_t st)
+{
+    for (void *p : w.outgrown) cudaFreeAsync(p, st);
+    if (w.ptr) cudaFreeAsync(w.ptr, st);
+    w.outgrown.clear();
+    w.ptr = nullptr;
+    w.bytes = 0;
 }
 
 LaunchScope::LaunchScope(llmtie_gpu *g_, const char *name_) : g(g_), name(name_)
@@ -194,6 +213,8 @@ extern "C" void llmtie_close(llmtie_gpu *g)
     if (g->ws_rope.ptr) cudaFreeAsync(g->ws_rope.ptr, g->stream);
     if (g->ws_part.ptr) cudaFreeAsync(g->ws_part.ptr, g->stream);
     if (g->ws_kv16.ptr) cudaFreeAsync(g->ws_kv16.ptr, g->stream);
+    workspace_free(g->ws_q8, g->stream);
+    workspace_free(g->ws_q8_part, g->stream);
     if (g->stream) cudaStreamSynchronize(g->stream);
     if (g->abort_epoch) cudaFree(g->abort_epoch);
     if (g->timeout_host) cudaFreeHost(g->timeout_host);
@@ -219,6 +240,7 @@ static llmtie_status report_device_timeout(llmtie_gpu *g)
     cudaMemsetAsync(g->abort_epoch, 0, sizeof(int), g->stream);
     for (llmtie_decode_scratch *s : g->scratches) {
         if (s->ctr) cudaMemsetAsync(s->ctr, 0, s->ctr_words * sizeof(unsigned), g->stream);
+        if (s->q8_ctr.ptr) cudaMemsetAsync(s->q8_ctr.ptr, 0, s->q8_ctr.bytes, g->stream);
     }
     return llmtie_fail(LLMTIE_ERR_TIMEOUT, "a bounded device wait gave up (site %d)", site);
 }
@@ -1047,6 +1069,9 @@ extern "C" void llmtie_decode_scratch_free(llmtie_gpu *g, llmtie_decode_scratch 
     if (g) {
         if (s->part) cudaFreeAsync(s->part, g->stream);
         if (s->ctr) cudaFreeAsync(s->ctr, g->stream);
+        workspace_free(s->q8_part, g->stream);
+        workspace_free(s->q8_ctr, g->stream);
+        workspace_free(s->q8_stats, g->stream);
         g->scratches.erase(std::remove(g->scratches.begin(), g->scratches.end(), s),
                            g->scratches.end());
     }
@@ -1852,6 +1877,17 @@ extern "C" llmtie_status llmtie_prefill_varlen(
     }
     return LLMTIE_OK;
 }
+
+// ---- what the entries of other files share ----------------------------------------
+
+llmtie_status llmtie_driver_fail(const char *what, cudaError_t e) { return driver_fail(what, e); }
+llmtie_status llmtie_misaligned(const char *what, const void *p, size_t align)
+{
+    return misaligned(what, p, align);
+}
+llmtie_status llmtie_unsupported(size_t hd, size_t heads, size_t kv) { return unsupported(hd, heads, kv); }
+WaitCtl llmtie_next_wait_ctl(llmtie_gpu *g) { return next_wait_ctl(g); }
+bool llmtie_use_tc(const PrefillParams &p, int hd) { return use_tc(p, hd); }
 
 // ---- profiling -------------------------------------------------------------------
 

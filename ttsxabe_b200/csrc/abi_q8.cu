@@ -1,0 +1,538 @@
+// The C ABI of the 8-bit KV cache: host-side refusals and the launches. As in
+// abi.cu every range is checked here, before anything is launched.
+#include "kv_q8.cuh"
+
+#include <stdlib.h>
+#include <string.h>
+
+#include <algorithm>
+#include <utility>
+#include <vector>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+bool fits_i32(size_t x) { return x <= 0x7fffffffu; }
+
+size_t cache_bytes(size_t kv_heads, size_t hd, size_t cap)
+{
+    return (size_t)q8_layout((int)kv_heads, (int)hd, (int)(cap / kQ8Block)).bytes;
+}
+
+// The shapes every entry takes.
+llmtie_status check_geometry(llmtie_gpu *g, size_t batch, size_t kv_heads, size_t hd)
+{
+    if (!g) return llmtie_fail(LLMTIE_ERR_INVALID, "null device handle");
+    cudaSetDevice(g->ordinal);
+    if ((hd != 64 && hd != 128) || kv_heads == 0) return llmtie_unsupported(hd, kv_heads, kv_heads);
+    if (kv_heads > 4096) return llmtie_fail(LLMTIE_ERR_INVALID, "an 8-bit cache of %zu KV heads", kv_heads);
+    if (!fits_i32(batch)) return llmtie_fail(LLMTIE_ERR_INVALID, "a batch of %zu", batch);
+    return LLMTIE_OK;
+}
+
+// One cache of a table, holding (or about to hold) `live` tokens.
+llmtie_status check_cache(const void *base, int32_t cap, long long live)
+{
+    if (!base) return llmtie_fail(LLMTIE_ERR_INVALID, "null 8-bit cache");
+    if (((uintptr_t)base & 15u) != 0) return llmtie_misaligned("an 8-bit cache", base, 16);
+    if (cap <= 0 || cap % kQ8Block != 0) {
+        return llmtie_fail(LLMTIE_ERR_RAGGED_BLOCK, "an 8-bit cache with a capacity of %d, which is not a multiple of %d",
+                           cap, kQ8Block);
+    }
+    if (live < 0 || live > cap) {
+        return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "appending at %lld to a cache with room for %d", live, cap);
+    }
+    return LLMTIE_OK;
+}
+
+// Caches that one call writes must not share memory: their writes would race.
+llmtie_status check_apart(std::vector<std::pair<uintptr_t, size_t>> &spans)
+{
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); i++) {
+        if (spans[i].first < spans[i - 1].first + spans[i - 1].second) {
+            return llmtie_fail(LLMTIE_ERR_INVALID, "two caches of one call share memory");
+        }
+    }
+    return LLMTIE_OK;
+}
+
+llmtie_status overrun(size_t need, size_t have)
+{
+    return llmtie_fail(LLMTIE_ERR_SLICE_OVERRUN, "reading to %zu in a buffer of %zu", need, have);
+}
+
+// cu_seqlens ascending from >= 0; *total is its last entry.
+llmtie_status check_rows(const int32_t *cu, size_t batch, size_t *total)
+{
+    if (cu[0] < 0) return llmtie_fail(LLMTIE_ERR_INVALID, "cu_seqlens starts at %d", cu[0]);
+    for (size_t b = 0; b < batch; b++) {
+        if (cu[b + 1] < cu[b]) return llmtie_fail(LLMTIE_ERR_INVALID, "cu_seqlens is not ascending");
+    }
+    *total = (size_t)cu[batch];
+    return LLMTIE_OK;
+}
+
+#define TRY(x)                              \
+    do {                                    \
+        const llmtie_status try_s = (x);    \
+        if (try_s != LLMTIE_OK) return try_s; \
+    } while (0)
+
+}  // namespace
+
+extern "C" size_t llmtie_kv_q8_bytes(size_t kv_heads, size_t head_dim, size_t cap)
+{
+    if ((head_dim != 64 && head_dim != 128) || kv_heads == 0 || kv_heads > 4096 || cap % kQ8Block != 0 || !fits_i32(cap)) return 0;
+    return cache_bytes(kv_heads, head_dim, cap);
+}
+
+extern "C" llmtie_status llmtie_kv_alloc_q8(llmtie_gpu *g, size_t kv_heads, size_t head_dim, size_t cap, void **cache)
+{
+    TRY(check_geometry(g, 0, kv_heads, head_dim));
+    if (!cache) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
+    if (cap == 0 || cap % kQ8Block != 0 || !fits_i32(cap)) {
+        return llmtie_fail(LLMTIE_ERR_RAGGED_BLOCK, "an 8-bit cache with a capacity of %zu, which is not a multiple of %d",
+                           cap, kQ8Block);
+    }
+    return llmtie_zeros(g, cache_bytes(kv_heads, head_dim, cap), cache);
+}
+
+extern "C" llmtie_status llmtie_rope_inv_freq(llmtie_gpu *g, const float *freq_div, size_t head_dim, float theta,
+                                              float *out, size_t out_len)
+{
+    if (!g) return llmtie_fail(LLMTIE_ERR_INVALID, "null device handle");
+    cudaSetDevice(g->ordinal);
+    if (head_dim == 0 || head_dim % 2 != 0) {
+        return llmtie_fail(LLMTIE_ERR_ODD_HEAD_DIM, "rotating heads of %zu, which is not even", head_dim);
+    }
+    if (!out) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
+    if (out_len < head_dim / 2) return overrun(head_dim / 2, out_len);
+    if (!fits_i32(head_dim)) return llmtie_fail(LLMTIE_ERR_INVALID, "a head of %zu", head_dim);
+    LaunchScope ls(g, "rope_inv_freq");
+    launch_rope_inv_freq(g->stream, out, freq_div, (int)head_dim, theta);
+    return ls.done();
+}
+
+extern "C" llmtie_status llmtie_rope_append_q8(llmtie_gpu *g, const float *q, size_t q_len, float *q_out, size_t q_out_len,
+                                               const float *k, size_t k_len, const float *v, size_t v_len,
+                                               const int32_t *cu_seqlens, size_t batch, void *const *caches,
+                                               const int32_t *past, const int32_t *pos, const int32_t *cap,
+                                               const float *inv_freq, size_t inv_len, size_t heads, size_t kv_heads,
+                                               size_t head_dim)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!cu_seqlens || !caches || !past || !pos || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    if (batch == 0) return LLMTIE_OK;
+    size_t total;
+    TRY(check_rows(cu_seqlens, batch, &total));
+    const bool turn_q = q != nullptr && inv_freq != nullptr;
+    if (turn_q && (heads == 0 || heads > 65536)) return llmtie_unsupported(head_dim, heads, kv_heads);
+    if (k_len < total * kv_heads * head_dim || v_len < total * kv_heads * head_dim) {
+        return overrun(total * kv_heads * head_dim, std::min(k_len, v_len));
+    }
+    if (total > (size_t)cu_seqlens[0] && (!k || !v)) return llmtie_fail(LLMTIE_ERR_INVALID, "null key or value rows");
+    if (((uintptr_t)k & 15u) != 0) return llmtie_misaligned("the key rows", k, 16);
+    if (((uintptr_t)v & 15u) != 0) return llmtie_misaligned("the value rows", v, 16);
+    if (inv_freq && inv_len < head_dim / 2) return overrun(head_dim / 2, inv_len);
+    if (turn_q) {
+        const size_t need = total * heads * head_dim;
+        if (!q_out) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
+        if (q_len < need || q_out_len < need) return overrun(need, std::min(q_len, q_out_len));
+        if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
+        if (((uintptr_t)q_out & 15u) != 0) return llmtie_misaligned("the rotated query", q_out, 16);
+        // in place, or clear of everything the call reads
+        const uintptr_t o0 = (uintptr_t)q_out, o1 = o0 + need * 4;
+        auto meets = [&](const float *x, size_t n) { return o0 < (uintptr_t)x + n * 4 && (uintptr_t)x < o1; };
+        if ((q_out != q && meets(q, need)) || meets(k, total * kv_heads * head_dim) || meets(v, total * kv_heads * head_dim)) {
+            return llmtie_fail(LLMTIE_ERR_INVALID, "the rotated query overlaps the rows the call reads");
+        }
+    }
+    std::vector<std::pair<uintptr_t, size_t>> spans;
+    for (size_t b = 0; b < batch; b++) {
+        const int n = cu_seqlens[b + 1] - cu_seqlens[b];
+        if (n == 0) continue;
+        TRY(check_cache(caches[b], cap[b], past[b] < 0 ? -1 : (long long)past[b] + n));
+        if (pos[b] < 0 || (long long)pos[b] + n > 0x7fffffffll) {
+            return llmtie_fail(LLMTIE_ERR_INVALID, "rows at position %d", pos[b]);
+        }
+        spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
+    }
+    TRY(check_apart(spans));
+    for (size_t b0 = 0; b0 < batch;) {
+        Q8AppendParams p;
+        memset(&p, 0, sizeof(p));
+        for (; b0 < batch && p.nseq < LLMTIE_Q8_MAX_SEQ; b0++) {
+            const int n = cu_seqlens[b0 + 1] - cu_seqlens[b0];
+            if (n == 0) continue;
+            Q8AppendSeq &s = p.seq[p.nseq++];
+            s.base = (unsigned char *)caches[b0];
+            s.nb = cap[b0] / kQ8Block;
+            s.past = past[b0];
+            s.n = n;
+            s.row0 = cu_seqlens[b0];
+            s.pos = pos[b0];
+            s.item0 = p.items;
+            const int rows = past[b0] % kQ8Block + n, blocks = (rows + kQ8Block - 1) / kQ8Block;
+            p.items += blocks - (blocks > 1 && rows % kQ8Block != 0 ? 1 : 0);
+        }
+        if (p.nseq == 0) break;
+        p.q = turn_q ? q : nullptr;
+        p.q_out = q_out;
+        p.k = k;
+        p.v = v;
+        p.inv_freq = inv_freq;
+        p.heads = (int)heads;
+        p.kv_heads = (int)kv_heads;
+        LaunchScope ls(g, "rope_append_q8");
+        const cudaError_t e = launch_q8_append(g->stream, p, (int)head_dim, g->sm_count);
+        if (e != cudaSuccess) return llmtie_driver_fail("rope_append_q8", e);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
+extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *caches, const int32_t *cap,
+                                              const int32_t *live, const int32_t *first, const int32_t *cu_seqlens,
+                                              size_t batch, size_t kv_heads, size_t head_dim, uint16_t *k_out,
+                                              size_t k_len, uint16_t *v_out, size_t v_len)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!cu_seqlens || !caches || !cap || !live || !first) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    if (batch == 0) return LLMTIE_OK;
+    size_t total;
+    TRY(check_rows(cu_seqlens, batch, &total));
+    if (k_len < total * kv_heads * head_dim || v_len < total * kv_heads * head_dim) {
+        return overrun(total * kv_heads * head_dim, std::min(k_len, v_len));
+    }
+    if (total > (size_t)cu_seqlens[0] && (!k_out || !v_out)) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
+    if (((uintptr_t)k_out & 7u) != 0) return llmtie_misaligned("the keys read", k_out, 8);
+    if (((uintptr_t)v_out & 7u) != 0) return llmtie_misaligned("the values read", v_out, 8);
+    for (size_t b = 0; b < batch; b++) {
+        const int n = cu_seqlens[b + 1] - cu_seqlens[b];
+        if (n == 0) continue;
+        TRY(check_cache(caches[b], cap[b], live[b]));
+        if (first[b] < 0 || (long long)first[b] + n > live[b]) {
+            return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "reading to %lld of a cache that holds %d", (long long)first[b] + n, live[b]);
+        }
+    }
+    for (size_t b0 = 0; b0 < batch;) {
+        Q8ReadParams p;
+        memset(&p, 0, sizeof(p));
+        for (; b0 < batch && p.nseq < LLMTIE_Q8_MAX_SEQ; b0++) {
+            const int n = cu_seqlens[b0 + 1] - cu_seqlens[b0];
+            if (n == 0) continue;
+            p.seq[p.nseq++] = {(const unsigned char *)caches[b0], cap[b0] / kQ8Block, live[b0], first[b0], n, cu_seqlens[b0], p.items};
+            p.items += (first[b0] + n - 1) / kQ8Block - first[b0] / kQ8Block + 1;
+        }
+        if (p.nseq == 0) break;
+        p.k = k_out;
+        p.v = v_out;
+        p.kv_heads = (int)kv_heads;
+        LaunchScope ls(g, "cache_read_q8");
+        const cudaError_t e = launch_q8_read(g->stream, p, (int)head_dim);
+        if (e != cudaSuccess) return llmtie_driver_fail("cache_read_q8", e);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
+extern "C" llmtie_status llmtie_cache_rewind_q8(llmtie_gpu *g, void *const *caches, const int32_t *cap,
+                                                const int32_t *live, const int32_t *to, size_t batch, size_t kv_heads,
+                                                size_t head_dim)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!caches || !cap || !live || !to) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    std::vector<std::pair<uintptr_t, size_t>> spans;
+    for (size_t b = 0; b < batch; b++) {
+        TRY(check_cache(caches[b], cap[b], live[b]));
+        if (to[b] < 0 || to[b] > live[b]) {
+            return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "cutting a cache that holds %d to %d", live[b], to[b]);
+        }
+        spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
+    }
+    TRY(check_apart(spans));
+    for (size_t b0 = 0; b0 < batch;) {
+        Q8RewindParams p;
+        memset(&p, 0, sizeof(p));
+        for (; b0 < batch && p.nseq < LLMTIE_Q8_MAX_SEQ; b0++) {
+            // a cut at a block's start needs no tail, one inside the tail has it
+            if (to[b0] % kQ8Block == 0 || to[b0] / kQ8Block == live[b0] / kQ8Block) continue;
+            p.seq[p.nseq++] = {(unsigned char *)caches[b0], cap[b0] / kQ8Block, to[b0]};
+        }
+        if (p.nseq == 0) break;
+        p.kv_heads = (int)kv_heads;
+        LaunchScope ls(g, "cache_rewind_q8");
+        const cudaError_t e = launch_q8_rewind(g->stream, p, (int)head_dim);
+        if (e != cudaSuccess) return llmtie_driver_fail("cache_rewind_q8", e);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
+extern "C" llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const *src, const int32_t *src_cap,
+                                               void *const *dst, const int32_t *dst_cap, const int32_t *live,
+                                               const int32_t *keep, size_t batch, size_t keep_first, size_t keep_recent,
+                                               size_t kv_heads, size_t head_dim, int32_t *index, size_t index_len)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!src || !src_cap || !dst || !dst_cap || !live || !keep) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    std::vector<std::pair<uintptr_t, size_t>> spans;
+    int most = 0;
+    for (size_t b = 0; b < batch; b++) {
+        TRY(check_cache(src[b], src_cap[b], live[b]));
+        const int full = live[b] / kQ8Block;
+        if (keep[b] < 0 || (full > keep[b] && keep_first + keep_recent > (size_t)keep[b])) {
+            return llmtie_fail(LLMTIE_ERR_INVALID, "keeping %d blocks of which the first %zu and the last %zu stay", keep[b],
+                               keep_first, keep_recent);
+        }
+        const int kept = std::min(full, keep[b]);
+        most = std::max(most, kept);
+        TRY(check_cache(dst[b], dst_cap[b], (long long)kept * kQ8Block + live[b] % kQ8Block));
+        spans.emplace_back((uintptr_t)src[b], cache_bytes(kv_heads, head_dim, (size_t)src_cap[b]));
+        if (dst[b] != src[b]) {
+            spans.emplace_back((uintptr_t)dst[b], cache_bytes(kv_heads, head_dim, (size_t)dst_cap[b]));
+        } else if (dst_cap[b] != src_cap[b]) {
+            return llmtie_fail(LLMTIE_ERR_INVALID, "a cache shortened in place keeps its capacity of %d, not %d", src_cap[b],
+                               dst_cap[b]);
+        }
+    }
+    TRY(check_apart(spans));
+    if (index && index_len < batch * kv_heads * (size_t)most) return overrun(batch * kv_heads * (size_t)most, index_len);
+    for (size_t b0 = 0; b0 < batch; b0 += LLMTIE_Q8_MAX_SEQ) {
+        Q8EvictParams p;
+        memset(&p, 0, sizeof(p));
+        p.nseq = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, batch - b0);
+        for (int b = 0; b < p.nseq; b++) {
+            Q8EvictSeq &s = p.seq[b];
+            s.src = (const unsigned char *)src[b0 + b];
+            s.dst = (unsigned char *)dst[b0 + b];
+            s.src_nb = src_cap[b0 + b] / kQ8Block;
+            s.dst_nb = dst_cap[b0 + b] / kQ8Block;
+            s.full = live[b0 + b] / kQ8Block;
+            s.tail = live[b0 + b] % kQ8Block;
+            s.keep = std::min(s.full, (int)keep[b0 + b]);
+            // (where nothing goes, everything is kept whatever these say)
+            s.first = s.keep < s.full ? (int)keep_first : 0;
+            s.recent = s.keep < s.full ? (int)keep_recent : 0;
+        }
+        p.kv_heads = (int)kv_heads;
+        p.max_keep = most;
+        p.user_stride = most;
+        p.user_index = index ? index + b0 * kv_heads * (size_t)most : nullptr;
+        cudaError_t err;
+        p.index = (int *)workspace_reserve(g->ws_q8, (size_t)p.nseq * kv_heads * std::max(most, 1) * sizeof(int), g->stream, &err);
+        if (!p.index) return llmtie_driver_fail("allocating", err);
+        LaunchScope ls(g, "cache_evict_q8");
+        const cudaError_t e = launch_q8_evict(g->stream, p, (int)head_dim, g->sm_count);
+        if (e != cudaSuccess) return llmtie_driver_fail("cache_evict_q8", e);
+        if (most > 0) g->launches++;   // two kernels in that launcher then
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
+extern "C" llmtie_status llmtie_cache_grow_q8(llmtie_gpu *g, const void *src, size_t src_len, void *dst, size_t dst_len,
+                                              size_t kv_heads, size_t head_dim, size_t old_cap, size_t new_cap,
+                                              size_t live)
+{
+    TRY(check_geometry(g, 1, kv_heads, head_dim));
+    if (live > old_cap || new_cap < old_cap || !fits_i32(new_cap)) {
+        return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "appending at %zu to a cache with room for %zu", std::max(live, old_cap),
+                           std::min(new_cap, old_cap));
+    }
+    const int32_t oc = (int32_t)old_cap, nc = (int32_t)new_cap, n = (int32_t)live, keep = n / kQ8Block;
+    TRY(check_cache(src, oc, n));
+    TRY(check_cache(dst, nc, n));
+    if (src_len < cache_bytes(kv_heads, head_dim, old_cap)) return overrun(cache_bytes(kv_heads, head_dim, old_cap), src_len);
+    if (dst_len < cache_bytes(kv_heads, head_dim, new_cap)) return overrun(cache_bytes(kv_heads, head_dim, new_cap), dst_len);
+    if (src == dst) return llmtie_fail(LLMTIE_ERR_INVALID, "a cache cannot grow in place");
+    if (n == 0) return LLMTIE_OK;
+    return llmtie_cache_evict_q8(g, &src, &oc, &dst, &nc, &n, &keep, 1, 0, 0, kv_heads, head_dim, nullptr, 0);
+}
+
+extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q, size_t q_len, void *const *caches,
+                                                  const int32_t *live, const int32_t *cap, size_t batch, size_t heads,
+                                                  size_t kv_heads, size_t head_dim, float scale, int32_t weigh,
+                                                  llmtie_decode_scratch *scratch, void *out, size_t out_len,
+                                                  int32_t out_f16)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!scratch) return llmtie_fail(LLMTIE_ERR_INVALID, "null decode scratch");
+    if (!caches || !live || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    if (heads % kv_heads != 0 || heads / kv_heads > 8 || heads == 0) return llmtie_unsupported(head_dim, heads, kv_heads);
+    const size_t n = heads * head_dim;
+    if (q_len < batch * n) return overrun(batch * n, q_len);
+    if (out_len < batch * n) return overrun(batch * n, out_len);
+    if (batch == 0) return LLMTIE_OK;
+    if (!q || !out) return llmtie_fail(LLMTIE_ERR_INVALID, "null query or output");
+    if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
+    if (((uintptr_t)out & 15u) != 0) return llmtie_misaligned("the output", out, 16);
+    std::vector<std::pair<uintptr_t, size_t>> spans;
+    for (size_t b = 0; b < batch; b++) {
+        TRY(check_cache(caches[b], cap[b], live[b]));
+        if (weigh) spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
+    }
+    TRY(check_apart(spans));
+    for (size_t b0 = 0; b0 < batch; b0 += LLMTIE_Q8_MAX_SEQ) {
+        DecodeQ8Params p;
+        memset(&p, 0, sizeof(p));
+        p.nseq = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, batch - b0);
+        long long units = 0, blocks = 0;
+        for (int b = 0; b < p.nseq; b++) {
+            const int32_t t = live[b0 + b];
+            p.seq[b] = {(unsigned char *)caches[b0 + b], cap[b0 + b] / kQ8Block, t};
+            p.unit0[b] = units;
+            p.stat0[b] = blocks;
+            units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
+            blocks += (long long)(t / kQ8Block) * (long long)kv_heads;
+        }
+        p.unit0[p.nseq] = units;
+        p.heads = (int)heads;
+        p.kv_heads = (int)kv_heads;
+        p.q = q + b0 * n;
+        p.out = out_f16 ? (void *)((uint16_t *)out + b0 * n) : (void *)((float *)out + b0 * n);
+        p.out_f16 = out_f16 ? 1 : 0;
+        p.sl2 = scale * kLog2e;
+        p.status = g->timeout_site;
+        p.wait_cycles = g->wait_cycles;
+        // A block of the grid an SM, and never fewer than four cache blocks for
+        // one: a finer cut spends longer merging than it saves.
+        const int most = std::min(g->sm_count, LLMTIE_Q8_MAX_BLOCKS);
+        const int grid = (int)std::min<long long>(most, (units + 3) / 4);
+        for (int c = 0; c <= grid; c++) p.ustart[c] = grid ? units * c / grid : 0;
+        const size_t pairs = (size_t)p.nseq * kv_heads;
+        cudaError_t err;
+        const size_t slots = (size_t)std::max(grid, 1) * 2 * 8;
+        p.part_o = (float *)workspace_reserve(scratch->q8_part, slots * (head_dim + 2) * sizeof(float), g->stream, &err);
+        if (!p.part_o) return llmtie_driver_fail("allocating", err);
+        p.part_ml = (float2 *)(p.part_o + slots * head_dim);
+        const size_t had = scratch->q8_ctr.bytes;
+        p.ctr = (unsigned *)workspace_reserve(scratch->q8_ctr, pairs * sizeof(unsigned), g->stream, &err);
+        if (!p.ctr) return llmtie_driver_fail("allocating", err);
+        if (scratch->q8_ctr.bytes != had) {
+            err = cudaMemsetAsync(p.ctr, 0, scratch->q8_ctr.bytes, g->stream);
+            if (err != cudaSuccess) return llmtie_driver_fail("zeroing", err);
+        }
+        if (weigh && blocks > 0) {
+            p.stats = (float2 *)workspace_reserve(scratch->q8_stats, (size_t)blocks * 8 * sizeof(float2), g->stream, &err);
+            if (!p.stats) return llmtie_driver_fail("allocating", err);
+        }
+        LaunchScope ls(g, head_dim == 128 ? "decode_q8_128" : "decode_q8_64");
+        err = launch_decode_q8(g->stream, p, (int)head_dim, grid);
+        if (err != cudaSuccess) return llmtie_driver_fail("decode_q8", err);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
+extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len, const int32_t *cu_seqlens,
+                                              size_t batch, const void *const *caches, const int32_t *past,
+                                              const int32_t *cap, size_t heads, size_t kv_heads, size_t head_dim,
+                                              float scale, int32_t causal, void *out, size_t out_len, int32_t out_f16)
+{
+    TRY(check_geometry(g, batch, kv_heads, head_dim));
+    if (!cu_seqlens || !caches || !past || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
+    if (heads % kv_heads != 0 || heads == 0 || heads > 65535) return llmtie_unsupported(head_dim, heads, kv_heads);
+    if (batch == 0) return LLMTIE_OK;
+    size_t total;
+    TRY(check_rows(cu_seqlens, batch, &total));
+    const size_t n = heads * head_dim;
+    if (q_len < total * n || out_len < total * n) return overrun(total * n, std::min(q_len, out_len));
+    if (total > (size_t)cu_seqlens[0] && (!q || !out)) return llmtie_fail(LLMTIE_ERR_INVALID, "null query or output");
+    if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
+    if (((uintptr_t)out & 15u) != 0) return llmtie_misaligned("the output", out, 16);
+    for (size_t b = 0; b < batch; b++) {
+        const int rows = cu_seqlens[b + 1] - cu_seqlens[b];
+        if (rows == 0) continue;
+        TRY(check_cache(caches[b], cap[b], past[b] < 0 ? -1 : (long long)past[b] + rows));
+    }
+    // A launch of the attention kernel takes LLMTIE_TC_MAX_SEQ sequences; a
+    // sequence of more than kRows rows is as many of them as it takes, over the
+    // same keys.
+    constexpr int kRows = 16384;
+    for (size_t b = 0, done = 0; b < batch;) {
+        Q8UnpackParams up;
+        PrefillParams pp;
+        memset(&up, 0, sizeof(up));
+        memset(&pp, 0, sizeof(pp));
+        size_t bytes = 0;
+        size_t at[LLMTIE_TC_MAX_SEQ];       // where the sequence's keys lie in the workspace
+        while (b < batch && pp.nseq < LLMTIE_TC_MAX_SEQ) {
+            const int rows = cu_seqlens[b + 1] - cu_seqlens[b];
+            if (rows == 0) {
+                b++;
+                continue;
+            }
+            const int live = past[b] + rows;
+            const size_t cap16 = ((size_t)live + 7) / 8 * 8, half = (kv_heads * cap16 * head_dim * 2 + 255) / 256 * 256;
+            Q8UnpackSeq &u = up.seq[up.nseq++];
+            u.base = (const unsigned char *)caches[b];
+            u.nb = cap[b] / kQ8Block;
+            u.live = live;
+            u.cap16 = (int)cap16;
+            u.item0 = up.items;
+            up.items += (live + 4 * kQ8Block - 1) / (4 * kQ8Block);
+            const size_t place = bytes;
+            u.k = (uint16_t *)place;             // (offsets until the workspace is known)
+            u.v = (uint16_t *)(place + half);
+            bytes += 2 * half;
+            while (done < (size_t)rows && pp.nseq < LLMTIE_TC_MAX_SEQ) {
+                const int take = (int)std::min<size_t>(kRows, rows - done);
+                PrefillSeq &s = pp.seq[pp.nseq];
+                at[pp.nseq++] = up.nseq - 1;
+                s.row0 = cu_seqlens[b] - cu_seqlens[0] + (int)done;
+                s.tq = take;
+                s.past = past[b] + (int)done;
+                s.cap = (int)cap16;
+                s.tk = live;
+                done += take;
+            }
+            if (done == (size_t)rows) {
+                b++;
+                done = 0;
+            }
+        }
+        if (pp.nseq == 0) break;
+        cudaError_t err;
+        char *work = (char *)workspace_reserve(g->ws_q8, bytes, g->stream, &err);
+        if (!work) return llmtie_driver_fail("allocating", err);
+        for (int i = 0; i < up.nseq; i++) {
+            up.seq[i].k = (uint16_t *)(work + (size_t)up.seq[i].k);
+            up.seq[i].v = (uint16_t *)(work + (size_t)up.seq[i].v);
+        }
+        for (int i = 0; i < pp.nseq; i++) {
+            pp.seq[i].k = up.seq[at[i]].k;
+            pp.seq[i].v = up.seq[at[i]].v;
+        }
+        up.kv_heads = (int)kv_heads;
+        {
+            LaunchScope ls(g, "q8_unpack");
+            const cudaError_t e = launch_q8_unpack(g->stream, up, (int)head_dim);
+            if (e != cudaSuccess) return llmtie_driver_fail("q8_unpack", e);
+            TRY(ls.done());
+        }
+        const size_t row0 = (size_t)cu_seqlens[0] * n;
+        pp.q = q + row0;
+        pp.q_stride = (long long)n;
+        pp.out = out_f16 ? (void *)((uint16_t *)out + row0) : (void *)((float *)out + row0);
+        pp.out_stride = (long long)n;
+        pp.out_f16 = out_f16 ? 1 : 0;
+        pp.heads = (int)heads;
+        pp.kv_heads = (int)kv_heads;
+        pp.causal = causal ? 1 : 0;
+        pp.q_scale = 1.0f;
+        pp.sl2 = scale * kLog2e;
+        const bool tc = llmtie_use_tc(pp, (int)head_dim);
+        static const bool no_pdl = getenv("LLMTIE_B200_NO_PDL") != nullptr;
+        pp.after_prepass = (tc && !no_pdl && !g->kprof) ? 1 : 0;
+        WaitCtl w = llmtie_next_wait_ctl(g);
+        w.part = &g->ws_q8_part;
+        LaunchScope ls(g, tc ? "flash_attn_q8_tc" : "flash_attn_q8");
+        err = tc ? launch_prefill_tc(g->stream, pp, (int)head_dim, w) : launch_prefill_mma(g->stream, pp, (int)head_dim);
+        if (err != cudaSuccess) return llmtie_driver_fail("flash_attn_q8", err);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}

@@ -22,9 +22,16 @@ struct KprofEntry {
 // A device buffer the handle keeps between calls and only ever grows, so that
 // a call which needs scratch memory allocates nothing once it is warm. Work
 // on a handle is stream-ordered, so one call's use ends before the next's begins.
+// With `keep` set a buffer that was outgrown is kept until the handle closes,
+// because a captured graph may still replay work in it, and growing under a
+// capture is refused, because the memory would belong to the graph.
 struct Workspace {
     void *ptr = nullptr;
     size_t bytes = 0;
+    bool keep = false;
+    std::vector<void *> outgrown;
+    Workspace() = default;
+    explicit Workspace(bool keep_) : keep(keep_) {}
 };
 // Returns at least `bytes` of it (null and *err set if the allocation failed).
 void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t *err);
@@ -57,6 +64,8 @@ struct llmtie_gpu {
     std::vector<llmtie_decode_scratch *> scratches;
     Workspace ws_rope;   // the ragged prefill's table of cosines and sines (or its copy of q)
     Workspace ws_part;   // partial results of a prefill whose long row blocks were cut
+    Workspace ws_q8{true};       // the 8-bit cache: its live keys as f16 for prefill, eviction's block lists
+    Workspace ws_q8_part{true};  // the pieces of cut row blocks of prefill over it
     Workspace ws_kv16;   // f16 copies of the live keys of caches the tensor-memory prefill cannot map
 };
 
@@ -74,6 +83,8 @@ struct llmtie_decode_scratch {
     unsigned *ctr = nullptr;   // [pairs], zero at rest
     size_t part_floats = 0;
     size_t ctr_words = 0;
+    // the same for decode over the 8-bit cache, and its blocks' statistics
+    Workspace q8_part{true}, q8_ctr{true}, q8_stats{true};
     // tensor maps of the caches this scratch was last used with, per sequence slot
     DecodeMapKey map_key[32];
     alignas(64) CUtensorMap kmap[32];
@@ -393,7 +404,7 @@ struct PrefillMergeGroup {
     int seq, slot, pslot0, pieces;
 };
 bool prefill_tc_eligible(const PrefillParams &p, int hd);
-// What a launch needs of the handle for its bounded waits.
+// What a launch needs of the handle for its bounded waits (and where its pieces go).
 struct WaitCtl {
     int *status;
     int *abort_epoch;
@@ -427,6 +438,14 @@ struct VarlenParams {
     float *rope_tab;
 };
 void launch_varlen_rope_append(cudaStream_t st, const VarlenParams &p);
+
+// abi.cu: refusals and choices the entries share.
+llmtie_status llmtie_driver_fail(const char *what, cudaError_t e);
+llmtie_status llmtie_misaligned(const char *what, const void *p, size_t align);
+llmtie_status llmtie_unsupported(size_t hd, size_t heads, size_t kv);
+WaitCtl llmtie_next_wait_ctl(llmtie_gpu *g);
+bool llmtie_use_tc(const PrefillParams &p, int hd);
+void workspace_free(Workspace &w, cudaStream_t st);
 
 // Name -> kernel table behind llmtie_kernel_resources: each kernel file
 // registers its entries from a static initialiser.

@@ -1,0 +1,562 @@
+// Split-KV decode over the 8-bit cache (kv_q8.cuh): one query row a head, the
+// codes go into the tensor cores as they lie in memory.
+//
+// Mathematics. With q of a row as 16-bit fixed point, q = f (256 H + L), H and L
+// int8, and a block's keys k = s_k c, the scores are f s_k (256 H.c + L.c): two
+// int8 products, exact in 32 bits. The probabilities of a block are taken
+// relative to the block's own maximum, p = 2^(s - m_blk) in [0, 1], and held as
+// 16-bit fixed point too, p = (256 P + Q) / 65535 with P and Q unsigned bytes:
+// their product with the value codes is exact as well, and is folded into the
+// f32 accumulator with the factor s_v 2^(m_blk - m) / 65535. So nothing is
+// converted code by code, every rounding is 2^-16 of a row's or a block's
+// largest value, and a key far below another block's maximum keeps its
+// precision.
+//
+// Tiles. One warp takes one cache block of 32 tokens: mma.m16n8k32 with the
+// query's H rows as rows 0-7 and its L rows as rows 8-15 of A (up to eight
+// query heads of a group), four key tiles of eight tokens as B; the result
+// fragment holds a row's H and L sums in one thread, and, with the tokens
+// dealt to the tiles' columns as below, exactly the eight tokens whose bytes
+// that thread needs of the A fragment of the second product. No shuffle but
+// the two of the block's maximum, no conversion of codes, no trip of the
+// probabilities through shared memory.
+//
+// The kernel is bound by reading the cache: each warp keeps a ring of its own
+// blocks in flight (cp.async.bulk, an mbarrier a stage), and the grid is cut by
+// work, one block of the grid an SM; a pair (sequence, KV head) that several of
+// them share is merged by the last to arrive.
+#include "kv_q8.cuh"
+
+#include <math_constants.h>
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 8;             // query rows a pair may have
+
+template <int HD>
+struct Geo {
+    static constexpr int BLOCK = kQ8Block * HD;          // bytes of a block's keys (or values)
+    static constexpr int STAGES = HD == 128 ? 3 : 6;
+    static constexpr int RING = kWarps * STAGES * 2 * BLOCK;
+    static constexpr int MERGE = kWarps * kRows * HD * 4;
+    static constexpr int SMEM = RING + MERGE;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Waits for a phase of the ring, at most p.wait_cycles.
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, int *status, long long cycles)
+{
+    long long start = 0;
+    for (uint32_t it = 0;; it++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (it == 0) start = clock64();
+        else if ((it & 15u) == 0 && clock64() - start > cycles) break;
+    }
+    report_timeout(status, 60);
+    return false;
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// One run of a block of the grid: blocks [first, last) of one pair, and its
+// tail if the run reaches the pair's end.
+struct Run {
+    int seq, head;
+    int first, last;      // complete blocks
+    bool tail;
+    bool whole;           // the pair has no other block of the grid
+    long long next;       // unit after the run
+};
+
+__device__ __forceinline__ Run run_at(const DecodeQ8Params &p, long long u, long long end)
+{
+    int lo = 0, hi = p.nseq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.unit0[mid] <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    Run r;
+    const DecodeQ8Seq &s = p.seq[lo];
+    const int units = (s.live + 31) >> 5;                       // never 0 here: such a sequence has no units
+    r.seq = lo;
+    r.head = (int)((u - p.unit0[lo]) / units);
+    const long long begin = p.unit0[lo] + (long long)r.head * units;
+    const int full = s.live >> 5;
+    r.first = (int)(u - begin);
+    const int stop = (int)min((long long)units, end - begin);
+    r.tail = stop > full;
+    r.last = min(stop, full);
+    r.whole = r.first == 0 && stop == units;
+    r.next = begin + stop;
+    return r;
+}
+
+// The block of the grid that holds unit u.
+__device__ __forceinline__ int block_of(const DecodeQ8Params &p, long long u)
+{
+    int lo = 0, hi = (int)gridDim.x - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.ustart[mid] <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <int HD>
+__device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at, int lane, const float (&o)[HD / 32])
+{
+    constexpr int V = HD / 32;
+    if (p.out_f16) {
+        __half2 *d = (__half2 *)((uint16_t *)p.out + at + V * lane);
+#pragma unroll
+        for (int e = 0; e < V / 2; e++) d[e] = __floats2half2_rn(o[2 * e], o[2 * e + 1]);
+    } else {
+        float2 *d = (float2 *)((float *)p.out + at + V * lane);
+#pragma unroll
+        for (int e = 0; e < V / 2; e++) d[e] = make_float2(o[2 * e], o[2 * e + 1]);
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_constant__ DecodeQ8Params p)
+{
+    using G = Geo<HD>;
+    constexpr int PANELS = HD / 64;
+    constexpr int NT = HD / 8;           // value tiles of eight channels
+    constexpr int V = HD / 32;           // channels a lane holds of a merged row
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t bars[kWarps * G::STAGES];
+    __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
+    __shared__ float2 final_s[kRows];
+    __shared__ int last_s;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = p.heads / p.kv_heads;
+    const long long u_begin = p.ustart[blockIdx.x], u_end = p.ustart[blockIdx.x + 1];
+    float *merge = (float *)(smem + G::RING);
+    const uint32_t ring0 = smem_u32(smem) + (uint32_t)warp * (G::STAGES * 2 * G::BLOCK);
+    const uint32_t bar0 = smem_u32(&bars[warp * G::STAGES]);
+    if (lane == 0) {
+        for (int s = 0; s < G::STAGES; s++) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s));
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+
+    // The warp's blocks in order, over all runs: `ahead` is what is fetched next.
+    Run ahead = run_at(p, u_begin, u_end);
+    int ahead_blk = ahead.first + warp;
+    int issued = 0, used = 0;
+    auto skip_done = [&] {
+        while (ahead_blk >= ahead.last && ahead.next < u_end) {
+            ahead = run_at(p, ahead.next, u_end);
+            ahead_blk = ahead.first + warp;
+        }
+        return ahead_blk < ahead.last;
+    };
+    auto fetch = [&] {
+        if (!skip_done()) return;
+        if (lane == 0) {
+            const DecodeQ8Seq &s = p.seq[ahead.seq];
+            const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
+            const long long off = ((long long)ahead.head * s.nb + ahead_blk) * G::BLOCK;
+            const int stage = issued % G::STAGES;
+            const uint32_t dst = ring0 + (uint32_t)stage * (2 * G::BLOCK), bar = bar0 + 8 * stage;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * G::BLOCK) : "memory");
+            bulk_load(dst, s.base + at.k + off, G::BLOCK, bar);
+            bulk_load(dst + G::BLOCK, s.base + at.v + off, G::BLOCK, bar);
+        }
+        issued++;
+        ahead_blk += kWarps;
+    };
+    for (int s = 0; s < G::STAGES; s++) fetch();
+
+    const int r = lane >> 2, c = lane & 3;
+    bool ok = true;
+    for (long long u = u_begin; u < u_end;) {
+        const Run run = run_at(p, u, u_end);
+        const bool is_first = u == u_begin;
+        u = run.next;
+        const DecodeQ8Seq &sq = p.seq[run.seq];
+        const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+        const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
+        const float *ks = (const float *)(sq.base + at.ks) + (long long)run.head * sq.nb;
+        const float *vs = (const float *)(sq.base + at.vs) + (long long)run.head * sq.nb;
+
+        // -- the query as fixed point: row r, the 16 channels of chunk c in each panel
+        uint32_t qa[PANELS][4], qb[PANELS][4];
+        float f_q;
+        {
+            float x[PANELS][16];
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < PANELS; j++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
+                    x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(x[j][i]) & 0x7fffffffu);
+            }
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const float top = __uint_as_float(most);
+            // (an infinity or NaN in the row makes every score NaN)
+            const bool some = most > 0u && most < 0x7f800000u;
+            f_q = some ? top * (1.0f / 32639.0f) * p.sl2 : (most ? __uint_as_float(0x7fffffffu) : 0.0f);
+            const float inv = some ? 32639.0f / top : 0.0f;
+#pragma unroll
+            for (int j = 0; j < PANELS; j++) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t hi = 0, lo = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int z = some ? max(-32639, min(32639, __float2int_rn(x[j][4 * w + i] * inv))) : 0;
+                        hi |= (uint32_t)(((z + 128) >> 8) & 255) << (8 * i);
+                        lo |= (uint32_t)(z & 255) << (8 * i);
+                    }
+                    qa[j][w] = hi;
+                    qb[j][w] = lo;
+                }
+            }
+        }
+
+        // -- the tail in f32: warp w takes query row w, a lane a token, then V channels
+        float t_m = -CUDART_INF_F, t_l = 0.0f, t_o[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) t_o[e] = 0.0f;
+        if (run.tail && warp < group) {
+            const int n = sq.live & 31;
+            const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + (long long)run.head * kQ8Block * HD;
+            const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + (long long)run.head * kQ8Block * HD;
+            float s = -CUDART_INF_F;
+            if (lane < n) {
+                s = 0.0f;
+#pragma unroll 4
+                for (int d = 0; d < HD; d += 8) {
+                    const uint4 kk = *(const uint4 *)(kt + lane * HD + d);
+                    const float4 q0 = __ldg((const float4 *)(qh + warp * HD + d));
+                    const float4 q1 = __ldg((const float4 *)(qh + warp * HD + d + 4));
+                    const float2 k0 = __half22float2(*(const __half2 *)&kk.x), k1 = __half22float2(*(const __half2 *)&kk.y);
+                    const float2 k2 = __half22float2(*(const __half2 *)&kk.z), k3 = __half22float2(*(const __half2 *)&kk.w);
+                    s += q0.x * k0.x + q0.y * k0.y + q0.z * k1.x + q0.w * k1.y + q1.x * k2.x + q1.y * k2.y + q1.z * k3.x + q1.w * k3.y;
+                }
+                s *= p.sl2;
+            }
+            t_m = s;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t_m = fmaxf(t_m, __shfl_xor_sync(0xffffffffu, t_m, o));
+            const float pr = lane < n ? ex2(s - t_m) : 0.0f;
+            t_l = pr;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t_l += __shfl_xor_sync(0xffffffffu, t_l, o);
+#pragma unroll 4
+            for (int t = 0; t < n; t++) {
+                const float w = __shfl_sync(0xffffffffu, pr, t);
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    const float2 x = __half22float2(*(const __half2 *)(vt + t * HD + V * lane + e));
+                    t_o[e] = fmaf(w, x.x, t_o[e]);
+                    t_o[e + 1] = fmaf(w, x.y, t_o[e + 1]);
+                }
+            }
+        }
+
+        // -- the warp's blocks
+        float acc[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0f;
+        float m = -CUDART_INF_F, l = 0.0f;       // reference maximum of row r; this lane's part of the sum
+        float k_scale = 0.0f, v_scale = 0.0f;
+        if (run.first + warp < run.last) {
+            k_scale = __ldg(ks + run.first + warp);
+            v_scale = __ldg(vs + run.first + warp);
+        }
+        for (int blk = run.first + warp; blk < run.last; blk += kWarps) {
+            const int stage = used % G::STAGES;
+            const uint32_t kb = ring0 + (uint32_t)stage * (2 * G::BLOCK), vb = kb + G::BLOCK;
+            const float sk = k_scale, sv = v_scale;
+            if (blk + kWarps < run.last) {
+                k_scale = __ldg(ks + blk + kWarps);
+                v_scale = __ldg(vs + blk + kWarps);
+            }
+            if (ok) ok = ring_wait(bar0 + 8 * stage, (uint32_t)(used / G::STAGES) & 1u, p.status, p.wait_cycles);
+            used++;
+            // scores: column n of tile t is token 8 (n / 2) + 2 t + n % 2
+            float s[8];
+            float mb = -CUDART_INF_F;
+            const float f = f_q * sk;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                int d[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < PANELS; j++) {
+                    const uint32_t src = kb + (uint32_t)(j * (kQ8Block * 64) + (8 * (r >> 1) + 2 * t + (r & 1)) * 64 + c * 16);
+                    uint32_t b0, b1, b2, b3;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(b0), "=r"(b1), "=r"(b2), "=r"(b3) : "r"(src) : "memory");
+                    mma_s8(d, qa[j][0], qb[j][0], qa[j][1], qb[j][1], b0, b1);
+                    mma_s8(d, qa[j][2], qb[j][2], qa[j][3], qb[j][3], b2, b3);
+                }
+                s[2 * t] = (float)(d[0] * 256 + d[2]) * f;          // token 8 c + 2 t of row r
+                s[2 * t + 1] = (float)(d[1] * 256 + d[3]) * f;      // and the next
+                mb = fmaxf(mb, fmaxf(s[2 * t], s[2 * t + 1]));
+            }
+            mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+            mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+            // The reference moves only when a block's maximum is far above it
+            // (2^16 times): f32 has room for the rest.
+            if (__any_sync(0xffffffffu, mb > m + 16.0f)) {
+                const float to = mb > m + 16.0f ? mb : m;
+                const float a = m == -CUDART_INF_F ? 0.0f : ex2(m - to);
+                l *= a;
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    acc[i][0] *= a;
+                    acc[i][1] *= a;
+                }
+                m = to;
+            }
+            float sum = 0.0f;
+            uint32_t z[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float e = ex2(s[i] - mb);
+                sum += e;
+                z[i] = __float_as_uint(fmaf(e, 65535.0f, 8388608.0f));
+            }
+            const float beta = ex2(mb - m);
+            l = fmaf(beta, sum, l);
+            if (p.stats) {
+                float whole = sum;
+                whole += __shfl_xor_sync(0xffffffffu, whole, 1);
+                whole += __shfl_xor_sync(0xffffffffu, whole, 2);
+                if (c == 0) {
+                    p.stats[(p.stat0[run.seq] + (long long)run.head * (sq.live >> 5) + blk) * kRows + r] = make_float2(mb, whole);
+                }
+            }
+            uint32_t a_hi[2], a_lo[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t x = __byte_perm(z[4 * i], z[4 * i + 1], 0x5410), y = __byte_perm(z[4 * i + 2], z[4 * i + 3], 0x5410);
+                a_hi[i] = __byte_perm(x, y, 0x7531);
+                a_lo[i] = __byte_perm(x, y, 0x6420);
+            }
+            const float w = beta * sv * (1.0f / 65535.0f);
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                int d[4] = {0, 0, 0, 0};
+                uint32_t b0, b1;
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(vb + (uint32_t)((8 * i + r) * kQ8Block + 8 * c)) : "memory");
+                mma_u8(d, a_hi[0], a_lo[0], a_hi[1], a_lo[1], b0, b1);
+                acc[i][0] = fmaf((float)(d[0] * 256 + d[2]), w, acc[i][0]);
+                acc[i][1] = fmaf((float)(d[1] * 256 + d[3]), w, acc[i][1]);
+            }
+            __syncwarp();   // every lane has read the stage
+            fetch();
+        }
+
+        // -- the run's result: warp w merges row w of the eight warps' (and its own tail's)
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (c == 0) {
+            m_s[warp][r] = m;
+            l_s[warp][r] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            // (groups of eight channels swizzled by the row: no bank conflicts on either side)
+            *(float2 *)(merge + (warp * kRows + r) * HD + 8 * (i ^ r) + 2 * c) = make_float2(acc[i][0], acc[i][1]);
+        }
+        __syncthreads();
+        const long long row_at = ((long long)run.seq * p.heads + (long long)run.head * group + warp) * HD;
+        const int pair = run.seq * p.kv_heads + run.head;
+        float M = -CUDART_INF_F, L = 0.0f, o[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) o[e] = 0.0f;
+        if (warp < group) {
+            M = t_m;
+#pragma unroll
+            for (int k = 0; k < kWarps; k++) M = fmaxf(M, m_s[k][warp]);
+            const float ft = t_m == -CUDART_INF_F ? 0.0f : ex2(t_m - M);
+            L = t_l * ft;
+#pragma unroll
+            for (int e = 0; e < V; e++) o[e] = t_o[e] * ft;
+#pragma unroll
+            for (int k = 0; k < kWarps; k++) {
+                const float mk = m_s[k][warp];
+                const float fk = mk == -CUDART_INF_F ? 0.0f : ex2(mk - M);
+                L = fmaf(fk, l_s[k][warp], L);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    o[e] = fmaf(fk, merge[(k * kRows + warp) * HD + 8 * ((V * lane / 8) ^ warp) + V * lane % 8 + e], o[e]);
+                }
+            }
+        }
+        bool done = run.whole;
+        if (!run.whole) {
+            const long long slot = (long long)blockIdx.x * 2 + (is_first ? 0 : 1);
+            if (warp < group) {
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    *(float2 *)(p.part_o + (slot * kRows + warp) * HD + V * lane + e) = make_float2(o[e], o[e + 1]);
+                }
+                if (lane == 0) p.part_ml[slot * kRows + warp] = make_float2(M, L);
+            }
+            __threadfence();
+            __syncthreads();
+            const int units = (sq.live + 31) >> 5;
+            const long long begin = p.unit0[run.seq] + (long long)run.head * units;
+            const int b0 = block_of(p, begin), b1 = block_of(p, begin + units - 1);
+            if (tid == 0) {
+                const unsigned seen = atomicAdd(&p.ctr[pair], 1u);
+                last_s = seen == (unsigned)(b1 - b0);
+                if (last_s) p.ctr[pair] = 0u;
+            }
+            __syncthreads();
+            done = last_s != 0;
+            if (done) {
+                __threadfence();
+                if (warp < group) {
+                    // the contributors in order, whoever came last: the same bits every time
+                    M = -CUDART_INF_F;
+                    for (int b = b0; b <= b1; b++) {
+                        const long long sl = (long long)b * 2 + (p.ustart[b] >= begin || b > b0 ? 0 : 1);
+                        M = fmaxf(M, __ldcg(&p.part_ml[sl * kRows + warp]).x);
+                    }
+                    L = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < V; e++) o[e] = 0.0f;
+                    for (int b = b0; b <= b1; b++) {
+                        const long long sl = (long long)b * 2 + (p.ustart[b] >= begin || b > b0 ? 0 : 1);
+                        const float2 ml = __ldcg(&p.part_ml[sl * kRows + warp]);
+                        const float fk = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - M);
+                        L = fmaf(fk, ml.y, L);
+#pragma unroll
+                        for (int e = 0; e < V; e += 2) {
+                            const float2 x = __ldcg((const float2 *)(p.part_o + (sl * kRows + warp) * HD + V * lane + e));
+                            o[e] = fmaf(fk, x.x, o[e]);
+                            o[e + 1] = fmaf(fk, x.y, o[e + 1]);
+                        }
+                    }
+                }
+            }
+        }
+        if (done) {
+            const float inv = 1.0f / L;
+            if (warp < group) {
+#pragma unroll
+                for (int e = 0; e < V; e++) o[e] *= inv;
+                store_row<HD>(p, row_at, lane, o);
+                if (lane == 0) final_s[warp] = make_float2(M, inv);
+            }
+            if (p.stats) {
+                // weights: what each block's keys got, over the group's heads
+                __syncthreads();
+                float *weight = (float *)(sq.base + at.w) + (long long)run.head * sq.nb;
+                const int full = sq.live >> 5;
+                const float2 *st = p.stats + (p.stat0[run.seq] + (long long)run.head * full) * kRows;
+                for (int b = tid; b < full; b += kThreads) {
+                    float sum = 0.0f;
+                    for (int k = 0; k < group; k++) {
+                        const float2 x = __ldcg(&st[(long long)b * kRows + k]);
+                        sum = fmaf(ex2(x.x - final_s[k].x) * final_s[k].y, x.y, sum);
+                    }
+                    weight[b] += sum;
+                }
+            }
+        }
+        __syncthreads();   // merge, m_s and final_s are free again
+    }
+    if (!ok) {
+        // a wait gave up: leave the copies still in flight time to land
+        for (int i = 0; i < 64; i++) __nanosleep(1000);
+    }
+}
+
+// Sequences that hold no token: zeros.
+__global__ void q8_zero_rows_kernel(const __grid_constant__ DecodeQ8Params p, int width)
+{
+    if (p.seq[blockIdx.x].live) return;
+    for (int i = threadIdx.x; i < width; i += blockDim.x) {
+        const long long at = (long long)blockIdx.x * width + i;
+        if (p.out_f16) ((uint16_t *)p.out)[at] = 0;
+        else ((float *)p.out)[at] = 0.0f;
+    }
+}
+
+const KernelReg reg128("decode_q8_128", (const void *)decode_q8_kernel<128>);
+const KernelReg reg64("decode_q8_64", (const void *)decode_q8_kernel<64>);
+
+}  // namespace
+
+cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, int grid)
+{
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<128>::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_q8_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<64>::SMEM);
+        if (e != cudaSuccess) return e;
+        configured[dev] = true;
+    }
+    bool empty = false;
+    for (int b = 0; b < p.nseq; b++) empty = empty || p.seq[b].live == 0;
+    if (empty) {
+        q8_zero_rows_kernel<<<p.nseq, 256, 0, st>>>(p, p.heads * hd);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    if (grid == 0) return cudaSuccess;
+    if (hd == 128) decode_q8_kernel<128><<<grid, kThreads, Geo<128>::SMEM, st>>>(p);
+    else decode_q8_kernel<64><<<grid, kThreads, Geo<64>::SMEM, st>>>(p);
+    return cudaGetLastError();
+}

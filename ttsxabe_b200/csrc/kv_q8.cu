@@ -1,0 +1,595 @@
+// The movers of the 8-bit KV cache: rows rotated and appended, read back,
+// unpacked for the prefill kernel, a cut block put back into the tail, and the
+// eviction of blocks by accumulated attention weight.
+#include "kv_q8.cuh"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+// Four int8 codes of one word as floats, exactly: a byte biased to unsigned in
+// the low mantissa byte of 2^23 is 2^23 + code + 128.
+__device__ __forceinline__ void codes_f32(uint32_t w, float (&f)[4])
+{
+    const uint32_t u = w ^ 0x80808080u;
+    f[0] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f;
+    f[1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f;
+    f[2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f;
+    f[3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// The values four codes stand for, rounded to f16.
+__device__ __forceinline__ uint2 dequant4(uint32_t w, float scale)
+{
+    float f[4];
+    codes_f32(w, f);
+    return make_uint2(pack_half2(f[0] * scale, f[1] * scale), pack_half2(f[2] * scale, f[3] * scale));
+}
+
+// A 4 x 4 byte transpose: byte j of r[i] <-> byte i of r[j].
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4])
+{
+    const uint32_t a = __byte_perm(r[0], r[1], 0x5140), b = __byte_perm(r[2], r[3], 0x5140);
+    const uint32_t c = __byte_perm(r[0], r[1], 0x7362), d = __byte_perm(r[2], r[3], 0x7362);
+    r[0] = __byte_perm(a, b, 0x5410);
+    r[1] = __byte_perm(a, b, 0x7632);
+    r[2] = __byte_perm(c, d, 0x5410);
+    r[3] = __byte_perm(c, d, 0x7632);
+}
+
+// The last sequence whose first work item is at or before `item`.
+template <typename Seq>
+__device__ __forceinline__ int seq_of(const Seq *seq, int nseq, int item)
+{
+    int lo = 0, hi = nseq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (seq[mid].item0 <= item) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// ---- append -------------------------------------------------------------------------
+//
+// A block of the grid takes the up to 32 new rows of one cache block for a
+// chunk of heads: blockIdx.y first runs over the chunks of KV heads (keys
+// rotated, then keys and values quantised or put into the tail), then over the
+// chunks of query heads (rotated only). The sines and cosines of those rows are
+// worked out once, into shared memory, and shared by the chunk's heads; the
+// angle is pos * inv_freq[j] in 64 bits, taken in half turns and reduced before
+// it is rounded to f32, so that far positions lose nothing.
+//
+// The sequence's first work item also writes its last, incomplete block: the
+// tail holds the first rows of the one and receives the rows of the other, and
+// one block of the grid does both in order.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_constant__ Q8AppendParams p)
+{
+    constexpr int LPR = HD / 8;                  // lanes of a row, each with four values of either half
+    constexpr int RPW = 32 / LPR;                // rows a warp loads at once
+    constexpr int ITER = kQ8Block / (kWarps * RPW);
+    constexpr int HALF = HD / 2;
+    constexpr int SW = HD / 4 + 1;               // words of a staged row, padded
+    __shared__ float2 turn[kQ8Block][HALF];      // (cosine, sine)
+    __shared__ uint32_t stage[kQ8Block * SW];
+    __shared__ uint32_t red[2][kWarps];
+
+    const int item = blockIdx.x;
+    const Q8AppendSeq sq = p.seq[seq_of(p.seq, p.nseq, item)];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kv_chunks = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
+    const bool is_q = (int)blockIdx.y >= kv_chunks;
+    const int r = sq.past & 31;                  // rows of the first block that lie in the tail
+    const int total = r + sq.n;
+    const int nblk = (total + 31) >> 5;
+    const int mine = item - sq.item0;
+    const bool rest = mine == 0 && nblk > 1 && (total & 31) != 0;   // the last block too
+    const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+
+    for (int pass = 0; pass < (rest ? 2 : 1); pass++) {
+        const int j = pass ? nblk - 1 : mine;
+        const int t_lo = j == 0 ? r : 0;                       // new rows of this block: [t_lo, t_hi)
+        const int t_hi = min(32, total - 32 * j);
+        const long long row_of = (long long)sq.row0 + 32 * j - r;   // + t: its packed row
+        __syncthreads();   // the pass before is done with `turn`, and with the tail rows it read
+        if (p.inv_freq) {
+            for (int i = tid; i < (t_hi - t_lo) * HALF; i += kThreads) {
+                const int t = t_lo + i / HALF, f = i % HALF;
+                const double half_turns = (double)(sq.pos + 32 * j - r + t) * (double)p.inv_freq[f] *
+                                          0.31830988618379067154;
+                float sn, cs;
+                sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &sn, &cs);
+                turn[t][f] = make_float2(cs, sn);
+            }
+        }
+        __syncthreads();
+        const int c = lane % LPR;
+        if (is_q) {
+            const int h0 = ((int)blockIdx.y - kv_chunks) * p.q_chunk;
+            const int nh = min(p.q_chunk, p.heads - h0);
+            const int rows = (t_hi - t_lo) * nh;
+            for (int i = warp * RPW + lane / LPR; i < rows; i += kWarps * RPW) {
+                const int t = t_lo + i / nh, h = h0 + i % nh;
+                const long long e = ((row_of + t) * p.heads + h) * HD + 4 * c;
+                const float4 a = *(const float4 *)(p.q + e), b = *(const float4 *)(p.q + e + HALF);
+                const float2 *w = &turn[t][4 * c];
+                float4 lo, hi;
+                rope_rotate(a.x, b.x, w[0].x, w[0].y, lo.x, hi.x);
+                rope_rotate(a.y, b.y, w[1].x, w[1].y, lo.y, hi.y);
+                rope_rotate(a.z, b.z, w[2].x, w[2].y, lo.z, hi.z);
+                rope_rotate(a.w, b.w, w[3].x, w[3].y, lo.w, hi.w);
+                *(float4 *)(p.q_out + e) = lo;
+                *(float4 *)(p.q_out + e + HALF) = hi;
+            }
+            continue;
+        }
+        const int blk = (sq.past >> 5) + j;
+        const bool complete = 32 * (j + 1) <= total;
+        const int h0 = (int)blockIdx.y * p.kv_chunk;
+        for (int hk = 2 * h0; hk < 2 * min(p.kv_heads, h0 + p.kv_chunk); hk++) {
+            const int h = hk >> 1, which = hk & 1;             // keys, then values
+            const float *src = which ? p.v : p.k;
+            uint16_t *tail = (uint16_t *)(sq.base + (which ? at.vt : at.kt)) + (long long)h * kQ8Block * HD;
+            __half2 x[ITER][4];                                // two halves of the row, four values each
+            uint32_t most = 0;
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                const int t = (warp * ITER + it) * RPW + lane / LPR;
+                uint2 lo16 = make_uint2(0u, 0u), hi16 = lo16;
+                if (t >= t_lo && t < t_hi) {
+                    const long long e = ((row_of + t) * p.kv_heads + h) * HD + 4 * c;
+                    float4 a = *(const float4 *)(src + e), b = *(const float4 *)(src + e + HALF);
+                    if (!which && p.inv_freq) {
+                        const float2 *w = &turn[t][4 * c];
+                        float4 lo, hi;
+                        rope_rotate(a.x, b.x, w[0].x, w[0].y, lo.x, hi.x);
+                        rope_rotate(a.y, b.y, w[1].x, w[1].y, lo.y, hi.y);
+                        rope_rotate(a.z, b.z, w[2].x, w[2].y, lo.z, hi.z);
+                        rope_rotate(a.w, b.w, w[3].x, w[3].y, lo.w, hi.w);
+                        a = lo;
+                        b = hi;
+                    }
+                    lo16 = make_uint2(pack_half2(a.x, a.y), pack_half2(a.z, a.w));
+                    hi16 = make_uint2(pack_half2(b.x, b.y), pack_half2(b.z, b.w));
+                    if (!complete) {
+                        *(uint2 *)(tail + t * HD + 4 * c) = lo16;
+                        *(uint2 *)(tail + t * HD + HALF + 4 * c) = hi16;
+                    }
+                } else if (complete) {                         // (t < t_lo: a row of the tail)
+                    lo16 = *(const uint2 *)(tail + t * HD + 4 * c);
+                    hi16 = *(const uint2 *)(tail + t * HD + HALF + 4 * c);
+                }
+                const uint32_t w[4] = {lo16.x, lo16.y, hi16.x, hi16.y};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[it][i] = *(const __half2 *)&w[i];
+                    most = max(most, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                }
+            }
+            if (!complete) continue;
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) red[which][warp] = most;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kWarps; i++) most = max(most, red[which][i]);
+            // A block that holds an infinity or NaN reads back as NaN throughout.
+            const float top = __half2float(__ushort_as_half((uint16_t)most));
+            const float scale = most >= 0x7c00u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(top, 127.0f);
+            const bool some = most > 0u && most < 0x7c00u;
+            uint32_t *codes = (uint32_t *)(sq.base + (which ? at.v : at.k) +
+                                           ((long long)h * sq.nb + blk) * (kQ8Block * HD));
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                const int t = (warp * ITER + it) * RPW + lane / LPR;
+                uint32_t word[2];
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+                    const float2 u = __half22float2(x[it][2 * side]), v = __half22float2(x[it][2 * side + 1]);
+                    const float y[4] = {u.x, u.y, v.x, v.y};
+                    uint32_t q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        q[i] = some ? (uint32_t)__float2int_rn(__fdiv_rn(y[i], scale)) : 0u;
+                    }
+                    word[side] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                }
+                if (!which) {
+                    // panels of 64 channels: word of token t, channel d in panel d / 64
+                    const int other = HD == 128 ? kQ8Block * 64 / 4 : HALF / 4;
+                    codes[t * 16 + c] = word[0];
+                    codes[t * 16 + c + other] = word[1];
+                } else {
+                    stage[t * SW + c] = word[0];
+                    stage[t * SW + HALF / 4 + c] = word[1];
+                }
+            }
+            if (which) {
+                // transposed: a thread turns four tokens x four channels
+                __syncthreads();
+                const int tq = lane & 7, dq = warp * 4 + (lane >> 3);
+                if (dq < HD / 4) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = stage[(4 * tq + i) * SW + dq];
+                    transpose4(w);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) codes[(4 * dq + i) * 8 + tq] = w[i];
+                }
+                __syncthreads();
+            }
+            if (tid == 0) {
+                const long long b = (long long)h * sq.nb + blk;
+                ((float *)(sq.base + (which ? at.vs : at.ks)))[b] = scale;
+                if (which) ((float *)(sq.base + at.w))[b] = 0.0f;
+            }
+        }
+    }
+}
+
+// ---- reading back -------------------------------------------------------------------
+
+// Tokens [first, first + n) as f16 rows [kv_heads*hd]: blockIdx = (cache block,
+// KV head, keys or values).
+template <int HD>
+__global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant__ Q8ReadParams p)
+{
+    const Q8ReadSeq sq = p.seq[seq_of(p.seq, p.nseq, (int)blockIdx.x)];
+    const int blk = (sq.first >> 5) + (int)blockIdx.x - sq.item0;
+    const int h = blockIdx.y, which = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+    const int t0 = 32 * blk;
+    const int lo = max(sq.first - t0, 0), hi = min(sq.first + sq.n - t0, 32);
+    // row of token t of this block
+    uint16_t *out = (which ? p.v : p.k) + (((long long)sq.row0 + t0 - sq.first) * p.kv_heads + h) * HD;
+    const long long step = (long long)p.kv_heads * HD;
+    if (blk >= sq.live >> 5) {
+        const uint16_t *tail = (const uint16_t *)(sq.base + (which ? at.vt : at.kt)) + (long long)h * kQ8Block * HD;
+        for (int i = tid; i < kQ8Block * HD / 4; i += kThreads) {
+            const int t = i / (HD / 4), d = i % (HD / 4) * 4;
+            if (t >= lo && t < hi) *(uint2 *)(out + t * step + d) = *(const uint2 *)(tail + t * HD + d);
+        }
+        return;
+    }
+    const long long b = (long long)h * sq.nb + blk;
+    const uint32_t *codes = (const uint32_t *)(sq.base + (which ? at.v : at.k) + b * (kQ8Block * HD));
+    const float scale = ((const float *)(sq.base + (which ? at.vs : at.ks)))[b];
+    if (!which) {
+        for (int i = tid; i < kQ8Block * HD / 4; i += kThreads) {
+            const int panel = i / (kQ8Block * 16), t = i / 16 % kQ8Block, d = panel * 64 + i % 16 * 4;
+            if (t >= lo && t < hi) *(uint2 *)(out + t * step + d) = dequant4(codes[i], scale);
+        }
+    } else if (lane < HD / 4) {
+        // a warp takes four tokens, a lane four channels of them
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = codes[(4 * lane + i) * 8 + warp];
+        transpose4(w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = 4 * warp + i;
+            if (t >= lo && t < hi) *(uint2 *)(out + t * step + 4 * lane) = dequant4(w[i], scale);
+        }
+    }
+}
+
+// The live tokens as f16 caches that the prefill kernel's tensor maps can be
+// laid over. blockIdx = (four cache blocks, KV head); a thread turns 16 codes
+// (16 bytes) into 32 bytes of either output. Past the live tokens, up to the
+// capacity (the next multiple of eight), lie zeros.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_constant__ Q8UnpackParams p)
+{
+    // (the attention kernel behind this one may set itself up meanwhile)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Q8UnpackSeq sq = p.seq[seq_of(p.seq, p.nseq, (int)blockIdx.x)];
+    const int blk0 = 4 * ((int)blockIdx.x - sq.item0);
+    const int h = blockIdx.y, tid = threadIdx.x;
+    const int full = sq.live >> 5;
+    const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+    const long long b0 = (long long)h * sq.nb;
+    const float *ks = (const float *)(sq.base + at.ks) + b0, *vs = (const float *)(sq.base + at.vs) + b0;
+    uint16_t *ko = sq.k + (long long)h * sq.cap16 * HD, *vo = sq.v + (long long)h * HD * sq.cap16;
+    constexpr int PER = kQ8Block * HD / 16;      // 16-byte pieces of a block
+#pragma unroll 1
+    for (int i = tid; i < 4 * PER; i += kThreads) {
+        const int blk = blk0 + i / PER, e = i % PER;
+        if (blk >= full) break;
+        const uint4 kc = ((const uint4 *)(sq.base + at.k + (b0 + blk) * (kQ8Block * HD)))[e];
+        const uint4 vc = ((const uint4 *)(sq.base + at.v + (b0 + blk) * (kQ8Block * HD)))[e];
+        const float ksc = ks[blk], vsc = vs[blk];
+        {
+            const int panel = e / (kQ8Block * 4), t = e / 4 % kQ8Block, d = panel * 64 + e % 4 * 16;
+            uint4 *o = (uint4 *)(ko + (long long)(32 * blk + t) * HD + d);
+            const uint2 w0 = dequant4(kc.x, ksc), w1 = dequant4(kc.y, ksc);
+            const uint2 w2 = dequant4(kc.z, ksc), w3 = dequant4(kc.w, ksc);
+            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
+            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
+        }
+        {
+            const int d = e / 2, t = e % 2 * 16;
+            uint4 *o = (uint4 *)(vo + (long long)d * sq.cap16 + 32 * blk + t);
+            const uint2 w0 = dequant4(vc.x, vsc), w1 = dequant4(vc.y, vsc);
+            const uint2 w2 = dequant4(vc.z, vsc), w3 = dequant4(vc.w, vsc);
+            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
+            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
+        }
+    }
+    const int tail = sq.live & 31;
+    if (tail && full >= blk0 && full < blk0 + 4) {
+        const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + (long long)h * kQ8Block * HD;
+        const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + (long long)h * kQ8Block * HD;
+        const int upto = sq.cap16 - 32 * full;                   // (and zeros up to the capacity)
+        for (int i = tid; i < upto * HD; i += kThreads) {
+            ko[(long long)32 * full * HD + i] = i < tail * HD ? kt[i] : (uint16_t)0;
+            const int d = i / upto, t = i % upto;
+            vo[(long long)d * sq.cap16 + 32 * full + t] = t < tail ? vt[t * HD + d] : (uint16_t)0;
+        }
+    }
+}
+
+// The first to % 32 tokens of block to / 32 back into the tail.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) q8_rewind_kernel(const __grid_constant__ Q8RewindParams p)
+{
+    const Q8RewindSeq sq = p.seq[blockIdx.y];
+    const int h = blockIdx.x, which = blockIdx.z, tid = threadIdx.x;
+    const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+    const long long b = (long long)h * sq.nb + (sq.to >> 5);
+    const signed char *codes = (const signed char *)(sq.base + (which ? at.v : at.k) + b * (kQ8Block * HD));
+    const float scale = ((const float *)(sq.base + (which ? at.vs : at.ks)))[b];
+    uint16_t *tail = (uint16_t *)(sq.base + (which ? at.vt : at.kt)) + (long long)h * kQ8Block * HD;
+    for (int i = tid; i < (sq.to & 31) * HD; i += kThreads) {
+        const int t = i / HD, d = i % HD;
+        const int code = which ? codes[d * kQ8Block + t] : codes[d / 64 * (kQ8Block * 64) + t * 64 + d % 64];
+        tail[i] = __half_as_ushort(__float2half_rn((float)code * scale));
+    }
+}
+
+// ---- eviction -----------------------------------------------------------------------
+//
+// Which blocks stay: one block of the grid a (sequence, KV head). The weight of
+// the m-th largest among the blocks that may go is found by its bits, eight at
+// a time (weights are not negative, so their bits order as they do; NaN and
+// negative ones count as zero); then one walk in order keeps what is protected,
+// what is above that weight, and as many of those at it, lowest first, as there
+// is room for. The walk also moves scales and weights: a tile is read before
+// anything of it is written, and a kept block only ever moves down, so source
+// and destination may be one cache.
+constexpr int kPickThreads = 512;
+
+__device__ __forceinline__ uint32_t weight_key(float w) { return w > 0.0f ? __float_as_uint(w) : 0u; }
+
+// Exclusive prefix sum of v over the block; *sum is the total. Every thread calls.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sum, uint32_t *sum)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();   // what was read of warp_sum before is done with
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < kPickThreads / 32; i++) {
+        const uint32_t s = warp_sum[i];
+        if (i < warp) before += s;
+        all += s;
+    }
+    *sum = all;
+    return before + x - v;
+}
+
+__global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_constant__ Q8EvictParams p, int hd)
+{
+    __shared__ uint32_t hist[256], warp_sum[kPickThreads / 32], found[2];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Q8EvictSeq sq = p.seq[blockIdx.y];
+    const int h = blockIdx.x, tid = threadIdx.x;
+    const Q8Layout a = q8_layout(p.kv_heads, hd, sq.src_nb), z = q8_layout(p.kv_heads, hd, sq.dst_nb);
+    const long long sb = (long long)h * sq.src_nb, db = (long long)h * sq.dst_nb;
+    const float *w = (const float *)(sq.src + a.w) + sb;
+    int *index = p.index + ((long long)blockIdx.y * p.kv_heads + h) * p.max_keep;
+    int *user = p.user_index ? p.user_index + ((long long)blockIdx.y * p.kv_heads + h) * p.user_stride : nullptr;
+    const int lo = sq.first, hi = sq.full - sq.recent;           // those that may go
+    const bool all = sq.keep >= sq.full;
+    uint32_t room = all ? 0u : (uint32_t)(sq.keep - sq.first - sq.recent);
+    uint32_t key = 0xffffffffu, ties = 0;                        // above key: stays; at it: the first `ties`
+    if (!all && room > 0) {
+        uint32_t prefix = 0, mask = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
+            __syncthreads();
+            for (int i = lo + tid; i < hi; i += kPickThreads) {
+                const uint32_t k = weight_key(w[i]);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            // digit 255 - tid, so that a prefix sum counts from the top
+            const uint32_t mineh = tid < 256 ? hist[255 - tid] : 0u;
+            uint32_t sum;
+            const uint32_t above = block_scan(mineh, warp_sum, &sum);
+            if (tid < 256 && above < room && above + mineh >= room) {
+                found[0] = 255u - tid;
+                found[1] = room - above;
+            }
+            __syncthreads();
+            prefix |= found[0] << shift;
+            mask |= 255u << shift;
+            room = found[1];
+        }
+        key = prefix;
+        ties = room;
+    }
+    uint32_t kept = 0, tied = 0;
+    for (int i0 = 0; i0 < sq.full; i0 += kPickThreads) {
+        const int i = i0 + tid;
+        const bool in = i < sq.full;
+        const bool safe = in && (all || i < lo || i >= hi);
+        const float wi = in ? w[i] : 0.0f;
+        const uint32_t k = weight_key(wi);
+        const bool tie = in && !safe && k == key;
+        uint32_t sum;
+        const uint32_t t_before = tied + block_scan(tie ? 1u : 0u, warp_sum, &sum);
+        tied += sum;
+        const bool stay = safe || (in && k > key) || (tie && t_before < ties);
+        const uint32_t to = kept + block_scan(stay ? 1u : 0u, warp_sum, &sum);
+        kept += sum;
+        float kscale = 0.0f, vscale = 0.0f;
+        if (stay) {
+            kscale = ((const float *)(sq.src + a.ks))[sb + i];
+            vscale = ((const float *)(sq.src + a.vs))[sb + i];
+        }
+        __syncthreads();   // the tile is read
+        if (stay) {
+            index[to] = i;
+            if (user) user[to] = i;
+            ((float *)(sq.dst + z.ks))[db + to] = kscale;
+            ((float *)(sq.dst + z.vs))[db + to] = vscale;
+            ((float *)(sq.dst + z.w))[db + to] = wi;
+        }
+    }
+    if (sq.dst != sq.src) {
+        const int n = sq.tail * hd;                              // tail rows of this head
+        const uint16_t *kt = (const uint16_t *)(sq.src + a.kt) + (long long)h * kQ8Block * hd;
+        const uint16_t *vt = (const uint16_t *)(sq.src + a.vt) + (long long)h * kQ8Block * hd;
+        uint16_t *ko = (uint16_t *)(sq.dst + z.kt) + (long long)h * kQ8Block * hd;
+        uint16_t *vo = (uint16_t *)(sq.dst + z.vt) + (long long)h * kQ8Block * hd;
+        for (int i = tid; i < n; i += kPickThreads) {
+            ko[i] = kt[i];
+            vo[i] = vt[i];
+        }
+    }
+}
+
+// Moves the kept blocks' codes: blockIdx = (slice of a block's bytes, keys or
+// values of a head, sequence). Slices move by the same list and never meet, so
+// each may go at its own pace; within one, a group of blocks is read before any
+// of it is written, and later groups lie above what it writes.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) q8_move_kernel(const __grid_constant__ Q8EvictParams p, int slices)
+{
+    constexpr int DEPTH = 8;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Q8EvictSeq sq = p.seq[blockIdx.z];
+    const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const int per = kQ8Block * HD / 16 / slices;                 // 16-byte pieces of a slice
+    const int lanes = kThreads / per;                            // blocks a pass of the threads takes
+    const int piece = (int)blockIdx.x * per + threadIdx.x % per, sub = threadIdx.x / per;
+    const Q8Layout a = q8_layout(p.kv_heads, HD, sq.src_nb), z = q8_layout(p.kv_heads, HD, sq.dst_nb);
+    const uint4 *src = (const uint4 *)(sq.src + (which ? a.v : a.k)) + (long long)h * sq.src_nb * (kQ8Block * HD / 16) + piece;
+    uint4 *dst = (uint4 *)(sq.dst + (which ? z.v : z.k)) + (long long)h * sq.dst_nb * (kQ8Block * HD / 16) + piece;
+    const int *index = p.index + ((long long)blockIdx.z * p.kv_heads + h) * p.max_keep;
+    const bool same = sq.src == sq.dst;
+    for (int j0 = 0; j0 < sq.keep; j0 += lanes * DEPTH) {
+        uint4 x[DEPTH];
+        bool go[DEPTH];
+#pragma unroll
+        for (int u = 0; u < DEPTH; u++) {
+            const int j = j0 + u * lanes + sub;
+            go[u] = j < sq.keep;
+            if (go[u]) {
+                const int i = index[j];
+                go[u] = !(same && i == j);
+                if (go[u]) x[u] = src[(long long)i * (kQ8Block * HD / 16)];
+            }
+        }
+        if (same) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < DEPTH; u++) {
+            const int j = j0 + u * lanes + sub;
+            if (go[u]) dst[(long long)j * (kQ8Block * HD / 16)] = x[u];
+        }
+    }
+}
+
+const KernelReg reg_append("q8_append", (const void *)q8_append_kernel<128>);
+const KernelReg reg_read("q8_read", (const void *)q8_read_kernel<128>);
+const KernelReg reg_unpack("q8_unpack", (const void *)q8_unpack_kernel<128>);
+const KernelReg reg_pick("q8_pick", (const void *)q8_pick_kernel);
+const KernelReg reg_move("q8_move", (const void *)q8_move_kernel<128>);
+
+}  // namespace
+
+cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count)
+{
+    // Heads share a block of the grid (and its sines and cosines) as long as the
+    // launch still has a few blocks for every SM.
+    p.kv_chunk = 8;
+    p.q_chunk = 16;
+    auto blocks = [&] {
+        const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
+        const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
+        return (long long)p.items * (kvc + qc);
+    };
+    while (p.kv_chunk > 1 && blocks() < 4ll * sm_count) {
+        p.kv_chunk /= 2;
+        p.q_chunk /= 2;
+    }
+    const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
+    const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
+    const dim3 grid((unsigned)p.items, (unsigned)(kvc + qc));
+    if (hd == 128) q8_append_kernel<128><<<grid, kThreads, 0, st>>>(p);
+    else q8_append_kernel<64><<<grid, kThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_q8_read(cudaStream_t st, const Q8ReadParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads, 2);
+    if (hd == 128) q8_read_kernel<128><<<grid, kThreads, 0, st>>>(p);
+    else q8_read_kernel<64><<<grid, kThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_q8_unpack(cudaStream_t st, const Q8UnpackParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads);
+    if (hd == 128) q8_unpack_kernel<128><<<grid, kThreads, 0, st>>>(p);
+    else q8_unpack_kernel<64><<<grid, kThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_q8_rewind(cudaStream_t st, const Q8RewindParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.kv_heads, (unsigned)p.nseq, 2);
+    if (hd == 128) q8_rewind_kernel<128><<<grid, kThreads, 0, st>>>(p);
+    else q8_rewind_kernel<64><<<grid, kThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_q8_evict(cudaStream_t st, const Q8EvictParams &p, int hd, int sm_count)
+{
+    q8_pick_kernel<<<dim3((unsigned)p.kv_heads, (unsigned)p.nseq), kPickThreads, 0, st>>>(p, hd);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || p.max_keep == 0) return e;
+    // Slices of no less than 256 bytes, until every SM has a few.
+    const int most = kQ8Block * hd / 256;
+    int slices = 1;
+    while (slices < most && (long long)slices * p.kv_heads * 2 * p.nseq < 4ll * sm_count) slices *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)slices, (unsigned)p.kv_heads * 2, (unsigned)p.nseq);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return hd == 128 ? cudaLaunchKernelEx(&cfg, q8_move_kernel<128>, p, slices)
+                     : cudaLaunchKernelEx(&cfg, q8_move_kernel<64>, p, slices);
+}

@@ -1,0 +1,162 @@
+// The 8-bit KV cache: where its sections lie, and the launchers of the kernels
+// that fill, read, shorten and attend over it.
+//
+// Tokens lie in blocks of 32. A complete block of one KV head is int8 codes
+// with one f32 scale for its keys and one for its values: code = rint(x /
+// scale), scale = max|x| / 127 over the block's 32 x hd elements, x the row
+// rounded to f16. The tokens of the last, incomplete block stay f16 rows (the
+// tail), so that a token is rounded to 8 bits once, together with its block,
+// and the codes do not depend on how the tokens arrived (one by one, or in
+// prompts cut anywhere).
+//
+// One buffer holds a layer's cache; its sections, each at a multiple of 128
+// bytes, nb = capacity / 32:
+//   key codes    [kv][nb][hd/64][32 tokens][64]   panels of 64 channels: eight
+//                lanes reading 16 bytes each of two neighbouring rows touch
+//                every bank once
+//   value codes  [kv][nb][hd][32 tokens]          transposed inside a block, as
+//                the product with the probabilities reads them
+//   key scales   f32 [kv][nb]
+//   value scales f32 [kv][nb]
+//   weights      f32 [kv][nb]     accumulated attention weight of each block
+//   key tail     f16 [kv][32][hd]
+//   value tail   f16 [kv][32][hd]
+#pragma once
+
+#include "common.cuh"
+
+constexpr int kQ8Block = 32;
+#define LLMTIE_Q8_MAX_SEQ 32
+
+struct Q8Layout {
+    long long k, v, ks, vs, w, kt, vt, bytes;
+};
+__host__ __device__ inline Q8Layout q8_layout(int kv_heads, int hd, int nb)
+{
+    const long long codes = (long long)kv_heads * nb * kQ8Block * hd;
+    const long long scales = ((long long)kv_heads * nb * 4 + 127) / 128 * 128;
+    const long long tail = (long long)kv_heads * kQ8Block * hd * 2;
+    Q8Layout l;
+    l.k = 0;
+    l.v = codes;
+    l.ks = 2 * codes;
+    l.vs = l.ks + scales;
+    l.w = l.vs + scales;
+    l.kt = l.w + scales;
+    l.vt = l.kt + tail;
+    l.bytes = l.vt + tail;
+    return l;
+}
+
+// ---- kv_q8.cu ---------------------------------------------------------------
+
+struct Q8AppendSeq {
+    unsigned char *base;
+    int nb;        // blocks of the cache's capacity
+    int past;      // tokens the cache holds
+    int n;         // rows this sequence brings (never 0 here)
+    int row0;      // its first row in q, k and v
+    int pos;       // rotary position of that row
+    int item0;     // first of its work items
+};
+struct Q8AppendParams {
+    Q8AppendSeq seq[LLMTIE_Q8_MAX_SEQ];
+    int nseq, items;
+    const float *q;          // null: no queries to rotate
+    float *q_out;            // may be q
+    const float *k, *v;
+    const float *inv_freq;   // null: the rows come rotated
+    int heads, kv_heads;
+    int kv_chunk, q_chunk;   // heads a block of the grid takes
+};
+cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count);
+
+struct Q8ReadSeq {
+    const unsigned char *base;
+    int nb, live;
+    int first, n;      // tokens [first, first + n)
+    int row0;          // where they go in the packed outputs
+    int item0;
+};
+struct Q8ReadParams {
+    Q8ReadSeq seq[LLMTIE_Q8_MAX_SEQ];
+    int nseq, items;
+    uint16_t *k, *v;   // f16 [rows][kv_heads*hd]
+    int kv_heads;
+};
+cudaError_t launch_q8_read(cudaStream_t st, const Q8ReadParams &p, int hd);
+
+// The first `live` tokens as f16 caches of capacity cap16 (a multiple of 8):
+// keys [kv][cap16][hd], values [kv][hd][cap16], for the prefill kernel.
+struct Q8UnpackSeq {
+    const unsigned char *base;
+    uint16_t *k, *v;
+    int nb, live, cap16;
+    int item0;
+};
+struct Q8UnpackParams {
+    Q8UnpackSeq seq[LLMTIE_Q8_MAX_SEQ];
+    int nseq, items;
+    int kv_heads;
+};
+cudaError_t launch_q8_unpack(cudaStream_t st, const Q8UnpackParams &p, int hd);
+
+struct Q8RewindSeq {
+    unsigned char *base;
+    int nb, to;        // the block of token `to` goes back into the tail
+};
+struct Q8RewindParams {
+    Q8RewindSeq seq[LLMTIE_Q8_MAX_SEQ];
+    int nseq;
+    int kv_heads;
+};
+cudaError_t launch_q8_rewind(cudaStream_t st, const Q8RewindParams &p, int hd);
+
+struct Q8EvictSeq {
+    const unsigned char *src;
+    unsigned char *dst;      // may be src
+    int src_nb, dst_nb;
+    int full;                // complete blocks in src
+    int tail;                // tokens of the tail
+    int keep;                // blocks that stay, <= full
+    int first, recent;       // blocks at either end that stay whatever their weight
+};
+struct Q8EvictParams {
+    Q8EvictSeq seq[LLMTIE_Q8_MAX_SEQ];
+    int nseq;
+    int kv_heads;
+    int max_keep;
+    int *index;              // [seq][kv][max_keep]: which source block each kept one was
+    int *user_index;         // the same for the caller (or null), rows user_stride apart
+    long long user_stride;
+};
+cudaError_t launch_q8_evict(cudaStream_t st, const Q8EvictParams &p, int hd, int sm_count);
+
+// f32 inverse frequencies theta^(-2j/hd) (/ freq_div[j]), the bits rope_scaled uses.
+void launch_rope_inv_freq(cudaStream_t st, float *out, const float *freq_div, int hd, float theta);
+
+// ---- decode_q8.cu -----------------------------------------------------------
+
+#define LLMTIE_Q8_MAX_BLOCKS 160
+struct DecodeQ8Seq {
+    unsigned char *base;     // (the weights are written)
+    int nb, live;
+};
+struct DecodeQ8Params {
+    DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
+    long long unit0[LLMTIE_Q8_MAX_SEQ + 1];            // first 32-token unit of each sequence
+    long long ustart[LLMTIE_Q8_MAX_BLOCKS + 1];        // block c takes units [ustart[c], ustart[c+1])
+    long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
+    int nseq, heads, kv_heads;
+    const float *q;          // [seq][heads*hd]
+    void *out;               // [seq][heads*hd], f16 or f32
+    int out_f16;
+    float sl2;               // scale * log2(e)
+    float *part_o;           // [block][2][8][hd]
+    float2 *part_ml;         // [block][2][8]
+    unsigned *ctr;           // arrivals of each (sequence, KV head), zero at rest
+    float2 *stats;           // [block of a sequence][8] (maximum, sum), or null: no weights
+    int *status;
+    long long wait_cycles;
+};
+cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, int grid);

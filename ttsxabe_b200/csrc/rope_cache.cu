@@ -144,6 +144,13 @@ __global__ void rope_gptj_kernel(float *__restrict__ x, const float *__restrict_
     }
 }
 
+__global__ void inv_freq_kernel(float *__restrict__ out, const float *__restrict__ freq_div, int hd,
+                                float theta)
+{
+    const int j = blockIdx.x * blockDim.x + threadIdx.x;
+    if (j < hd / 2) out[j] = inv_freq(theta, j, hd, freq_div);
+}
+
 // The decode step's RoPE and cache write for a batch of sequences (one is a
 // batch of one): sequence blockIdx.y rotates its q row in place, writes its
 // rotated k row into its f16 K cache and its v row into its transposed f16 V
@@ -886,4 +893,9 @@ void launch_rope_cache_batched(cudaStream_t st, const RopeBatchParams &p)
 {
     const size_t n = (size_t)(p.heads + p.kv_heads) * (p.hd / 2);
     rope_cache_batched_kernel<<<dim3(flat_blocks(n, 128), p.nseq), 128, 0, st>>>(p);
+}
+
+void launch_rope_inv_freq(cudaStream_t st, float *out, const float *freq_div, int hd, float theta)
+{
+    inv_freq_kernel<<<(hd / 2 + 63) / 64, 64, 0, st>>>(out, freq_div, hd, theta);
 }

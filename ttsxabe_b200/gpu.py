@@ -176,6 +176,17 @@ def decode_plan(tk, kv_heads: int, rows: int, head_dim: int, sm_count: int = 148
     return mode.value, list(table[:grid.value + 1])
 
 
+def kv_q8_bytes(kv_heads: int, head_dim: int, cap: int) -> int:
+    """Bytes of an 8-bit cache (host only); 0 for a shape that there is none of."""
+    return int(_lib.load().llmtie_kv_q8_bytes(kv_heads, head_dim, cap))
+
+
+def evicted_len(live: int, keep: int) -> int:
+    """Tokens that an 8-bit cache of `live` holds after an eviction that keeps
+    `keep` complete blocks."""
+    return min(live // 32, keep) * 32 + live % 32
+
+
 class Gpu:
     """One device handle with its own stream (device.rs:737-842)."""
 
@@ -605,6 +616,152 @@ class Gpu:
             self._i32_table(past), self._i32_table(cap), _ptr(freq_div), heads, kv_heads,
             head_dim, theta, scale, out.data_ptr(), out.numel()))
         return out
+
+    # ---- the 8-bit KV cache ------------------------------------------------------------------
+    #
+    # Caches are torch.uint8 tensors of `kv_q8_bytes` bytes (include/llmtie_b200.h has
+    # the layout). Where a list of them is given, each is checked against its
+    # capacity; a table made by `ptr_table` is taken as it is.
+
+    @staticmethod
+    def _q8_table(caches, cap, kv_heads, head_dim) -> C.Array:
+        if isinstance(caches, C.Array):
+            return caches
+        if len(caches) != len(cap):
+            raise InvalidArgument(f"{len(caches)} caches and {len(cap)} capacities")
+        for t, c in zip(caches, cap):
+            need = kv_q8_bytes(kv_heads, head_dim, int(c)) if c > 0 else 0
+            have = t.numel() * t.element_size()
+            if not t.is_cuda:
+                raise InvalidArgument("an 8-bit cache in host memory")
+            if have < need or not t.is_contiguous():
+                raise SliceOverrun(f"reading to {need} in a buffer of {have}")
+        return Gpu._ptr_table(caches)
+
+    @staticmethod
+    def _tables_of(n: int, *tables) -> None:
+        """Every host table must be as long as the batch that reads it."""
+        for t in tables:
+            if len(t) < n:
+                raise InvalidArgument(f"a sequence table of {len(t)} for a batch of {n}")
+
+    def kv_alloc_q8(self, kv_heads, head_dim, cap) -> torch.Tensor:
+        """A zeroed 8-bit cache."""
+        need = kv_q8_bytes(kv_heads, head_dim, cap)
+        if need == 0 or cap <= 0:
+            raise RaggedBlock(f"an 8-bit cache of {kv_heads} heads of {head_dim} with a capacity "
+                              f"of {cap}, which is not a multiple of 32")
+        with torch.cuda.stream(self.stream):
+            return torch.zeros(need, dtype=torch.uint8, device=self.device)
+
+    def rope_inv_freq(self, theta, head_dim, freq_div=None) -> torch.Tensor:
+        """The inverse frequencies that `rope_scaled` goes by, to be kept for
+        `rope_append_q8`."""
+        out = self.uninit(head_dim // 2)
+        _check(self._lib.llmtie_rope_inv_freq(self._h, _ptr(freq_div), head_dim, theta,
+                                              out.data_ptr(), out.numel()))
+        return out
+
+    def rope_append_q8(self, q, k, v, cu_seqlens, caches, cap, past, pos, inv_freq, heads,
+                       kv_heads, head_dim, q_out=None) -> None:
+        """Rotates and appends packed rows (see include/llmtie_b200.h). `q` is
+        rotated in place unless `q_out` is given; it may be None, as may
+        `inv_freq`, with which nothing is rotated."""
+        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        n = len(table)
+        self._tables_of(n, cap, past, pos)
+        self._tables_of(n + 1, cu_seqlens)
+        if q_out is None:
+            q_out = q
+        _check(self._lib.llmtie_rope_append_q8(
+            self._h, _ptr(q), 0 if q is None else q.numel(), _ptr(q_out),
+            0 if q_out is None else q_out.numel(), k.data_ptr(), k.numel(), v.data_ptr(),
+            v.numel(), self._i32_table(cu_seqlens), n, table, self._i32_table(past),
+            self._i32_table(pos), self._i32_table(cap), _ptr(inv_freq),
+            0 if inv_freq is None else inv_freq.numel(), heads, kv_heads, head_dim))
+
+    def cache_read_q8(self, caches, cap, live, first, cu_seqlens, kv_heads, head_dim, k_out=None,
+                      v_out=None):
+        """Tokens of 8-bit caches as the f16 values they stand for: packed rows
+        [kv_heads*head_dim] of keys and of values."""
+        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        n = len(table)
+        self._tables_of(n, cap, live, first)
+        self._tables_of(n + 1, cu_seqlens)
+        total = int(cu_seqlens[n]) * kv_heads * head_dim
+        if k_out is None:
+            k_out = self._empty(total, torch.float16)
+        if v_out is None:
+            v_out = self._empty(total, torch.float16)
+        _check(self._lib.llmtie_cache_read_q8(
+            self._h, table, self._i32_table(cap), self._i32_table(live), self._i32_table(first),
+            self._i32_table(cu_seqlens), n, kv_heads, head_dim, k_out.data_ptr(), k_out.numel(),
+            v_out.data_ptr(), v_out.numel()))
+        return k_out, v_out
+
+    def cache_rewind_q8(self, caches, cap, live, to, kv_heads, head_dim) -> None:
+        """Cuts 8-bit caches back from `live` tokens to `to`."""
+        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        self._tables_of(len(table), cap, live, to)
+        _check(self._lib.llmtie_cache_rewind_q8(
+            self._h, table, self._i32_table(cap), self._i32_table(live), self._i32_table(to),
+            len(table), kv_heads, head_dim))
+
+    def cache_grow_q8(self, src, dst, kv_heads, head_dim, old_cap, new_cap, live) -> None:
+        _check(self._lib.llmtie_cache_grow_q8(
+            self._h, src.data_ptr(), src.numel(), dst.data_ptr(), dst.numel(), kv_heads, head_dim,
+            old_cap, new_cap, live))
+
+    def decode_batched_q8(self, q, caches, live, cap, heads, kv_heads, head_dim, scale,
+                          scratch: DecodeScratch, out=None, weigh=False) -> torch.Tensor:
+        """`decode_batched` over 8-bit caches; `out` may be f32 (as by default) or
+        f16. `weigh` adds to the caches' block weights."""
+        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        self._tables_of(len(table), cap, live)
+        if out is None:
+            out = self.uninit(len(table) * heads * head_dim)
+        _check(self._lib.llmtie_decode_batched_q8(
+            self._h, q.data_ptr(), q.numel(), table, self._i32_table(live), self._i32_table(cap),
+            len(table), heads, kv_heads, head_dim, scale, int(bool(weigh)), scratch._bind(self),
+            out.data_ptr(), out.numel(), self._f16_out(out)))
+        return out
+
+    def flash_attn_q8(self, q, cu_seqlens, caches, cap, past, heads, kv_heads, head_dim, scale,
+                      causal, out=None) -> torch.Tensor:
+        """`flash_attn_f16` over 8-bit caches for packed ragged rows; `out` may be
+        f32 (as by default) or f16."""
+        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        n = len(table)
+        self._tables_of(n, cap, past)
+        self._tables_of(n + 1, cu_seqlens)
+        if out is None:
+            out = self.uninit(int(cu_seqlens[n]) * heads * head_dim)
+        _check(self._lib.llmtie_flash_attn_q8(
+            self._h, q.data_ptr(), q.numel(), self._i32_table(cu_seqlens), n, table,
+            self._i32_table(past), self._i32_table(cap), heads, kv_heads, head_dim, scale,
+            int(bool(causal)), out.data_ptr(), out.numel(), self._f16_out(out)))
+        return out
+
+    @staticmethod
+    def _f16_out(out: torch.Tensor) -> int:
+        if out.dtype not in (torch.float32, torch.float16):
+            raise InvalidArgument(f"an output of {out.dtype}")
+        return int(out.dtype == torch.float16)
+
+    def cache_evict_q8(self, src, src_cap, dst, dst_cap, live, keep, keep_first, keep_recent,
+                       kv_heads, head_dim, index=None) -> None:
+        """Keeps the `keep` complete blocks of each cache that attention cared
+        most for (see include/llmtie_b200.h), in `dst` (which may be `src`). The
+        cache then holds `evicted_len(live, keep)` tokens."""
+        s = self._q8_table(src, src_cap, kv_heads, head_dim)
+        d = self._q8_table(dst, dst_cap, kv_heads, head_dim)
+        self._tables_of(len(s), d, src_cap, dst_cap, live, keep)
+        if index is not None and index.dtype != torch.int32:
+            raise InvalidArgument(f"an index of {index.dtype}")
+        _check(self._lib.llmtie_cache_evict_q8(
+            self._h, s, self._i32_table(src_cap), d, self._i32_table(dst_cap),
+            self._i32_table(live), self._i32_table(keep), len(s), keep_first, keep_recent,
+            kv_heads, head_dim, _ptr(index), 0 if index is None else index.numel()))
 
     # ---- profiling ------------------------------------------------------------------------
 
