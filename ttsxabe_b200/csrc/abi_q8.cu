@@ -383,12 +383,13 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
         for (int b = 0; b < p.nseq; b++) {
             const int32_t t = live[b0 + b];
             p.seq[b] = {(unsigned char *)caches[b0 + b], cap[b0 + b] / kQ8Block, t};
-            p.unit0[b] = units;
+            p.unit0[b] = (int)units;
             p.stat0[b] = blocks;
             units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
             blocks += (long long)(t / kQ8Block) * (long long)kv_heads;
         }
-        p.unit0[p.nseq] = units;
+        if (units > 0x7fffffffll) return llmtie_fail(LLMTIE_ERR_INVALID, "a launch over %lld blocks of the caches", units);
+        p.unit0[p.nseq] = (int)units;
         p.heads = (int)heads;
         p.kv_heads = (int)kv_heads;
         p.q = q + b0 * n;
@@ -397,11 +398,12 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
         p.sl2 = scale * kLog2e;
         p.status = g->timeout_site;
         p.wait_cycles = g->wait_cycles;
-        // A block of the grid an SM, and never fewer than four cache blocks for
-        // one: a finer cut spends longer merging than it saves.
-        const int most = std::min(g->sm_count, LLMTIE_Q8_MAX_BLOCKS);
+        // As many blocks of the grid as fit the device at once, and never fewer
+        // than four cache blocks for one, a warp each: a finer cut spends longer
+        // merging than it saves.
+        const int most = std::min(g->sm_count * decode_q8_resident((int)head_dim), LLMTIE_Q8_MAX_BLOCKS);
         const int grid = (int)std::min<long long>(most, (units + 3) / 4);
-        for (int c = 0; c <= grid; c++) p.ustart[c] = grid ? units * c / grid : 0;
+        for (int c = 0; c <= grid; c++) p.ustart[c] = grid ? (int)(units * c / grid) : 0;
         const size_t pairs = (size_t)p.nseq * kv_heads;
         cudaError_t err;
         const size_t slots = (size_t)std::max(grid, 1) * 2 * 8;
@@ -473,7 +475,7 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
             u.live = live;
             u.cap16 = (int)cap16;
             u.item0 = up.items;
-            up.items += (live + 4 * kQ8Block - 1) / (4 * kQ8Block);
+            up.items += (live + q8_unpack_tokens((int)head_dim) - 1) / q8_unpack_tokens((int)head_dim);
             const size_t place = bytes;
             u.k = (uint16_t *)place;             // (offsets until the workspace is known)
             u.v = (uint16_t *)(place + half);

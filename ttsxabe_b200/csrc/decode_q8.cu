@@ -23,7 +23,7 @@
 //
 // The kernel is bound by reading the cache: each warp keeps a ring of its own
 // blocks in flight (cp.async.bulk, an mbarrier a stage), and the grid is cut by
-// work, one block of the grid an SM; a pair (sequence, KV head) that several of
+// work over the blocks of the grid that fit the device at once; a pair (sequence, KV head) that several of
 // them share is merged by the last to arrive.
 #include "kv_q8.cuh"
 
@@ -31,14 +31,15 @@
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;             // query rows a pair may have
 
 template <int HD>
 struct Geo {
     static constexpr int BLOCK = kQ8Block * HD;          // bytes of a block's keys (or values)
-    static constexpr int STAGES = HD == 128 ? 3 : 6;
+    static constexpr int STAGES = 3;
+    static constexpr int RESIDENT = HD == 128 ? 2 : 4;   // blocks of the grid that fit an SM
     static constexpr int RING = kWarps * STAGES * 2 * BLOCK;
     static constexpr int MERGE = kWarps * kRows * HD * 4;
     static constexpr int SMEM = RING + MERGE;
@@ -105,12 +106,14 @@ __device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 struct Run {
     int seq, head;
     int first, last;      // complete blocks
+    int units;            // of the whole pair
+    int begin;            // its first unit
     bool tail;
     bool whole;           // the pair has no other block of the grid
-    long long next;       // unit after the run
+    int next;             // unit after the run
 };
 
-__device__ __forceinline__ Run run_at(const DecodeQ8Params &p, long long u, long long end)
+__device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
 {
     int lo = 0, hi = p.nseq - 1;
     while (lo < hi) {
@@ -119,23 +122,23 @@ __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, long long u, long
         else hi = mid - 1;
     }
     Run r;
-    const DecodeQ8Seq &s = p.seq[lo];
-    const int units = (s.live + 31) >> 5;                       // never 0 here: such a sequence has no units
+    const int live = p.seq[lo].live;
+    const int full = live >> 5;
+    r.units = (live + 31) >> 5;                                 // never 0 here: such a sequence has no units
     r.seq = lo;
-    r.head = (int)((u - p.unit0[lo]) / units);
-    const long long begin = p.unit0[lo] + (long long)r.head * units;
-    const int full = s.live >> 5;
-    r.first = (int)(u - begin);
-    const int stop = (int)min((long long)units, end - begin);
+    r.head = (int)((unsigned)(u - p.unit0[lo]) / (unsigned)r.units);
+    r.begin = p.unit0[lo] + r.head * r.units;
+    r.first = u - r.begin;
+    const int stop = min(r.units, end - r.begin);
     r.tail = stop > full;
     r.last = min(stop, full);
-    r.whole = r.first == 0 && stop == units;
-    r.next = begin + stop;
+    r.whole = r.first == 0 && stop == r.units;
+    r.next = r.begin + stop;
     return r;
 }
 
 // The block of the grid that holds unit u.
-__device__ __forceinline__ int block_of(const DecodeQ8Params &p, long long u)
+__device__ __forceinline__ int block_of(const DecodeQ8Params &p, int u)
 {
     int lo = 0, hi = (int)gridDim.x - 1;
     while (lo < hi) {
@@ -162,7 +165,7 @@ __device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at,
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_constant__ DecodeQ8Params p)
+__global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(const __grid_constant__ DecodeQ8Params p)
 {
     using G = Geo<HD>;
     constexpr int PANELS = HD / 64;
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.heads / p.kv_heads;
-    const long long u_begin = p.ustart[blockIdx.x], u_end = p.ustart[blockIdx.x + 1];
+    const int u_begin = p.ustart[blockIdx.x], u_end = p.ustart[blockIdx.x + 1];
     float *merge = (float *)(smem + G::RING);
     const uint32_t ring0 = smem_u32(smem) + (uint32_t)warp * (G::STAGES * 2 * G::BLOCK);
     const uint32_t bar0 = smem_u32(&bars[warp * G::STAGES]);
@@ -187,6 +190,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    // The next kernel of the stream may set itself up; nothing of the one before
+    // is read until it has ended.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // The warp's blocks in order, over all runs: `ahead` is what is fetched next.
     Run ahead = run_at(p, u_begin, u_end);
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
 
     const int r = lane >> 2, c = lane & 3;
     bool ok = true;
-    for (long long u = u_begin; u < u_end;) {
+    for (int u = u_begin; u < u_end;) {
         const Run run = run_at(p, u, u_end);
         const bool is_first = u == u_begin;
         u = run.next;
@@ -228,20 +235,46 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
         const float *ks = (const float *)(sq.base + at.ks) + (long long)run.head * sq.nb;
         const float *vs = (const float *)(sq.base + at.vs) + (long long)run.head * sq.nb;
 
-        // -- the query as fixed point: row r, the 16 channels of chunk c in each panel
+        // -- everything the run needs besides its blocks is asked for at once: the
+        // query (row r, the 16 channels of chunk c in each panel), and of the tail
+        // the warp's eight tokens, four lanes each
+        float x[PANELS][16];
+#pragma unroll
+        for (int j = 0; j < PANELS; j++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
+                x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
+            }
+        }
+        const int tail_n = run.tail ? min(8, (sq.live & 31) - 8 * warp) : 0;    // the warp's tokens
+        uint4 tk[HD / 32];
+        uint2 tv[8][V / 4 ? V / 4 : 1];
+        if (tail_n > 0) {
+            const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
+            const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) {
+                tk[i] = r < tail_n ? *(const uint4 *)(kt + r * HD + 32 * i + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                tv[t][0] = make_uint2(0u, 0u);
+                if (t < tail_n) {
+                    if (V == 4) tv[t][0] = *(const uint2 *)(vt + t * HD + V * lane);
+                    else tv[t][0].x = *(const uint32_t *)(vt + t * HD + V * lane);
+                }
+            }
+        }
+
+        // -- the query as fixed point
         uint32_t qa[PANELS][4], qb[PANELS][4];
         float f_q;
         {
-            float x[PANELS][16];
             uint32_t most = 0;
 #pragma unroll
             for (int j = 0; j < PANELS; j++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
-                    x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
-                }
 #pragma unroll
                 for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(x[j][i]) & 0x7fffffffu);
             }
@@ -256,65 +289,84 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
             for (int j = 0; j < PANELS; j++) {
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
-                    uint32_t hi = 0, lo = 0;
+                    uint32_t z[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int z = some ? max(-32639, min(32639, __float2int_rn(x[j][4 * w + i] * inv))) : 0;
-                        hi |= (uint32_t)(((z + 128) >> 8) & 255) << (8 * i);
-                        lo |= (uint32_t)(z & 255) << (8 * i);
+                        z[i] = (uint32_t)(some ? max(-32639, min(32639, __float2int_rn(x[j][4 * w + i] * inv))) : 0);
                     }
-                    qa[j][w] = hi;
-                    qb[j][w] = lo;
+                    // z = 256 H + L: L its low byte, signed, H what is left
+                    qb[j][w] = __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
+                    qa[j][w] = __byte_perm(__byte_perm(z[0] + 128u, z[1] + 128u, 0x0051),
+                                           __byte_perm(z[2] + 128u, z[3] + 128u, 0x0051), 0x5410);
                 }
             }
         }
 
-        // -- the tail in f32: warp w takes query row w, a lane a token, then V channels
-        float t_m = -CUDART_INF_F, t_l = 0.0f, t_o[V];
-#pragma unroll
-        for (int e = 0; e < V; e++) t_o[e] = 0.0f;
-        if (run.tail && warp < group) {
-            const int n = sq.live & 31;
-            const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + (long long)run.head * kQ8Block * HD;
-            const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + (long long)run.head * kQ8Block * HD;
-            float s = -CUDART_INF_F;
-            if (lane < n) {
-                s = 0.0f;
-#pragma unroll 4
-                for (int d = 0; d < HD; d += 8) {
-                    const uint4 kk = *(const uint4 *)(kt + lane * HD + d);
-                    const float4 q0 = __ldg((const float4 *)(qh + warp * HD + d));
-                    const float4 q1 = __ldg((const float4 *)(qh + warp * HD + d + 4));
-                    const float2 k0 = __half22float2(*(const __half2 *)&kk.x), k1 = __half22float2(*(const __half2 *)&kk.y);
-                    const float2 k2 = __half22float2(*(const __half2 *)&kk.z), k3 = __half22float2(*(const __half2 *)&kk.w);
-                    s += q0.x * k0.x + q0.y * k0.y + q0.z * k1.x + q0.w * k1.y + q1.x * k2.x + q1.y * k2.y + q1.z * k3.x + q1.w * k3.y;
-                }
-                s *= p.sl2;
-            }
-            t_m = s;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t_m = fmaxf(t_m, __shfl_xor_sync(0xffffffffu, t_m, o));
-            const float pr = lane < n ? ex2(s - t_m) : 0.0f;
-            t_l = pr;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t_l += __shfl_xor_sync(0xffffffffu, t_l, o);
-#pragma unroll 4
-            for (int t = 0; t < n; t++) {
-                const float w = __shfl_sync(0xffffffffu, pr, t);
-#pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    const float2 x = __half22float2(*(const __half2 *)(vt + t * HD + V * lane + e));
-                    t_o[e] = fmaf(w, x.x, t_o[e]);
-                    t_o[e + 1] = fmaf(w, x.y, t_o[e + 1]);
-                }
-            }
-        }
-
-        // -- the warp's blocks
+        // -- the warp's part of the tail, in f32: what its sums start from
         float acc[NT][2];
 #pragma unroll
         for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0f;
         float m = -CUDART_INF_F, l = 0.0f;       // reference maximum of row r; this lane's part of the sum
+        if (tail_n > 0) {
+            float *mine = merge + warp * kRows * HD;
+            for (int g = 0; g < group; g++) {
+                // lane (r, c): channels 32 i + 8 c of token r
+                float s = 0.0f;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) {
+                    const float4 q0 = __ldg((const float4 *)(qh + g * HD + 32 * i + 8 * c));
+                    const float4 q1 = __ldg((const float4 *)(qh + g * HD + 32 * i + 8 * c + 4));
+                    const float2 k0 = __half22float2(*(const __half2 *)&tk[i].x), k1 = __half22float2(*(const __half2 *)&tk[i].y);
+                    const float2 k2 = __half22float2(*(const __half2 *)&tk[i].z), k3 = __half22float2(*(const __half2 *)&tk[i].w);
+                    s = fmaf(q0.x, k0.x, s); s = fmaf(q0.y, k0.y, s); s = fmaf(q0.z, k1.x, s); s = fmaf(q0.w, k1.y, s);
+                    s = fmaf(q1.x, k2.x, s); s = fmaf(q1.y, k2.y, s); s = fmaf(q1.z, k3.x, s); s = fmaf(q1.w, k3.y, s);
+                }
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s = r < tail_n ? s * p.sl2 : -CUDART_INF_F;
+                float top = s;
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float e = r < tail_n ? ex2(s - top) : 0.0f;
+                float sum = e;
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                float o4[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) o4[i] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 8; t++) {
+                    const float w = __shfl_sync(0xffffffffu, e, 4 * t);
+                    const float2 v0 = __half22float2(*(const __half2 *)&tv[t][0].x);
+                    o4[0] = fmaf(w, v0.x, o4[0]);
+                    o4[1] = fmaf(w, v0.y, o4[1]);
+                    if (V == 4) {
+                        const float2 v1 = __half22float2(*(const __half2 *)&tv[t][0].y);
+                        o4[V - 2] = fmaf(w, v1.x, o4[V - 2]);
+                        o4[V - 1] = fmaf(w, v1.y, o4[V - 1]);
+                    }
+                }
+                // channels V lane .. of row g, where the fragment layout finds them
+#pragma unroll
+                for (int i = 0; i < V; i++) mine[g * HD + 8 * ((V * lane / 8) ^ g) + V * lane % 8 + i] = o4[i];
+                if (r == g) {
+                    m = top;
+                    l = c == 0 ? sum : 0.0f;
+                }
+            }
+            __syncwarp();
+            if (r < group) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const float2 y = *(const float2 *)(mine + r * HD + 8 * (i ^ r) + 2 * c);
+                    acc[i][0] = y.x;
+                    acc[i][1] = y.y;
+                }
+            }
+            __syncwarp();
+        }
+
+        // -- the warp's blocks
         float k_scale = 0.0f, v_scale = 0.0f;
         if (run.first + warp < run.last) {
             k_scale = __ldg(ks + run.first + warp);
@@ -403,114 +455,140 @@ __global__ void __launch_bounds__(kThreads, 1) decode_q8_kernel(const __grid_con
             fetch();
         }
 
-        // -- the run's result: warp w merges row w of the eight warps' (and its own tail's)
+        // -- the run's result: a warp merges rows warp, warp + kWarps of the block's warps'
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (c == 0) {
             m_s[warp][r] = m;
             l_s[warp][r] = l;
         }
+        if (r < group) {
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            // (groups of eight channels swizzled by the row: no bank conflicts on either side)
-            *(float2 *)(merge + (warp * kRows + r) * HD + 8 * (i ^ r) + 2 * c) = make_float2(acc[i][0], acc[i][1]);
+            for (int i = 0; i < NT; i++) {
+                // (groups of eight channels swizzled by the row: no bank conflicts on either side)
+                *(float2 *)(merge + (warp * kRows + r) * HD + 8 * (i ^ r) + 2 * c) = make_float2(acc[i][0], acc[i][1]);
+            }
         }
         __syncthreads();
-        const long long row_at = ((long long)run.seq * p.heads + (long long)run.head * group + warp) * HD;
-        const int pair = run.seq * p.kv_heads + run.head;
-        float M = -CUDART_INF_F, L = 0.0f, o[V];
+        const long long row0 = (long long)run.seq * p.heads + (long long)run.head * group;
+        const int slot = (int)blockIdx.x * 2 + (is_first ? 0 : 1);
+        for (int row = warp; row < group; row += kWarps) {
+            float M = -CUDART_INF_F, L = 0.0f, o[V];
 #pragma unroll
-        for (int e = 0; e < V; e++) o[e] = 0.0f;
-        if (warp < group) {
-            M = t_m;
+            for (int e = 0; e < V; e++) o[e] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kWarps; k++) M = fmaxf(M, m_s[k][warp]);
-            const float ft = t_m == -CUDART_INF_F ? 0.0f : ex2(t_m - M);
-            L = t_l * ft;
-#pragma unroll
-            for (int e = 0; e < V; e++) o[e] = t_o[e] * ft;
+            for (int k = 0; k < kWarps; k++) M = fmaxf(M, m_s[k][row]);
 #pragma unroll
             for (int k = 0; k < kWarps; k++) {
-                const float mk = m_s[k][warp];
+                const float mk = m_s[k][row];
                 const float fk = mk == -CUDART_INF_F ? 0.0f : ex2(mk - M);
-                L = fmaf(fk, l_s[k][warp], L);
+                L = fmaf(fk, l_s[k][row], L);
 #pragma unroll
                 for (int e = 0; e < V; e++) {
-                    o[e] = fmaf(fk, merge[(k * kRows + warp) * HD + 8 * ((V * lane / 8) ^ warp) + V * lane % 8 + e], o[e]);
+                    o[e] = fmaf(fk, merge[(k * kRows + row) * HD + 8 * ((V * lane / 8) ^ row) + V * lane % 8 + e], o[e]);
                 }
+            }
+            if (run.whole) {
+                const float inv = 1.0f / L;
+#pragma unroll
+                for (int e = 0; e < V; e++) o[e] *= inv;
+                store_row<HD>(p, (row0 + row) * HD, lane, o);
+                if (lane == 0) final_s[row] = make_float2(M, inv);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    *(float2 *)(p.part_o + ((long long)slot * kRows + row) * HD + V * lane + e) = make_float2(o[e], o[e + 1]);
+                }
+                if (lane == 0) p.part_ml[slot * kRows + row] = make_float2(M, L);
             }
         }
         bool done = run.whole;
         if (!run.whole) {
-            const long long slot = (long long)blockIdx.x * 2 + (is_first ? 0 : 1);
-            if (warp < group) {
-#pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    *(float2 *)(p.part_o + (slot * kRows + warp) * HD + V * lane + e) = make_float2(o[e], o[e + 1]);
-                }
-                if (lane == 0) p.part_ml[slot * kRows + warp] = make_float2(M, L);
-            }
             __threadfence();
             __syncthreads();
-            const int units = (sq.live + 31) >> 5;
-            const long long begin = p.unit0[run.seq] + (long long)run.head * units;
-            const int b0 = block_of(p, begin), b1 = block_of(p, begin + units - 1);
+            const int b0 = block_of(p, run.begin), b1 = block_of(p, run.begin + run.units - 1);
             if (tid == 0) {
-                const unsigned seen = atomicAdd(&p.ctr[pair], 1u);
+                unsigned *ctr = &p.ctr[run.seq * p.kv_heads + run.head];
+                const unsigned seen = atomicAdd(ctr, 1u);
                 last_s = seen == (unsigned)(b1 - b0);
-                if (last_s) p.ctr[pair] = 0u;
+                if (last_s) *ctr = 0u;
             }
             __syncthreads();
             done = last_s != 0;
             if (done) {
                 __threadfence();
-                if (warp < group) {
-                    // the contributors in order, whoever came last: the same bits every time
-                    M = -CUDART_INF_F;
-                    for (int b = b0; b <= b1; b++) {
-                        const long long sl = (long long)b * 2 + (p.ustart[b] >= begin || b > b0 ? 0 : 1);
-                        M = fmaxf(M, __ldcg(&p.part_ml[sl * kRows + warp]).x);
-                    }
-                    L = 0.0f;
+                // The contributors in order, whoever came last: the same bits every
+                // time. A block's first run has slot 0, and only b0 may hold the pair
+                // in its last.
+                const int skew = p.ustart[b0] >= run.begin ? 0 : 1;
+                for (int row = warp; row < group; row += kWarps) {
+                    float M = -CUDART_INF_F, L = 0.0f, o[V];
 #pragma unroll
                     for (int e = 0; e < V; e++) o[e] = 0.0f;
-                    for (int b = b0; b <= b1; b++) {
-                        const long long sl = (long long)b * 2 + (p.ustart[b] >= begin || b > b0 ? 0 : 1);
-                        const float2 ml = __ldcg(&p.part_ml[sl * kRows + warp]);
-                        const float fk = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - M);
-                        L = fmaf(fk, ml.y, L);
+                    for (int bb = b0; bb <= b1; bb += 32) {
+                        const int n = min(32, b1 + 1 - bb);
+                        const int my_slot = 2 * (bb + lane) + (bb + lane == b0 ? skew : 0);
+                        float2 ml = make_float2(-CUDART_INF_F, 0.0f);
+                        if (lane < n) ml = __ldcg(&p.part_ml[my_slot * kRows + row]);
+                        float top = ml.x;
 #pragma unroll
-                        for (int e = 0; e < V; e += 2) {
-                            const float2 x = __ldcg((const float2 *)(p.part_o + (sl * kRows + warp) * HD + V * lane + e));
-                            o[e] = fmaf(fk, x.x, o[e]);
-                            o[e + 1] = fmaf(fk, x.y, o[e + 1]);
+                        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        top = fmaxf(top, M);
+                        const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
+                        const float f = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+                        float sum = f * ml.y;
+#pragma unroll
+                        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                        L = fmaf(L, keep, sum);
+#pragma unroll
+                        for (int e = 0; e < V; e++) o[e] *= keep;
+                        for (int i0 = 0; i0 < n; i0 += 8) {
+                            float2 y[8][V / 2];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const int b = min(bb + i0 + i, b1);
+                                const long long sl = 2 * b + (b == b0 ? skew : 0);
+#pragma unroll
+                                for (int e = 0; e < V; e += 2) {
+                                    y[i][e / 2] = __ldcg((const float2 *)(p.part_o + (sl * kRows + row) * HD + V * lane + e));
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const float fi = __shfl_sync(0xffffffffu, f, i0 + i);   // (0 past the last)
+#pragma unroll
+                                for (int e = 0; e < V; e += 2) {
+                                    o[e] = fmaf(fi, y[i][e / 2].x, o[e]);
+                                    o[e + 1] = fmaf(fi, y[i][e / 2].y, o[e + 1]);
+                                }
+                            }
                         }
+                        M = top;
                     }
+                    const float inv = 1.0f / L;
+#pragma unroll
+                    for (int e = 0; e < V; e++) o[e] *= inv;
+                    store_row<HD>(p, (row0 + row) * HD, lane, o);
+                    if (lane == 0) final_s[row] = make_float2(M, inv);
                 }
             }
         }
-        if (done) {
-            const float inv = 1.0f / L;
-            if (warp < group) {
+        if (done && p.stats) {
+            // weights: what each block's keys got, over the group's heads
+            __syncthreads();
+            float *weight = (float *)(sq.base + at.w) + (long long)run.head * sq.nb;
+            const int full = sq.live >> 5;
+            const float2 *st = p.stats + (p.stat0[run.seq] + (long long)run.head * full) * kRows;
+            for (int b = tid; b < full; b += kThreads) {
+                float2 y[kRows];
 #pragma unroll
-                for (int e = 0; e < V; e++) o[e] *= inv;
-                store_row<HD>(p, row_at, lane, o);
-                if (lane == 0) final_s[warp] = make_float2(M, inv);
-            }
-            if (p.stats) {
-                // weights: what each block's keys got, over the group's heads
-                __syncthreads();
-                float *weight = (float *)(sq.base + at.w) + (long long)run.head * sq.nb;
-                const int full = sq.live >> 5;
-                const float2 *st = p.stats + (p.stat0[run.seq] + (long long)run.head * full) * kRows;
-                for (int b = tid; b < full; b += kThreads) {
-                    float sum = 0.0f;
-                    for (int k = 0; k < group; k++) {
-                        const float2 x = __ldcg(&st[(long long)b * kRows + k]);
-                        sum = fmaf(ex2(x.x - final_s[k].x) * final_s[k].y, x.y, sum);
-                    }
-                    weight[b] += sum;
+                for (int k = 0; k < kRows; k++) y[k] = k < group ? __ldcg(&st[(long long)b * kRows + k]) : make_float2(0.f, 0.f);
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kRows; k++) {
+                    if (k < group) sum = fmaf(ex2(y[k].x - final_s[k].x) * final_s[k].y, y[k].y, sum);
                 }
+                weight[b] += sum;
             }
         }
         __syncthreads();   // merge, m_s and final_s are free again
@@ -556,7 +634,17 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
         if (e != cudaSuccess) return e;
     }
     if (grid == 0) return cudaSuccess;
-    if (hd == 128) decode_q8_kernel<128><<<grid, kThreads, Geo<128>::SMEM, st>>>(p);
-    else decode_q8_kernel<64><<<grid, kThreads, Geo<64>::SMEM, st>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = hd == 128 ? Geo<128>::SMEM : Geo<64>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return hd == 128 ? cudaLaunchKernelEx(&cfg, decode_q8_kernel<128>, p) : cudaLaunchKernelEx(&cfg, decode_q8_kernel<64>, p);
 }
+
+int decode_q8_resident(int hd) { return hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT; }

@@ -60,21 +60,29 @@ __device__ __forceinline__ int seq_of(const Seq *seq, int nseq, int item)
     return lo;
 }
 
+// A kernel of this file may be set up while the one before it in the stream
+// still runs; nothing is read or written before that one has ended.
+__device__ __forceinline__ void after_previous()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- append -------------------------------------------------------------------------
 //
 // A block of the grid takes the up to 32 new rows of one cache block for a
-// chunk of heads: blockIdx.y first runs over the chunks of KV heads (keys
-// rotated, then keys and values quantised or put into the tail), then over the
-// chunks of query heads (rotated only). The sines and cosines of those rows are
-// worked out once, into shared memory, and shared by the chunk's heads; the
-// angle is pos * inv_freq[j] in 64 bits, taken in half turns and reduced before
-// it is rounded to f32, so that far positions lose nothing.
+// chunk of heads: blockIdx.y runs over the chunks of key heads (rotated, then
+// quantised or put into the tail), of value heads (the same without the
+// rotation), and of query heads (rotated only). The sines and cosines of those
+// rows are worked out once, into shared memory, and shared by the chunk's
+// heads; the angle is pos * inv_freq[j] in 64 bits, taken in half turns and
+// reduced before it is rounded to f32, so that far positions lose nothing.
 //
 // The sequence's first work item also writes its last, incomplete block: the
 // tail holds the first rows of the one and receives the rows of the other, and
 // one block of the grid does both in order.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_constant__ Q8AppendParams p)
+__global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_constant__ Q8AppendParams p)
 {
     constexpr int LPR = HD / 8;                  // lanes of a row, each with four values of either half
     constexpr int RPW = 32 / LPR;                // rows a warp loads at once
@@ -89,13 +97,17 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
     const Q8AppendSeq sq = p.seq[seq_of(p.seq, p.nseq, item)];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kv_chunks = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
-    const bool is_q = (int)blockIdx.y >= kv_chunks;
+    const bool is_q = (int)blockIdx.y >= 2 * kv_chunks;
+    const int which = !is_q && (int)blockIdx.y >= kv_chunks ? 1 : 0;        // values, not keys
+    const bool turns = p.inv_freq != nullptr && !which;
     const int r = sq.past & 31;                  // rows of the first block that lie in the tail
     const int total = r + sq.n;
     const int nblk = (total + 31) >> 5;
     const int mine = item - sq.item0;
     const bool rest = mine == 0 && nblk > 1 && (total & 31) != 0;   // the last block too
     const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+    const int c = lane % LPR;
+    after_previous();
 
     for (int pass = 0; pass < (rest ? 2 : 1); pass++) {
         const int j = pass ? nblk - 1 : mine;
@@ -103,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
         const int t_hi = min(32, total - 32 * j);
         const long long row_of = (long long)sq.row0 + 32 * j - r;   // + t: its packed row
         __syncthreads();   // the pass before is done with `turn`, and with the tail rows it read
-        if (p.inv_freq) {
+        auto fill_turns = [&] {
             for (int i = tid; i < (t_hi - t_lo) * HALF; i += kThreads) {
                 const int t = t_lo + i / HALF, f = i % HALF;
                 const double half_turns = (double)(sq.pos + 32 * j - r + t) * (double)p.inv_freq[f] *
@@ -112,34 +124,74 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
                 sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &sn, &cs);
                 turn[t][f] = make_float2(cs, sn);
             }
-        }
-        __syncthreads();
-        const int c = lane % LPR;
+            __syncthreads();
+        };
+        auto rotate4 = [&](int t, float4 &a, float4 &b) {
+            const float4 w0 = *(const float4 *)&turn[t][4 * c], w1 = *(const float4 *)&turn[t][4 * c + 2];
+            float4 lo, hi;
+            rope_rotate(a.x, b.x, w0.x, w0.y, lo.x, hi.x);
+            rope_rotate(a.y, b.y, w0.z, w0.w, lo.y, hi.y);
+            rope_rotate(a.z, b.z, w1.x, w1.y, lo.z, hi.z);
+            rope_rotate(a.w, b.w, w1.z, w1.w, lo.w, hi.w);
+            a = lo;
+            b = hi;
+        };
         if (is_q) {
-            const int h0 = ((int)blockIdx.y - kv_chunks) * p.q_chunk;
+            const int h0 = ((int)blockIdx.y - 2 * kv_chunks) * p.q_chunk;
             const int nh = min(p.q_chunk, p.heads - h0);
             const int rows = (t_hi - t_lo) * nh;
-            for (int i = warp * RPW + lane / LPR; i < rows; i += kWarps * RPW) {
-                const int t = t_lo + i / nh, h = h0 + i % nh;
-                const long long e = ((row_of + t) * p.heads + h) * HD + 4 * c;
-                const float4 a = *(const float4 *)(p.q + e), b = *(const float4 *)(p.q + e + HALF);
-                const float2 *w = &turn[t][4 * c];
-                float4 lo, hi;
-                rope_rotate(a.x, b.x, w[0].x, w[0].y, lo.x, hi.x);
-                rope_rotate(a.y, b.y, w[1].x, w[1].y, lo.y, hi.y);
-                rope_rotate(a.z, b.z, w[2].x, w[2].y, lo.z, hi.z);
-                rope_rotate(a.w, b.w, w[3].x, w[3].y, lo.w, hi.w);
-                *(float4 *)(p.q_out + e) = lo;
-                *(float4 *)(p.q_out + e + HALF) = hi;
+            constexpr int U = 4;                               // rows in flight
+            constexpr int STEP = kWarps * RPW;
+            bool ready = false;
+            for (int i0 = warp * RPW + lane / LPR; !ready || i0 < rows; i0 += U * STEP) {
+                float4 a[U], b[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int i = i0 + u * STEP;
+                    if (i < rows) {
+                        const float *x = p.q + ((row_of + t_lo + i / nh) * p.heads + h0 + i % nh) * HD + 4 * c;
+                        a[u] = *(const float4 *)x;
+                        b[u] = *(const float4 *)(x + HALF);
+                    }
+                }
+                if (!ready) {                                  // (the first rows are on their way meanwhile)
+                    fill_turns();
+                    ready = true;
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int i = i0 + u * STEP;
+                    if (i < rows) {
+                        const int t = t_lo + i / nh;
+                        rotate4(t, a[u], b[u]);
+                        float *y = p.q_out + ((row_of + t) * p.heads + h0 + i % nh) * HD + 4 * c;
+                        *(float4 *)y = a[u];
+                        *(float4 *)(y + HALF) = b[u];
+                    }
+                }
             }
             continue;
         }
         const int blk = (sq.past >> 5) + j;
         const bool complete = 32 * (j + 1) <= total;
-        const int h0 = (int)blockIdx.y * p.kv_chunk;
-        for (int hk = 2 * h0; hk < 2 * min(p.kv_heads, h0 + p.kv_chunk); hk++) {
-            const int h = hk >> 1, which = hk & 1;             // keys, then values
-            const float *src = which ? p.v : p.k;
+        const float *src = which ? p.v : p.k;
+        const int h0 = ((int)blockIdx.y - (which ? kv_chunks : 0)) * p.kv_chunk;
+        const int h1 = min(p.kv_heads, h0 + p.kv_chunk);
+        float4 a[ITER], b[ITER];
+        auto load = [&](int h) {
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                const int t = (warp * ITER + it) * RPW + lane / LPR;
+                if (t >= t_lo && t < t_hi) {
+                    const float *x = src + ((row_of + t) * p.kv_heads + h) * HD + 4 * c;
+                    a[it] = *(const float4 *)x;
+                    b[it] = *(const float4 *)(x + HALF);
+                }
+            }
+        };
+        load(h0);
+        if (turns) fill_turns();
+        for (int h = h0; h < h1; h++) {
             uint16_t *tail = (uint16_t *)(sq.base + (which ? at.vt : at.kt)) + (long long)h * kQ8Block * HD;
             __half2 x[ITER][4];                                // two halves of the row, four values each
             uint32_t most = 0;
@@ -148,20 +200,9 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
                 const int t = (warp * ITER + it) * RPW + lane / LPR;
                 uint2 lo16 = make_uint2(0u, 0u), hi16 = lo16;
                 if (t >= t_lo && t < t_hi) {
-                    const long long e = ((row_of + t) * p.kv_heads + h) * HD + 4 * c;
-                    float4 a = *(const float4 *)(src + e), b = *(const float4 *)(src + e + HALF);
-                    if (!which && p.inv_freq) {
-                        const float2 *w = &turn[t][4 * c];
-                        float4 lo, hi;
-                        rope_rotate(a.x, b.x, w[0].x, w[0].y, lo.x, hi.x);
-                        rope_rotate(a.y, b.y, w[1].x, w[1].y, lo.y, hi.y);
-                        rope_rotate(a.z, b.z, w[2].x, w[2].y, lo.z, hi.z);
-                        rope_rotate(a.w, b.w, w[3].x, w[3].y, lo.w, hi.w);
-                        a = lo;
-                        b = hi;
-                    }
-                    lo16 = make_uint2(pack_half2(a.x, a.y), pack_half2(a.z, a.w));
-                    hi16 = make_uint2(pack_half2(b.x, b.y), pack_half2(b.z, b.w));
+                    if (turns) rotate4(t, a[it], b[it]);
+                    lo16 = make_uint2(pack_half2(a[it].x, a[it].y), pack_half2(a[it].z, a[it].w));
+                    hi16 = make_uint2(pack_half2(b[it].x, b[it].y), pack_half2(b[it].z, b[it].w));
                     if (!complete) {
                         *(uint2 *)(tail + t * HD + 4 * c) = lo16;
                         *(uint2 *)(tail + t * HD + HALF + 4 * c) = hi16;
@@ -177,12 +218,13 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
                     most = max(most, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
                 }
             }
+            if (h + 1 < h1) load(h + 1);                       // (under this head's arithmetic)
             if (!complete) continue;
             most = __reduce_max_sync(0xffffffffu, most);
-            if (lane == 0) red[which][warp] = most;
+            if (lane == 0) red[h & 1][warp] = most;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kWarps; i++) most = max(most, red[which][i]);
+            for (int i = 0; i < kWarps; i++) most = max(most, red[h & 1][i]);
             // A block that holds an infinity or NaN reads back as NaN throughout.
             const float top = __half2float(__ushort_as_half((uint16_t)most));
             const float scale = most >= 0x7c00u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(top, 127.0f);
@@ -226,12 +268,12 @@ __global__ void __launch_bounds__(kThreads) q8_append_kernel(const __grid_consta
 #pragma unroll
                     for (int i = 0; i < 4; i++) codes[(4 * dq + i) * 8 + tq] = w[i];
                 }
-                __syncthreads();
+                // (the next head's maximum is exchanged, with a barrier, before `stage` is written again)
             }
             if (tid == 0) {
-                const long long b = (long long)h * sq.nb + blk;
-                ((float *)(sq.base + (which ? at.vs : at.ks)))[b] = scale;
-                if (which) ((float *)(sq.base + at.w))[b] = 0.0f;
+                const long long at_b = (long long)h * sq.nb + blk;
+                ((float *)(sq.base + (which ? at.vs : at.ks)))[at_b] = scale;
+                if (which) ((float *)(sq.base + at.w))[at_b] = 0.0f;
             }
         }
     }
@@ -245,6 +287,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant__ Q8ReadParams p)
 {
     const Q8ReadSeq sq = p.seq[seq_of(p.seq, p.nseq, (int)blockIdx.x)];
+    after_previous();
     const int blk = (sq.first >> 5) + (int)blockIdx.x - sq.item0;
     const int h = blockIdx.y, which = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -263,71 +306,98 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant
         return;
     }
     const long long b = (long long)h * sq.nb + blk;
-    const uint32_t *codes = (const uint32_t *)(sq.base + (which ? at.v : at.k) + b * (kQ8Block * HD));
+    const uint4 *codes = (const uint4 *)(sq.base + (which ? at.v : at.k) + b * (kQ8Block * HD));
     const float scale = ((const float *)(sq.base + (which ? at.vs : at.ks)))[b];
+    const uint4 w = tid < kQ8Block * HD / 16 ? codes[tid] : make_uint4(0u, 0u, 0u, 0u);
     if (!which) {
-        for (int i = tid; i < kQ8Block * HD / 4; i += kThreads) {
-            const int panel = i / (kQ8Block * 16), t = i / 16 % kQ8Block, d = panel * 64 + i % 16 * 4;
-            if (t >= lo && t < hi) *(uint2 *)(out + t * step + d) = dequant4(codes[i], scale);
+        // 16 channels of a token
+        const int panel = tid / (kQ8Block * 4), t = tid / 4 % kQ8Block, d = panel * 64 + tid % 4 * 16;
+        if (tid < kQ8Block * HD / 16 && t >= lo && t < hi) {
+            uint2 *o = (uint2 *)(out + t * step + d);
+            o[0] = dequant4(w.x, scale);
+            o[1] = dequant4(w.y, scale);
+            o[2] = dequant4(w.z, scale);
+            o[3] = dequant4(w.w, scale);
         }
-    } else if (lane < HD / 4) {
-        // a warp takes four tokens, a lane four channels of them
-        uint32_t w[4];
+        return;
+    }
+    // 16 tokens of a channel in, four channels of four tokens out (rows of eight
+    // words padded to ten: neither side meets a bank twice)
+    __shared__ uint32_t stage[HD * 10];
+    if (tid < kQ8Block * HD / 16) {
+        uint32_t *to = stage + tid / 2 * 10 + tid % 2 * 4;
+        *(uint2 *)to = make_uint2(w.x, w.y);
+        *(uint2 *)(to + 2) = make_uint2(w.z, w.w);
+    }
+    __syncthreads();
+    const int tq = lane & 7, dq = warp * 4 + (lane >> 3);
+    if (dq < HD / 4) {
+        uint32_t x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = codes[(4 * lane + i) * 8 + warp];
-        transpose4(w);
+        for (int i = 0; i < 4; i++) x[i] = stage[(4 * dq + i) * 10 + tq];
+        transpose4(x);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int t = 4 * warp + i;
-            if (t >= lo && t < hi) *(uint2 *)(out + t * step + 4 * lane) = dequant4(w[i], scale);
+            const int t = 4 * tq + i;
+            if (t >= lo && t < hi) *(uint2 *)(out + t * step + 4 * dq) = dequant4(x[i], scale);
         }
     }
 }
 
 // The live tokens as f16 caches that the prefill kernel's tensor maps can be
-// laid over. blockIdx = (four cache blocks, KV head); a thread turns 16 codes
-// (16 bytes) into 32 bytes of either output. Past the live tokens, up to the
+// laid over. blockIdx = (kUnpack cache blocks, KV head); a thread turns twice 16
+// codes (16 bytes) of either into 32 bytes, all four loads in flight. Past the live tokens, up to the
 // capacity (the next multiple of eight), lie zeros.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_constant__ Q8UnpackParams p)
 {
-    // (the attention kernel behind this one may set itself up meanwhile)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int PER = kQ8Block * HD / 16;      // 16-byte pieces of a block
+    constexpr int kUnpack = 2 * kThreads / PER;
     const Q8UnpackSeq sq = p.seq[seq_of(p.seq, p.nseq, (int)blockIdx.x)];
-    const int blk0 = 4 * ((int)blockIdx.x - sq.item0);
+    const int blk0 = kUnpack * ((int)blockIdx.x - sq.item0);
     const int h = blockIdx.y, tid = threadIdx.x;
     const int full = sq.live >> 5;
     const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
     const long long b0 = (long long)h * sq.nb;
     const float *ks = (const float *)(sq.base + at.ks) + b0, *vs = (const float *)(sq.base + at.vs) + b0;
     uint16_t *ko = sq.k + (long long)h * sq.cap16 * HD, *vo = sq.v + (long long)h * HD * sq.cap16;
-    constexpr int PER = kQ8Block * HD / 16;      // 16-byte pieces of a block
-#pragma unroll 1
-    for (int i = tid; i < 4 * PER; i += kThreads) {
-        const int blk = blk0 + i / PER, e = i % PER;
-        if (blk >= full) break;
-        const uint4 kc = ((const uint4 *)(sq.base + at.k + (b0 + blk) * (kQ8Block * HD)))[e];
-        const uint4 vc = ((const uint4 *)(sq.base + at.v + (b0 + blk) * (kQ8Block * HD)))[e];
-        const float ksc = ks[blk], vsc = vs[blk];
+    // (the attention kernel behind this one sets itself up meanwhile)
+    after_previous();
+    uint4 kc[2], vc[2];
+    float ksc[2], vsc[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int i = tid + u * kThreads, blk = blk0 + i / PER, e = i % PER;
+        if (blk < full) {
+            kc[u] = ((const uint4 *)(sq.base + at.k + (b0 + blk) * (kQ8Block * HD)))[e];
+            vc[u] = ((const uint4 *)(sq.base + at.v + (b0 + blk) * (kQ8Block * HD)))[e];
+            ksc[u] = ks[blk];
+            vsc[u] = vs[blk];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int i = tid + u * kThreads, blk = blk0 + i / PER, e = i % PER;
+        if (blk >= full) continue;
         {
             const int panel = e / (kQ8Block * 4), t = e / 4 % kQ8Block, d = panel * 64 + e % 4 * 16;
             uint4 *o = (uint4 *)(ko + (long long)(32 * blk + t) * HD + d);
-            const uint2 w0 = dequant4(kc.x, ksc), w1 = dequant4(kc.y, ksc);
-            const uint2 w2 = dequant4(kc.z, ksc), w3 = dequant4(kc.w, ksc);
+            const uint2 w0 = dequant4(kc[u].x, ksc[u]), w1 = dequant4(kc[u].y, ksc[u]);
+            const uint2 w2 = dequant4(kc[u].z, ksc[u]), w3 = dequant4(kc[u].w, ksc[u]);
             o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
             o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
         }
         {
             const int d = e / 2, t = e % 2 * 16;
             uint4 *o = (uint4 *)(vo + (long long)d * sq.cap16 + 32 * blk + t);
-            const uint2 w0 = dequant4(vc.x, vsc), w1 = dequant4(vc.y, vsc);
-            const uint2 w2 = dequant4(vc.z, vsc), w3 = dequant4(vc.w, vsc);
+            const uint2 w0 = dequant4(vc[u].x, vsc[u]), w1 = dequant4(vc[u].y, vsc[u]);
+            const uint2 w2 = dequant4(vc[u].z, vsc[u]), w3 = dequant4(vc[u].w, vsc[u]);
             o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
             o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
         }
     }
     const int tail = sq.live & 31;
-    if (tail && full >= blk0 && full < blk0 + 4) {
+    if (tail && full >= blk0 && full < blk0 + kUnpack) {
         const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + (long long)h * kQ8Block * HD;
         const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + (long long)h * kQ8Block * HD;
         const int upto = sq.cap16 - 32 * full;                   // (and zeros up to the capacity)
@@ -344,6 +414,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_rewind_kernel(const __grid_constant__ Q8RewindParams p)
 {
     const Q8RewindSeq sq = p.seq[blockIdx.y];
+    after_previous();
     const int h = blockIdx.x, which = blockIdx.z, tid = threadIdx.x;
     const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
     const long long b = (long long)h * sq.nb + (sq.to >> 5);
@@ -359,15 +430,17 @@ __global__ void __launch_bounds__(kThreads) q8_rewind_kernel(const __grid_consta
 
 // ---- eviction -----------------------------------------------------------------------
 //
-// Which blocks stay: one block of the grid a (sequence, KV head). The weight of
-// the m-th largest among the blocks that may go is found by its bits, eight at
-// a time (weights are not negative, so their bits order as they do; NaN and
-// negative ones count as zero); then one walk in order keeps what is protected,
-// what is above that weight, and as many of those at it, lowest first, as there
-// is room for. The walk also moves scales and weights: a tile is read before
-// anything of it is written, and a kept block only ever moves down, so source
-// and destination may be one cache.
-constexpr int kPickThreads = 512;
+// Which blocks stay: one block of the grid a (sequence, KV head). Among the
+// blocks that may go, `room` stay: those above the weight `key`, and of those at
+// it the first `ties`. Up to kPickThreads blocks every thread counts the weights
+// that come before its own; of more the room-th largest is found by its bits,
+// eleven at a time (weights are not negative, so their bits order as they do;
+// NaN and negative ones count as zero). One walk in order then moves scales and
+// weights: a tile is read before anything of it is written, and a kept block
+// only ever moves down, so source and destination may be one cache.
+constexpr int kPickThreads = 1024;
+constexpr int kPickKeys = 8192;              // weights held in shared memory
+constexpr int kPickBins = 2048;
 
 __device__ __forceinline__ uint32_t weight_key(float w) { return w > 0.0f ? __float_as_uint(w) : 0u; }
 
@@ -384,20 +457,22 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sum, u
     __syncthreads();   // what was read of warp_sum before is done with
     if (lane == 31) warp_sum[warp] = x;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int i = 0; i < kPickThreads / 32; i++) {
-        const uint32_t s = warp_sum[i];
-        if (i < warp) before += s;
-        all += s;
+    static_assert(kPickThreads == 1024, "a warp sum for every lane");
+    uint32_t s = warp_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
     }
-    *sum = all;
-    return before + x - v;
+    *sum = __shfl_sync(0xffffffffu, s, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, s, max(warp, 1) - 1);
+    return (warp ? before : 0u) + x - v;
 }
 
 __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_constant__ Q8EvictParams p, int hd)
 {
-    __shared__ uint32_t hist[256], warp_sum[kPickThreads / 32], found[2];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ uint32_t hist[kPickBins], warp_sum[32], found[2];
+    __shared__ __align__(16) uint32_t keys[kPickKeys];
     const Q8EvictSeq sq = p.seq[blockIdx.y];
     const int h = blockIdx.x, tid = threadIdx.x;
     const Q8Layout a = q8_layout(p.kv_heads, hd, sq.src_nb), z = q8_layout(p.kv_heads, hd, sq.dst_nb);
@@ -409,52 +484,89 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
     const bool all = sq.keep >= sq.full;
     uint32_t room = all ? 0u : (uint32_t)(sq.keep - sq.first - sq.recent);
     uint32_t key = 0xffffffffu, ties = 0;                        // above key: stays; at it: the first `ties`
+    bool chosen = false;                                         // (few blocks: this thread's own stays)
+    const bool few = sq.full <= kPickThreads;
+    after_previous();
     if (!all && room > 0) {
-        uint32_t prefix = 0, mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = lo + tid; i < hi; i += kPickThreads) {
-                const uint32_t k = weight_key(w[i]);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+        const bool held = sq.full <= kPickKeys;
+        if (held) {
+            for (int i = tid; i < (few ? (sq.full + 3) / 4 * 4 : sq.full); i += kPickThreads) {
+                keys[i] = i >= lo && i < hi ? weight_key(w[i]) : 0u;
             }
             __syncthreads();
-            // digit 255 - tid, so that a prefix sum counts from the top
-            const uint32_t mineh = tid < 256 ? hist[255 - tid] : 0u;
-            uint32_t sum;
-            const uint32_t above = block_scan(mineh, warp_sum, &sum);
-            if (tid < 256 && above < room && above + mineh >= room) {
-                found[0] = 255u - tid;
-                found[1] = room - above;
-            }
-            __syncthreads();
-            prefix |= found[0] << shift;
-            mask |= 255u << shift;
-            room = found[1];
         }
-        key = prefix;
-        ties = room;
+        if (few) {
+            if (tid >= lo && tid < hi) {
+                const uint32_t k = keys[tid];
+                uint32_t ahead = 0;                              // those that go before it
+                for (int i = lo / 4 * 4; i < hi; i += 4) {
+                    const uint4 y = *(const uint4 *)&keys[i];
+                    const uint32_t v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int o = i + e;
+                        ahead += (v[e] > k || (v[e] == k && o < tid)) && o >= lo && o < hi ? 1u : 0u;
+                    }
+                }
+                chosen = ahead < room;
+            }
+        } else {
+            uint32_t prefix = 0, mask = 0;
+            for (int round = 0; round < 3; round++) {
+                const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+                const uint32_t digits = round == 2 ? 1023u : 2047u;
+                hist[tid] = 0;
+                hist[tid + kPickThreads] = 0;
+                __syncthreads();
+                for (int i = lo + tid; i < hi; i += kPickThreads) {
+                    const uint32_t k = held ? keys[i] : weight_key(w[i]);
+                    if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1u);
+                }
+                __syncthreads();
+                // digits from the top, two a thread
+                const uint32_t d0 = kPickBins - 1 - 2 * tid;
+                const uint32_t n0 = hist[d0], n1 = hist[d0 - 1];
+                uint32_t sum;
+                const uint32_t above = block_scan(n0 + n1, warp_sum, &sum);
+                if (above < room && above + n0 >= room) {
+                    found[0] = d0;
+                    found[1] = room - above;
+                } else if (above + n0 < room && above + n0 + n1 >= room) {
+                    found[0] = d0 - 1;
+                    found[1] = room - above - n0;
+                }
+                __syncthreads();
+                prefix |= found[0] << shift;
+                mask |= digits << shift;
+                room = found[1];
+            }
+            key = prefix;
+            ties = room;
+        }
     }
     uint32_t kept = 0, tied = 0;
     for (int i0 = 0; i0 < sq.full; i0 += kPickThreads) {
         const int i = i0 + tid;
         const bool in = i < sq.full;
         const bool safe = in && (all || i < lo || i >= hi);
-        const float wi = in ? w[i] : 0.0f;
-        const uint32_t k = weight_key(wi);
-        const bool tie = in && !safe && k == key;
-        uint32_t sum;
-        const uint32_t t_before = tied + block_scan(tie ? 1u : 0u, warp_sum, &sum);
-        tied += sum;
-        const bool stay = safe || (in && k > key) || (tie && t_before < ties);
-        const uint32_t to = kept + block_scan(stay ? 1u : 0u, warp_sum, &sum);
-        kept += sum;
-        float kscale = 0.0f, vscale = 0.0f;
-        if (stay) {
+        float wi = 0.0f, kscale = 0.0f, vscale = 0.0f;
+        if (in) {
+            wi = w[i];
             kscale = ((const float *)(sq.src + a.ks))[sb + i];
             vscale = ((const float *)(sq.src + a.vs))[sb + i];
         }
-        __syncthreads();   // the tile is read
+        const uint32_t k = weight_key(wi);
+        const bool sure = safe || (few ? chosen : in && k > key);
+        const bool tie = !few && in && !safe && k == key;
+        // both counts in one sum: a tile has no more than 1024 of either
+        uint32_t sum;
+        const uint32_t before = block_scan((sure ? 1u : 0u) | (tie ? 0x10000u : 0u), warp_sum, &sum);
+        const uint32_t t_before = min(tied + (before >> 16), ties), t_tile = min(tied, ties);
+        const bool stay = sure || (tie && tied + (before >> 16) < ties);
+        const uint32_t to = kept + (before & 0xffffu) + t_before - t_tile;
+        kept += (sum & 0xffffu) + min(tied + (sum >> 16), ties) - t_tile;
+        tied += sum >> 16;
+        // (the tile is read: every thread has passed the scan's barriers with its values)
         if (stay) {
             index[to] = i;
             if (user) user[to] = i;
@@ -484,7 +596,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_move_kernel(const __grid_constant__ Q8EvictParams p, int slices)
 {
     constexpr int DEPTH = 8;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous();
     const Q8EvictSeq sq = p.seq[blockIdx.z];
     const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
     const int per = kQ8Block * HD / 16 / slices;                 // 16-byte pieces of a slice
@@ -525,71 +637,70 @@ const KernelReg reg_move("q8_move", (const void *)q8_move_kernel<128>);
 
 }  // namespace
 
-cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count)
+// Launches as the programmatic dependent of the kernel before it in the stream
+// (see after_previous, which every kernel launched here calls).
+template <typename... Params, typename... Args>
+static cudaError_t launch(cudaStream_t st, dim3 grid, int threads, void (*kernel)(Params...), Args... args)
 {
-    // Heads share a block of the grid (and its sines and cosines) as long as the
-    // launch still has a few blocks for every SM.
-    p.kv_chunk = 8;
-    p.q_chunk = 16;
-    auto blocks = [&] {
-        const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
-        const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
-        return (long long)p.items * (kvc + qc);
-    };
-    while (p.kv_chunk > 1 && blocks() < 4ll * sm_count) {
-        p.kv_chunk /= 2;
-        p.q_chunk /= 2;
-    }
-    const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
-    const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
-    const dim3 grid((unsigned)p.items, (unsigned)(kvc + qc));
-    if (hd == 128) q8_append_kernel<128><<<grid, kThreads, 0, st>>>(p);
-    else q8_append_kernel<64><<<grid, kThreads, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_q8_read(cudaStream_t st, const Q8ReadParams &p, int hd)
-{
-    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads, 2);
-    if (hd == 128) q8_read_kernel<128><<<grid, kThreads, 0, st>>>(p);
-    else q8_read_kernel<64><<<grid, kThreads, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_q8_unpack(cudaStream_t st, const Q8UnpackParams &p, int hd)
-{
-    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads);
-    if (hd == 128) q8_unpack_kernel<128><<<grid, kThreads, 0, st>>>(p);
-    else q8_unpack_kernel<64><<<grid, kThreads, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_q8_rewind(cudaStream_t st, const Q8RewindParams &p, int hd)
-{
-    const dim3 grid((unsigned)p.kv_heads, (unsigned)p.nseq, 2);
-    if (hd == 128) q8_rewind_kernel<128><<<grid, kThreads, 0, st>>>(p);
-    else q8_rewind_kernel<64><<<grid, kThreads, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_q8_evict(cudaStream_t st, const Q8EvictParams &p, int hd, int sm_count)
-{
-    q8_pick_kernel<<<dim3((unsigned)p.kv_heads, (unsigned)p.nseq), kPickThreads, 0, st>>>(p, hd);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || p.max_keep == 0) return e;
-    // Slices of no less than 256 bytes, until every SM has a few.
-    const int most = kQ8Block * hd / 256;
-    int slices = 1;
-    while (slices < most && (long long)slices * p.kv_heads * 2 * p.nseq < 4ll * sm_count) slices *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)slices, (unsigned)p.kv_heads * 2, (unsigned)p.nseq);
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return hd == 128 ? cudaLaunchKernelEx(&cfg, q8_move_kernel<128>, p, slices)
-                     : cudaLaunchKernelEx(&cfg, q8_move_kernel<64>, p, slices);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count)
+{
+    // Heads share a block of the grid (and its sines and cosines) as long as the
+    // launch still has a few blocks for every SM.
+    p.kv_chunk = 2;
+    p.q_chunk = 16;
+    auto rows = [&] {
+        const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
+        const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
+        return 2 * kvc + qc;
+    };
+    while (p.q_chunk > 2 && (long long)p.items * rows() < 8ll * sm_count) {
+        p.kv_chunk = 1;
+        p.q_chunk /= 2;
+    }
+    const dim3 grid((unsigned)p.items, (unsigned)rows());
+    return hd == 128 ? launch(st, grid, kThreads, q8_append_kernel<128>, p) : launch(st, grid, kThreads, q8_append_kernel<64>, p);
+}
+
+cudaError_t launch_q8_read(cudaStream_t st, const Q8ReadParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads, 2);
+    return hd == 128 ? launch(st, grid, kThreads, q8_read_kernel<128>, p) : launch(st, grid, kThreads, q8_read_kernel<64>, p);
+}
+
+int q8_unpack_tokens(int hd) { return kQ8Block * (2 * kThreads * 16 / (kQ8Block * hd)); }
+
+cudaError_t launch_q8_unpack(cudaStream_t st, const Q8UnpackParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.items, (unsigned)p.kv_heads);
+    return hd == 128 ? launch(st, grid, kThreads, q8_unpack_kernel<128>, p) : launch(st, grid, kThreads, q8_unpack_kernel<64>, p);
+}
+
+cudaError_t launch_q8_rewind(cudaStream_t st, const Q8RewindParams &p, int hd)
+{
+    const dim3 grid((unsigned)p.kv_heads, (unsigned)p.nseq, 2);
+    return hd == 128 ? launch(st, grid, kThreads, q8_rewind_kernel<128>, p) : launch(st, grid, kThreads, q8_rewind_kernel<64>, p);
+}
+
+cudaError_t launch_q8_evict(cudaStream_t st, const Q8EvictParams &p, int hd, int sm_count)
+{
+    const cudaError_t e = launch(st, dim3((unsigned)p.kv_heads, (unsigned)p.nseq), kPickThreads, q8_pick_kernel, p, hd);
+    if (e != cudaSuccess || p.max_keep == 0) return e;
+    // Slices of no less than 256 bytes, until every SM has a few.
+    const int most = kQ8Block * hd / 256;
+    int slices = 1;
+    while (slices < most && (long long)slices * p.kv_heads * 2 * p.nseq < 4ll * sm_count) slices *= 2;
+    const dim3 grid((unsigned)slices, (unsigned)p.kv_heads * 2, (unsigned)p.nseq);
+    return hd == 128 ? launch(st, grid, kThreads, q8_move_kernel<128>, p, slices) : launch(st, grid, kThreads, q8_move_kernel<64>, p, slices);
 }

@@ -99,6 +99,7 @@ struct Q8UnpackParams {
     int nseq, items;
     int kv_heads;
 };
+int q8_unpack_tokens(int hd);    // tokens of a work item
 cudaError_t launch_q8_unpack(cudaStream_t st, const Q8UnpackParams &p, int hd);
 
 struct Q8RewindSeq {
@@ -137,15 +138,15 @@ void launch_rope_inv_freq(cudaStream_t st, float *out, const float *freq_div, in
 
 // ---- decode_q8.cu -----------------------------------------------------------
 
-#define LLMTIE_Q8_MAX_BLOCKS 160
+#define LLMTIE_Q8_MAX_BLOCKS 640
 struct DecodeQ8Seq {
     unsigned char *base;     // (the weights are written)
     int nb, live;
 };
 struct DecodeQ8Params {
     DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
-    long long unit0[LLMTIE_Q8_MAX_SEQ + 1];            // first 32-token unit of each sequence
-    long long ustart[LLMTIE_Q8_MAX_BLOCKS + 1];        // block c takes units [ustart[c], ustart[c+1])
+    int unit0[LLMTIE_Q8_MAX_SEQ + 1];                  // first 32-token unit of each sequence
+    int ustart[LLMTIE_Q8_MAX_BLOCKS + 1];              // block c takes units [ustart[c], ustart[c+1])
     long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
     int nseq, heads, kv_heads;
     const float *q;          // [seq][heads*hd]
@@ -160,3 +161,5 @@ struct DecodeQ8Params {
     long long wait_cycles;
 };
 cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, int grid);
+// Blocks of that kernel that an SM holds at once.
+int decode_q8_resident(int hd);
