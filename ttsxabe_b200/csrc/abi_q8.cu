@@ -401,9 +401,10 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
         // As many blocks of the grid as fit the device at once, and never fewer
         // than four cache blocks for one, a warp each: a finer cut spends longer
         // merging than it saves.
-        const int most = std::min(g->sm_count * decode_q8_resident((int)head_dim), LLMTIE_Q8_MAX_BLOCKS);
+        const int most = g->sm_count * decode_q8_resident((int)head_dim);
         const int grid = (int)std::min<long long>(most, (units + 3) / 4);
-        for (int c = 0; c <= grid; c++) p.ustart[c] = grid ? (int)(units * c / grid) : 0;
+        p.each = grid ? (int)(units / grid) : 0;
+        p.more = grid ? (int)(units % grid) : 0;
         const size_t pairs = (size_t)p.nseq * kv_heads;
         cudaError_t err;
         const size_t slots = (size_t)std::max(grid, 1) * 2 * 8;

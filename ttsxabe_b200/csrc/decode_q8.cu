@@ -40,7 +40,9 @@ struct Geo {
     static constexpr int BLOCK = kQ8Block * HD;          // bytes of a block's keys (or values)
     static constexpr int STAGES = 3;
     static constexpr int RESIDENT = HD == 128 ? 2 : 4;   // blocks of the grid that fit an SM
-    static constexpr int RING = kWarps * STAGES * 2 * BLOCK;
+    // a stage: keys, values, and the 16 bytes of either's scales that hold the block's
+    static constexpr int STAGE = 2 * BLOCK + 32;
+    static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int MERGE = kWarps * kRows * HD * 4;
     static constexpr int SMEM = RING + MERGE;
 };
@@ -137,16 +139,16 @@ __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
     return r;
 }
 
+// The cut: the first `more` blocks of the grid take each + 1 units, the others each.
+__device__ __forceinline__ int first_unit(const DecodeQ8Params &p, int block)
+{
+    return block * p.each + min(block, p.more);
+}
 // The block of the grid that holds unit u.
 __device__ __forceinline__ int block_of(const DecodeQ8Params &p, int u)
 {
-    int lo = 0, hi = (int)gridDim.x - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.ustart[mid] <= u) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+    const int seam = p.more * (p.each + 1);
+    return u < seam ? (int)((unsigned)u / (unsigned)(p.each + 1)) : p.more + (int)((unsigned)(u - seam) / (unsigned)p.each);
 }
 
 template <int HD>
@@ -179,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.heads / p.kv_heads;
-    const int u_begin = p.ustart[blockIdx.x], u_end = p.ustart[blockIdx.x + 1];
+    const int u_begin = first_unit(p, (int)blockIdx.x), u_end = first_unit(p, (int)blockIdx.x + 1);
     float *merge = (float *)(smem + G::RING);
-    const uint32_t ring0 = smem_u32(smem) + (uint32_t)warp * (G::STAGES * 2 * G::BLOCK);
+    const uint32_t ring0 = smem_u32(smem) + (uint32_t)warp * (G::STAGES * G::STAGE);
     const uint32_t bar0 = smem_u32(&bars[warp * G::STAGES]);
     if (lane == 0) {
         for (int s = 0; s < G::STAGES; s++) {
@@ -190,13 +192,57 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    const int r = lane >> 2, c = lane & 3;
+    Run run = run_at(p, u_begin, u_end);
+
+    // What a run needs besides its blocks: the query (row r, the 16 channels of
+    // chunk c in each panel), and of the tail the warp's eight tokens (keys: token
+    // r, channels 32 i + 8 c; values: V channels of each). It is asked for in front
+    // of the blocks, and for the next run in front of this one's merge: behind a
+    // full ring of blocks a load waits for all of them.
+    float x[PANELS][16];
+    uint4 tk[HD / 32];
+    uint2 tv[8];
+    auto load_run = [&] {
+        const DecodeQ8Seq &s = p.seq[run.seq];
+        const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
+#pragma unroll
+        for (int j = 0; j < PANELS; j++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
+                x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
+            }
+        }
+        const int n = run.tail ? (s.live & 31) - 8 * warp : 0;
+        if (n > 0) {
+            const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
+            const uint16_t *kt = (const uint16_t *)(s.base + at.kt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
+            const uint16_t *vt = (const uint16_t *)(s.base + at.vt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) {
+                tk[i] = r < n ? *(const uint4 *)(kt + r * HD + 32 * i + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                tv[t] = make_uint2(0u, 0u);
+                if (t < n) {
+                    if (V == 4) tv[t] = *(const uint2 *)(vt + t * HD + V * lane);
+                    else tv[t].x = *(const uint32_t *)(vt + t * HD + V * lane);
+                }
+            }
+        }
+    };
+
     // The next kernel of the stream may set itself up; nothing of the one before
     // is read until it has ended.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    load_run();
 
     // The warp's blocks in order, over all runs: `ahead` is what is fetched next.
-    Run ahead = run_at(p, u_begin, u_end);
+    Run ahead = run;
     int ahead_blk = ahead.first + warp;
     int issued = 0, used = 0;
     auto skip_done = [&] {
@@ -211,63 +257,28 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (lane == 0) {
             const DecodeQ8Seq &s = p.seq[ahead.seq];
             const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
-            const long long off = ((long long)ahead.head * s.nb + ahead_blk) * G::BLOCK;
+            const long long b = (long long)ahead.head * s.nb + ahead_blk;
             const int stage = issued % G::STAGES;
-            const uint32_t dst = ring0 + (uint32_t)stage * (2 * G::BLOCK), bar = bar0 + 8 * stage;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * G::BLOCK) : "memory");
-            bulk_load(dst, s.base + at.k + off, G::BLOCK, bar);
-            bulk_load(dst + G::BLOCK, s.base + at.v + off, G::BLOCK, bar);
+            const uint32_t dst = ring0 + (uint32_t)stage * G::STAGE, bar = bar0 + 8 * stage;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(G::STAGE) : "memory");
+            bulk_load(dst, s.base + at.k + b * G::BLOCK, G::BLOCK, bar);
+            bulk_load(dst + G::BLOCK, s.base + at.v + b * G::BLOCK, G::BLOCK, bar);
+            bulk_load(dst + 2 * G::BLOCK, s.base + at.ks + (b & ~3ll) * 4, 16, bar);
+            bulk_load(dst + 2 * G::BLOCK + 16, s.base + at.vs + (b & ~3ll) * 4, 16, bar);
         }
         issued++;
         ahead_blk += kWarps;
     };
     for (int s = 0; s < G::STAGES; s++) fetch();
 
-    const int r = lane >> 2, c = lane & 3;
-    bool ok = true;
-    for (int u = u_begin; u < u_end;) {
-        const Run run = run_at(p, u, u_end);
-        const bool is_first = u == u_begin;
-        u = run.next;
+    bool ok = true, is_first = true;
+    for (;;) {
         const DecodeQ8Seq &sq = p.seq[run.seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
         const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
-        const float *ks = (const float *)(sq.base + at.ks) + (long long)run.head * sq.nb;
-        const float *vs = (const float *)(sq.base + at.vs) + (long long)run.head * sq.nb;
+        const uint32_t scale0 = (uint32_t)((long long)run.head * sq.nb) & 3u;
 
-        // -- everything the run needs besides its blocks is asked for at once: the
-        // query (row r, the 16 channels of chunk c in each panel), and of the tail
-        // the warp's eight tokens, four lanes each
-        float x[PANELS][16];
-#pragma unroll
-        for (int j = 0; j < PANELS; j++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
-                x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
-            }
-        }
         const int tail_n = run.tail ? min(8, (sq.live & 31) - 8 * warp) : 0;    // the warp's tokens
-        uint4 tk[HD / 32];
-        uint2 tv[8][V / 4 ? V / 4 : 1];
-        if (tail_n > 0) {
-            const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
-            const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
-#pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                tk[i] = r < tail_n ? *(const uint4 *)(kt + r * HD + 32 * i + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                tv[t][0] = make_uint2(0u, 0u);
-                if (t < tail_n) {
-                    if (V == 4) tv[t][0] = *(const uint2 *)(vt + t * HD + V * lane);
-                    else tv[t][0].x = *(const uint32_t *)(vt + t * HD + V * lane);
-                }
-            }
-        }
-
         // -- the query as fixed point
         uint32_t qa[PANELS][4], qb[PANELS][4];
         float f_q;
@@ -337,11 +348,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 #pragma unroll
                 for (int t = 0; t < 8; t++) {
                     const float w = __shfl_sync(0xffffffffu, e, 4 * t);
-                    const float2 v0 = __half22float2(*(const __half2 *)&tv[t][0].x);
+                    const float2 v0 = __half22float2(*(const __half2 *)&tv[t].x);
                     o4[0] = fmaf(w, v0.x, o4[0]);
                     o4[1] = fmaf(w, v0.y, o4[1]);
                     if (V == 4) {
-                        const float2 v1 = __half22float2(*(const __half2 *)&tv[t][0].y);
+                        const float2 v1 = __half22float2(*(const __half2 *)&tv[t].y);
                         o4[V - 2] = fmaf(w, v1.x, o4[V - 2]);
                         o4[V - 1] = fmaf(w, v1.y, o4[V - 1]);
                     }
@@ -367,24 +378,18 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
 
         // -- the warp's blocks
-        float k_scale = 0.0f, v_scale = 0.0f;
-        if (run.first + warp < run.last) {
-            k_scale = __ldg(ks + run.first + warp);
-            v_scale = __ldg(vs + run.first + warp);
-        }
         for (int blk = run.first + warp; blk < run.last; blk += kWarps) {
             const int stage = used % G::STAGES;
-            const uint32_t kb = ring0 + (uint32_t)stage * (2 * G::BLOCK), vb = kb + G::BLOCK;
-            const float sk = k_scale, sv = v_scale;
-            if (blk + kWarps < run.last) {
-                k_scale = __ldg(ks + blk + kWarps);
-                v_scale = __ldg(vs + blk + kWarps);
-            }
+            const uint32_t kb = ring0 + (uint32_t)stage * G::STAGE, vb = kb + G::BLOCK;
             if (ok) ok = ring_wait(bar0 + 8 * stage, (uint32_t)(used / G::STAGES) & 1u, p.status, p.wait_cycles);
             used++;
             // scores: column n of tile t is token 8 (n / 2) + 2 t + n % 2
             float s[8];
             float mb = -CUDART_INF_F;
+            float sk, sv;
+            const uint32_t scales = kb + 2 * G::BLOCK + ((scale0 + (uint32_t)blk) & 3u) * 4;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk) : "r"(scales) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sv) : "r"(scales + 16) : "memory");
             const float f = f_q * sk;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
@@ -455,6 +460,14 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             fetch();
         }
 
+        // the next run's query and tail are on their way under the merge
+        const Run now = run;
+        const bool more = now.next < u_end;
+        if (more) {
+            run = run_at(p, now.next, u_end);
+            load_run();
+        }
+
         // -- the run's result: a warp merges rows warp, warp + kWarps of the block's warps'
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -470,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             }
         }
         __syncthreads();
-        const long long row0 = (long long)run.seq * p.heads + (long long)run.head * group;
+        const long long row0 = (long long)now.seq * p.heads + (long long)now.head * group;
         const int slot = (int)blockIdx.x * 2 + (is_first ? 0 : 1);
         for (int row = warp; row < group; row += kWarps) {
             float M = -CUDART_INF_F, L = 0.0f, o[V];
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                     o[e] = fmaf(fk, merge[(k * kRows + row) * HD + 8 * ((V * lane / 8) ^ row) + V * lane % 8 + e], o[e]);
                 }
             }
-            if (run.whole) {
+            if (now.whole) {
                 const float inv = 1.0f / L;
 #pragma unroll
                 for (int e = 0; e < V; e++) o[e] *= inv;
@@ -502,25 +515,24 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 if (lane == 0) p.part_ml[slot * kRows + row] = make_float2(M, L);
             }
         }
-        bool done = run.whole;
-        if (!run.whole) {
-            __threadfence();
+        bool done = now.whole;
+        if (!now.whole) {
+            const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
             __syncthreads();
-            const int b0 = block_of(p, run.begin), b1 = block_of(p, run.begin + run.units - 1);
             if (tid == 0) {
-                unsigned *ctr = &p.ctr[run.seq * p.kv_heads + run.head];
-                const unsigned seen = atomicAdd(ctr, 1u);
+                // (releases what the barrier ordered before it, acquires the others')
+                unsigned *ctr = &p.ctr[now.seq * p.kv_heads + now.head], seen;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(ctr) : "memory");
                 last_s = seen == (unsigned)(b1 - b0);
                 if (last_s) *ctr = 0u;
             }
             __syncthreads();
             done = last_s != 0;
             if (done) {
-                __threadfence();
                 // The contributors in order, whoever came last: the same bits every
                 // time. A block's first run has slot 0, and only b0 may hold the pair
                 // in its last.
-                const int skew = p.ustart[b0] >= run.begin ? 0 : 1;
+                const int skew = first_unit(p, b0) >= now.begin ? 0 : 1;
                 for (int row = warp; row < group; row += kWarps) {
                     float M = -CUDART_INF_F, L = 0.0f, o[V];
 #pragma unroll
@@ -576,9 +588,9 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (done && p.stats) {
             // weights: what each block's keys got, over the group's heads
             __syncthreads();
-            float *weight = (float *)(sq.base + at.w) + (long long)run.head * sq.nb;
+            float *weight = (float *)(sq.base + at.w) + (long long)now.head * sq.nb;
             const int full = sq.live >> 5;
-            const float2 *st = p.stats + (p.stat0[run.seq] + (long long)run.head * full) * kRows;
+            const float2 *st = p.stats + (p.stat0[now.seq] + (long long)now.head * full) * kRows;
             for (int b = tid; b < full; b += kThreads) {
                 float2 y[kRows];
 #pragma unroll
@@ -591,6 +603,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 weight[b] += sum;
             }
         }
+        if (!more) break;
+        is_first = false;
         __syncthreads();   // merge, m_s and final_s are free again
     }
     if (!ok) {
@@ -634,17 +648,9 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
         if (e != cudaSuccess) return e;
     }
     if (grid == 0) return cudaSuccess;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = hd == 128 ? Geo<128>::SMEM : Geo<64>::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return hd == 128 ? cudaLaunchKernelEx(&cfg, decode_q8_kernel<128>, p) : cudaLaunchKernelEx(&cfg, decode_q8_kernel<64>, p);
+    const dim3 blocks((unsigned)grid);
+    return hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, decode_q8_kernel<128>, p)
+                     : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, decode_q8_kernel<64>, p);
 }
 
 int decode_q8_resident(int hd) { return hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT; }

@@ -637,21 +637,11 @@ const KernelReg reg_move("q8_move", (const void *)q8_move_kernel<128>);
 
 }  // namespace
 
-// Launches as the programmatic dependent of the kernel before it in the stream
-// (see after_previous, which every kernel launched here calls).
+// (every kernel launched here calls after_previous)
 template <typename... Params, typename... Args>
 static cudaError_t launch(cudaStream_t st, dim3 grid, int threads, void (*kernel)(Params...), Args... args)
 {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
+    return launch_dependent(st, grid, threads, 0, kernel, args...);
 }
 
 cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count)

@@ -25,6 +25,8 @@
 
 #include "common.cuh"
 
+#include <stdlib.h>
+
 constexpr int kQ8Block = 32;
 #define LLMTIE_Q8_MAX_SEQ 32
 
@@ -46,6 +48,26 @@ __host__ __device__ inline Q8Layout q8_layout(int kv_heads, int hd, int nb)
     l.vt = l.kt + tail;
     l.bytes = l.vt + tail;
     return l;
+}
+
+// Launches `kernel` as the programmatic dependent of the kernel before it in the
+// stream: it may be set up while that one still runs, and waits for its end
+// (griddepcontrol.wait) before it reads or writes anything.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_dependent(cudaStream_t st, dim3 grid, int threads, size_t smem, void (*kernel)(Params...), Args... args)
+{
+    static const bool no_pdl = getenv("LLMTIE_B200_NO_PDL") != nullptr;   // an A/B switch
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = no_pdl ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // ---- kv_q8.cu ---------------------------------------------------------------
@@ -138,7 +160,6 @@ void launch_rope_inv_freq(cudaStream_t st, float *out, const float *freq_div, in
 
 // ---- decode_q8.cu -----------------------------------------------------------
 
-#define LLMTIE_Q8_MAX_BLOCKS 640
 struct DecodeQ8Seq {
     unsigned char *base;     // (the weights are written)
     int nb, live;
@@ -146,7 +167,7 @@ struct DecodeQ8Seq {
 struct DecodeQ8Params {
     DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
     int unit0[LLMTIE_Q8_MAX_SEQ + 1];                  // first 32-token unit of each sequence
-    int ustart[LLMTIE_Q8_MAX_BLOCKS + 1];              // block c takes units [ustart[c], ustart[c+1])
+    int each, more;                                    // units a block of the grid takes; the first `more` one more
     long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
     int nseq, heads, kv_heads;
     const float *q;          // [seq][heads*hd]
