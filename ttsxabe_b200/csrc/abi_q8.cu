@@ -207,8 +207,8 @@ extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *
         return overrun(total * kv_heads * head_dim, std::min(k_len, v_len));
     }
     if (total > (size_t)cu_seqlens[0] && (!k_out || !v_out)) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
-    if (((uintptr_t)k_out & 7u) != 0) return llmtie_misaligned("the keys read", k_out, 8);
-    if (((uintptr_t)v_out & 7u) != 0) return llmtie_misaligned("the values read", v_out, 8);
+    if (((uintptr_t)k_out & 15u) != 0) return llmtie_misaligned("the keys read", k_out, 16);
+    if (((uintptr_t)v_out & 15u) != 0) return llmtie_misaligned("the values read", v_out, 16);
     for (size_t b = 0; b < batch; b++) {
         const int n = cu_seqlens[b + 1] - cu_seqlens[b];
         if (n == 0) continue;

@@ -38,10 +38,9 @@ constexpr int kRows = 8;             // query rows a pair may have
 template <int HD>
 struct Geo {
     static constexpr int BLOCK = kQ8Block * HD;          // bytes of a block's keys (or values)
-    static constexpr int STAGES = 3;
-    static constexpr int RESIDENT = HD == 128 ? 2 : 4;   // blocks of the grid that fit an SM
-    // a stage: keys, values, and the 16 bytes of either's scales that hold the block's
-    static constexpr int STAGE = 2 * BLOCK + 32;
+    static constexpr int STAGES = 2;
+    static constexpr int RESIDENT = HD == 128 ? 2 : 3;   // blocks of the grid that fit an SM
+    static constexpr int STAGE = 2 * BLOCK;              // keys, then values
     static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int MERGE = kWarps * kRows * HD * 4;
     static constexpr int SMEM = RING + MERGE;
@@ -166,6 +165,35 @@ __device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at,
     }
 }
 
+// The weights of finished pairs (two at most, side by side: what this costs is
+// the latency of its loads): what each complete block's tokens got, summed over
+// the group's heads; `fin` has each row's maximum and the inverse of its sum.
+template <int HD>
+__device__ __forceinline__ void weigh(const DecodeQ8Params &p, const Run *pair, bool both, const float2 *fin, int tid, int group)
+{
+    const int full0 = p.seq[pair[0].seq].live >> 5, total = full0 + (both ? p.seq[pair[1].seq].live >> 5 : 0);
+    for (int i = tid; i < total; i += kThreads) {
+        const bool second = i >= full0;
+        const Run &now = pair[second];
+        const int b = second ? i - full0 : i;
+        const DecodeQ8Seq &sq = p.seq[now.seq];
+        const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+        float *weight = (float *)(sq.base + at.w) + (long long)now.head * sq.nb + b;
+        const float2 *st = p.stats + (p.stat0[now.seq] + (long long)now.head * (sq.live >> 5) + b) * kRows;
+        const float2 *f = fin + (second ? group : 0);
+        float2 y[kRows];
+        const float before = *weight;
+#pragma unroll
+        for (int k = 0; k < kRows; k++) y[k] = k < group ? __ldcg(&st[k]) : make_float2(0.f, 0.f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRows; k++) {
+            if (k < group) sum = fmaf(ex2(y[k].x - f[k].x) * f[k].y, y[k].y, sum);
+        }
+        *weight = before + sum;
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(const __grid_constant__ DecodeQ8Params p)
 {
@@ -176,8 +204,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[kWarps * G::STAGES];
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
-    __shared__ float2 final_s[kRows];
-    __shared__ int last_s;
+    __shared__ float2 final_s[2 * kRows];
+    __shared__ int last_s[2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.heads / p.kv_heads;
@@ -197,14 +225,29 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 
     // What a run needs besides its blocks: the query (row r, the 16 channels of
     // chunk c in each panel), and of the tail the warp's eight tokens (keys: token
-    // r, channels 32 i + 8 c; values: V channels of each). It is asked for in front
+    // r, the same channels; values: V channels of each). It is asked for in front
     // of the blocks, and for the next run in front of this one's merge: behind a
     // full ring of blocks a load waits for all of them.
     float x[PANELS][16];
-    uint4 tk[HD / 32];
+    uint4 tk[PANELS][2];
     uint2 tv[8];
+    // The scales of the warp's next 32 blocks, a lane each (half of them ahead of
+    // use, later on).
+    float k_scale, v_scale, k_next = 0.0f, v_next = 0.0f;
+    const float *ks, *vs;
+    auto load_scales = [&](int blk, float &a, float &b) {
+        blk += lane * kWarps;
+        if (blk < run.last) {
+            a = __ldg(ks + blk);
+            b = __ldg(vs + blk);
+        }
+    };
     auto load_run = [&] {
         const DecodeQ8Seq &s = p.seq[run.seq];
+        const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
+        ks = (const float *)(s.base + at.ks) + (long long)run.head * s.nb;
+        vs = (const float *)(s.base + at.vs) + (long long)run.head * s.nb;
+        load_scales(run.first + warp, k_scale, v_scale);
         const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
 #pragma unroll
         for (int j = 0; j < PANELS; j++) {
@@ -217,12 +260,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
         const int n = run.tail ? (s.live & 31) - 8 * warp : 0;
         if (n > 0) {
-            const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
             const uint16_t *kt = (const uint16_t *)(s.base + at.kt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
             const uint16_t *vt = (const uint16_t *)(s.base + at.vt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                tk[i] = r < n ? *(const uint4 *)(kt + r * HD + 32 * i + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 2 * PANELS; i++) {
+                tk[i / 2][i % 2] = r < n ? *(const uint4 *)(kt + r * HD + 64 * (i / 2) + 16 * c + 8 * (i % 2)) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
             for (int t = 0; t < 8; t++) {
@@ -235,36 +277,43 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
     };
 
+    // The warp's blocks in order, over all runs: `ahead` is what is fetched next.
+    Run ahead = run;
+    int ahead_blk = ahead.first + warp;
+    const unsigned char *ahead_k, *ahead_v;      // of the head's first block
+    auto aim = [&] {
+        const DecodeQ8Seq &s = p.seq[ahead.seq];
+        const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
+        const long long b = (long long)ahead.head * s.nb;
+        ahead_k = s.base + at.k + b * G::BLOCK;
+        ahead_v = s.base + at.v + b * G::BLOCK;
+    };
+    aim();
+
     // The next kernel of the stream may set itself up; nothing of the one before
     // is read until it has ended.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     load_run();
 
-    // The warp's blocks in order, over all runs: `ahead` is what is fetched next.
-    Run ahead = run;
-    int ahead_blk = ahead.first + warp;
     int issued = 0, used = 0;
     auto skip_done = [&] {
         while (ahead_blk >= ahead.last && ahead.next < u_end) {
             ahead = run_at(p, ahead.next, u_end);
             ahead_blk = ahead.first + warp;
+            aim();
         }
         return ahead_blk < ahead.last;
     };
     auto fetch = [&] {
         if (!skip_done()) return;
         if (lane == 0) {
-            const DecodeQ8Seq &s = p.seq[ahead.seq];
-            const Q8Layout at = q8_layout(p.kv_heads, HD, s.nb);
-            const long long b = (long long)ahead.head * s.nb + ahead_blk;
             const int stage = issued % G::STAGES;
             const uint32_t dst = ring0 + (uint32_t)stage * G::STAGE, bar = bar0 + 8 * stage;
+            const size_t off = (size_t)ahead_blk * G::BLOCK;
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(G::STAGE) : "memory");
-            bulk_load(dst, s.base + at.k + b * G::BLOCK, G::BLOCK, bar);
-            bulk_load(dst + G::BLOCK, s.base + at.v + b * G::BLOCK, G::BLOCK, bar);
-            bulk_load(dst + 2 * G::BLOCK, s.base + at.ks + (b & ~3ll) * 4, 16, bar);
-            bulk_load(dst + 2 * G::BLOCK + 16, s.base + at.vs + (b & ~3ll) * 4, 16, bar);
+            bulk_load(dst, ahead_k + off, G::BLOCK, bar);
+            bulk_load(dst + G::BLOCK, ahead_v + off, G::BLOCK, bar);
         }
         issued++;
         ahead_blk += kWarps;
@@ -272,11 +321,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     for (int s = 0; s < G::STAGES; s++) fetch();
 
     bool ok = true, is_first = true;
+    Run pending[2];
+    pending[0].units = pending[1].units = 0;
     for (;;) {
         const DecodeQ8Seq &sq = p.seq[run.seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
-        const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
-        const uint32_t scale0 = (uint32_t)((long long)run.head * sq.nb) & 3u;
 
         const int tail_n = run.tail ? min(8, (sq.live & 31) - 8 * warp) : 0;    // the warp's tokens
         // -- the query as fixed point
@@ -321,16 +370,19 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (tail_n > 0) {
             float *mine = merge + warp * kRows * HD;
             for (int g = 0; g < group; g++) {
-                // lane (r, c): channels 32 i + 8 c of token r
+                // lane (r, c): chunk c of token r's key against that of row g's query, which
+                // lane (g, c) holds (read again from memory it would wait behind the ring)
                 float s = 0.0f;
 #pragma unroll
-                for (int i = 0; i < HD / 32; i++) {
-                    const float4 q0 = __ldg((const float4 *)(qh + g * HD + 32 * i + 8 * c));
-                    const float4 q1 = __ldg((const float4 *)(qh + g * HD + 32 * i + 8 * c + 4));
-                    const float2 k0 = __half22float2(*(const __half2 *)&tk[i].x), k1 = __half22float2(*(const __half2 *)&tk[i].y);
-                    const float2 k2 = __half22float2(*(const __half2 *)&tk[i].z), k3 = __half22float2(*(const __half2 *)&tk[i].w);
-                    s = fmaf(q0.x, k0.x, s); s = fmaf(q0.y, k0.y, s); s = fmaf(q0.z, k1.x, s); s = fmaf(q0.w, k1.y, s);
-                    s = fmaf(q1.x, k2.x, s); s = fmaf(q1.y, k2.y, s); s = fmaf(q1.z, k3.x, s); s = fmaf(q1.w, k3.y, s);
+                for (int i = 0; i < 2 * PANELS; i++) {
+                    const uint4 kk = tk[i / 2][i % 2];
+                    const float2 k4[4] = {__half22float2(*(const __half2 *)&kk.x), __half22float2(*(const __half2 *)&kk.y),
+                                          __half22float2(*(const __half2 *)&kk.z), __half22float2(*(const __half2 *)&kk.w)};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        s = fmaf(__shfl_sync(0xffffffffu, x[i / 2][8 * (i % 2) + 2 * e], 4 * g + c), k4[e].x, s);
+                        s = fmaf(__shfl_sync(0xffffffffu, x[i / 2][8 * (i % 2) + 2 * e + 1], 4 * g + c), k4[e].y, s);
+                    }
                 }
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
@@ -386,10 +438,13 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             // scores: column n of tile t is token 8 (n / 2) + 2 t + n % 2
             float s[8];
             float mb = -CUDART_INF_F;
-            float sk, sv;
-            const uint32_t scales = kb + 2 * G::BLOCK + ((scale0 + (uint32_t)blk) & 3u) * 4;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk) : "r"(scales) : "memory");
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sv) : "r"(scales + 16) : "memory");
+            const int turn = (blk - run.first - warp) / kWarps & 31;
+            const float sk = __shfl_sync(0xffffffffu, k_scale, turn), sv = __shfl_sync(0xffffffffu, v_scale, turn);
+            if (turn == 15) load_scales(blk + 17 * kWarps, k_next, v_next);
+            if (turn == 31) {
+                k_scale = k_next;
+                v_scale = v_next;
+            }
             const float f = f_q * sk;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
@@ -515,97 +570,103 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 if (lane == 0) p.part_ml[slot * kRows + row] = make_float2(M, L);
             }
         }
-        bool done = now.whole;
-        if (!now.whole) {
-            const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
-            __syncthreads();
-            if (tid == 0) {
-                // (releases what the barrier ordered before it, acquires the others')
-                unsigned *ctr = &p.ctr[now.seq * p.kv_heads + now.head], seen;
-                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(ctr) : "memory");
-                last_s = seen == (unsigned)(b1 - b0);
-                if (last_s) *ctr = 0u;
+        if (now.whole) {
+            if (p.stats) {
+                __syncthreads();
+                weigh<HD>(p, &now, false, final_s, tid, group);
             }
-            __syncthreads();
-            done = last_s != 0;
-            if (done) {
-                // The contributors in order, whoever came last: the same bits every
-                // time. A block's first run has slot 0, and only b0 may hold the pair
-                // in its last.
-                const int skew = first_unit(p, b0) >= now.begin ? 0 : 1;
-                for (int row = warp; row < group; row += kWarps) {
-                    float M = -CUDART_INF_F, L = 0.0f, o[V];
-#pragma unroll
-                    for (int e = 0; e < V; e++) o[e] = 0.0f;
-                    for (int bb = b0; bb <= b1; bb += 32) {
-                        const int n = min(32, b1 + 1 - bb);
-                        const int my_slot = 2 * (bb + lane) + (bb + lane == b0 ? skew : 0);
-                        float2 ml = make_float2(-CUDART_INF_F, 0.0f);
-                        if (lane < n) ml = __ldcg(&p.part_ml[my_slot * kRows + row]);
-                        float top = ml.x;
-#pragma unroll
-                        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        top = fmaxf(top, M);
-                        const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
-                        const float f = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
-                        float sum = f * ml.y;
-#pragma unroll
-                        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                        L = fmaf(L, keep, sum);
-#pragma unroll
-                        for (int e = 0; e < V; e++) o[e] *= keep;
-                        for (int i0 = 0; i0 < n; i0 += 8) {
-                            float2 y[8][V / 2];
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const int b = min(bb + i0 + i, b1);
-                                const long long sl = 2 * b + (b == b0 ? skew : 0);
-#pragma unroll
-                                for (int e = 0; e < V; e += 2) {
-                                    y[i][e / 2] = __ldcg((const float2 *)(p.part_o + (sl * kRows + row) * HD + V * lane + e));
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const float fi = __shfl_sync(0xffffffffu, f, i0 + i);   // (0 past the last)
-#pragma unroll
-                                for (int e = 0; e < V; e += 2) {
-                                    o[e] = fmaf(fi, y[i][e / 2].x, o[e]);
-                                    o[e + 1] = fmaf(fi, y[i][e / 2].y, o[e + 1]);
-                                }
-                            }
-                        }
-                        M = top;
-                    }
-                    const float inv = 1.0f / L;
-#pragma unroll
-                    for (int e = 0; e < V; e++) o[e] *= inv;
-                    store_row<HD>(p, (row0 + row) * HD, lane, o);
-                    if (lane == 0) final_s[row] = make_float2(M, inv);
-                }
-            }
-        }
-        if (done && p.stats) {
-            // weights: what each block's keys got, over the group's heads
-            __syncthreads();
-            float *weight = (float *)(sq.base + at.w) + (long long)now.head * sq.nb;
-            const int full = sq.live >> 5;
-            const float2 *st = p.stats + (p.stat0[now.seq] + (long long)now.head * full) * kRows;
-            for (int b = tid; b < full; b += kThreads) {
-                float2 y[kRows];
-#pragma unroll
-                for (int k = 0; k < kRows; k++) y[k] = k < group ? __ldcg(&st[(long long)b * kRows + k]) : make_float2(0.f, 0.f);
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kRows; k++) {
-                    if (k < group) sum = fmaf(ex2(y[k].x - final_s[k].x) * final_s[k].y, y[k].y, sum);
-                }
-                weight[b] += sum;
-            }
+        } else {
+            pending[is_first ? 0 : 1] = now;
         }
         if (!more) break;
         is_first = false;
         __syncthreads();   // merge, m_s and final_s are free again
+    }
+
+    // -- pairs shared with other blocks of the grid (the first run's and the last's,
+    // at most): the last to arrive merges. All arrivals wait until the block's own
+    // work is done: an arrival takes as long as the memory is busy.
+    __syncthreads();
+    if (tid < 2) {
+        last_s[tid] = 0;
+        const Run &now = tid ? pending[1] : pending[0];
+        if (now.units > 0) {
+            const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
+            // (releases what the barrier ordered before it, acquires the others')
+            unsigned *ctr = &p.ctr[now.seq * p.kv_heads + now.head], seen;
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(ctr) : "memory");
+            last_s[tid] = seen == (unsigned)(b1 - b0);
+            if (last_s[tid]) *ctr = 0u;
+        }
+    }
+    __syncthreads();
+    // (a warp takes a row of either pair)
+    for (int item = warp; item < 2 * group; item += kWarps) {
+        if (!last_s[item >= group]) continue;
+        const int row = item >= group ? item - group : item;
+        const Run &now = pending[item >= group];
+        const long long row0 = (long long)now.seq * p.heads + (long long)now.head * group;
+        const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
+        // The contributors in order, whoever came last: the same bits every time. A
+        // block's first run has slot 0, and only b0 may hold the pair in its last.
+        const int skew = first_unit(p, b0) >= now.begin ? 0 : 1;
+        float M = -CUDART_INF_F, L = 0.0f, o[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) o[e] = 0.0f;
+        for (int bb = b0; bb <= b1; bb += 32) {
+            const int n = min(32, b1 + 1 - bb);
+            const int my_slot = 2 * (bb + lane) + (bb + lane == b0 ? skew : 0);
+            float2 ml = make_float2(-CUDART_INF_F, 0.0f);
+            if (lane < n) ml = __ldcg(&p.part_ml[my_slot * kRows + row]);
+            float2 y[8][V / 2];
+            auto load8 = [&](int i0) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int b = min(bb + i0 + i, b1);
+                    const long long sl = 2 * b + (b == b0 ? skew : 0);
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        y[i][e / 2] = __ldcg((const float2 *)(p.part_o + (sl * kRows + row) * HD + V * lane + e));
+                    }
+                }
+            };
+            load8(0);
+            float top = ml.x;
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+            top = fmaxf(top, M);
+            const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
+            const float f = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+            float sum = f * ml.y;
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            L = fmaf(L, keep, sum);
+#pragma unroll
+            for (int e = 0; e < V; e++) o[e] *= keep;
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                if (i0) load8(i0);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i0 + i);   // (0 past the last)
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        o[e] = fmaf(fi, y[i][e / 2].x, o[e]);
+                        o[e + 1] = fmaf(fi, y[i][e / 2].y, o[e + 1]);
+                    }
+                }
+            }
+            M = top;
+        }
+        const float inv = 1.0f / L;
+#pragma unroll
+        for (int e = 0; e < V; e++) o[e] *= inv;
+        store_row<HD>(p, (row0 + row) * HD, lane, o);
+        if (lane == 0) final_s[item] = make_float2(M, inv);
+    }
+    if (p.stats && (last_s[0] || last_s[1])) {
+        __syncthreads();
+        const int e = last_s[0] ? 0 : 1;
+        weigh<HD>(p, pending + e, last_s[0] && last_s[1], final_s + e * group, tid, group);
     }
     if (!ok) {
         // a wait gave up: leave the copies still in flight time to land

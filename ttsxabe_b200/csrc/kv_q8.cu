@@ -116,10 +116,10 @@ __global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_con
         const long long row_of = (long long)sq.row0 + 32 * j - r;   // + t: its packed row
         __syncthreads();   // the pass before is done with `turn`, and with the tail rows it read
         auto fill_turns = [&] {
-            for (int i = tid; i < (t_hi - t_lo) * HALF; i += kThreads) {
-                const int t = t_lo + i / HALF, f = i % HALF;
-                const double half_turns = (double)(sq.pos + 32 * j - r + t) * (double)p.inv_freq[f] *
-                                          0.31830988618379067154;
+            const int f = tid % HALF;
+            const double each = (double)p.inv_freq[f] * 0.31830988618379067154;
+            for (int t = t_lo + tid / HALF; t < t_hi; t += kThreads / HALF) {
+                const double half_turns = (double)(sq.pos + 32 * j - r + t) * each;
                 float sn, cs;
                 sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &sn, &cs);
                 turn[t][f] = make_float2(cs, sn);
@@ -137,19 +137,19 @@ __global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_con
             b = hi;
         };
         if (is_q) {
-            const int h0 = ((int)blockIdx.y - 2 * kv_chunks) * p.q_chunk;
-            const int nh = min(p.q_chunk, p.heads - h0);
-            const int rows = (t_hi - t_lo) * nh;
+            const int h0 = ((int)blockIdx.y - 2 * kv_chunks) << p.q_log, mask = (1 << p.q_log) - 1;
+            const int rows = (t_hi - t_lo) << p.q_log;
             constexpr int U = 4;                               // rows in flight
             constexpr int STEP = kWarps * RPW;
+            const long long base = ((row_of + t_lo) * p.heads + h0) * HD + 4 * c;
             bool ready = false;
             for (int i0 = warp * RPW + lane / LPR; !ready || i0 < rows; i0 += U * STEP) {
                 float4 a[U], b[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const int i = i0 + u * STEP;
-                    if (i < rows) {
-                        const float *x = p.q + ((row_of + t_lo + i / nh) * p.heads + h0 + i % nh) * HD + 4 * c;
+                    const int i = i0 + u * STEP, h = i & mask;
+                    if (i < rows && h0 + h < p.heads) {
+                        const float *x = p.q + base + ((long long)(i >> p.q_log) * p.heads + h) * HD;
                         a[u] = *(const float4 *)x;
                         b[u] = *(const float4 *)(x + HALF);
                     }
@@ -160,11 +160,10 @@ __global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_con
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const int i = i0 + u * STEP;
-                    if (i < rows) {
-                        const int t = t_lo + i / nh;
-                        rotate4(t, a[u], b[u]);
-                        float *y = p.q_out + ((row_of + t) * p.heads + h0 + i % nh) * HD + 4 * c;
+                    const int i = i0 + u * STEP, h = i & mask;
+                    if (i < rows && h0 + h < p.heads) {
+                        rotate4(t_lo + (i >> p.q_log), a[u], b[u]);
+                        float *y = p.q_out + base + ((long long)(i >> p.q_log) * p.heads + h) * HD;
                         *(float4 *)y = a[u];
                         *(float4 *)(y + HALF) = b[u];
                     }
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_con
             // A block that holds an infinity or NaN reads back as NaN throughout.
             const float top = __half2float(__ushort_as_half((uint16_t)most));
             const float scale = most >= 0x7c00u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(top, 127.0f);
-            const bool some = most > 0u && most < 0x7c00u;
+            const float inv = most > 0u && most < 0x7c00u ? __fdiv_rn(127.0f, top) : 0.0f;
             uint32_t *codes = (uint32_t *)(sq.base + (which ? at.v : at.k) +
                                            ((long long)h * sq.nb + blk) * (kQ8Block * HD));
 #pragma unroll
@@ -238,11 +237,21 @@ __global__ void __launch_bounds__(kThreads, 3) q8_append_kernel(const __grid_con
 #pragma unroll
                 for (int side = 0; side < 2; side++) {
                     const float2 u = __half22float2(x[it][2 * side]), v = __half22float2(x[it][2 * side + 1]);
-                    const float y[4] = {u.x, u.y, v.x, v.y};
+                    float y[4] = {u.x, u.y, v.x, v.y};
+                    if (inv == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
+                    // rint(y / scale) by the reciprocal, whose product is within 2^-15 of the
+                    // quotient (2^-22 of at most 127): only next to a tie is it divided
                     uint32_t q[4];
+                    bool near = false;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        q[i] = some ? (uint32_t)__float2int_rn(__fdiv_rn(y[i], scale)) : 0u;
+                        const float t = y[i] * inv, n = t + 12582912.0f;         // the integer in its low bits
+                        q[i] = __float_as_uint(n);
+                        near = near || fabsf(t - (n - 12582912.0f)) > 0.4999f;
+                    }
+                    if (near) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) q[i] = (uint32_t)__float2int_rn(__fdiv_rn(y[i], scale));
                     }
                     word[side] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                 }
@@ -313,11 +322,11 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant
         // 16 channels of a token
         const int panel = tid / (kQ8Block * 4), t = tid / 4 % kQ8Block, d = panel * 64 + tid % 4 * 16;
         if (tid < kQ8Block * HD / 16 && t >= lo && t < hi) {
-            uint2 *o = (uint2 *)(out + t * step + d);
-            o[0] = dequant4(w.x, scale);
-            o[1] = dequant4(w.y, scale);
-            o[2] = dequant4(w.z, scale);
-            o[3] = dequant4(w.w, scale);
+            uint4 *o = (uint4 *)(out + t * step + d);
+            const uint2 w0 = dequant4(w.x, scale), w1 = dequant4(w.y, scale);
+            const uint2 w2 = dequant4(w.z, scale), w3 = dequant4(w.w, scale);
+            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
+            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
         }
         return;
     }
@@ -648,16 +657,16 @@ cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_
 {
     // Heads share a block of the grid (and its sines and cosines) as long as the
     // launch still has a few blocks for every SM.
-    p.kv_chunk = 2;
-    p.q_chunk = 16;
+    p.kv_chunk = 4;
+    p.q_log = 4;
     auto rows = [&] {
         const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
-        const int qc = p.q ? (p.heads + p.q_chunk - 1) / p.q_chunk : 0;
+        const int qc = p.q ? (p.heads + (1 << p.q_log) - 1) >> p.q_log : 0;
         return 2 * kvc + qc;
     };
-    while (p.q_chunk > 2 && (long long)p.items * rows() < 8ll * sm_count) {
-        p.kv_chunk = 1;
-        p.q_chunk /= 2;
+    while (p.q_log > 1 && (long long)p.items * rows() < 8ll * sm_count) {
+        if (p.kv_chunk > 1) p.kv_chunk /= 2;
+        p.q_log--;
     }
     const dim3 grid((unsigned)p.items, (unsigned)rows());
     return hd == 128 ? launch(st, grid, kThreads, q8_append_kernel<128>, p) : launch(st, grid, kThreads, q8_append_kernel<64>, p);

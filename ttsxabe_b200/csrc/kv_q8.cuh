@@ -89,7 +89,7 @@ struct Q8AppendParams {
     const float *k, *v;
     const float *inv_freq;   // null: the rows come rotated
     int heads, kv_heads;
-    int kv_chunk, q_chunk;   // heads a block of the grid takes
+    int kv_chunk, q_log;     // heads a block of the grid takes: kv_chunk, or 1 << q_log of the query
 };
 cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count);
 

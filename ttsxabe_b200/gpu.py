@@ -641,9 +641,8 @@ class Gpu:
     @staticmethod
     def _tables_of(n: int, *tables) -> None:
         """Every host table must be as long as the batch that reads it."""
-        for t in tables:
-            if len(t) < n:
-                raise InvalidArgument(f"a sequence table of {len(t)} for a batch of {n}")
+        if min(map(len, tables)) < n:
+            raise InvalidArgument(f"a sequence table of {min(map(len, tables))} for a batch of {n}")
 
     def kv_alloc_q8(self, kv_heads, head_dim, cap) -> torch.Tensor:
         """A zeroed 8-bit cache."""
@@ -670,7 +669,8 @@ class Gpu:
         table = self._q8_table(caches, cap, kv_heads, head_dim)
         n = len(table)
         self._tables_of(n, cap, past, pos)
-        self._tables_of(n + 1, cu_seqlens)
+        if len(cu_seqlens) <= n:
+            raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if q_out is None:
             q_out = q
         _check(self._lib.llmtie_rope_append_q8(
@@ -687,12 +687,12 @@ class Gpu:
         table = self._q8_table(caches, cap, kv_heads, head_dim)
         n = len(table)
         self._tables_of(n, cap, live, first)
-        self._tables_of(n + 1, cu_seqlens)
-        total = int(cu_seqlens[n]) * kv_heads * head_dim
+        if len(cu_seqlens) <= n:
+            raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if k_out is None:
-            k_out = self._empty(total, torch.float16)
+            k_out = self._empty(cu_seqlens[n] * kv_heads * head_dim, torch.float16)
         if v_out is None:
-            v_out = self._empty(total, torch.float16)
+            v_out = self._empty(cu_seqlens[n] * kv_heads * head_dim, torch.float16)
         _check(self._lib.llmtie_cache_read_q8(
             self._h, table, self._i32_table(cap), self._i32_table(live), self._i32_table(first),
             self._i32_table(cu_seqlens), n, kv_heads, head_dim, k_out.data_ptr(), k_out.numel(),
@@ -733,7 +733,8 @@ class Gpu:
         table = self._q8_table(caches, cap, kv_heads, head_dim)
         n = len(table)
         self._tables_of(n, cap, past)
-        self._tables_of(n + 1, cu_seqlens)
+        if len(cu_seqlens) <= n:
+            raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if out is None:
             out = self.uninit(int(cu_seqlens[n]) * heads * head_dim)
         _check(self._lib.llmtie_flash_attn_q8(
