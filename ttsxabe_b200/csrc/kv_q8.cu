@@ -407,13 +407,30 @@ __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_consta
     }
     const int tail = sq.live & 31;
     if (tail && full >= blk0 && full < blk0 + kUnpack) {
-        const uint16_t *kt = (const uint16_t *)(sq.base + at.kt) + (long long)h * kQ8Block * HD;
-        const uint16_t *vt = (const uint16_t *)(sq.base + at.vt) + (long long)h * kQ8Block * HD;
-        const int upto = sq.cap16 - 32 * full;                   // (and zeros up to the capacity)
-        for (int i = tid; i < upto * HD; i += kThreads) {
-            ko[(long long)32 * full * HD + i] = i < tail * HD ? kt[i] : (uint16_t)0;
-            const int d = i / upto, t = i % upto;
-            vo[(long long)d * sq.cap16 + 32 * full + t] = t < tail ? vt[t * HD + d] : (uint16_t)0;
+        // the tail's rows, and zeros up to the capacity, a multiple of eight
+        __shared__ uint32_t rows[kQ8Block][HD / 2 + 1];
+        const uint4 *kt = (const uint4 *)(sq.base + at.kt) + (long long)h * PER * 2;
+        const uint4 *vt = (const uint4 *)(sq.base + at.vt) + (long long)h * PER * 2;
+        const int upto = sq.cap16 - 32 * full;
+        for (int i = tid; i < 2 * PER; i += kThreads) {
+            const int t = i / (HD / 8), d = i % (HD / 8);
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u), k = t < tail ? kt[i] : zero, v = t < tail ? vt[i] : zero;
+            if (t < upto) ((uint4 *)(ko + (long long)32 * full * HD))[i] = k;
+            rows[t][4 * d] = v.x;
+            rows[t][4 * d + 1] = v.y;
+            rows[t][4 * d + 2] = v.z;
+            rows[t][4 * d + 3] = v.w;
+        }
+        __syncthreads();
+        for (int i = tid; i < HD * 4; i += kThreads) {
+            const int d = i / 4, t = i % 4 * 8;                  // eight tokens of a channel
+            if (t >= upto) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                w[e] = __byte_perm(rows[t + 2 * e][d / 2], rows[t + 2 * e + 1][d / 2], d % 2 ? 0x7632 : 0x5410);
+            }
+            *(uint4 *)(vo + (long long)d * sq.cap16 + 32 * full + t) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
@@ -496,11 +513,30 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
     bool chosen = false;                                         // (few blocks: this thread's own stays)
     const bool few = sq.full <= kPickThreads;
     after_previous();
+    // Everything whose address is known is asked for first: the first tile's
+    // weights and scales, and the tail's rows of this head.
+    const float *ks = (const float *)(sq.src + a.ks) + sb, *vs = (const float *)(sq.src + a.vs) + sb;
+    float wi = 0.0f, kscale = 0.0f, vscale = 0.0f;
+    if (tid < sq.full) {
+        wi = w[tid];
+        kscale = ks[tid];
+        vscale = vs[tid];
+    }
+    if (sq.dst != sq.src) {
+        const int n = sq.tail * hd / 8;                          // 16-byte pieces, no more than 512
+        const uint4 *kt = (const uint4 *)(sq.src + a.kt) + (long long)h * (kQ8Block * hd / 8);
+        const uint4 *vt = (const uint4 *)(sq.src + a.vt) + (long long)h * (kQ8Block * hd / 8);
+        if (tid < n) {
+            const uint4 x = kt[tid], y = vt[tid];
+            ((uint4 *)(sq.dst + z.kt))[(long long)h * (kQ8Block * hd / 8) + tid] = x;
+            ((uint4 *)(sq.dst + z.vt))[(long long)h * (kQ8Block * hd / 8) + tid] = y;
+        }
+    }
     if (!all && room > 0) {
         const bool held = sq.full <= kPickKeys;
         if (held) {
-            for (int i = tid; i < (few ? (sq.full + 3) / 4 * 4 : sq.full); i += kPickThreads) {
-                keys[i] = i >= lo && i < hi ? weight_key(w[i]) : 0u;
+            for (int i = tid; i < (sq.full + 3) / 4 * 4; i += kPickThreads) {
+                keys[i] = i >= lo && i < hi ? weight_key(i == tid ? wi : w[i]) : 0u;
             }
             __syncthreads();
         }
@@ -558,11 +594,13 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
         const int i = i0 + tid;
         const bool in = i < sq.full;
         const bool safe = in && (all || i < lo || i >= hi);
-        float wi = 0.0f, kscale = 0.0f, vscale = 0.0f;
-        if (in) {
-            wi = w[i];
-            kscale = ((const float *)(sq.src + a.ks))[sb + i];
-            vscale = ((const float *)(sq.src + a.vs))[sb + i];
+        // the next tile's are asked for before this one's are written: they lie above
+        const int next = i + kPickThreads;
+        float w_next = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+        if (next < sq.full) {
+            w_next = w[next];
+            ks_next = ks[next];
+            vs_next = vs[next];
         }
         const uint32_t k = weight_key(wi);
         const bool sure = safe || (few ? chosen : in && k > key);
@@ -583,17 +621,9 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
             ((float *)(sq.dst + z.vs))[db + to] = vscale;
             ((float *)(sq.dst + z.w))[db + to] = wi;
         }
-    }
-    if (sq.dst != sq.src) {
-        const int n = sq.tail * hd;                              // tail rows of this head
-        const uint16_t *kt = (const uint16_t *)(sq.src + a.kt) + (long long)h * kQ8Block * hd;
-        const uint16_t *vt = (const uint16_t *)(sq.src + a.vt) + (long long)h * kQ8Block * hd;
-        uint16_t *ko = (uint16_t *)(sq.dst + z.kt) + (long long)h * kQ8Block * hd;
-        uint16_t *vo = (uint16_t *)(sq.dst + z.vt) + (long long)h * kQ8Block * hd;
-        for (int i = tid; i < n; i += kPickThreads) {
-            ko[i] = kt[i];
-            vo[i] = vt[i];
-        }
+        wi = w_next;
+        kscale = ks_next;
+        vscale = vs_next;
     }
 }
 
@@ -658,13 +688,13 @@ cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_
     // Heads share a block of the grid (and its sines and cosines) as long as the
     // launch still has a few blocks for every SM.
     p.kv_chunk = 4;
-    p.q_log = 4;
+    p.q_log = 3;
     auto rows = [&] {
         const int kvc = (p.kv_heads + p.kv_chunk - 1) / p.kv_chunk;
         const int qc = p.q ? (p.heads + (1 << p.q_log) - 1) >> p.q_log : 0;
         return 2 * kvc + qc;
     };
-    while (p.q_log > 1 && (long long)p.items * rows() < 8ll * sm_count) {
+    while (p.q_log > 1 && (long long)p.items * rows() < 4ll * sm_count) {
         if (p.kv_chunk > 1) p.kv_chunk /= 2;
         p.q_log--;
     }
