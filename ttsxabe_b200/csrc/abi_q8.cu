@@ -388,7 +388,7 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
             units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
             blocks += (long long)(t / kQ8Block) * (long long)kv_heads;
         }
-        if (units > 0x7fffffffll) return llmtie_fail(LLMTIE_ERR_INVALID, "a launch over %lld blocks of the caches", units);
+        if (units > 0x3fffffffll) return llmtie_fail(LLMTIE_ERR_INVALID, "a launch over %lld blocks of the caches", units);
         p.unit0[p.nseq] = (int)units;
         p.heads = (int)heads;
         p.kv_heads = (int)kv_heads;
@@ -403,8 +403,12 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
         // merging than it saves.
         const int most = g->sm_count * decode_q8_resident((int)head_dim);
         const int grid = (int)std::min<long long>(most, (units + 3) / 4);
-        p.each = grid ? (int)(units / grid) : 0;
-        p.more = grid ? (int)(units % grid) : 0;
+        // A run costs about what 16 more blocks would (its query, its merge); where the
+        // shares are so short that a pair is many blocks' anyway, nothing is charged.
+        p.over = grid && units / grid >= 8 ? 16 : 0;
+        const long long shares = units + (long long)p.over * p.nseq * (long long)kv_heads;
+        p.each = grid ? (int)(shares / grid) : 0;
+        p.more = grid ? (int)(shares % grid) : 0;
         const size_t pairs = (size_t)p.nseq * kv_heads;
         cudaError_t err;
         const size_t slots = (size_t)std::max(grid, 1) * 2 * 8;

@@ -102,6 +102,15 @@ __device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // One run of a block of the grid: blocks [first, last) of one pair, and its
 // tail if the run reaches the pair's end.
 struct Run {
@@ -114,6 +123,15 @@ struct Run {
     int next;             // unit after the run
 };
 
+// A pair that several blocks of the grid hold (units 0: none).
+struct Shared {
+    int seq, head, begin, units;
+};
+__device__ __forceinline__ Shared pick(bool second, const Shared &a, const Shared &b)
+{
+    return {second ? b.seq : a.seq, second ? b.head : a.head, second ? b.begin : a.begin, second ? b.units : a.units};
+}
+
 __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
 {
     int lo = 0, hi = p.nseq - 1;
@@ -125,9 +143,9 @@ __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
     Run r;
     const int live = p.seq[lo].live;
     const int full = live >> 5;
-    r.units = (live + 31) >> 5;                                 // never 0 here: such a sequence has no units
+    r.units = (live + 31) >> 5;                                 // (0 only where the block has no units)
     r.seq = lo;
-    r.head = (int)((unsigned)(u - p.unit0[lo]) / (unsigned)r.units);
+    r.head = (int)((unsigned)(u - p.unit0[lo]) / (unsigned)max(1, r.units));
     r.begin = p.unit0[lo] + r.head * r.units;
     r.first = u - r.begin;
     const int stop = min(r.units, end - r.begin);
@@ -138,16 +156,31 @@ __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
     return r;
 }
 
-// The cut: the first `more` blocks of the grid take each + 1 units, the others each.
+// The cut is one of virtual units: a pair is its units behind `over` more that
+// stand for what a run costs besides its blocks. A block of the grid whose share
+// starts among those takes the pair from its first unit, one whose share ends
+// there stops at the pair before; a share of nothing else is empty. The first
+// `more` blocks take each + 1, the others each.
 __device__ __forceinline__ int first_unit(const DecodeQ8Params &p, int block)
 {
-    return block * p.each + min(block, p.more);
+    const int v = block * p.each + min(block, p.more);
+    int lo = 0, hi = p.nseq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.unit0[mid] + p.over * mid * p.kv_heads <= v) lo = mid;
+        else hi = mid - 1;
+    }
+    const int units = (p.seq[lo].live + 31) >> 5;
+    if (units == 0) return p.unit0[lo];                         // (only past the last unit)
+    const int in = v - p.unit0[lo] - p.over * lo * p.kv_heads;
+    const int pair = (int)((unsigned)in / (unsigned)(units + p.over));
+    return p.unit0[lo] + pair * units + max(0, in - pair * (units + p.over) - p.over);
 }
-// The block of the grid that holds unit u.
-__device__ __forceinline__ int block_of(const DecodeQ8Params &p, int u)
+// The block of the grid that holds unit u, of pair number `pair` of the launch.
+__device__ __forceinline__ int block_of(const DecodeQ8Params &p, int u, int pair)
 {
-    const int seam = p.more * (p.each + 1);
-    return u < seam ? (int)((unsigned)u / (unsigned)(p.each + 1)) : p.more + (int)((unsigned)(u - seam) / (unsigned)p.each);
+    const int v = u + p.over * (pair + 1), seam = p.more * (p.each + 1);
+    return v < seam ? (int)((unsigned)v / (unsigned)(p.each + 1)) : p.more + (int)((unsigned)(v - seam) / (unsigned)p.each);
 }
 
 template <int HD>
@@ -169,17 +202,17 @@ __device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at,
 // the latency of its loads): what each complete block's tokens got, summed over
 // the group's heads; `fin` has each row's maximum and the inverse of its sum.
 template <int HD>
-__device__ __forceinline__ void weigh(const DecodeQ8Params &p, const Run *pair, bool both, const float2 *fin, int tid, int group)
+__device__ __forceinline__ void weigh(const DecodeQ8Params &p, int seq0, int head0, int seq1, int head1, const float2 *fin,
+                                      int tid, int group)
 {
-    const int full0 = p.seq[pair[0].seq].live >> 5, total = full0 + (both ? p.seq[pair[1].seq].live >> 5 : 0);
+    const int full0 = p.seq[seq0].live >> 5, total = full0 + (seq1 >= 0 ? p.seq[seq1].live >> 5 : 0);
     for (int i = tid; i < total; i += kThreads) {
         const bool second = i >= full0;
-        const Run &now = pair[second];
-        const int b = second ? i - full0 : i;
-        const DecodeQ8Seq &sq = p.seq[now.seq];
+        const int b = second ? i - full0 : i, seq = second ? seq1 : seq0, head = second ? head1 : head0;
+        const DecodeQ8Seq &sq = p.seq[seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
-        float *weight = (float *)(sq.base + at.w) + (long long)now.head * sq.nb + b;
-        const float2 *st = p.stats + (p.stat0[now.seq] + (long long)now.head * (sq.live >> 5) + b) * kRows;
+        float *weight = (float *)(sq.base + at.w) + (long long)head * sq.nb + b;
+        const float2 *st = p.stats + (p.stat0[seq] + (long long)head * (sq.live >> 5) + b) * kRows;
         const float2 *f = fin + (second ? group : 0);
         float2 y[kRows];
         const float before = *weight;
@@ -294,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     // is read until it has ended.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (u_begin >= u_end) return;        // (a share that was all charges)
     load_run();
 
     int issued = 0, used = 0;
@@ -321,8 +355,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     for (int s = 0; s < G::STAGES; s++) fetch();
 
     bool ok = true, is_first = true;
-    Run pending[2];
-    pending[0].units = pending[1].units = 0;
+    Shared shared0 = {0, 0, 0, 0}, shared1 = {0, 0, 0, 0};       // of the first run and the last
     for (;;) {
         const DecodeQ8Seq &sq = p.seq[run.seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
@@ -341,9 +374,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const float top = __uint_as_float(most);
-            // (an infinity or NaN in the row makes every score NaN)
-            const bool some = most > 0u && most < 0x7f800000u;
-            f_q = some ? top * (1.0f / 32639.0f) * p.sl2 : (most ? __uint_as_float(0x7fffffffu) : 0.0f);
+            // (an infinity or NaN in the row makes every score NaN; a row of nothing
+            // above 1e-30 scores nothing)
+            const bool some = top > 1e-30f && most < 0x7f800000u;
+            f_q = some ? top * (1.0f / 32639.0f) * p.sl2 : (most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : 0.0f);
             const float inv = some ? 32639.0f / top : 0.0f;
 #pragma unroll
             for (int j = 0; j < PANELS; j++) {
@@ -362,44 +396,47 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             }
         }
 
-        // -- the warp's part of the tail, in f32: what its sums start from
-        float acc[NT][2];
-#pragma unroll
-        for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0f;
+        // -- the warp's part of the tail: what its sums start from. The keys are f16 and
+        // so is the query, as two parts again: x / f_q's top = hi + lo to 2^-22, hi as
+        // rows 0-7 and lo as rows 8-15 of A, both in the lane that holds x already
         float m = -CUDART_INF_F, l = 0.0f;       // reference maximum of row r; this lane's part of the sum
+        float acc[NT][2];
         if (tail_n > 0) {
+            const float unit = f_q * 32639.0f, over = f_q != 0.0f ? p.sl2 / unit : 0.0f;   // sl2 top, 1 / top
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < PANELS; j++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t a[4];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float y0 = x[j][4 * k + 2 * i] * over, y1 = x[j][4 * k + 2 * i + 1] * over;
+                        const __half2 hi = __floats2half2_rn(y0, y1);
+                        const __half2 lo = __floats2half2_rn(y0 - __low2float(hi), y1 - __high2float(hi));
+                        a[2 * i] = *(const uint32_t *)&hi;
+                        a[2 * i + 1] = *(const uint32_t *)&lo;
+                    }
+                    const uint4 kk = tk[j][k / 2];
+                    mma_f16(d, a[0], a[1], a[2], a[3], k % 2 ? kk.z : kk.x, k % 2 ? kk.w : kk.y);
+                }
+            }
+            // row r against tokens 2 c and 2 c + 1
+            const float s0 = 2 * c < tail_n ? (d[0] + d[2]) * unit : -CUDART_INF_F;
+            const float s1 = 2 * c + 1 < tail_n ? (d[1] + d[3]) * unit : -CUDART_INF_F;
+            m = fmaxf(s0, s1);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float e0 = 2 * c < tail_n ? ex2(s0 - m) : 0.0f, e1 = 2 * c + 1 < tail_n ? ex2(s1 - m) : 0.0f;
+            l = e0 + e1;
             float *mine = merge + warp * kRows * HD;
             for (int g = 0; g < group; g++) {
-                // lane (r, c): chunk c of token r's key against that of row g's query, which
-                // lane (g, c) holds (read again from memory it would wait behind the ring)
-                float s = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2 * PANELS; i++) {
-                    const uint4 kk = tk[i / 2][i % 2];
-                    const float2 k4[4] = {__half22float2(*(const __half2 *)&kk.x), __half22float2(*(const __half2 *)&kk.y),
-                                          __half22float2(*(const __half2 *)&kk.z), __half22float2(*(const __half2 *)&kk.w)};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        s = fmaf(__shfl_sync(0xffffffffu, x[i / 2][8 * (i % 2) + 2 * e], 4 * g + c), k4[e].x, s);
-                        s = fmaf(__shfl_sync(0xffffffffu, x[i / 2][8 * (i % 2) + 2 * e + 1], 4 * g + c), k4[e].y, s);
-                    }
-                }
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                s = r < tail_n ? s * p.sl2 : -CUDART_INF_F;
-                float top = s;
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float e = r < tail_n ? ex2(s - top) : 0.0f;
-                float sum = e;
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 float o4[V];
 #pragma unroll
                 for (int i = 0; i < V; i++) o4[i] = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 8; t++) {
-                    const float w = __shfl_sync(0xffffffffu, e, 4 * t);
+                    const float w = __shfl_sync(0xffffffffu, t % 2 ? e1 : e0, 4 * g + t / 2);
                     const float2 v0 = __half22float2(*(const __half2 *)&tv[t].x);
                     o4[0] = fmaf(w, v0.x, o4[0]);
                     o4[1] = fmaf(w, v0.y, o4[1]);
@@ -412,21 +449,18 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 // channels V lane .. of row g, where the fragment layout finds them
 #pragma unroll
                 for (int i = 0; i < V; i++) mine[g * HD + 8 * ((V * lane / 8) ^ g) + V * lane % 8 + i] = o4[i];
-                if (r == g) {
-                    m = top;
-                    l = c == 0 ? sum : 0.0f;
-                }
             }
             __syncwarp();
-            if (r < group) {
 #pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const float2 y = *(const float2 *)(mine + r * HD + 8 * (i ^ r) + 2 * c);
-                    acc[i][0] = y.x;
-                    acc[i][1] = y.y;
-                }
+            for (int i = 0; i < NT; i++) {
+                const float2 y = r < group ? *(const float2 *)(mine + r * HD + 8 * (i ^ r) + 2 * c) : make_float2(0.f, 0.f);
+                acc[i][0] = y.x;
+                acc[i][1] = y.y;
             }
             __syncwarp();
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0f;
         }
 
         // -- the warp's blocks
@@ -573,10 +607,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (now.whole) {
             if (p.stats) {
                 __syncthreads();
-                weigh<HD>(p, &now, false, final_s, tid, group);
+                weigh<HD>(p, now.seq, now.head, -1, 0, final_s, tid, group);
             }
+        } else if (is_first) {
+            shared0 = {now.seq, now.head, now.begin, now.units};
         } else {
-            pending[is_first ? 0 : 1] = now;
+            shared1 = {now.seq, now.head, now.begin, now.units};
         }
         if (!more) break;
         is_first = false;
@@ -589,11 +625,12 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     __syncthreads();
     if (tid < 2) {
         last_s[tid] = 0;
-        const Run &now = tid ? pending[1] : pending[0];
+        const Shared now = pick(tid != 0, shared0, shared1);
         if (now.units > 0) {
-            const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
+            const int pair = now.seq * p.kv_heads + now.head;
+            const int b0 = block_of(p, now.begin, pair), b1 = block_of(p, now.begin + now.units - 1, pair);
             // (releases what the barrier ordered before it, acquires the others')
-            unsigned *ctr = &p.ctr[now.seq * p.kv_heads + now.head], seen;
+            unsigned *ctr = &p.ctr[pair], seen;
             asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(ctr) : "memory");
             last_s[tid] = seen == (unsigned)(b1 - b0);
             if (last_s[tid]) *ctr = 0u;
@@ -604,9 +641,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     for (int item = warp; item < 2 * group; item += kWarps) {
         if (!last_s[item >= group]) continue;
         const int row = item >= group ? item - group : item;
-        const Run &now = pending[item >= group];
+        const Shared now = pick(item >= group, shared0, shared1);
         const long long row0 = (long long)now.seq * p.heads + (long long)now.head * group;
-        const int b0 = block_of(p, now.begin), b1 = block_of(p, now.begin + now.units - 1);
+        const int pair = now.seq * p.kv_heads + now.head;
+        const int b0 = block_of(p, now.begin, pair), b1 = block_of(p, now.begin + now.units - 1, pair);
         // The contributors in order, whoever came last: the same bits every time. A
         // block's first run has slot 0, and only b0 may hold the pair in its last.
         const int skew = first_unit(p, b0) >= now.begin ? 0 : 1;
@@ -665,8 +703,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     }
     if (p.stats && (last_s[0] || last_s[1])) {
         __syncthreads();
-        const int e = last_s[0] ? 0 : 1;
-        weigh<HD>(p, pending + e, last_s[0] && last_s[1], final_s + e * group, tid, group);
+        weigh<HD>(p, last_s[0] ? shared0.seq : shared1.seq, last_s[0] ? shared0.head : shared1.head,
+                  last_s[0] && last_s[1] ? shared1.seq : -1, shared1.head, final_s + (last_s[0] ? 0 : group), tid, group);
     }
     if (!ok) {
         // a wait gave up: leave the copies still in flight time to land

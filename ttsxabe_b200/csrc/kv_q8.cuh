@@ -167,7 +167,7 @@ struct DecodeQ8Seq {
 struct DecodeQ8Params {
     DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
     int unit0[LLMTIE_Q8_MAX_SEQ + 1];                  // first 32-token unit of each sequence
-    int each, more;                                    // units a block of the grid takes; the first `more` one more
+    int each, more, over;                              // the cut over the grid: see first_unit in decode_q8.cu
     long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
     int nseq, heads, kv_heads;
     const float *q;          // [seq][heads*hd]

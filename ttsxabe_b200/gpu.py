@@ -666,9 +666,11 @@ class Gpu:
         """Rotates and appends packed rows (see include/llmtie_b200.h). `q` is
         rotated in place unless `q_out` is given; it may be None, as may
         `inv_freq`, with which nothing is rotated."""
-        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        table = (caches if isinstance(caches, C.Array)
+                 else self._q8_table(caches, cap, kv_heads, head_dim))
         n = len(table)
-        self._tables_of(n, cap, past, pos)
+        if len(cap) < n or len(past) < n or len(pos) < n:
+            self._tables_of(n, cap, past, pos)
         if len(cu_seqlens) <= n:
             raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if q_out is None:
@@ -684,9 +686,11 @@ class Gpu:
                       v_out=None):
         """Tokens of 8-bit caches as the f16 values they stand for: packed rows
         [kv_heads*head_dim] of keys and of values."""
-        table = self._q8_table(caches, cap, kv_heads, head_dim)
+        table = (caches if isinstance(caches, C.Array)
+                 else self._q8_table(caches, cap, kv_heads, head_dim))
         n = len(table)
-        self._tables_of(n, cap, live, first)
+        if len(cap) < n or len(live) < n or len(first) < n:
+            self._tables_of(n, cap, live, first)
         if len(cu_seqlens) <= n:
             raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if k_out is None:
@@ -716,13 +720,16 @@ class Gpu:
                           scratch: DecodeScratch, out=None, weigh=False) -> torch.Tensor:
         """`decode_batched` over 8-bit caches; `out` may be f32 (as by default) or
         f16. `weigh` adds to the caches' block weights."""
-        table = self._q8_table(caches, cap, kv_heads, head_dim)
-        self._tables_of(len(table), cap, live)
+        table = (caches if isinstance(caches, C.Array)
+                 else self._q8_table(caches, cap, kv_heads, head_dim))
+        n = len(table)
+        if len(cap) < n or len(live) < n:
+            self._tables_of(n, cap, live)
         if out is None:
-            out = self.uninit(len(table) * heads * head_dim)
+            out = self.uninit(n * heads * head_dim)
         _check(self._lib.llmtie_decode_batched_q8(
             self._h, q.data_ptr(), q.numel(), table, self._i32_table(live), self._i32_table(cap),
-            len(table), heads, kv_heads, head_dim, scale, int(bool(weigh)), scratch._bind(self),
+            n, heads, kv_heads, head_dim, scale, int(bool(weigh)), scratch._bind(self),
             out.data_ptr(), out.numel(), self._f16_out(out)))
         return out
 
