@@ -213,6 +213,7 @@ extern "C" void llmtie_close(llmtie_gpu *g)
     if (g->ws_rope.ptr) cudaFreeAsync(g->ws_rope.ptr, g->stream);
     if (g->ws_part.ptr) cudaFreeAsync(g->ws_part.ptr, g->stream);
     if (g->ws_kv16.ptr) cudaFreeAsync(g->ws_kv16.ptr, g->stream);
+    llmtie_decode_scratch_free(g, g->q8_scratch);
     workspace_free(g->ws_q8, g->stream);
     workspace_free(g->ws_q8_part, g->stream);
     if (g->stream) cudaStreamSynchronize(g->stream);

@@ -80,6 +80,81 @@ llmtie_status check_rows(const int32_t *cu, size_t batch, size_t *total)
         if (try_s != LLMTIE_OK) return try_s; \
     } while (0)
 
+// How the decode kernel would go over jobs [b0, b0 + LLMTIE_Q8_MAX_SEQ).
+llmtie_status plan_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, size_t b0, size_t kv_heads, size_t head_dim,
+                        DecodeQ8Plan &plan)
+{
+    int per[LLMTIE_Q8_MAX_SEQ], clusters[2];
+    const int n = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, jobs.size() - b0);
+    for (int b = 0; b < n; b++) per[b] = (jobs[b0 + b].live + kQ8Block - 1) / kQ8Block;
+    const cudaError_t e = decode_q8_clusters((int)head_dim, clusters);
+    if (e != cudaSuccess) return llmtie_driver_fail("decode_q8", e);
+    plan_decode_q8(plan, per, n, (int)kv_heads, (int)head_dim, g->sm_count, clusters);
+    return LLMTIE_OK;
+}
+
+// The decode kernel over any number of jobs, LLMTIE_Q8_MAX_SEQ a launch.
+llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, const float *q, void *out, int32_t out_f16,
+                       size_t heads, size_t kv_heads, size_t head_dim, float scale, int32_t causal, int32_t weigh,
+                       llmtie_decode_scratch *scratch)
+{
+    for (size_t b0 = 0; b0 < jobs.size(); b0 += LLMTIE_Q8_MAX_SEQ) {
+        DecodeQ8Params p;
+        memset(&p, 0, sizeof(p));
+        p.nseq = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, jobs.size() - b0);
+        long long units = 0, blocks = 0;
+        for (int b = 0; b < p.nseq; b++) {
+            p.seq[b] = jobs[b0 + b];
+            const int t = p.seq[b].live;
+            p.unit0[b] = (int)units;
+            p.stat0[b] = blocks;
+            units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
+            blocks += (long long)p.seq[b].full * (long long)kv_heads;
+        }
+        p.causal = causal ? 1 : 0;
+        p.q = q;
+        p.out = out;
+        if (units > 0x3fffffffll) return llmtie_fail(LLMTIE_ERR_INVALID, "a launch over %lld blocks of the caches", units);
+        p.unit0[p.nseq] = (int)units;
+        p.heads = (int)heads;
+        p.kv_heads = (int)kv_heads;
+        p.out_f16 = out_f16 ? 1 : 0;
+        p.sl2 = scale * kLog2e;
+        p.status = g->timeout_site;
+        p.wait_cycles = g->wait_cycles;
+        DecodeQ8Plan plan;
+        TRY(plan_jobs(g, jobs, b0, kv_heads, head_dim, plan));
+        cudaError_t err;
+        const int grid = plan.grid;
+        p.cluster = plan.cluster;
+        p.over = plan.over;
+        const long long shares = units + (long long)p.over * p.nseq * (long long)kv_heads;
+        p.each = grid ? (int)(shares / grid) : 0;
+        p.more = grid ? (int)(shares % grid) : 0;
+        const size_t pairs = (size_t)p.nseq * kv_heads;
+        const size_t slots = (size_t)std::max(p.cluster ? 1 : grid, 1) * 2 * 8;
+        p.part_o = (float *)workspace_reserve(scratch->q8_part, slots * (head_dim + 2) * sizeof(float), g->stream, &err);
+        if (!p.part_o) return llmtie_driver_fail("allocating", err);
+        p.part_ml = (float2 *)(p.part_o + slots * head_dim);
+        const size_t had = scratch->q8_ctr.bytes;
+        p.ctr = (unsigned *)workspace_reserve(scratch->q8_ctr, pairs * sizeof(unsigned), g->stream, &err);
+        if (!p.ctr) return llmtie_driver_fail("allocating", err);
+        if (scratch->q8_ctr.bytes != had) {
+            err = cudaMemsetAsync(p.ctr, 0, scratch->q8_ctr.bytes, g->stream);
+            if (err != cudaSuccess) return llmtie_driver_fail("zeroing", err);
+        }
+        if (weigh && blocks > 0) {
+            p.stats = (float2 *)workspace_reserve(scratch->q8_stats, (size_t)blocks * 8 * sizeof(float2), g->stream, &err);
+            if (!p.stats) return llmtie_driver_fail("allocating", err);
+        }
+        LaunchScope ls(g, head_dim == 128 ? "decode_q8_128" : "decode_q8_64");
+        err = launch_decode_q8(g->stream, p, (int)head_dim, grid);
+        if (err != cudaSuccess) return llmtie_driver_fail("decode_q8", err);
+        TRY(ls.done());
+    }
+    return LLMTIE_OK;
+}
+
 }  // namespace
 
 extern "C" size_t llmtie_kv_q8_bytes(size_t kv_heads, size_t head_dim, size_t cap)
@@ -375,63 +450,11 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
         if (weigh) spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
     }
     TRY(check_apart(spans));
-    for (size_t b0 = 0; b0 < batch; b0 += LLMTIE_Q8_MAX_SEQ) {
-        DecodeQ8Params p;
-        memset(&p, 0, sizeof(p));
-        p.nseq = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, batch - b0);
-        long long units = 0, blocks = 0;
-        for (int b = 0; b < p.nseq; b++) {
-            const int32_t t = live[b0 + b];
-            p.seq[b] = {(unsigned char *)caches[b0 + b], cap[b0 + b] / kQ8Block, t};
-            p.unit0[b] = (int)units;
-            p.stat0[b] = blocks;
-            units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
-            blocks += (long long)(t / kQ8Block) * (long long)kv_heads;
-        }
-        if (units > 0x3fffffffll) return llmtie_fail(LLMTIE_ERR_INVALID, "a launch over %lld blocks of the caches", units);
-        p.unit0[p.nseq] = (int)units;
-        p.heads = (int)heads;
-        p.kv_heads = (int)kv_heads;
-        p.q = q + b0 * n;
-        p.out = out_f16 ? (void *)((uint16_t *)out + b0 * n) : (void *)((float *)out + b0 * n);
-        p.out_f16 = out_f16 ? 1 : 0;
-        p.sl2 = scale * kLog2e;
-        p.status = g->timeout_site;
-        p.wait_cycles = g->wait_cycles;
-        // As many blocks of the grid as fit the device at once, and never fewer
-        // than four cache blocks for one, a warp each: a finer cut spends longer
-        // merging than it saves.
-        const int most = g->sm_count * decode_q8_resident((int)head_dim);
-        const int grid = (int)std::min<long long>(most, (units + 3) / 4);
-        // A run costs about what 16 more blocks would (its query, its merge); where the
-        // shares are so short that a pair is many blocks' anyway, nothing is charged.
-        p.over = grid && units / grid >= 8 ? 16 : 0;
-        const long long shares = units + (long long)p.over * p.nseq * (long long)kv_heads;
-        p.each = grid ? (int)(shares / grid) : 0;
-        p.more = grid ? (int)(shares % grid) : 0;
-        const size_t pairs = (size_t)p.nseq * kv_heads;
-        cudaError_t err;
-        const size_t slots = (size_t)std::max(grid, 1) * 2 * 8;
-        p.part_o = (float *)workspace_reserve(scratch->q8_part, slots * (head_dim + 2) * sizeof(float), g->stream, &err);
-        if (!p.part_o) return llmtie_driver_fail("allocating", err);
-        p.part_ml = (float2 *)(p.part_o + slots * head_dim);
-        const size_t had = scratch->q8_ctr.bytes;
-        p.ctr = (unsigned *)workspace_reserve(scratch->q8_ctr, pairs * sizeof(unsigned), g->stream, &err);
-        if (!p.ctr) return llmtie_driver_fail("allocating", err);
-        if (scratch->q8_ctr.bytes != had) {
-            err = cudaMemsetAsync(p.ctr, 0, scratch->q8_ctr.bytes, g->stream);
-            if (err != cudaSuccess) return llmtie_driver_fail("zeroing", err);
-        }
-        if (weigh && blocks > 0) {
-            p.stats = (float2 *)workspace_reserve(scratch->q8_stats, (size_t)blocks * 8 * sizeof(float2), g->stream, &err);
-            if (!p.stats) return llmtie_driver_fail("allocating", err);
-        }
-        LaunchScope ls(g, head_dim == 128 ? "decode_q8_128" : "decode_q8_64");
-        err = launch_decode_q8(g->stream, p, (int)head_dim, grid);
-        if (err != cudaSuccess) return llmtie_driver_fail("decode_q8", err);
-        TRY(ls.done());
+    std::vector<DecodeQ8Seq> jobs(batch);
+    for (size_t b = 0; b < batch; b++) {
+        jobs[b] = {(unsigned char *)caches[b], cap[b] / kQ8Block, live[b] / kQ8Block, live[b], (int)b, 1};
     }
-    return LLMTIE_OK;
+    return run_jobs(g, jobs, q, out, out_f16, heads, kv_heads, head_dim, scale, 1, weigh, scratch);
 }
 
 extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len, const int32_t *cu_seqlens,
@@ -455,6 +478,45 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
         if (rows == 0) continue;
         TRY(check_cache(caches[b], cap[b], past[b] < 0 ? -1 : (long long)past[b] + rows));
     }
+    // Sequences of few rows may go through the decode kernel, which reads their codes
+    // as they lie, as a job for every eight rows of a group: where that is estimated to
+    // take less than unpacking them, 13 us for a launch and a microsecond for every 77
+    // cache blocks (155 at head_dim 64) as measured. (8 x 512 tokens, 32 / 8 heads x
+    // 128: 8 rows 9 against 26 us, 32 rows 31 against 27.)
+    const size_t group = heads / kv_heads;
+    constexpr int kMostJobs = 16;
+    std::vector<DecodeQ8Seq> jobs;
+    std::vector<char> few(batch, 0);
+    double unpacked = 0.0, decoded = 0.0;
+    bool others = false;
+    for (size_t b = 0; b < batch; b++) {
+        const int rows = cu_seqlens[b + 1] - cu_seqlens[b], each = group <= 8 ? (int)(8 / group) : 0;
+        if (rows == 0) continue;
+        if (each == 0 || (rows + each - 1) / each > kMostJobs) {
+            others = true;                                  // (there is such a launch anyway)
+            continue;
+        }
+        few[b] = 1;
+        unpacked += (double)((past[b] + rows + kQ8Block - 1) / kQ8Block) * (double)kv_heads / (head_dim == 128 ? 77.0 : 155.0);
+        for (int r = 0; r < rows; r += each) {
+            const int n = std::min(each, rows - r);
+            jobs.push_back({(unsigned char *)caches[b], cap[b] / kQ8Block, (past[b] + rows) / kQ8Block,
+                            past[b] + (causal ? r + n : rows), cu_seqlens[b] + r, n});
+        }
+    }
+    for (size_t j = 0; j < jobs.size(); j += LLMTIE_Q8_MAX_SEQ) {
+        DecodeQ8Plan plan;
+        TRY(plan_jobs(g, jobs, j, kv_heads, head_dim, plan));
+        decoded += plan.us;
+    }
+    if (decoded > unpacked + (others ? 0.0 : 13.0)) {
+        jobs.clear();
+        std::fill(few.begin(), few.end(), 0);
+    }
+    if (!jobs.empty()) {
+        if (!g->q8_scratch) TRY(llmtie_decode_scratch_new(g, &g->q8_scratch));
+        TRY(run_jobs(g, jobs, q, out, out_f16, heads, kv_heads, head_dim, scale, causal, 0, g->q8_scratch));
+    }
     // A launch of the attention kernel takes LLMTIE_TC_MAX_SEQ sequences; a
     // sequence of more than kRows rows is as many of them as it takes, over the
     // same keys.
@@ -468,7 +530,7 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
         size_t at[LLMTIE_TC_MAX_SEQ];       // where the sequence's keys lie in the workspace
         while (b < batch && pp.nseq < LLMTIE_TC_MAX_SEQ) {
             const int rows = cu_seqlens[b + 1] - cu_seqlens[b];
-            if (rows == 0) {
+            if (rows == 0 || few[b]) {
                 b++;
                 continue;
             }

@@ -64,6 +64,7 @@ struct llmtie_gpu {
     std::vector<llmtie_decode_scratch *> scratches;
     Workspace ws_rope;   // the ragged prefill's table of cosines and sines (or its copy of q)
     Workspace ws_part;   // partial results of a prefill whose long row blocks were cut
+    llmtie_decode_scratch *q8_scratch = nullptr;   // for prompts of few rows over the 8-bit cache
     Workspace ws_q8{true};       // the 8-bit cache: its live keys as f16 for prefill, eviction's block lists
     Workspace ws_q8_part{true};  // the pieces of cut row blocks of prefill over it
     Workspace ws_kv16;   // f16 copies of the live keys of caches the tensor-memory prefill cannot map

@@ -1,4 +1,5 @@
-// Split-KV decode over the 8-bit cache (kv_q8.cuh): one query row a head, the
+// Split-KV decode over the 8-bit cache (kv_q8.cuh): one query row a head, or
+// the few of a short prompt (as long as a group's are no more than eight); the
 // codes go into the tensor cores as they lie in memory.
 //
 // Mathematics. With q of a row as 16-bit fixed point, q = f (256 H + L), H and L
@@ -14,7 +15,7 @@
 //
 // Tiles. One warp takes one cache block of 32 tokens: mma.m16n8k32 with the
 // query's H rows as rows 0-7 and its L rows as rows 8-15 of A (up to eight
-// query heads of a group), four key tiles of eight tokens as B; the result
+// query rows of a group), four key tiles of eight tokens as B; the result
 // fragment holds a row's H and L sums in one thread, and, with the tokens
 // dealt to the tiles' columns as below, exactly the eight tokens whose bytes
 // that thread needs of the A fragment of the second product. No shuffle but
@@ -28,6 +29,8 @@
 #include "kv_q8.cuh"
 
 #include <math_constants.h>
+
+#include <algorithm>
 
 namespace {
 
@@ -141,8 +144,7 @@ __device__ __forceinline__ Run run_at(const DecodeQ8Params &p, int u, int end)
         else hi = mid - 1;
     }
     Run r;
-    const int live = p.seq[lo].live;
-    const int full = live >> 5;
+    const int live = p.seq[lo].live, full = p.seq[lo].full;
     r.units = (live + 31) >> 5;                                 // (0 only where the block has no units)
     r.seq = lo;
     r.head = (int)((unsigned)(u - p.unit0[lo]) / (unsigned)max(1, r.units));
@@ -198,22 +200,61 @@ __device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at,
     }
 }
 
-// The weights of finished pairs (two at most, side by side: what this costs is
-// the latency of its loads): what each complete block's tokens got, summed over
+// By cluster: pair blockIdx.x / p.cluster, cut evenly over the cluster's blocks.
+__device__ __forceinline__ Run run_of_rank(const DecodeQ8Params &p)
+{
+    const int pair = (int)blockIdx.x / p.cluster, rank = (int)blockIdx.x - pair * p.cluster;
+    Run r;
+    r.seq = pair / p.kv_heads;
+    r.head = pair - r.seq * p.kv_heads;
+    const int full = p.seq[r.seq].full;
+    r.units = (p.seq[r.seq].live + 31) >> 5;
+    r.begin = 0;
+    r.first = (int)((long long)r.units * rank / p.cluster);
+    const int stop = (int)((long long)r.units * (rank + 1) / p.cluster);
+    r.tail = stop > full && r.first < stop;
+    r.last = min(stop, full);
+    r.whole = p.cluster == 1;
+    r.next = 0;
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// An address of this block's shared memory in that of cluster rank `rank`.
+__device__ __forceinline__ uint32_t peer(uint32_t addr, int rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float2 peer_f2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// The weights of blocks [first, last) of one finished pair and of all of a second
+// (or of none: seq1 < 0), side by side, because what this costs is the latency of
+// its loads: what each complete block's tokens got, summed over
 // the group's heads; `fin` has each row's maximum and the inverse of its sum.
 template <int HD>
-__device__ __forceinline__ void weigh(const DecodeQ8Params &p, int seq0, int head0, int seq1, int head1, const float2 *fin,
-                                      int tid, int group)
+__device__ __forceinline__ void weigh(const DecodeQ8Params &p, int seq0, int head0, int first, int last, int seq1, int head1,
+                                      const float2 *fin, int tid, int group)
 {
-    const int full0 = p.seq[seq0].live >> 5, total = full0 + (seq1 >= 0 ? p.seq[seq1].live >> 5 : 0);
+    const int full0 = last - first, total = full0 + (seq1 >= 0 ? p.seq[seq1].full : 0);
     for (int i = tid; i < total; i += kThreads) {
         const bool second = i >= full0;
-        const int b = second ? i - full0 : i, seq = second ? seq1 : seq0, head = second ? head1 : head0;
+        const int b = second ? i - full0 : first + i, seq = second ? seq1 : seq0, head = second ? head1 : head0;
         const DecodeQ8Seq &sq = p.seq[seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
         float *weight = (float *)(sq.base + at.w) + (long long)head * sq.nb + b;
-        const float2 *st = p.stats + (p.stat0[seq] + (long long)head * (sq.live >> 5) + b) * kRows;
-        const float2 *f = fin + (second ? group : 0);
+        const float2 *st = p.stats + (p.stat0[seq] + (long long)head * sq.full + b) * kRows;
+        const float2 *f = fin + (second ? kRows : 0);
         float2 y[kRows];
         const float before = *weight;
 #pragma unroll
@@ -239,10 +280,17 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
     __shared__ float2 final_s[2 * kRows];
     __shared__ int last_s[2];
+    __shared__ float2 part_s[kRows];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.heads / p.kv_heads;
-    const int u_begin = first_unit(p, (int)blockIdx.x), u_end = first_unit(p, (int)blockIdx.x + 1);
+    // Row `row` of a job: head row % group of the group, at its query row / group.
+    auto row_at = [&](int seq, int head, int row) {
+        const int pos = row / group;
+        return ((long long)(p.seq[seq].row0 + pos) * p.heads + head * group + (row - pos * group)) * HD;
+    };
+    const int u_begin = p.cluster ? 0 : first_unit(p, (int)blockIdx.x);
+    const int u_end = p.cluster ? 0 : first_unit(p, (int)blockIdx.x + 1);
     float *merge = (float *)(smem + G::RING);
     const uint32_t ring0 = smem_u32(smem) + (uint32_t)warp * (G::STAGES * G::STAGE);
     const uint32_t bar0 = smem_u32(&bars[warp * G::STAGES]);
@@ -254,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     }
     __syncwarp();
     const int r = lane >> 2, c = lane & 3;
-    Run run = run_at(p, u_begin, u_end);
+    Run run = p.cluster ? run_of_rank(p) : run_at(p, u_begin, u_end);
 
     // What a run needs besides its blocks: the query (row r, the 16 channels of
     // chunk c in each panel), and of the tail the warp's eight tokens (keys: token
@@ -281,17 +329,18 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         ks = (const float *)(s.base + at.ks) + (long long)run.head * s.nb;
         vs = (const float *)(s.base + at.vs) + (long long)run.head * s.nb;
         load_scales(run.first + warp, k_scale, v_scale);
-        const float *qh = p.q + ((long long)run.seq * p.heads + (long long)run.head * group) * HD;
+        const bool mine = r < group * s.n;
+        const float *qr = p.q + row_at(run.seq, run.head, mine ? r : 0);
 #pragma unroll
         for (int j = 0; j < PANELS; j++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < group) y = __ldg((const float4 *)(qh + r * HD + 64 * j + 16 * c + 4 * i));
+                if (mine) y = __ldg((const float4 *)(qr + 64 * j + 16 * c + 4 * i));
                 x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
             }
         }
-        const int n = run.tail ? (s.live & 31) - 8 * warp : 0;
+        const int n = run.tail ? s.live - 32 * s.full - 8 * warp : 0;
         if (n > 0) {
             const uint16_t *kt = (const uint16_t *)(s.base + at.kt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
             const uint16_t *vt = (const uint16_t *)(s.base + at.vt) + ((long long)run.head * kQ8Block + 8 * warp) * HD;
@@ -327,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     // is read until it has ended.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (u_begin >= u_end) return;        // (a share that was all charges)
+    if (p.cluster ? run.units == 0 : u_begin >= u_end) return;   // (a sequence of no tokens; a share that was all charges)
     load_run();
 
     int issued = 0, used = 0;
@@ -360,7 +409,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         const DecodeQ8Seq &sq = p.seq[run.seq];
         const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
 
-        const int tail_n = run.tail ? min(8, (sq.live & 31) - 8 * warp) : 0;    // the warp's tokens
+        const int rows = group * sq.n;
+        // the last token that row r sees, and the last that all rows see
+        const int lim = p.causal && r < rows ? sq.live - sq.n + r / group : sq.live - 1;
+        const int lim_all = p.causal ? sq.live - sq.n : sq.live - 1;
+        const int tail_n = run.tail ? min(8, sq.live - 32 * sq.full - 8 * warp) : 0;    // the warp's tokens
         // -- the query as fixed point
         uint32_t qa[PANELS][4], qb[PANELS][4];
         float f_q;
@@ -422,15 +475,16 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 }
             }
             // row r against tokens 2 c and 2 c + 1
-            const float s0 = 2 * c < tail_n ? (d[0] + d[2]) * unit : -CUDART_INF_F;
-            const float s1 = 2 * c + 1 < tail_n ? (d[1] + d[3]) * unit : -CUDART_INF_F;
+            const int seen = min(tail_n, lim + 1 - 32 * sq.full - 8 * warp);      // of the warp's tokens
+            const float s0 = 2 * c < seen ? (d[0] + d[2]) * unit : -CUDART_INF_F;
+            const float s1 = 2 * c + 1 < seen ? (d[1] + d[3]) * unit : -CUDART_INF_F;
             m = fmaxf(s0, s1);
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float e0 = 2 * c < tail_n ? ex2(s0 - m) : 0.0f, e1 = 2 * c + 1 < tail_n ? ex2(s1 - m) : 0.0f;
+            const float e0 = 2 * c < seen ? ex2(s0 - m) : 0.0f, e1 = 2 * c + 1 < seen ? ex2(s1 - m) : 0.0f;
             l = e0 + e1;
             float *mine = merge + warp * kRows * HD;
-            for (int g = 0; g < group; g++) {
+            for (int g = 0; g < rows; g++) {
                 float o4[V];
 #pragma unroll
                 for (int i = 0; i < V; i++) o4[i] = 0.0f;
@@ -453,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                const float2 y = r < group ? *(const float2 *)(mine + r * HD + 8 * (i ^ r) + 2 * c) : make_float2(0.f, 0.f);
+                const float2 y = r < rows ? *(const float2 *)(mine + r * HD + 8 * (i ^ r) + 2 * c) : make_float2(0.f, 0.f);
                 acc[i][0] = y.x;
                 acc[i][1] = y.y;
             }
@@ -493,8 +547,16 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 }
                 s[2 * t] = (float)(d[0] * 256 + d[2]) * f;          // token 8 c + 2 t of row r
                 s[2 * t + 1] = (float)(d[1] * 256 + d[3]) * f;      // and the next
-                mb = fmaxf(mb, fmaxf(s[2 * t], s[2 * t + 1]));
             }
+            if (32 * blk + 31 > lim_all) {
+                // (a block among a prompt's own rows: the first of them may see nothing of it)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (32 * blk + 8 * c + i > lim) s[i] = -CUDART_INF_F;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) mb = fmaxf(mb, s[i]);
             mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
             mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
             // The reference moves only when a block's maximum is far above it
@@ -510,22 +572,24 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 }
                 m = to;
             }
+            const bool seen = mb != -CUDART_INF_F;
+            const float top = seen ? mb : 0.0f;
             float sum = 0.0f;
             uint32_t z[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float e = ex2(s[i] - mb);
+                const float e = ex2(s[i] - top);
                 sum += e;
                 z[i] = __float_as_uint(fmaf(e, 65535.0f, 8388608.0f));
             }
-            const float beta = ex2(mb - m);
+            const float beta = seen ? ex2(mb - m) : 0.0f;
             l = fmaf(beta, sum, l);
             if (p.stats) {
                 float whole = sum;
                 whole += __shfl_xor_sync(0xffffffffu, whole, 1);
                 whole += __shfl_xor_sync(0xffffffffu, whole, 2);
                 if (c == 0) {
-                    p.stats[(p.stat0[run.seq] + (long long)run.head * (sq.live >> 5) + blk) * kRows + r] = make_float2(mb, whole);
+                    p.stats[(p.stat0[run.seq] + (long long)run.head * sq.full + blk) * kRows + r] = make_float2(mb, whole);
                 }
             }
             uint32_t a_hi[2], a_lo[2];
@@ -564,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             m_s[warp][r] = m;
             l_s[warp][r] = l;
         }
-        if (r < group) {
+        if (r < rows) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 // (groups of eight channels swizzled by the row: no bank conflicts on either side)
@@ -572,9 +636,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             }
         }
         __syncthreads();
-        const long long row0 = (long long)now.seq * p.heads + (long long)now.head * group;
         const int slot = (int)blockIdx.x * 2 + (is_first ? 0 : 1);
-        for (int row = warp; row < group; row += kWarps) {
+        for (int row = warp; row < rows; row += kWarps) {
             float M = -CUDART_INF_F, L = 0.0f, o[V];
 #pragma unroll
             for (int e = 0; e < V; e++) o[e] = 0.0f;
@@ -594,8 +657,15 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 const float inv = 1.0f / L;
 #pragma unroll
                 for (int e = 0; e < V; e++) o[e] *= inv;
-                store_row<HD>(p, (row0 + row) * HD, lane, o);
+                store_row<HD>(p, row_at(now.seq, now.head, row), lane, o);
                 if (lane == 0) final_s[row] = make_float2(M, inv);
+            } else if (p.cluster) {
+                // (the ring is empty: there is no other run)
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    *(float2 *)((float *)smem + row * HD + V * lane + e) = make_float2(o[e], o[e + 1]);
+                }
+                if (lane == 0) part_s[row] = make_float2(M, L);
             } else {
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
@@ -607,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (now.whole) {
             if (p.stats) {
                 __syncthreads();
-                weigh<HD>(p, now.seq, now.head, -1, 0, final_s, tid, group);
+                weigh<HD>(p, now.seq, now.head, 0, sq.full, -1, 0, final_s, tid, rows);
             }
         } else if (is_first) {
             shared0 = {now.seq, now.head, now.begin, now.units};
@@ -617,6 +687,76 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         if (!more) break;
         is_first = false;
         __syncthreads();   // merge, m_s and final_s are free again
+    }
+
+    if (p.cluster > 1) {
+        // -- by cluster: the blocks' results meet through distributed shared memory, row
+        // k of them merged by the block of rank k mod the cluster's size
+        const int rank = (int)blockIdx.x % p.cluster, rows = group * p.seq[run.seq].n;
+        cluster_sync();
+        for (int i = warp; rank + i * p.cluster < rows; i += kWarps) {
+            const int row = rank + i * p.cluster;
+            const uint32_t ml_at = smem_u32(&part_s[row]), o_at = smem_u32(smem) + (uint32_t)(row * HD + V * lane) * 4;
+            float M = -CUDART_INF_F, L = 0.0f, o[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) o[e] = 0.0f;
+            for (int k0 = 0; k0 < p.cluster; k0 += 8) {
+                float2 ml[8], y[8][V / 2];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (k0 + k < p.cluster) {
+                        ml[k] = peer_f2(peer(ml_at, k0 + k));
+#pragma unroll
+                        for (int e = 0; e < V / 2; e++) y[k][e] = peer_f2(peer(o_at, k0 + k) + 8 * e);
+                    }
+                }
+                float top = M;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (k0 + k < p.cluster) top = fmaxf(top, ml[k].x);
+                }
+                const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
+                L *= keep;
+#pragma unroll
+                for (int e = 0; e < V; e++) o[e] *= keep;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (k0 + k < p.cluster) {
+                        const float f = ml[k].x == -CUDART_INF_F ? 0.0f : ex2(ml[k].x - top);
+                        L = fmaf(f, ml[k].y, L);
+#pragma unroll
+                        for (int e = 0; e < V / 2; e++) {
+                            o[2 * e] = fmaf(f, y[k][e].x, o[2 * e]);
+                            o[2 * e + 1] = fmaf(f, y[k][e].y, o[2 * e + 1]);
+                        }
+                    }
+                }
+                M = top;
+            }
+            const float inv = 1.0f / L;
+#pragma unroll
+            for (int e = 0; e < V; e++) o[e] *= inv;
+            store_row<HD>(p, row_at(run.seq, run.head, row), lane, o);
+        }
+        if (p.stats) {
+            // each block weighs its own cache blocks, and works the rows' sums out itself
+            if (tid < rows) {
+                float M = -CUDART_INF_F, L = 0.0f;
+                for (int k = 0; k < p.cluster; k++) M = fmaxf(M, peer_f2(peer(smem_u32(&part_s[tid]), k)).x);
+                for (int k = 0; k < p.cluster; k++) {
+                    const float2 ml = peer_f2(peer(smem_u32(&part_s[tid]), k));
+                    L = fmaf(ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - M), ml.y, L);
+                }
+                final_s[tid] = make_float2(M, 1.0f / L);
+            }
+            __syncthreads();
+            weigh<HD>(p, run.seq, run.head, run.first, run.last, -1, 0, final_s, tid, rows);
+        }
+        cluster_sync();   // no block leaves while another reads its results
+        if (!ok) {
+            for (int i = 0; i < 64; i++) __nanosleep(1000);
+        }
+        return;
     }
 
     // -- pairs shared with other blocks of the grid (the first run's and the last's,
@@ -638,11 +778,10 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     }
     __syncthreads();
     // (a warp takes a row of either pair)
-    for (int item = warp; item < 2 * group; item += kWarps) {
-        if (!last_s[item >= group]) continue;
-        const int row = item >= group ? item - group : item;
-        const Shared now = pick(item >= group, shared0, shared1);
-        const long long row0 = (long long)now.seq * p.heads + (long long)now.head * group;
+    for (int item = warp; item < 2 * kRows; item += kWarps) {
+        const int row = item % kRows;
+        const Shared now = pick(item >= kRows, shared0, shared1);
+        if (!last_s[item >= kRows] || row >= group * p.seq[now.seq].n) continue;
         const int pair = now.seq * p.kv_heads + now.head;
         const int b0 = block_of(p, now.begin, pair), b1 = block_of(p, now.begin + now.units - 1, pair);
         // The contributors in order, whoever came last: the same bits every time. A
@@ -656,19 +795,25 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             const int my_slot = 2 * (bb + lane) + (bb + lane == b0 ? skew : 0);
             float2 ml = make_float2(-CUDART_INF_F, 0.0f);
             if (lane < n) ml = __ldcg(&p.part_ml[my_slot * kRows + row]);
-            float2 y[8][V / 2];
-            auto load8 = [&](int i0) {
+            constexpr int U = 16;
+            float y[U][V];
+            auto load = [&](int i0) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int b = min(bb + i0 + i, b1);
-                    const long long sl = 2 * b + (b == b0 ? skew : 0);
-#pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        y[i][e / 2] = __ldcg((const float2 *)(p.part_o + (sl * kRows + row) * HD + V * lane + e));
+                for (int i = 0; i < U; i++) {
+                    if (i0 + i < n) {
+                        const int b = bb + i0 + i;
+                        const float *src = p.part_o + ((long long)(2 * b + (b == b0 ? skew : 0)) * kRows + row) * HD + V * lane;
+                        if constexpr (V == 4) {
+                            const float4 z = __ldcg((const float4 *)src);
+                            y[i][0] = z.x; y[i][1] = z.y; y[i][2] = z.z; y[i][3] = z.w;
+                        } else {
+                            const float2 z = __ldcg((const float2 *)src);
+                            y[i][0] = z.x; y[i][1] = z.y;
+                        }
                     }
                 }
             };
-            load8(0);
+            load(0);
             float top = ml.x;
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
@@ -681,15 +826,14 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             L = fmaf(L, keep, sum);
 #pragma unroll
             for (int e = 0; e < V; e++) o[e] *= keep;
-            for (int i0 = 0; i0 < n; i0 += 8) {
-                if (i0) load8(i0);
+            for (int i0 = 0; i0 < n; i0 += U) {
+                if (i0) load(i0);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float fi = __shfl_sync(0xffffffffu, f, i0 + i);   // (0 past the last)
+                for (int i = 0; i < U; i++) {
+                    const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+                    if (i0 + i < n) {
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        o[e] = fmaf(fi, y[i][e / 2].x, o[e]);
-                        o[e + 1] = fmaf(fi, y[i][e / 2].y, o[e + 1]);
+                        for (int e = 0; e < V; e++) o[e] = fmaf(fi, y[i][e], o[e]);
                     }
                 }
             }
@@ -698,13 +842,13 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         const float inv = 1.0f / L;
 #pragma unroll
         for (int e = 0; e < V; e++) o[e] *= inv;
-        store_row<HD>(p, (row0 + row) * HD, lane, o);
+        store_row<HD>(p, row_at(now.seq, now.head, row), lane, o);
         if (lane == 0) final_s[item] = make_float2(M, inv);
     }
     if (p.stats && (last_s[0] || last_s[1])) {
         __syncthreads();
-        weigh<HD>(p, last_s[0] ? shared0.seq : shared1.seq, last_s[0] ? shared0.head : shared1.head,
-                  last_s[0] && last_s[1] ? shared1.seq : -1, shared1.head, final_s + (last_s[0] ? 0 : group), tid, group);
+        const int seq = last_s[0] ? shared0.seq : shared1.seq;
+        weigh<HD>(p, seq, last_s[0] ? shared0.head : shared1.head, 0, p.seq[seq].full, last_s[0] && last_s[1] ? shared1.seq : -1, shared1.head, final_s + (last_s[0] ? 0 : kRows), tid, group);
     }
     if (!ok) {
         // a wait gave up: leave the copies still in flight time to land
@@ -717,7 +861,7 @@ __global__ void q8_zero_rows_kernel(const __grid_constant__ DecodeQ8Params p, in
 {
     if (p.seq[blockIdx.x].live) return;
     for (int i = threadIdx.x; i < width; i += blockDim.x) {
-        const long long at = (long long)blockIdx.x * width + i;
+        const long long at = (long long)p.seq[blockIdx.x].row0 * width + i;
         if (p.out_f16) ((uint16_t *)p.out)[at] = 0;
         else ((float *)p.out)[at] = 0.0f;
     }
@@ -728,17 +872,49 @@ const KernelReg reg64("decode_q8_64", (const void *)decode_q8_kernel<64>);
 
 }  // namespace
 
+// Once a device: what the kernels may take of it, and how many clusters of 8 and
+// of 16 blocks it holds at once.
+static cudaError_t configure(int dev, int hd, int (**resident)[2])
+{
+    static bool done[64] = {false};
+    static int clusters[64][2][2];
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev]) {
+        const void *kernel[2] = {(const void *)decode_q8_kernel<128>, (const void *)decode_q8_kernel<64>};
+        const int smem[2] = {Geo<128>::SMEM, Geo<64>::SMEM};
+        for (int i = 0; i < 2; i++) {
+            cudaError_t e = cudaFuncSetAttribute(kernel[i], cudaFuncAttributeMaxDynamicSharedMemorySize, smem[i]);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return e;
+            for (int c = 0; c < 2; c++) {
+                cudaLaunchConfig_t cfg = {};
+                cudaLaunchAttribute attr[1];
+                cfg.gridDim = dim3(c ? 16 : 8);
+                cfg.blockDim = dim3(kThreads);
+                cfg.dynamicSmemBytes = (size_t)smem[i];
+                attr[0].id = cudaLaunchAttributeClusterDimension;
+                attr[0].val.clusterDim.x = c ? 16 : 8;
+                attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+                cfg.attrs = attr;
+                cfg.numAttrs = 1;
+                if (cudaOccupancyMaxActiveClusters(&clusters[dev][i][c], kernel[i], &cfg) != cudaSuccess) {
+                    cudaGetLastError();
+                    clusters[dev][i][c] = 0;
+                }
+            }
+        }
+        done[dev] = true;
+    }
+    if (resident) *resident = &clusters[dev][hd == 128 ? 0 : 1];
+    return cudaSuccess;
+}
+
 cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, int grid)
 {
-    static bool configured[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && !configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<128>::SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_q8_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<64>::SMEM);
-        if (e != cudaSuccess) return e;
-        configured[dev] = true;
-    }
+    const cudaError_t ce = configure(dev, hd, nullptr);
+    if (ce != cudaSuccess) return ce;
     bool empty = false;
     for (int b = 0; b < p.nseq; b++) empty = empty || p.seq[b].live == 0;
     if (empty) {
@@ -748,8 +924,70 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
     }
     if (grid == 0) return cudaSuccess;
     const dim3 blocks((unsigned)grid);
-    return hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, decode_q8_kernel<128>, p)
-                     : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, decode_q8_kernel<64>, p);
+    return hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, p.cluster, decode_q8_kernel<128>, p)
+                     : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, p.cluster, decode_q8_kernel<64>, p);
 }
 
-int decode_q8_resident(int hd) { return hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT; }
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters)
+{
+    // Microseconds, as measured (148 SMs): cache blocks a microsecond that the memory
+    // gives (6.9 TB/s), a warp's time for one when nothing but the warp itself bounds
+    // it, and what a launch costs besides: by a cluster of 1, 2, 4, 8 or 16 blocks of
+    // the grid (the last are packed onto half as many SMs), by the cut (whose merge
+    // goes through memory, and is long where many blocks share a pair: short
+    // launches), and for a further wave of blocks of the grid.
+    const double all = (hd == 128 ? 842.0 : 1684.0) * sm_count / 148, one = hd == 128 ? 0.7 : 0.6;
+    constexpr double kCluster[5] = {4.0, 4.5, 5.0, 5.4, 6.3}, kPacked = 1.15, kCut = 7.0, kShort = 12.0, kWave = 3.5;
+    const int most = sm_count * (hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT);
+    long long total = 0, longest = 0;
+    for (int i = 0; i < n; i++) {
+        total += (long long)units[i] * kv_heads;
+        longest = std::max<long long>(longest, units[i]);
+    }
+    const long long pairs = (long long)n * kv_heads;
+    plan = DecodeQ8Plan{0, 0, 0, 0.0};
+    if (total == 0) return;
+    // the cut by work: never fewer than four cache blocks, one a warp, for a block of
+    // the grid; where a launch is short, as many that what the warps take in turn (0.5
+    // us each) and what the merge takes for each block that a pair is spread over (0.04
+    // us) is least. Where it is long a run is charged for what it costs besides its
+    // cache blocks, about 16 of them.
+    long long grid = most;
+    int over = 16;
+    if (total < 8ll * most) {
+        double best = 0.0;
+        for (int k = 1; k <= 32; k++) {
+            const long long blocks = (total + 4 * k - 1) / (4 * k);
+            const double cost = 0.5 * k + 0.04 * (double)blocks / (double)pairs;
+            if (blocks <= most && (best == 0.0 || cost < best)) {
+                best = cost;
+                grid = blocks;
+            }
+        }
+        over = 0;
+    }
+    const long long share = (total + grid - 1) / grid;
+    plan = DecodeQ8Plan{(int)grid, 0, over, (over ? kCut : kShort) + std::max((double)total / all, one * (double)((share + 3) / 4))};
+    for (int i = 0, c = 1; i < 5; i++, c *= 2) {
+        const long long blocks = pairs * c;
+        if (c > 1 && blocks > most) break;
+        if (c >= 8 && clusters[c == 16] < pairs) break;
+        const double waves = (double)((blocks + most - 1) / most), part = std::max(1.0, (double)blocks / most);
+        const double own = one * (double)(((longest + c - 1) / c + 3) / 4) * (c == 16 ? kPacked : 1.0);
+        const double cost = kCluster[i] + kWave * (waves - 1.0) + std::max((double)total / all * waves / part, own * waves);
+        if (cost < plan.us && blocks <= 0x7fffffff) plan = DecodeQ8Plan{(int)blocks, c, 0, cost};
+    }
+}
+
+cudaError_t decode_q8_clusters(int hd, int (&clusters)[2])
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int(*held)[2];
+    const cudaError_t e = configure(dev, hd, &held);
+    if (e == cudaSuccess) {
+        clusters[0] = (*held)[0];
+        clusters[1] = (*held)[1];
+    }
+    return e;
+}

@@ -680,7 +680,7 @@ const KernelReg reg_move("q8_move", (const void *)q8_move_kernel<128>);
 template <typename... Params, typename... Args>
 static cudaError_t launch(cudaStream_t st, dim3 grid, int threads, void (*kernel)(Params...), Args... args)
 {
-    return launch_dependent(st, grid, threads, 0, kernel, args...);
+    return launch_dependent(st, grid, threads, 0, 1, kernel, args...);
 }
 
 cudaError_t launch_q8_append(cudaStream_t st, Q8AppendParams &p, int hd, int sm_count)

@@ -54,7 +54,8 @@ __host__ __device__ inline Q8Layout q8_layout(int kv_heads, int hd, int nb)
 // stream: it may be set up while that one still runs, and waits for its end
 // (griddepcontrol.wait) before it reads or writes anything.
 template <typename... Params, typename... Args>
-inline cudaError_t launch_dependent(cudaStream_t st, dim3 grid, int threads, size_t smem, void (*kernel)(Params...), Args... args)
+inline cudaError_t launch_dependent(cudaStream_t st, dim3 grid, int threads, size_t smem, int cluster, void (*kernel)(Params...),
+                                    Args... args)
 {
     static const bool no_pdl = getenv("LLMTIE_B200_NO_PDL") != nullptr;   // an A/B switch
     cudaLaunchConfig_t cfg = {};
@@ -62,11 +63,18 @@ inline cudaError_t launch_dependent(cudaStream_t st, dim3 grid, int threads, siz
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = no_pdl ? 0 : 1;
+    if (!no_pdl) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+    }
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -160,18 +168,23 @@ void launch_rope_inv_freq(cudaStream_t st, float *out, const float *freq_div, in
 
 // ---- decode_q8.cu -----------------------------------------------------------
 
+// One job: n queries (n * heads / kv_heads at most eight) of one sequence.
 struct DecodeQ8Seq {
     unsigned char *base;     // (the weights are written)
-    int nb, live;
+    int nb, full;            // blocks of the capacity, and complete ones (what is past them lies in the tail)
+    int live;                // the last query sees that many tokens
+    int row0, n;             // its first row in q and out
 };
 struct DecodeQ8Params {
     DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
     int unit0[LLMTIE_Q8_MAX_SEQ + 1];                  // first 32-token unit of each sequence
     int each, more, over;                              // the cut over the grid: see first_unit in decode_q8.cu
+    int cluster;                                       // or: a cluster of so many blocks a pair, no cut (0: the cut)
     long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
     int nseq, heads, kv_heads;
-    const float *q;          // [seq][heads*hd]
-    void *out;               // [seq][heads*hd], f16 or f32
+    int causal;              // query i sees live - n + 1 + i tokens, else all
+    const float *q;          // rows [heads*hd]
+    void *out;               // the same, f16 or f32
     int out_f16;
     float sl2;               // scale * log2(e)
     float *part_o;           // [block][2][8][hd]
@@ -182,5 +195,14 @@ struct DecodeQ8Params {
     long long wait_cycles;
 };
 cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, int grid);
-// Blocks of that kernel that an SM holds at once.
-int decode_q8_resident(int hd);
+// How a launch over pairs of `units` cache blocks (the tail counts as one), each
+// kv_heads times, is laid over the device.
+struct DecodeQ8Plan {
+    int grid;      // blocks of the grid (0: nothing to do)
+    int cluster;   // a cluster of so many a pair, or 0: cut by work
+    int over;      // what the cut charges a run
+    double us;     // about what it takes
+};
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters);
+// How many clusters of 8 and of 16 blocks the current device holds at once.
+cudaError_t decode_q8_clusters(int hd, int (&clusters)[2]);
