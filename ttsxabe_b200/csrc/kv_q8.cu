@@ -535,8 +535,19 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
     if (!all && room > 0) {
         const bool held = sq.full <= kPickKeys;
         if (held) {
-            for (int i = tid; i < (sq.full + 3) / 4 * 4; i += kPickThreads) {
-                keys[i] = i >= lo && i < hi ? weight_key(i == tid ? wi : w[i]) : 0u;
+            // (four loads in flight; the first tile's is there already)
+            for (int i0 = tid; i0 < (sq.full + 3) / 4 * 4; i0 += 4 * kPickThreads) {
+                float x[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int i = i0 + u * kPickThreads;
+                    x[u] = i == tid ? wi : i >= lo && i < hi ? w[i] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int i = i0 + u * kPickThreads;
+                    if (i < kPickKeys) keys[i] = i >= lo && i < hi ? weight_key(x[u]) : 0u;
+                }
             }
             __syncthreads();
         }
