@@ -616,13 +616,25 @@ llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q, size_t q_l
                                        int32_t weigh, llmtie_decode_scratch *scratch, void *out,
                                        size_t out_len, int32_t out_f16);
 
+/* How llmtie_decode_batched_q8 would lay a launch over the device (host only,
+ * no device): for contexts of live[0..batch) tokens, batch <= 32, on sm_count
+ * SMs that hold resident8 / resident16 thread-block clusters of 8 and of 16 of
+ * its blocks at once, the blocks of the grid, the cluster that takes each
+ * (sequence, KV head) pair (0: the launch is cut by work) and about how long it
+ * takes in nanoseconds. */
+llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads,
+                                    size_t head_dim, int32_t sm_count, int32_t resident8,
+                                    int32_t resident16, int32_t *grid, int32_t *cluster,
+                                    int64_t *ns);
+
 /* llmtie_flash_attn_f16 over 8-bit caches, for a packed ragged batch: sequence
  * b's rows cu_seqlens[b] .. cu_seqlens[b+1] of q f32 [rows][heads*head_dim]
  * (already rotated) attend to its cache, which holds past[b] tokens before
  * theirs and theirs (llmtie_rope_append_q8 puts them there): causal, or all to
- * all. out [rows][heads*head_dim], f16 or f32. The live keys are unpacked to
- * f16 once, into memory that the handle keeps for the purpose, for at most
- * eight sequences at a time. */
+ * all. out [rows][heads*head_dim], f16 or f32. Sequences of few rows go through
+ * the decode kernel; of the others the live keys are unpacked to f16 once, into
+ * memory that the handle keeps for the purpose, for at most eight sequences at
+ * a time. */
 llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len,
                                    const int32_t *cu_seqlens, size_t batch,
                                    const void *const *caches, const int32_t *past,

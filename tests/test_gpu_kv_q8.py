@@ -7,7 +7,7 @@ import torch
 from tests.helpers import assert_parity, rel_l2
 from tests.q8_model import Q8Model, attend, rotate
 from ttsxabe_b200 import (CacheOverrun, DecodeScratch, InvalidArgument, KvCacheQ8, Misaligned, OddHeadDim, Prefix,
-                          RaggedBlock, SliceOverrun, UnsupportedAttention, evicted_len, kv_q8_bytes)
+                          RaggedBlock, SliceOverrun, UnsupportedAttention, decode_plan_q8, evicted_len, kv_q8_bytes)
 
 pytestmark = pytest.mark.gpu
 
@@ -321,6 +321,39 @@ def test_decode_ragged_batch(gpu, heads, kv, hd):
         assert np.array_equal(again.reshape(q.shape), out)
 
 
+@pytest.mark.parametrize("heads,kv,hd,batch,live,cluster", [
+    (8, 8, 128, 1, 30, 1), (32, 8, 128, 16, 600, 2), (32, 8, 128, 8, 1800, 4), (32, 8, 128, 1, 1999, 8), (4, 1, 128, 1, 7000, 16),
+    (32, 8, 128, 1, 33000, 0), (20, 20, 64, 8, 1500, 2), (20, 20, 64, 1, 1500, 8), (8, 1, 64, 1, 9000, 16), (4, 1, 64, 40, 5, 1),
+    (8, 8, 64, 2, 20000, 0)])
+def test_decode_by_every_way_over_the_device(gpu, heads, kv, hd, batch, live, cluster):
+    """A cluster of each size a pair, and the cut by work; lengths that differ by
+    a block or two, and weights."""
+    rng = np.random.default_rng(live)
+    lives = [live - int(x) for x in rng.integers(0, min(live, 70), batch)]
+    assert decode_plan_q8(lives[:32], kv, hd)[1] == cluster
+    cap = [(n + 31) // 32 * 32 for n in lives]
+    ms = []
+    for c, n in zip(cap, lives):
+        m = Q8Model(kv, hd, c, fill=0x7f)
+        full = n // 32
+        m.k[:, :full], m.v[:, :full] = (rng.integers(-127, 128, x.shape) for x in (m.k[:, :full], m.v[:, :full]))
+        m.ks[:], m.vs[:] = np.nan, np.nan
+        m.ks[:, :full], m.vs[:, :full] = rng.uniform(0.005, 0.02, (2, kv, full))
+        m.kt[:, :n % 32], m.vt[:, :n % 32] = rng.standard_normal((2, kv, n % 32, hd))
+        m.w[:] = 0.5
+        ms.append(m)
+    ts = [put(gpu, m) for m in ms]
+    q = rng.standard_normal((batch, heads, hd)).astype(np.float32)
+    scratch = DecodeScratch()
+    out = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch, weigh=True)).reshape(q.shape)
+    for b, n in enumerate(lives):
+        want, share = decode_want(q[b], ms[b], n, heads, hd ** -0.5)
+        assert rel_l2(want, out[b]) <= DECODE_REL, f"sequence {b} of {n}"
+        w = got(gpu, ts[b], ms[b]).w
+        assert np.abs(w[:, :n // 32] - (0.5 + share)).max(initial=0) <= 2e-4 * (1.5 + share.max(initial=0))
+        assert (w[:, n // 32:] == 0.5).all()
+
+
 def test_decode_sink_and_long_faint_context(gpu):
     """One key far above all others, whose sum is as large as its own: no key's
     probability may be lost below it."""
@@ -402,8 +435,8 @@ def test_decode_offsets_past_32_bits(gpu):
 
 # ---- prefill ---------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (20, 20, 64), (12, 4, 128), (8, 1, 64)])
-@pytest.mark.parametrize("past,n", [(0, 1), (0, 5), (0, 32), (0, 129), (63, 1), (40, 90), (700, 33)])
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (20, 20, 64), (12, 4, 128), (8, 1, 64), (16, 1, 128), (5, 1, 64)])
+@pytest.mark.parametrize("past,n", [(0, 1), (0, 5), (0, 32), (0, 129), (63, 1), (40, 90), (700, 33), (62, 4), (31, 2), (1000, 8), (300, 17)])
 def test_flash(gpu, heads, kv, hd, past, n):
     rng = np.random.default_rng(past + n)
     live = past + n

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from tests.q8_model import Q8Model, attend, rotate, sections
-from ttsxabe_b200 import _lib, evicted_len, kv_q8_bytes
+from ttsxabe_b200 import InvalidArgument, UnsupportedAttention, _lib, decode_plan_q8, evicted_len, kv_q8_bytes
 
 
 @pytest.mark.parametrize("kv,hd,cap", [(8, 128, 4096), (20, 64, 1504), (1, 64, 32), (3, 128, 96)])
@@ -71,3 +71,39 @@ def test_model_attention_and_rotation():
     a, b = rotate(q[:1], 3, f), rotate(q[1:2], 10, f)
     c, d = rotate(q[:1], 103, f), rotate(q[1:2], 110, f)
     assert np.allclose((a * b).sum(-1), (c * d).sum(-1))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_plan(hd):
+    most = 148 * (2 if hd == 128 else 3)
+    rng = np.random.default_rng(hd)
+    seen = set()
+    for _ in range(400):
+        kv = int(rng.choice([1, 2, 8, 20]))
+        n = int(rng.integers(1, 33))
+        live = [int(x) for x in np.exp(rng.uniform(0, np.log(40000), n))]
+        grid, cluster, ns = decode_plan_q8(live, kv, hd)
+        pairs, units = n * kv, kv * sum((t + 31) // 32 for t in live)
+        seen.add(cluster)
+        assert ns > 0
+        if cluster:
+            assert grid == pairs * cluster and cluster in (1, 2, 4, 8, 16)
+            assert cluster == 1 or grid <= most
+            assert cluster < 8 or pairs <= (36 if cluster == 8 else 16)
+        else:
+            assert 1 <= grid <= min(most, (units + 3) // 4)
+    assert {0, 1, 2, 4} <= seen
+    assert decode_plan_q8([2048], 8, hd)[1] in (8, 16)
+    assert decode_plan_q8([131072] * 8, 8, hd)[0] <= most
+    # no clusters where the device holds none; nothing for no tokens
+    assert decode_plan_q8([2048], 8, hd, resident=(0, 0))[1] <= 4
+    assert decode_plan_q8([0, 0], 8, hd)[:2] == (0, 0)
+
+
+def test_decode_plan_refusals():
+    with pytest.raises(UnsupportedAttention):
+        decode_plan_q8([5], 8, 96)
+    with pytest.raises(InvalidArgument):
+        decode_plan_q8([5] * 33, 8, 64)
+    with pytest.raises(InvalidArgument):
+        decode_plan_q8([5], 8, 64, sm_count=0)

@@ -25,6 +25,7 @@ from .gpu import (  # noqa: F401
     UnsupportedAttention,
     decode_cut,
     decode_plan,
+    decode_plan_q8,
     evicted_len,
     kv_q8_bytes,
 )

@@ -457,6 +457,28 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
     return run_jobs(g, jobs, q, out, out_f16, heads, kv_heads, head_dim, scale, 1, weigh, scratch);
 }
 
+extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads, size_t head_dim,
+                                               int32_t sm_count, int32_t resident8, int32_t resident16, int32_t *grid,
+                                               int32_t *cluster, int64_t *ns)
+{
+    if ((head_dim != 64 && head_dim != 128) || kv_heads == 0 || kv_heads > 4096) return llmtie_unsupported(head_dim, kv_heads, kv_heads);
+    if (!live || !grid || !cluster || !ns || batch > LLMTIE_Q8_MAX_SEQ || sm_count <= 0) {
+        return llmtie_fail(LLMTIE_ERR_INVALID, "a malformed plan request");
+    }
+    int units[LLMTIE_Q8_MAX_SEQ];
+    for (size_t b = 0; b < batch; b++) {
+        if (live[b] < 0) return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "a context of %d", live[b]);
+        units[b] = (int)(((long long)live[b] + kQ8Block - 1) / kQ8Block);
+    }
+    const int clusters[2] = {resident8, resident16};
+    DecodeQ8Plan plan;
+    plan_decode_q8(plan, units, (int)batch, (int)kv_heads, (int)head_dim, sm_count, clusters);
+    *grid = plan.grid;
+    *cluster = plan.cluster;
+    *ns = (int64_t)(plan.us * 1000.0);
+    return LLMTIE_OK;
+}
+
 extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len, const int32_t *cu_seqlens,
                                               size_t batch, const void *const *caches, const int32_t *past,
                                               const int32_t *cap, size_t heads, size_t kv_heads, size_t head_dim,
