@@ -937,7 +937,7 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
     // goes through memory, and is long where many blocks share a pair: short
     // launches), and for a further wave of blocks of the grid.
     const double all = (hd == 128 ? 842.0 : 1684.0) * sm_count / 148, one = hd == 128 ? 0.7 : 0.6;
-    constexpr double kCluster[5] = {4.0, 4.5, 5.0, 5.4, 6.3}, kPacked = 1.15, kCut = 7.0, kShort = 12.0, kWave = 3.5;
+    constexpr double kCluster[5] = {4.0, 4.5, 5.0, 5.4, 6.3}, kPacked = 1.15, kCut = 7.0, kShort = 16.0, kWave = 3.5;
     const int most = sm_count * (hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT);
     long long total = 0, longest = 0;
     for (int i = 0; i < n; i++) {

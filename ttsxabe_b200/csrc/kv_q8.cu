@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kThreads) q8_rewind_kernel(const __grid_consta
 //
 // Which blocks stay: one block of the grid a (sequence, KV head). Among the
 // blocks that may go, `room` stay: those above the weight `key`, and of those at
-// it the first `ties`. Up to kPickThreads blocks every thread counts the weights
+// it the first `ties`. Up to kPickFew blocks every thread counts the weights
 // that come before its own; of more the room-th largest is found by its bits,
 // eleven at a time (weights are not negative, so their bits order as they do;
 // NaN and negative ones count as zero). One walk in order then moves scales and
@@ -467,6 +467,7 @@ __global__ void __launch_bounds__(kThreads) q8_rewind_kernel(const __grid_consta
 constexpr int kPickThreads = 1024;
 constexpr int kPickKeys = 8192;              // weights held in shared memory
 constexpr int kPickBins = 2048;
+constexpr int kPickFew = 512;                // counting 512 takes 3 us, their bits 6; 1024 the other way about
 
 __device__ __forceinline__ uint32_t weight_key(float w) { return w > 0.0f ? __float_as_uint(w) : 0u; }
 
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
     uint32_t room = all ? 0u : (uint32_t)(sq.keep - sq.first - sq.recent);
     uint32_t key = 0xffffffffu, ties = 0;                        // above key: stays; at it: the first `ties`
     bool chosen = false;                                         // (few blocks: this thread's own stays)
-    const bool few = sq.full <= kPickThreads;
+    const bool few = sq.full <= kPickFew;
     after_previous();
     // Everything whose address is known is asked for first: the first tile's
     // weights and scales, and the tail's rows of this head.
@@ -546,24 +547,26 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int i = i0 + u * kPickThreads;
-                    if (i < kPickKeys) keys[i] = i >= lo && i < hi ? weight_key(x[u]) : 0u;
+                    if (i < kPickKeys) keys[i] = i >= lo && i < hi ? weight_key(x[u]) + (few ? 1u : 0u) : 0u;
                 }
             }
             __syncthreads();
         }
         if (few) {
+            // (keys are one up here, so that 0 stands for blocks that are not to choose from)
             if (tid >= lo && tid < hi) {
-                const uint32_t k = keys[tid];
+                const uint32_t k = keys[tid] + 1u;               // above its own
+                const int at = tid / 4 * 4;
                 uint32_t ahead = 0;                              // those that go before it
-                for (int i = lo / 4 * 4; i < hi; i += 4) {
-                    const uint4 y = *(const uint4 *)&keys[i];
-                    const uint32_t v[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int o = i + e;
-                        ahead += (v[e] > k || (v[e] == k && o < tid)) && o >= lo && o < hi ? 1u : 0u;
+                auto count = [&](int from, int to, uint32_t least) {
+                    for (int i = from; i < to; i += 4) {
+                        const uint4 y = *(const uint4 *)&keys[i];
+                        ahead += (y.x >= least) + (y.y >= least) + (y.z >= least) + (y.w >= least);
                     }
-                }
+                };
+                count(lo / 4 * 4, at, k - 1u);                   // lower ones: as heavy or heavier
+                for (int i = at; i < min(at + 4, hi); i++) ahead += i != tid && keys[i] >= (i < tid ? k - 1u : k);
+                count(at + 4, hi, k);                            // higher ones: heavier
                 chosen = ahead < room;
             }
         } else {
@@ -638,44 +641,78 @@ __global__ void __launch_bounds__(kPickThreads) q8_pick_kernel(const __grid_cons
     }
 }
 
-// Moves the kept blocks' codes: blockIdx = (slice of a block's bytes, keys or
-// values of a head, sequence). Slices move by the same list and never meet, so
-// each may go at its own pace; within one, a group of blocks is read before any
-// of it is written, and later groups lie above what it writes.
+// Moves the kept blocks' codes. Into another cache every block is a copy of its
+// own: blockIdx = (share of the list, keys or values of a head, sequence), a
+// pass of the threads takes kThreads * 16 bytes.
+//
+// In place blockIdx.x is a slice of every block's bytes instead. Slices move by
+// the same list and never meet, so each may go at its own pace; within one, a
+// group of blocks is read before any of it is written, and later groups lie
+// above what it writes, so the next one is on its way meanwhile.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_move_kernel(const __grid_constant__ Q8EvictParams p, int slices)
 {
-    constexpr int DEPTH = 8;
+    constexpr int PIECES = kQ8Block * HD / 16;                   // 16-byte pieces of a block
     after_previous();
     const Q8EvictSeq sq = p.seq[blockIdx.z];
     const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    const int per = kQ8Block * HD / 16 / slices;                 // 16-byte pieces of a slice
-    const int lanes = kThreads / per;                            // blocks a pass of the threads takes
-    const int piece = (int)blockIdx.x * per + threadIdx.x % per, sub = threadIdx.x / per;
     const Q8Layout a = q8_layout(p.kv_heads, HD, sq.src_nb), z = q8_layout(p.kv_heads, HD, sq.dst_nb);
-    const uint4 *src = (const uint4 *)(sq.src + (which ? a.v : a.k)) + (long long)h * sq.src_nb * (kQ8Block * HD / 16) + piece;
-    uint4 *dst = (uint4 *)(sq.dst + (which ? z.v : z.k)) + (long long)h * sq.dst_nb * (kQ8Block * HD / 16) + piece;
+    const uint4 *src = (const uint4 *)(sq.src + (which ? a.v : a.k)) + (long long)h * sq.src_nb * PIECES;
+    uint4 *dst = (uint4 *)(sq.dst + (which ? z.v : z.k)) + (long long)h * sq.dst_nb * PIECES;
     const int *index = p.index + ((long long)blockIdx.z * p.kv_heads + h) * p.max_keep;
-    const bool same = sq.src == sq.dst;
-    for (int j0 = 0; j0 < sq.keep; j0 += lanes * DEPTH) {
-        uint4 x[DEPTH];
-        bool go[DEPTH];
+    if (sq.src != sq.dst) {
+        constexpr int DEPTH = 8, LANES = kThreads / PIECES;
+        const int piece = threadIdx.x % PIECES, sub = threadIdx.x / PIECES;
+        const int share = (sq.keep + (int)gridDim.x - 1) / (int)gridDim.x;
+        const int j1 = min(sq.keep, (int)(blockIdx.x + 1) * share);
+        for (int j0 = (int)blockIdx.x * share; j0 < j1; j0 += LANES * DEPTH) {
+            uint4 x[DEPTH];
 #pragma unroll
-        for (int u = 0; u < DEPTH; u++) {
-            const int j = j0 + u * lanes + sub;
-            go[u] = j < sq.keep;
-            if (go[u]) {
-                const int i = index[j];
-                go[u] = !(same && i == j);
-                if (go[u]) x[u] = src[(long long)i * (kQ8Block * HD / 16)];
+            for (int u = 0; u < DEPTH; u++) {
+                const int j = j0 + u * LANES + sub;
+                if (j < j1) x[u] = src[(long long)index[j] * PIECES + piece];
+            }
+#pragma unroll
+            for (int u = 0; u < DEPTH; u++) {
+                const int j = j0 + u * LANES + sub;
+                if (j < j1) dst[(long long)j * PIECES + piece] = x[u];
             }
         }
-        if (same) __syncthreads();
+        return;
+    }
+    constexpr int DEPTH = 4;
+    if ((int)blockIdx.x >= slices) return;
+    const int per = PIECES / slices, lanes = kThreads / per;     // blocks a pass of the threads takes
+    const int piece = (int)blockIdx.x * per + threadIdx.x % per, sub = threadIdx.x / per;
+    uint4 x[2][DEPTH];
+    bool go[2][DEPTH];
+    auto load = [&](int b, int j0) {
 #pragma unroll
         for (int u = 0; u < DEPTH; u++) {
             const int j = j0 + u * lanes + sub;
-            if (go[u]) dst[(long long)j * (kQ8Block * HD / 16)] = x[u];
+            go[b][u] = false;
+            if (j < sq.keep) {
+                const int i = index[j];
+                go[b][u] = i != j;
+                if (go[b][u]) x[b][u] = src[(long long)i * PIECES + piece];
+            }
         }
+    };
+    auto store = [&](int b, int j0) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; u++) {
+            if (go[b][u]) dst[(long long)(j0 + u * lanes + sub) * PIECES + piece] = x[b][u];
+        }
+    };
+    const int step = lanes * DEPTH;
+    load(0, 0);
+    for (int j0 = 0; j0 < sq.keep; j0 += 2 * step) {
+        load(1, j0 + step);
+        __syncthreads();       // group j0 has been read by all
+        store(0, j0);
+        load(0, j0 + 2 * step);
+        __syncthreads();
+        store(1, j0 + step);
     }
 }
 
@@ -737,10 +774,18 @@ cudaError_t launch_q8_evict(cudaStream_t st, const Q8EvictParams &p, int hd, int
 {
     const cudaError_t e = launch(st, dim3((unsigned)p.kv_heads, (unsigned)p.nseq), kPickThreads, q8_pick_kernel, p, hd);
     if (e != cudaSuccess || p.max_keep == 0) return e;
-    // Slices of no less than 256 bytes, until every SM has a few.
-    const int most = kQ8Block * hd / 256;
-    int slices = 1;
-    while (slices < most && (long long)slices * p.kv_heads * 2 * p.nseq < 4ll * sm_count) slices *= 2;
-    const dim3 grid((unsigned)slices, (unsigned)p.kv_heads * 2, (unsigned)p.nseq);
+    // In place: slices of no less than 256 bytes, until every SM has a few. Into
+    // another cache: shares of no less than a pass of eight loads, the same way.
+    const int most = kQ8Block * hd / 256, rows = p.kv_heads * 2 * p.nseq;
+    bool in_place = false, apart = false;
+    for (int b = 0; b < p.nseq; b++) {
+        if (p.seq[b].src == p.seq[b].dst) in_place = true;
+        else apart = true;
+    }
+    int slices = 1, shares = 1;
+    while (slices < most && (long long)slices * rows < 4ll * sm_count) slices *= 2;
+    const int pass = 8 * kThreads * 16 / (kQ8Block * hd);
+    while (shares * 2 * pass <= p.max_keep + pass && (long long)shares * rows < 8ll * sm_count) shares *= 2;
+    const dim3 grid((unsigned)std::max(in_place ? slices : 1, apart ? shares : 1), (unsigned)p.kv_heads * 2, (unsigned)p.nseq);
     return hd == 128 ? launch(st, grid, kThreads, q8_move_kernel<128>, p, slices) : launch(st, grid, kThreads, q8_move_kernel<64>, p, slices);
 }
