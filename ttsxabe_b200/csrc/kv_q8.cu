@@ -317,19 +317,20 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant
     const long long b = (long long)h * sq.nb + blk;
     const uint4 *codes = (const uint4 *)(sq.base + (which ? at.v : at.k) + b * (kQ8Block * HD));
     const float scale = ((const float *)(sq.base + (which ? at.vs : at.ks)))[b];
-    const uint4 w = tid < kQ8Block * HD / 16 ? codes[tid] : make_uint4(0u, 0u, 0u, 0u);
     if (!which) {
-        // 16 channels of a token
-        const int panel = tid / (kQ8Block * 4), t = tid / 4 % kQ8Block, d = panel * 64 + tid % 4 * 16;
-        if (tid < kQ8Block * HD / 16 && t >= lo && t < hi) {
-            uint4 *o = (uint4 *)(out + t * step + d);
+        // eight channels of a token, so that the lanes of a store write whole sectors
+        constexpr int PER = kQ8Block * HD / 8;
+#pragma unroll
+        for (int i = tid; i < PER; i += kThreads) {
+            const uint2 w = ((const uint2 *)codes)[i];
+            const int panel = i / (kQ8Block * 8), t = i / 8 % kQ8Block, d = panel * 64 + i % 8 * 8;
+            if (t < lo || t >= hi) continue;
             const uint2 w0 = dequant4(w.x, scale), w1 = dequant4(w.y, scale);
-            const uint2 w2 = dequant4(w.z, scale), w3 = dequant4(w.w, scale);
-            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
-            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
+            *(uint4 *)(out + t * step + d) = make_uint4(w0.x, w0.y, w1.x, w1.y);
         }
         return;
     }
+    const uint4 w = tid < kQ8Block * HD / 16 ? codes[tid] : make_uint4(0u, 0u, 0u, 0u);
     // 16 tokens of a channel in, four channels of four tokens out (rows of eight
     // words padded to ten: neither side meets a bank twice)
     __shared__ uint32_t stage[HD * 10];
@@ -354,14 +355,15 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant
 }
 
 // The live tokens as f16 caches that the prefill kernel's tensor maps can be
-// laid over. blockIdx = (kUnpack cache blocks, KV head); a thread turns twice 16
-// codes (16 bytes) of either into 32 bytes, all four loads in flight. Past the live tokens, up to the
+// laid over. blockIdx = (kUnpack cache blocks, KV head); a thread turns four times
+// eight codes of either into 16 bytes (so that the lanes of a store write whole
+// sectors), all eight loads in flight. Past the live tokens, up to the
 // capacity (the next multiple of eight), lie zeros.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_constant__ Q8UnpackParams p)
 {
-    constexpr int PER = kQ8Block * HD / 16;      // 16-byte pieces of a block
-    constexpr int kUnpack = 2 * kThreads / PER;
+    constexpr int PER = kQ8Block * HD / 8;       // pieces of eight codes of a block
+    constexpr int U = 4, kUnpack = U * kThreads / PER;
     const Q8UnpackSeq sq = p.seq[seq_of(p.seq, p.nseq, (int)blockIdx.x)];
     const int blk0 = kUnpack * ((int)blockIdx.x - sq.item0);
     const int h = blockIdx.y, tid = threadIdx.x;
@@ -372,47 +374,36 @@ __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_consta
     uint16_t *ko = sq.k + (long long)h * sq.cap16 * HD, *vo = sq.v + (long long)h * HD * sq.cap16;
     // (the attention kernel behind this one sets itself up meanwhile)
     after_previous();
-    uint4 kc[2], vc[2];
-    float ksc[2], vsc[2];
+    uint2 kc[U], vc[U];
+    float ksc[U], vsc[U];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < U; u++) {
         const int i = tid + u * kThreads, blk = blk0 + i / PER, e = i % PER;
         if (blk < full) {
-            kc[u] = ((const uint4 *)(sq.base + at.k + (b0 + blk) * (kQ8Block * HD)))[e];
-            vc[u] = ((const uint4 *)(sq.base + at.v + (b0 + blk) * (kQ8Block * HD)))[e];
+            kc[u] = ((const uint2 *)(sq.base + at.k + (b0 + blk) * (kQ8Block * HD)))[e];
+            vc[u] = ((const uint2 *)(sq.base + at.v + (b0 + blk) * (kQ8Block * HD)))[e];
             ksc[u] = ks[blk];
             vsc[u] = vs[blk];
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < U; u++) {
         const int i = tid + u * kThreads, blk = blk0 + i / PER, e = i % PER;
         if (blk >= full) continue;
-        {
-            const int panel = e / (kQ8Block * 4), t = e / 4 % kQ8Block, d = panel * 64 + e % 4 * 16;
-            uint4 *o = (uint4 *)(ko + (long long)(32 * blk + t) * HD + d);
-            const uint2 w0 = dequant4(kc[u].x, ksc[u]), w1 = dequant4(kc[u].y, ksc[u]);
-            const uint2 w2 = dequant4(kc[u].z, ksc[u]), w3 = dequant4(kc[u].w, ksc[u]);
-            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
-            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
-        }
-        {
-            const int d = e / 2, t = e % 2 * 16;
-            uint4 *o = (uint4 *)(vo + (long long)d * sq.cap16 + 32 * blk + t);
-            const uint2 w0 = dequant4(vc[u].x, vsc[u]), w1 = dequant4(vc[u].y, vsc[u]);
-            const uint2 w2 = dequant4(vc[u].z, vsc[u]), w3 = dequant4(vc[u].w, vsc[u]);
-            o[0] = make_uint4(w0.x, w0.y, w1.x, w1.y);
-            o[1] = make_uint4(w2.x, w2.y, w3.x, w3.y);
-        }
+        const int panel = e / (kQ8Block * 8), t = e / 8 % kQ8Block, d = panel * 64 + e % 8 * 8;
+        const uint2 k0 = dequant4(kc[u].x, ksc[u]), k1 = dequant4(kc[u].y, ksc[u]);
+        *(uint4 *)(ko + (long long)(32 * blk + t) * HD + d) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+        const uint2 v0 = dequant4(vc[u].x, vsc[u]), v1 = dequant4(vc[u].y, vsc[u]);
+        *(uint4 *)(vo + (long long)(e / 4) * sq.cap16 + 32 * blk + e % 4 * 8) = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
     const int tail = sq.live & 31;
     if (tail && full >= blk0 && full < blk0 + kUnpack) {
         // the tail's rows, and zeros up to the capacity, a multiple of eight
         __shared__ uint32_t rows[kQ8Block][HD / 2 + 1];
-        const uint4 *kt = (const uint4 *)(sq.base + at.kt) + (long long)h * PER * 2;
-        const uint4 *vt = (const uint4 *)(sq.base + at.vt) + (long long)h * PER * 2;
+        const uint4 *kt = (const uint4 *)(sq.base + at.kt) + (long long)h * PER;
+        const uint4 *vt = (const uint4 *)(sq.base + at.vt) + (long long)h * PER;
         const int upto = sq.cap16 - 32 * full;
-        for (int i = tid; i < 2 * PER; i += kThreads) {
+        for (int i = tid; i < PER; i += kThreads) {
             const int t = i / (HD / 8), d = i % (HD / 8);
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u), k = t < tail ? kt[i] : zero, v = t < tail ? vt[i] : zero;
             if (t < upto) ((uint4 *)(ko + (long long)32 * full * HD))[i] = k;
