@@ -185,8 +185,8 @@ static llmtie_status open_impl(int32_t ordinal, void *stream, bool adopt, llmtie
         *g->timeout_host = 0;
         e = cudaHostGetDevicePointer((void **)&g->timeout_site, g->timeout_host, 0);
     }
-    if (e == cudaSuccess) e = cudaMalloc(&g->abort_epoch, sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(g->abort_epoch, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&g->abort_epoch, 4 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(g->abort_epoch, 0, 4 * sizeof(int));
     if (e != cudaSuccess) {
         llmtie_close(g);
         return driver_fail("allocating the status word", e);
@@ -238,7 +238,7 @@ static llmtie_status report_device_timeout(llmtie_gpu *g)
     const int site = *(volatile int *)g->timeout_host;
     if (site == 0) return LLMTIE_OK;
     *(volatile int *)g->timeout_host = 0;
-    cudaMemsetAsync(g->abort_epoch, 0, sizeof(int), g->stream);
+    cudaMemsetAsync(g->abort_epoch, 0, 4 * sizeof(int), g->stream);
     for (llmtie_decode_scratch *s : g->scratches) {
         if (s->ctr) cudaMemsetAsync(s->ctr, 0, s->ctr_words * sizeof(unsigned), g->stream);
         if (s->q8_ctr.ptr) cudaMemsetAsync(s->q8_ctr.ptr, 0, s->q8_ctr.bytes, g->stream);
@@ -267,7 +267,7 @@ static WaitCtl next_wait_ctl(llmtie_gpu *g)
 {
     g->epoch = g->epoch == 0x7fffffff ? 1 : g->epoch + 1;
     return WaitCtl{g->timeout_site, g->abort_epoch, g->epoch, g->wait_cycles, g->sm_count,
-                   &g->ws_part};
+                   g->abort_epoch + 1, &g->ws_part};
 }
 
 extern "C" llmtie_status llmtie_alloc(llmtie_gpu *g, size_t bytes, void **dptr)

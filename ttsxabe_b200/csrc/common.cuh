@@ -378,16 +378,22 @@ struct PrefillTcParams {
     int out_f16;
     int heads, kv_heads, causal;
     int pair_rows;            // pair two row blocks of one head instead of two heads of a group
+    // The launch's items: column x (heads) and row y of item i are i % items_x and
+    // i / items_x (a further items_y rows for each further sequence, where there is no
+    // order). rounds: the grid is a block an SM, which take one after another;
+    // next_item: how many were taken beyond each block's first, and how many blocks are
+    // done; zero between launches.
+    int items, items_x, items_y, rounds;
+    int *next_item;
     float q_scale, sl2;
     int *status;              // set to a site code when a bounded wait gives up
     int *abort_epoch;         // set to `epoch` then: later blocks of this launch leave at once
     int epoch;
     long long wait_cycles;    // how long a wait on a barrier may spin
-    // The work of grid row blockIdx.y, longest first over the whole launch and
+    // The work of row y, longest first over the whole launch and
     // without the empty ones: a (sequence, row-block slot) or, where long row
     // blocks are cut so that a small launch still fills the device, one piece
-    // of its key tiles. n_order == 0 means blockIdx.z is the sequence and
-    // blockIdx.y the row block, whole.
+    // of its key tiles. n_order == 0 means y is the row block, whole.
     int n_order;
     uint32_t order[LLMTIE_TC_MAX_ORDER];   // pieces << 20 | piece << 14 | sequence << 8 | slot
     uint16_t pslot[LLMTIE_TC_MAX_ORDER];   // where a piece's partial result goes
@@ -412,6 +418,7 @@ struct WaitCtl {
     int epoch;
     long long cycles;
     int sm_count;             // SMs of the device (decides whether long row blocks are cut)
+    int *next_item;           // the counters of PrefillTcParams
     Workspace *part;          // where the pieces of cut row blocks leave their partial results
 };
 cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, const WaitCtl &w);

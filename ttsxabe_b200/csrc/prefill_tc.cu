@@ -75,7 +75,8 @@ enum Bar {
     P_FULL = 12,   // +t
     O_DONE = 14,   // +t
     S_FREE = 16,   // +t (head_dim 64 only)
-    NBARS = 18
+    ITEM = 18,     // +slot
+    NBARS = 22
 };
 
 // ---- PTX wrappers -----------------------------------------------------------------
@@ -336,6 +337,13 @@ struct Tile {
     int n;   // key tiles it attends to (0: idle)
 };
 
+struct Item {
+    int x, y;            // grid column and row it stands for
+    int seq, kh, pieces, jbeg, all_keys;
+    int row0, tq, past;  // of the sequence
+    int head[2], r0[2], n[2];
+};
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
@@ -346,6 +354,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
     __shared__ __align__(8) uint64_t bars[NBARS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag_s;
+    __shared__ Item items[4];
     volatile int *abort_flag = &abort_flag_s;
     const Waiter wt = {abort_flag, p.status, p.abort_epoch, p.epoch, p.wait_cycles};
 
@@ -353,49 +362,67 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
     const int warp = tid >> 5;
     const int lane = tid & 31;
 
-    // ---- which two tiles this block carries ------------------------------------------
-    // which sequence and which of its row-block slots (0 = the longest rows)
-    const uint32_t item = p.n_order ? p.order[blockIdx.y] : 0u;
-    const int seq_i = p.n_order ? (int)((item >> 8) & 63u) : (int)blockIdx.z;
-    const int slot_y = p.n_order ? (int)(item & 255u) : (int)blockIdx.y;
-    const int pieces = p.n_order ? (int)(item >> 20) : 1;      // 1: the row block is whole
-    const int piece = (int)((item >> 14) & 63u);
-    const PrefillTcSeq sq = p.seq[seq_i];
-    const int group = p.heads / p.kv_heads;
-    const int row_blocks = (sq.tq + BM - 1) / BM;
-    int kh, head_a, head_b, r0_a, r0_b;
-    // blockIdx.x runs over the heads (neighbours share a KV head's tiles in L2),
-    // blockIdx.y over the row blocks, longest rows first.
-    if (!p.pair_rows) {
-        const int pairs = group >> 1;
-        kh = blockIdx.x / pairs;
-        const int rb = row_blocks - 1 - slot_y;
-        head_a = kh * group + 2 * (blockIdx.x % pairs);
-        head_b = head_a + 1;
-        r0_a = r0_b = rb * BM;
-    } else {
-        kh = blockIdx.x / group;
-        const int rp = (row_blocks + 1) / 2 - 1 - slot_y;
-        head_a = head_b = blockIdx.x;
-        r0_a = 2 * rp * BM;
-        r0_b = (2 * rp + 1) * BM;
-    }
-    const int all_keys = p.causal ? sq.past + sq.tq : sq.tk;
-    auto tiles_of = [&](int r0) {
-        if (r0 < 0 || r0 >= sq.tq) return 0;
-        const int last = p.causal ? min(sq.past + r0 + BM, all_keys) : all_keys;
-        return (last + BN - 1) / BN;
+    // ---- the items this block carries, one after another ------------------------------
+    // An item is two query tiles over a range of key tiles. A launch that fits the
+    // device has a block for each, at its coordinates (p.rounds == 0). Otherwise the
+    // grid is a block an SM; a block's first item is its own number's, and the producer
+    // takes each further one off the launch's counter when it has asked for the last
+    // tiles of the one before, and leaves it in a slot of `items`. (Four of them: the
+    // producer is never more than two steps ahead of the MMAs, and every item but the
+    // first has a step at least.)
+    auto unpack_item = [&](int x, int yz) {
+        Item it;
+        it.x = x;
+        it.y = yz;
+        const int z = it.y / p.items_y;
+        it.y -= z * p.items_y;
+        // which sequence and which of its row-block slots (0 = the longest rows)
+        const uint32_t item = p.n_order ? p.order[it.y] : 0u;
+        it.seq = p.n_order ? (int)((item >> 8) & 63u) : z;
+        const int slot = p.n_order ? (int)(item & 255u) : it.y;
+        it.pieces = p.n_order ? (int)(item >> 20) : 1;         // 1: the row block is whole
+        const int piece = (int)((item >> 14) & 63u);
+        const PrefillTcSeq &sq = p.seq[it.seq];
+        const int group = p.heads / p.kv_heads;
+        const int row_blocks = (sq.tq + BM - 1) / BM;
+        int r0[2];
+        // x runs over the heads (neighbours share a KV head's tiles in L2), y over the
+        // row blocks, longest rows first.
+        if (!p.pair_rows) {
+            const int pairs = group >> 1;
+            it.kh = it.x / pairs;
+            it.head[0] = it.kh * group + 2 * (it.x % pairs);
+            it.head[1] = it.head[0] + 1;
+            r0[0] = r0[1] = (row_blocks - 1 - slot) * BM;
+        } else {
+            it.kh = it.x / group;
+            const int rp = (row_blocks + 1) / 2 - 1 - slot;
+            it.head[0] = it.head[1] = it.x;
+            r0[0] = 2 * rp * BM;
+            r0[1] = (2 * rp + 1) * BM;
+        }
+        it.row0 = sq.row0;
+        it.tq = sq.tq;
+        it.past = sq.past;
+        it.all_keys = p.causal ? sq.past + sq.tq : sq.tk;
+        int all[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            it.r0[t] = r0[t];
+            all[t] = 0;
+            if (r0[t] >= 0 && r0[t] < sq.tq) {
+                const int last = p.causal ? min(sq.past + r0[t] + BM, it.all_keys) : it.all_keys;
+                all[t] = (last + BN - 1) / BN;
+            }
+        }
+        // The key tiles of the item: all of the row block's, or piece `piece` of
+        // `pieces` equal shares (both tiles see the same keys then: pieces are only
+        // cut where the two tiles are two heads at the same rows).
+        it.jbeg = it.pieces > 1 ? (piece * all[0]) / it.pieces : 0;
+        it.n[0] = it.pieces > 1 ? ((piece + 1) * all[0]) / it.pieces - it.jbeg : all[0];
+        it.n[1] = it.pieces > 1 ? it.n[0] : all[1];
+        return it;
     };
-    // The key tiles this block takes: all of the row block's, or piece `piece`
-    // of `pieces` equal shares (both tiles see the same keys then: pieces are
-    // only cut where the two tiles are two heads at the same rows).
-    const int all_a = tiles_of(r0_a), all_b = tiles_of(r0_b);
-    const int jbeg = pieces > 1 ? (piece * all_a) / pieces : 0;
-    const int n_a = pieces > 1 ? ((piece + 1) * all_a) / pieces - jbeg : all_a;
-    const int n_b = pieces > 1 ? n_a : all_b;
-    auto n_of = [n_a, n_b](int t) { return t == 0 ? n_a : n_b; };
-    const int n_max = max(n_a, n_b);
-    if (n_max == 0) return;
 
     // ---- shared memory carve-up (1024-byte aligned for the swizzle) -------------------
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -433,7 +460,12 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
             mbar_init(BAR(O_DONE + s), 1);
             mbar_init(BAR(S_FREE + s), 4);
         }
+        for (int s = 0; s < 4; s++) mbar_init(BAR(ITEM + s), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid == 64) {
+        items[0] = p.rounds ? unpack_item((int)blockIdx.x % p.items_x, (int)blockIdx.x / p.items_x)
+                            : unpack_item((int)blockIdx.x, (int)(blockIdx.y + gridDim.y * blockIdx.z));
     }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
@@ -466,13 +498,25 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
     } else if (warp < 8) {
         // =========================== softmax warpgroups ===================================
         const int t = warp >> 2;
+        bool ok = true;
+        uint32_t steps = 0, done_items = 0;              // this tile's, over the items before
+        for (uint32_t i = 0; ok; i++) {
+        if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 50);
+        if (!ok) break;
+        const Item it = items[i & 3u];
+        if (it.seq < 0) break;
+        const Item &sq = it;
+        const int pieces = it.pieces, jbeg = it.jbeg, all_keys = it.all_keys;
         Tile me;
-        me.head = t == 0 ? head_a : head_b;
-        me.r0 = t == 0 ? r0_a : r0_b;
-        me.n = n_of(t);
+        me.head = t == 0 ? it.head[0] : it.head[1];
+        me.r0 = t == 0 ? it.r0[0] : it.r0[1];
+        me.n = t == 0 ? it.n[0] : it.n[1];
         const int row = tid & 127;                       // query row in the tile = lane
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         if (me.n > 0) {
+            // The tile's four warps are past the item before: its epilogue may have gone
+            // through this memory.
+            if (i > 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
             // -- stage Q: f32 rows -> f16, scaled, into the swizzled K-major layout ------
             {
                 const float *qh = p.q + (long long)sq.row0 * p.q_stride + me.head * HD;
@@ -571,10 +615,9 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
             float m_ref = -CUDART_INF_F;       // in score units
             float l = 0.0f;
             const int my_pos = sq.past + me.r0 + row;   // causal: last key this row sees
-            bool ok = true;
 
             for (int j = 0; j < me.n && ok; j++) {
-                ok = mbar_wait(BAR(S_FULL + t), (uint32_t)(j & 1), wt, 10 + t);
+                ok = mbar_wait(BAR(S_FULL + t), (steps + j) & 1u, wt, 10 + t);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[4][32];
@@ -629,7 +672,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                         // complete. With P over S that is implied (this step's S was
                         // committed after it).
                         if (!pv_done) {
-                            ok = mbar_wait(BAR(O_DONE + t), (uint32_t)((j - 1) & 1), wt, 22 + t);
+                            ok = mbar_wait(BAR(O_DONE + t), (steps + j - 1) & 1u, wt, 22 + t);
                             if (!ok) break;
                             tc_fence_after();
                             pv_done = true;
@@ -652,7 +695,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 }
 
                 if (!pv_done) {
-                    ok = mbar_wait(BAR(O_DONE + t), (uint32_t)((j - 1) & 1), wt, 22 + t);
+                    ok = mbar_wait(BAR(O_DONE + t), (steps + j - 1) & 1u, wt, 22 + t);
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -700,7 +743,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
 
             // -- epilogue: O / l to global ------------------------------------------------
             if (ok) {
-                ok = mbar_wait(BAR(O_DONE + t), kSplit ? (uint32_t)((me.n - 1) & 1) : 0u, wt, 20 + t);
+                ok = mbar_wait(BAR(O_DONE + t), (kSplit ? steps + me.n - 1 : done_items) & 1u, wt, 20 + t);
             }
             if (ok) {
                 tc_fence_after();
@@ -709,7 +752,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 const bool part = pieces > 1;
                 const float inv = part ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
                 const long long ptile =
-                    ((long long)p.pslot[blockIdx.y] * gridDim.x + blockIdx.x) * 2 + t;
+                    ((long long)p.pslot[it.y] * p.items_x + it.x) * 2 + t;
                 if (part) p.part_ml[ptile * BM + row] = make_float2(m_ref * sl2, l);
                 const bool out16 = p.out_f16 && !part;
                 const long long ostride = part ? HD : p.out_stride;      // elements
@@ -806,35 +849,58 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 }
             }
             tc_fence_before();
+            steps += (uint32_t)me.n;
+            done_items++;
+        }
         }
     } else if (warp == 8) {
         // =============================== TMA producer =======================================
+        // (runs ahead into the next item as soon as stages are free)
         if (lane == 0) {
-            const CUtensorMap *kmap = &p.kmap[seq_i];
-            const CUtensorMap *vmap = &p.vmap[seq_i];
-            for (int j = 0; j < n_max; j++) {
-                const int s = j & 1;
-                const uint32_t ph = (uint32_t)((j >> 1) & 1);
-                if (!mbar_wait(BAR(K_EMPTY + s), ph ^ 1u, wt, 30)) break;
-                mbar_expect_tx(BAR(K_FULL + s), TILE_QK);
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++) {
-                    tma_load_3d(k_smem(s) + kt * SUB, kmap, BAR(K_FULL + s), 64 * kt,
-                                (jbeg + j) * BN, kh);
+            bool ok = true;
+            uint32_t k = 0;                                  // steps over all items
+            for (uint32_t i = 0; ok; i++) {
+                Item it = items[0];
+                if (i > 0) {
+                    it.seq = -1;
+                    while (p.rounds) {
+                        const int next = (int)gridDim.x + atomicAdd(p.next_item, 1);
+                        if (next >= p.items) break;
+                        it = unpack_item(next % p.items_x, next / p.items_x);
+                        if (max(it.n[0], it.n[1]) > 0) break;
+                        it.seq = -1;
+                    }
                 }
-                if (!mbar_wait(BAR(V_EMPTY + s), ph ^ 1u, wt, 31)) break;
-                mbar_expect_tx(BAR(V_FULL + s), TILE_V);
-                tma_load_3d(v_smem(s), vmap, BAR(V_FULL + s), (jbeg + j) * BN, 0, kh);
-                tma_load_3d(v_smem(s) + SUBV, vmap, BAR(V_FULL + s), (jbeg + j) * BN + 64, 0, kh);
+                if (i > 0) items[i & 3u] = it;
+                mbar_arrive(BAR(ITEM + (i & 3u)));
+                if (it.seq < 0) break;
+                const CUtensorMap *kmap = &p.kmap[it.seq];
+                const CUtensorMap *vmap = &p.vmap[it.seq];
+                const int n_max = max(it.n[0], it.n[1]);
+                for (int j = 0; j < n_max; j++, k++) {
+                    const int s = (int)(k & 1u);
+                    const uint32_t ph = (k >> 1) & 1u;
+                    ok = mbar_wait(BAR(K_EMPTY + s), ph ^ 1u, wt, 30);
+                    if (!ok) break;
+                    mbar_expect_tx(BAR(K_FULL + s), TILE_QK);
+#pragma unroll
+                    for (int kt = 0; kt < KT; kt++) {
+                        tma_load_3d(k_smem(s) + kt * SUB, kmap, BAR(K_FULL + s), 64 * kt,
+                                    (it.jbeg + j) * BN, it.kh);
+                    }
+                    ok = mbar_wait(BAR(V_EMPTY + s), ph ^ 1u, wt, 31);
+                    if (!ok) break;
+                    mbar_expect_tx(BAR(V_FULL + s), TILE_V);
+                    tma_load_3d(v_smem(s), vmap, BAR(V_FULL + s), (it.jbeg + j) * BN, 0, it.kh);
+                    tma_load_3d(v_smem(s) + SUBV, vmap, BAR(V_FULL + s), (it.jbeg + j) * BN + 64, 0,
+                                it.kh);
+                }
             }
         }
     } else if (warp == 9) {
         // ================================ MMA issuer =========================================
         if (lane == 0) {
             bool ok = true;
-            for (int t = 0; t < 2 && ok; t++) {
-                if (n_of(t) > 0) ok = mbar_wait(BAR(Q_FULL + t), 0u, wt, 40 + t);
-            }
             // Descriptors are built once; a k-step of 16 halves (32 bytes) adds 2
             // to the start-address field, the second 64-wide sub-tile SUB >> 4.
             const uint64_t dq0 = smem_desc(q_smem(0)), dk0 = smem_desc(k_smem(0)),
@@ -862,62 +928,93 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 }
                 if (last || kSplit) tc_commit(BAR(O_DONE + t));
             };
-            if (ok) ok = mbar_wait(BAR(K_FULL + 0), 0u, wt, 42);
-            if (ok) {
-                tc_fence_after();
+            uint32_t k = 0, steps0 = 0, steps1 = 0, q_items = 0;      // over the items before (q_items: bit t)
+            for (uint32_t i = 0; ok; i++) {
+                if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 51);
+                if (!ok) break;
+                const Item it = items[i & 3u];
+                if (it.seq < 0) break;
+                const int n_a = it.n[0], n_b = it.n[1], n_max = max(n_a, n_b);
+                auto n_of = [n_a, n_b](int t) { return t ? n_b : n_a; };
+                if (n_max == 0) continue;
+#pragma unroll 1
                 for (int t = 0; t < 2; t++) {
-                    if (n_of(t) > 0) issue_s(t, 0);
+                    if (n_of(t) > 0 && ok) {
+                        ok = mbar_wait(BAR(Q_FULL + t), (q_items >> t) & 1u, wt, 40 + t);
+                        q_items ^= 1u << t;
+                    }
                 }
-                tc_commit(BAR(K_EMPTY + 0));
-            }
-            for (int j = 0; j < n_max && ok; j++) {
-                const int s = j & 1;
-                const uint32_t ph = (uint32_t)((j >> 1) & 1);
-                bool k_ready = false;
-                if (kSplit) {
-                    // The next step's scores first, each as soon as its softmax
-                    // has taken this step's out of tensor memory.
-                    for (int t = 0; t < 2 && ok; t++) {
-                        if (j + 1 < n_of(t)) {
-                            ok = mbar_wait(BAR(S_FREE + t), (uint32_t)(j & 1), wt, 47 + t);
-                            if (!ok) break;
+                if (!ok) break;
+                ok = mbar_wait(BAR(K_FULL + (k & 1u)), (k >> 1) & 1u, wt, 42);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int t = 0; t < 2; t++) {
+                    if (n_of(t) > 0) issue_s(t, (int)(k & 1u));
+                }
+                tc_commit(BAR(K_EMPTY + (k & 1u)));
+                for (int j = 0; j < n_max && ok; j++) {
+                    const int s = (int)((k + j) & 1u);
+                    const uint32_t ph = ((k + j) >> 1) & 1u, ph_next = ((k + j + 1) >> 1) & 1u;
+                    bool k_ready = false;
+                    if (kSplit) {
+                        // The next step's scores first, each as soon as its softmax
+                        // has taken this step's out of tensor memory.
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (ok && j + 1 < n_of(t)) {
+                                ok = mbar_wait(BAR(S_FREE + t), ((t ? steps1 : steps0) + j) & 1u, wt, 47 + t);
+                                if (ok && !k_ready) {
+                                    ok = mbar_wait(BAR(K_FULL + (s ^ 1)), ph_next, wt, 44);
+                                    k_ready = true;
+                                }
+                                if (ok) {
+                                    tc_fence_after();
+                                    issue_s(t, s ^ 1);
+                                }
+                            }
+                        }
+                        if (!ok) break;
+                        if (j + 1 < n_max) tc_commit(BAR(K_EMPTY + (s ^ 1)));
+                    }
+                    ok = mbar_wait(BAR(V_FULL + s), ph, wt, 43);
+                    if (!ok) break;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        if (ok && j < n_of(t)) {
+                            ok = mbar_wait(BAR(P_FULL + t), ((t ? steps1 : steps0) + j) & 1u, wt, 45 + t);
+                            if (ok) {
+                                tc_fence_after();
+                                issue_pv(t, s, j == 0, j == n_of(t) - 1);
+                            }
+                        }
+                        if (ok && !kSplit && j + 1 < n_of(t)) {
                             if (!k_ready) {
-                                ok = mbar_wait(BAR(K_FULL + (s ^ 1)),
-                                               (uint32_t)(((j + 1) >> 1) & 1), wt, 44);
-                                if (!ok) break;
+                                ok = mbar_wait(BAR(K_FULL + (s ^ 1)), ph_next, wt, 44);
+                                if (ok) tc_fence_after();
                                 k_ready = true;
                             }
-                            tc_fence_after();
-                            issue_s(t, s ^ 1);
+                            if (ok) issue_s(t, s ^ 1);
                         }
                     }
                     if (!ok) break;
-                    if (j + 1 < n_max) tc_commit(BAR(K_EMPTY + (s ^ 1)));
+                    tc_commit(BAR(V_EMPTY + s));
+                    if (!kSplit && j + 1 < n_max) tc_commit(BAR(K_EMPTY + (s ^ 1)));
                 }
-                ok = mbar_wait(BAR(V_FULL + s), ph, wt, 43);
-                if (!ok) break;
-                for (int t = 0; t < 2 && ok; t++) {
-                    if (j < n_of(t)) {
-                        ok = mbar_wait(BAR(P_FULL + t), (uint32_t)(j & 1), wt, 45 + t);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_pv(t, s, j == 0, j == n_of(t) - 1);
-                    }
-                    if (!kSplit && j + 1 < n_of(t)) {
-                        if (!k_ready) {
-                            ok = mbar_wait(BAR(K_FULL + (s ^ 1)), (uint32_t)(((j + 1) >> 1) & 1),
-                                           wt, 44);
-                            if (!ok) break;
-                            tc_fence_after();
-                            k_ready = true;
-                        }
-                        issue_s(t, s ^ 1);
-                    }
-                }
-                if (!ok) break;
-                tc_commit(BAR(V_EMPTY + s));
-                if (!kSplit && j + 1 < n_max) tc_commit(BAR(K_EMPTY + (s ^ 1)));
+                k += (uint32_t)n_max;
+                steps0 += (uint32_t)n_a;
+                steps1 += (uint32_t)n_b;
             }
+        }
+    }
+
+    // The last producer to come here, whether its work is done or given up, leaves the
+    // counters at zero for the next launch: the other roles still have two steps to go.
+    if (warp == 8 && lane == 0 && p.rounds) {
+        __threadfence();
+        if (atomicAdd(p.next_item + 1, 1) == (int)gridDim.x - 1) {
+            atomicExch(p.next_item, 0);
+            atomicExch(p.next_item + 1, 0);
         }
     }
 
@@ -1205,7 +1302,7 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         const int sms = std::max(1, w.sm_count);
         const double share = (double)work * grid.x / sms;
         if (!never && !tp.pair_rows && p.nseq <= 64 && longest >= 8 && longest > 1.25 * share) {
-            constexpr double kBlockCost = 5.5;   // a block's fixed costs, in tile steps
+            constexpr double kBlockCost = 4.0;   // an item's fixed costs, in tile steps
             constexpr double kMergeCost = 5.0;   // the merge kernel, in tile steps
             auto makespan = [&](int c) {
                 std::vector<int> items;
@@ -1297,9 +1394,17 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
             n_pslots = 0;
         }
     }
+    // A block of the grid for every item, or an SM's taking one after another.
+    tp.next_item = w.next_item;
+    tp.items_x = (int)grid.x;
+    tp.items_y = (int)grid.y;
+    tp.items = (int)(grid.x * grid.y * grid.z);
+    const int columns = (int)grid.x, sms = std::max(1, w.sm_count);
+    tp.rounds = tp.items > sms ? 1 : 0;
+    if (tp.rounds) grid = dim3((unsigned)sms);
     void *part = nullptr;
     if (n_pslots > 0) {
-        const size_t tiles = (size_t)n_pslots * grid.x * 2;
+        const size_t tiles = (size_t)n_pslots * columns * 2;
         const size_t o_bytes = tiles * BM * (size_t)hd * sizeof(float);
         const size_t ml_bytes = tiles * BM * sizeof(float2);
         cudaError_t e;
@@ -1334,7 +1439,7 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
             mp.out_stride = p.out_stride;
             mp.out_f16 = p.out_f16;
             mp.heads_per_x = 2;
-            mp.grid_x = (int)grid.x;
+            mp.grid_x = columns;
             for (int b = 0; b < p.nseq; b++) {
                 mp.row0[b] = p.seq[b].row0;
                 mp.tq[b] = p.seq[b].tq;
@@ -1342,7 +1447,7 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
             for (size_t g0 = 0; g0 < groups.size() && err == cudaSuccess; g0 += kMergeGroups) {
                 mp.n_groups = (int)std::min<size_t>(kMergeGroups, groups.size() - g0);
                 for (int i = 0; i < mp.n_groups; i++) mp.group[i] = groups[g0 + i];
-                const dim3 mg((unsigned)mp.n_groups, grid.x * 2, BM / 4);
+                const dim3 mg((unsigned)mp.n_groups, (unsigned)columns * 2, BM / 4);
                 // A programmatic dependent of the attention kernel: its blocks are
                 // set up while that kernel's last blocks still run, and wait for
                 // its end (griddepcontrol.wait) before they read anything.
