@@ -1006,6 +1006,21 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 steps1 += (uint32_t)n_b;
             }
         }
+    } else if (p.rounds) {
+        // ============== the two other warps: the next item's queries into L2 ===================
+        for (uint32_t i = 1;; i++) {
+            if (!mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 52)) break;
+            const Item it = items[i & 3u];
+            if (it.seq < 0) break;
+            // (a warp a tile; the lanes of a line of 128 bytes are one row's)
+            const int t = warp - 10, rows = min(BM, it.tq - (t ? it.r0[1] : it.r0[0]));
+            if ((t ? it.n[1] : it.n[0]) == 0) continue;
+            constexpr int LINES = HD * 4 / 128;
+            const float *q = p.q + (long long)(it.row0 + (t ? it.r0[1] : it.r0[0])) * p.q_stride + (t ? it.head[1] : it.head[0]) * HD;
+            for (int e = lane; e < rows * LINES; e += 32) {
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q + (long long)(e / LINES) * p.q_stride + e % LINES * 32));
+            }
+        }
     }
 
     // The last producer to come here, whether its work is done or given up, leaves the
