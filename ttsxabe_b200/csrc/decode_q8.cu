@@ -23,9 +23,13 @@
 // probabilities through shared memory.
 //
 // The kernel is bound by reading the cache: each warp keeps a ring of its own
-// blocks in flight (cp.async.bulk, an mbarrier a stage), and the grid is cut by
-// work over the blocks of the grid that fit the device at once; a pair (sequence, KV head) that several of
-// them share is merged by the last to arrive.
+// blocks in flight (cp.async.bulk, an mbarrier a stage; two stages, since with
+// three the queue at the memory makes every other load wait: 344 against 301 us
+// for 8 x 131072 keys of 8 heads x 128, which is 6.9-7.1 TB/s). A pair
+// (sequence, KV head) is taken by a cluster of blocks of the grid that merge
+// through distributed shared memory, or the grid is cut by work and the last
+// block to arrive merges (see plan_decode_q8, and there what either costs). The
+// tensor pipe is 20 % busy, so there is no more to gain from tcgen05 here.
 #include "kv_q8.cuh"
 
 #include <math_constants.h>

@@ -11,15 +11,21 @@
 // units), so probabilities are bounded by 2^8 rather than 1 - well inside f16
 // - and the accumulator in tensor memory is rescaled only on those tiles.
 //
-// A block carries two query tiles of 128 rows that share their K/V tiles: two
+// An item of work is two query tiles of 128 rows that share their K/V tiles: two
 // query heads of one KV group at the same positions (grouped models), or two
-// consecutive row blocks of one head (ungrouped). Roles by warp:
+// consecutive row blocks of one head (ungrouped). A launch of more items than SMs
+// runs a block an SM, which takes one item after another (what a block sets up,
+// and the gap to the next, 2 us an item before, it pays once; the next item's
+// first tiles and queries are asked for under the last steps of the one before:
+// 8192 causal positions 492 -> 478 us, the encoder's batch of eight 206 -> 190).
+// Roles by warp:
 //
 //   warps 0-3   softmax of tile A: thread r owns row r (tensor-memory lane r)
 //   warps 4-7   softmax of tile B
 //   warp  8     TMA producer: K tile [128 keys][128] and V tile [128][128 keys]
 //               per step, two stages each, 128-byte swizzle, no multicast
-//   warps 10-11 idle (they complete the third warpgroup for setmaxnreg)
+//   warps 10-11 the next item's queries into L2 (they complete the third warpgroup
+//               for setmaxnreg)
 //   warp  9     MMA issuer: S_t = Q_t K^T (SS), O_t += P_t V (P from tensor
 //               memory), in the order S_A S_B | PV_A S_A' PV_B S_B' | ... so
 //               that one tile's softmax runs under the other tile's MMAs
