@@ -777,7 +777,9 @@ def test_refusals(gpu):
     def evict(src=(t,), sc=(cap,), dst=(u,), dc=(cap,), live=(64,), keep=(1,), first=0, recent=0, **kw):
         gpu.cache_evict_q8(list(src), list(sc), list(dst), list(dc), list(live), list(keep), first, recent, kv, hd, **kw)
 
-    for error, args in [(InvalidArgument, dict(first=1, recent=1)), (InvalidArgument, dict(keep=(-1,))), (CacheOverrun, dict(live=(65,))),
+    for error, args in [(InvalidArgument, dict(first=1, recent=1)), (InvalidArgument, dict(keep=(-1,))),
+                        (InvalidArgument, dict(first=-1, recent=2)), (InvalidArgument, dict(recent=-1)),
+                        (InvalidArgument, dict(first=(1 << 63) + 1, recent=1 << 63)), (CacheOverrun, dict(live=(65,))),
                         (InvalidArgument, dict(dst=(t,), dc=(32,))), (CacheOverrun, dict(dc=(32,), live=(63,), sc=(64,))),
                         (InvalidArgument, dict(src=(t, t), sc=(cap,) * 2, dst=(u, u), dc=(cap,) * 2, live=(64,) * 2, keep=(1,) * 2)),
                         (SliceOverrun, dict(index=torch.zeros(1, dtype=torch.int32, device=gpu.device))),

@@ -358,7 +358,7 @@ extern "C" llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const 
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(src[b], src_cap[b], live[b]));
         const int full = live[b] / kQ8Block;
-        if (keep[b] < 0 || (full > keep[b] && keep_first + keep_recent > (size_t)keep[b])) {
+        if (keep[b] < 0 || (full > keep[b] && (keep_first > (size_t)keep[b] || keep_recent > (size_t)keep[b] - keep_first))) {
             return llmtie_fail(LLMTIE_ERR_INVALID, "keeping %d blocks of which the first %zu and the last %zu stay", keep[b],
                                keep_first, keep_recent);
         }
