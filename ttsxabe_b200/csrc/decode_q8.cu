@@ -323,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     auto load_scales = [&](int blk, float &a, float &b) {
         blk += lane * kWarps;
         if (blk < run.last) {
-            a = __ldg(ks + blk);
-            b = __ldg(vs + blk);
+            a = __ldcg(ks + blk);
+            b = __ldcg(vs + blk);
         }
     };
     auto load_run = [&] {
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (mine) y = __ldg((const float4 *)(qr + 64 * j + 16 * c + 4 * i));
+                if (mine) y = __ldcg((const float4 *)(qr + 64 * j + 16 * c + 4 * i));
                 x[j][4 * i] = y.x; x[j][4 * i + 1] = y.y; x[j][4 * i + 2] = y.z; x[j][4 * i + 3] = y.w;
             }
         }
