@@ -750,6 +750,8 @@ def test_refusals(gpu):
         (SliceOverrun, dict(inv=f[:hd // 2 - 1])), (Misaligned, dict(k=gpu.zeros(2 * kv * hd + 1)[1:])),
         (SliceOverrun, dict(q_out=q[:heads * hd])), (InvalidArgument, dict(q_out=q[4:], cu=(0, 0, 1))), (InvalidArgument, dict(q=gpu.zeros(2 * heads * hd), q_out=k.new_zeros(1), cu=(0, 0, 0), past=(0,))),
         (InvalidArgument, dict(caches=(t, torch.zeros(t.numel(), dtype=torch.uint8)))), (SliceOverrun, dict(caches=(t, u[:-1]))),
+        (InvalidArgument, dict(k=k.half())), (InvalidArgument, dict(v=gpu.zeros(4 * kv * hd)[::2])), (InvalidArgument, dict(q=q.half())),
+        (InvalidArgument, dict(inv=f.double())), (InvalidArgument, dict(q_out=q.double())), (InvalidArgument, dict(cu=(0, 1))),
     ]:
         with pytest.raises(error):
             append(**args)
@@ -761,6 +763,7 @@ def test_refusals(gpu):
         (CacheOverrun, dict(live=(65, 1))), (CacheOverrun, dict(live=(-1, 1))), (UnsupportedAttention, dict(heads=7)),
         (UnsupportedAttention, dict(heads=18, q=gpu.zeros(4 * 18 * hd))), (SliceOverrun, dict(q=q[:-4])), (SliceOverrun, dict(out=q[:-4])),
         (InvalidArgument, dict(caches=(t, t), weigh=True)), (InvalidArgument, dict(out=q.double())), (InvalidArgument, dict(live=(1,))),
+        (InvalidArgument, dict(q=q.half())), (InvalidArgument, dict(out=gpu.zeros(4 * heads * hd)[::2])),
         (Misaligned, dict(out=gpu.zeros(2 * heads * hd + 1)[1:])), (RaggedBlock, dict(caps=(40, 64))),
     ]:
         with pytest.raises(error):

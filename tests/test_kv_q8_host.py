@@ -4,9 +4,10 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 from tests.q8_model import Q8Model, attend, rotate, sections
-from ttsxabe_b200 import InvalidArgument, UnsupportedAttention, _lib, decode_plan_q8, evicted_len, kv_q8_bytes
+from ttsxabe_b200 import Gpu, InvalidArgument, UnsupportedAttention, _lib, decode_plan_q8, evicted_len, kv_q8_bytes
 
 
 @pytest.mark.parametrize("kv,hd,cap", [(8, 128, 4096), (20, 64, 1504), (1, 64, 32), (3, 128, 96)])
@@ -107,3 +108,31 @@ def test_decode_plan_refusals():
         decode_plan_q8([5] * 33, 8, 64)
     with pytest.raises(InvalidArgument):
         decode_plan_q8([5], 8, 64, sm_count=0)
+
+
+def test_a_cache_of_another_device_is_refused():
+    """A list of caches is checked before the table of their addresses is made."""
+    class Cache:
+        is_cuda, device = True, torch.device("cuda", 1)
+
+        def numel(self):
+            return 1 << 20
+
+        def element_size(self):
+            return 1
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 1 << 20
+
+    def table(ordinal, caches, cap):
+        gpu = Gpu.__new__(Gpu)
+        gpu._h, gpu.ordinal = None, ordinal
+        return gpu._q8_table(caches, cap, 2, 64)
+
+    assert table(1, [Cache()], [64])[0] == 1 << 20
+    for args in [(0, [Cache()], [64]), (1, [torch.zeros(1 << 20)], [64])]:
+        with pytest.raises(InvalidArgument, match="not cuda"):
+            table(*args)

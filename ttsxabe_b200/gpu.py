@@ -634,8 +634,7 @@ class Gpu:
     # the layout). Where a list of them is given, each is checked against its
     # capacity; a table made by `ptr_table` is taken as it is.
 
-    @staticmethod
-    def _q8_table(caches, cap, kv_heads, head_dim) -> C.Array:
+    def _q8_table(self, caches, cap, kv_heads, head_dim) -> C.Array:
         if isinstance(caches, C.Array):
             return caches
         if len(caches) != len(cap):
@@ -643,11 +642,16 @@ class Gpu:
         for t, c in zip(caches, cap):
             need = kv_q8_bytes(kv_heads, head_dim, int(c)) if c > 0 else 0
             have = t.numel() * t.element_size()
-            if not t.is_cuda:
-                raise InvalidArgument("an 8-bit cache in host memory")
+            if not t.is_cuda or t.device.index != self.ordinal:
+                raise InvalidArgument(f"an 8-bit cache on {t.device}, not cuda:{self.ordinal}")
             if have < need or not t.is_contiguous():
                 raise SliceOverrun(f"reading to {need} in a buffer of {have}")
         return Gpu._ptr_table(caches)
+
+    @staticmethod
+    def _not_rows(*tensors) -> InvalidArgument:
+        bad = [f"{t.dtype}{'' if t.is_contiguous() else ', strided'}" for t in tensors if t is not None]
+        return InvalidArgument(f"rows want contiguous float32 tensors, got {'; '.join(bad)}")
 
     @staticmethod
     def _tables_of(n: int, *tables) -> None:
@@ -684,6 +688,13 @@ class Gpu:
             self._tables_of(n, cap, past, pos)
         if len(cu_seqlens) <= n:
             raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
+        f32 = torch.float32
+        if (k.dtype is not f32 or v.dtype is not f32 or not k.is_contiguous()
+                or not v.is_contiguous()
+                or (inv_freq is not None and inv_freq.dtype is not f32)
+                or (q is not None and (q.dtype is not f32 or not q.is_contiguous()))
+                or (q_out is not None and (q_out.dtype is not f32 or not q_out.is_contiguous()))):
+            raise self._not_rows(q, k, v, inv_freq, q_out)
         if q_out is None:
             q_out = q
         _check(self._lib.llmtie_rope_append_q8(
@@ -708,6 +719,10 @@ class Gpu:
             k_out = self._empty(cu_seqlens[n] * kv_heads * head_dim, torch.float16)
         if v_out is None:
             v_out = self._empty(cu_seqlens[n] * kv_heads * head_dim, torch.float16)
+        f16 = torch.float16
+        if k_out.dtype is not f16 or v_out.dtype is not f16 or not (k_out.is_contiguous()
+                                                                     and v_out.is_contiguous()):
+            raise InvalidArgument(f"reading into {k_out.dtype} and {v_out.dtype}")
         _check(self._lib.llmtie_cache_read_q8(
             self._h, table, self._i32_table(cap), self._i32_table(live), self._i32_table(first),
             self._i32_table(cu_seqlens), n, kv_heads, head_dim, k_out.data_ptr(), k_out.numel(),
@@ -738,6 +753,8 @@ class Gpu:
             self._tables_of(n, cap, live)
         if out is None:
             out = self.uninit(n * heads * head_dim)
+        if q.dtype is not torch.float32 or not q.is_contiguous():
+            raise self._not_rows(q)
         _check(self._lib.llmtie_decode_batched_q8(
             self._h, q.data_ptr(), q.numel(), table, self._i32_table(live), self._i32_table(cap),
             n, heads, kv_heads, head_dim, scale, int(bool(weigh)), scratch._bind(self),
@@ -755,6 +772,8 @@ class Gpu:
             raise InvalidArgument(f"{len(cu_seqlens)} row offsets for a batch of {n}")
         if out is None:
             out = self.uninit(int(cu_seqlens[n]) * heads * head_dim)
+        if q.dtype is not torch.float32 or not q.is_contiguous():
+            raise self._not_rows(q)
         _check(self._lib.llmtie_flash_attn_q8(
             self._h, q.data_ptr(), q.numel(), self._i32_table(cu_seqlens), n, table,
             self._i32_table(past), self._i32_table(cap), heads, kv_heads, head_dim, scale,
@@ -763,9 +782,10 @@ class Gpu:
 
     @staticmethod
     def _f16_out(out: torch.Tensor) -> int:
-        if out.dtype not in (torch.float32, torch.float16):
-            raise InvalidArgument(f"an output of {out.dtype}")
-        return int(out.dtype == torch.float16)
+        kind = out.dtype
+        if (kind is not torch.float16 and kind is not torch.float32) or not out.is_contiguous():
+            raise InvalidArgument(f"an output of {kind} with strides {out.stride()}")
+        return kind is torch.float16
 
     def cache_evict_q8(self, src, src_cap, dst, dst_cap, live, keep, keep_first, keep_recent,
                        kv_heads, head_dim, index=None) -> None:
@@ -775,8 +795,8 @@ class Gpu:
         s = self._q8_table(src, src_cap, kv_heads, head_dim)
         d = self._q8_table(dst, dst_cap, kv_heads, head_dim)
         self._tables_of(len(s), d, src_cap, dst_cap, live, keep)
-        if index is not None and index.dtype != torch.int32:
-            raise InvalidArgument(f"an index of {index.dtype}")
+        if index is not None and (index.dtype != torch.int32 or not index.is_contiguous()):
+            raise InvalidArgument(f"an index of {index.dtype} with strides {index.stride()}")
         _check(self._lib.llmtie_cache_evict_q8(
             self._h, s, self._i32_table(src_cap), d, self._i32_table(dst_cap),
             self._i32_table(live), self._i32_table(keep), len(s), keep_first, keep_recent,
