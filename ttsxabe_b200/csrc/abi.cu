@@ -126,6 +126,11 @@ llmtie_status LaunchScope::done()
 
 // ---- handle ---------------------------------------------------------------
 
+// The words of a handle: its abort_epoch, two counters for the prefill launches of its
+// stream, and two for each that is captured.
+constexpr int kCapturedLaunches = 8192;
+constexpr size_t kHandleWords = 3 + 2 * (size_t)kCapturedLaunches;
+
 static llmtie_status open_impl(int32_t ordinal, void *stream, bool adopt, llmtie_gpu **out)
 {
     if (!out) return llmtie_fail(LLMTIE_ERR_INVALID, "null output handle");
@@ -185,8 +190,8 @@ static llmtie_status open_impl(int32_t ordinal, void *stream, bool adopt, llmtie
         *g->timeout_host = 0;
         e = cudaHostGetDevicePointer((void **)&g->timeout_site, g->timeout_host, 0);
     }
-    if (e == cudaSuccess) e = cudaMalloc(&g->abort_epoch, 4 * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(g->abort_epoch, 0, 4 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&g->abort_epoch, kHandleWords * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(g->abort_epoch, 0, kHandleWords * sizeof(int));
     if (e != cudaSuccess) {
         llmtie_close(g);
         return driver_fail("allocating the status word", e);
@@ -238,7 +243,7 @@ static llmtie_status report_device_timeout(llmtie_gpu *g)
     const int site = *(volatile int *)g->timeout_host;
     if (site == 0) return LLMTIE_OK;
     *(volatile int *)g->timeout_host = 0;
-    cudaMemsetAsync(g->abort_epoch, 0, 4 * sizeof(int), g->stream);
+    cudaMemsetAsync(g->abort_epoch, 0, kHandleWords * sizeof(int), g->stream);
     for (llmtie_decode_scratch *s : g->scratches) {
         if (s->ctr) cudaMemsetAsync(s->ctr, 0, s->ctr_words * sizeof(unsigned), g->stream);
         if (s->q8_ctr.ptr) cudaMemsetAsync(s->q8_ctr.ptr, 0, s->q8_ctr.bytes, g->stream);
@@ -262,12 +267,20 @@ extern "C" llmtie_status llmtie_set_wait_limit_cycles(llmtie_gpu *g, int64_t cyc
 }
 
 // What a tensor-memory prefill launch is given for its bounded waits; every
-// launch gets a number of its own.
+// launch gets a number of its own. The counters its blocks go by belong to the
+// handle for a launch on its stream, where one follows another; a captured launch has
+// its own, since graphs may be replayed beside each other on other streams. Once those
+// are used up a captured launch has none and takes a block for every item.
 static WaitCtl next_wait_ctl(llmtie_gpu *g)
 {
     g->epoch = g->epoch == 0x7fffffff ? 1 : g->epoch + 1;
-    return WaitCtl{g->timeout_site, g->abort_epoch, g->epoch, g->wait_cycles, g->sm_count,
-                   g->abort_epoch + 1, &g->ws_part};
+    int *counters = g->abort_epoch + 1;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(g->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+        counters = g->captured < kCapturedLaunches ? g->abort_epoch + 3 + 2 * g->captured++ : nullptr;
+    }
+    return WaitCtl{g->timeout_site, g->abort_epoch, g->epoch, g->wait_cycles, g->sm_count, counters,
+                   &g->ws_part};
 }
 
 extern "C" llmtie_status llmtie_alloc(llmtie_gpu *g, size_t bytes, void **dptr)

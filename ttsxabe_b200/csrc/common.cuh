@@ -56,6 +56,7 @@ struct llmtie_gpu {
     // later leave at once; other launches are not affected.
     int *abort_epoch = nullptr;
     int epoch = 0;
+    int captured = 0;    // prefill launches that were captured (the counters of each lie behind that word)
     // How long a device-side wait may spin, in SM cycles (about a second).
     long long wait_cycles = 1ll << 31;
     // Every DecodeScratch made through this handle: their arrival counters
@@ -418,7 +419,7 @@ struct WaitCtl {
     int epoch;
     long long cycles;
     int sm_count;             // SMs of the device (decides whether long row blocks are cut)
-    int *next_item;           // the counters of PrefillTcParams
+    int *next_item;           // the counters of PrefillTcParams, or null: a block for every item
     Workspace *part;          // where the pieces of cut row blocks leave their partial results
 };
 cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, const WaitCtl &w);

@@ -1421,7 +1421,7 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
     tp.items_y = (int)grid.y;
     tp.items = (int)(grid.x * grid.y * grid.z);
     const int columns = (int)grid.x, sms = std::max(1, w.sm_count);
-    tp.rounds = tp.items > sms ? 1 : 0;
+    tp.rounds = tp.next_item && tp.items > sms ? 1 : 0;
     if (tp.rounds) grid = dim3((unsigned)sms);
     void *part = nullptr;
     if (n_pslots > 0) {
