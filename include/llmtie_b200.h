@@ -535,8 +535,9 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
  *   value tail   f16  [kv_heads][32][head_dim]
  * How many tokens it holds is the caller's to know (its `live` or `past`).
  * head_dim is 64 or 128. The entries take HOST tables with a cache, a capacity
- * and lengths for each sequence, any number of sequences a call; caches that
- * one call writes must not share memory. A capacity that is not a multiple of
+ * and lengths for each sequence, up to 65536 sequences a call; caches that one
+ * call writes must not share memory, nor may an output share any with the
+ * query (but for rows that are rotated in place). A capacity that is not a multiple of
  * 32 is refused with LLMTIE_ERR_RAGGED_BLOCK.
  *
  * Calls may be captured into a CUDA graph once the same call has been made

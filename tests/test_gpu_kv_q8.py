@@ -764,6 +764,7 @@ def test_refusals(gpu):
         (UnsupportedAttention, dict(heads=18, q=gpu.zeros(4 * 18 * hd))), (SliceOverrun, dict(q=q[:-4])), (SliceOverrun, dict(out=q[:-4])),
         (InvalidArgument, dict(caches=(t, t), weigh=True)), (InvalidArgument, dict(out=q.double())), (InvalidArgument, dict(live=(1,))),
         (InvalidArgument, dict(q=q.half())), (InvalidArgument, dict(out=gpu.zeros(4 * heads * hd)[::2])),
+        (InvalidArgument, dict(out=q)), (InvalidArgument, dict(out=q.view(torch.float16)[heads * hd:])),
         (Misaligned, dict(out=gpu.zeros(2 * heads * hd + 1)[1:])), (RaggedBlock, dict(caps=(40, 64))),
     ]:
         with pytest.raises(error):
@@ -773,7 +774,8 @@ def test_refusals(gpu):
         gpu.flash_attn_q8(q, list(cu), list(caches), list(caps), list(past), heads, kv, hd, 0.1, True, **kw)
 
     for error, args in [(CacheOverrun, dict(past=(64, 0))), (CacheOverrun, dict(past=(-1, 0))), (UnsupportedAttention, dict(heads=7)),
-                        (SliceOverrun, dict(cu=(0, 1, 3))), (InvalidArgument, dict(cu=(0, 2, 1))), (Misaligned, dict(q=gpu.zeros(2 * heads * hd + 1)[1:]))]:
+                        (SliceOverrun, dict(cu=(0, 1, 3))), (InvalidArgument, dict(cu=(0, 2, 1))), (Misaligned, dict(q=gpu.zeros(2 * heads * hd + 1)[1:])),
+                        (InvalidArgument, dict(out=q)), (InvalidArgument, dict(q=q.half()))]:
         with pytest.raises(error):
             flash(**args)
 
@@ -795,6 +797,11 @@ def test_refusals(gpu):
         gpu.cache_rewind_q8([t, t], [cap] * 2, [40] * 2, [33] * 2, kv, hd)
     with pytest.raises(CacheOverrun):
         gpu.cache_read_q8([t], [cap], [10], [5], [0, 6], kv, hd)
+    rows = torch.empty(5 * kv * hd, dtype=torch.float16, device=gpu.device)
+    with pytest.raises(InvalidArgument):
+        gpu.cache_read_q8([t], [cap], [10], [5], [0, 5], kv, hd, k_out=rows, v_out=rows)
+    with pytest.raises(InvalidArgument):
+        gpu.cache_read_q8([t], [cap], [10], [5], [0, 5], kv, hd, k_out=rows.float(), v_out=rows)
     with pytest.raises(SliceOverrun):
         gpu.cache_read_q8([t], [cap], [10], [5], [0, 5], kv, hd, k_out=torch.empty(4, dtype=torch.float16, device=gpu.device))
     with pytest.raises(CacheOverrun):

@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <new>
 #include <utility>
 #include <vector>
 
@@ -27,7 +28,7 @@ llmtie_status check_geometry(llmtie_gpu *g, size_t batch, size_t kv_heads, size_
     cudaSetDevice(g->ordinal);
     if ((hd != 64 && hd != 128) || kv_heads == 0) return llmtie_unsupported(hd, kv_heads, kv_heads);
     if (kv_heads > 4096) return llmtie_fail(LLMTIE_ERR_INVALID, "an 8-bit cache of %zu KV heads", kv_heads);
-    if (!fits_i32(batch)) return llmtie_fail(LLMTIE_ERR_INVALID, "a batch of %zu", batch);
+    if (batch > 65536) return llmtie_fail(LLMTIE_ERR_INVALID, "a batch of %zu", batch);
     return LLMTIE_OK;
 }
 
@@ -58,6 +59,11 @@ llmtie_status check_apart(std::vector<std::pair<uintptr_t, size_t>> &spans)
     return LLMTIE_OK;
 }
 
+bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
+{
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
 llmtie_status overrun(size_t need, size_t have)
 {
     return llmtie_fail(LLMTIE_ERR_SLICE_OVERRUN, "reading to %zu in a buffer of %zu", need, have);
@@ -73,6 +79,13 @@ llmtie_status check_rows(const int32_t *cu, size_t batch, size_t *total)
     *total = (size_t)cu[batch];
     return LLMTIE_OK;
 }
+
+// (the tables an entry makes may find no memory: an error, not an exception)
+#define NO_MEMORY_IS_AN_ERROR                                                              \
+    catch (const std::bad_alloc &)                                                         \
+    {                                                                                      \
+        return llmtie_fail(LLMTIE_ERR_DRIVER, "no host memory for the tables of the call"); \
+    }
 
 #define TRY(x)                              \
     do {                                    \
@@ -196,7 +209,7 @@ extern "C" llmtie_status llmtie_rope_append_q8(llmtie_gpu *g, const float *q, si
                                                const int32_t *past, const int32_t *pos, const int32_t *cap,
                                                const float *inv_freq, size_t inv_len, size_t heads, size_t kv_heads,
                                                size_t head_dim)
-{
+try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!cu_seqlens || !caches || !past || !pos || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
     if (batch == 0) return LLMTIE_OK;
@@ -218,9 +231,8 @@ extern "C" llmtie_status llmtie_rope_append_q8(llmtie_gpu *g, const float *q, si
         if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
         if (((uintptr_t)q_out & 15u) != 0) return llmtie_misaligned("the rotated query", q_out, 16);
         // in place, or clear of everything the call reads
-        const uintptr_t o0 = (uintptr_t)q_out, o1 = o0 + need * 4;
-        auto meets = [&](const float *x, size_t n) { return o0 < (uintptr_t)x + n * 4 && (uintptr_t)x < o1; };
-        if ((q_out != q && meets(q, need)) || meets(k, total * kv_heads * head_dim) || meets(v, total * kv_heads * head_dim)) {
+        const size_t kv_bytes = total * kv_heads * head_dim * 4;
+        if ((q_out != q && meet(q_out, need * 4, q, need * 4)) || meet(q_out, need * 4, k, kv_bytes) || meet(q_out, need * 4, v, kv_bytes)) {
             return llmtie_fail(LLMTIE_ERR_INVALID, "the rotated query overlaps the rows the call reads");
         }
     }
@@ -267,6 +279,7 @@ extern "C" llmtie_status llmtie_rope_append_q8(llmtie_gpu *g, const float *q, si
     }
     return LLMTIE_OK;
 }
+NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *caches, const int32_t *cap,
                                               const int32_t *live, const int32_t *first, const int32_t *cu_seqlens,
@@ -284,6 +297,9 @@ extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *
     if (total > (size_t)cu_seqlens[0] && (!k_out || !v_out)) return llmtie_fail(LLMTIE_ERR_INVALID, "null output pointer");
     if (((uintptr_t)k_out & 15u) != 0) return llmtie_misaligned("the keys read", k_out, 16);
     if (((uintptr_t)v_out & 15u) != 0) return llmtie_misaligned("the values read", v_out, 16);
+    if (meet(k_out, total * kv_heads * head_dim * 2, v_out, total * kv_heads * head_dim * 2)) {
+        return llmtie_fail(LLMTIE_ERR_INVALID, "the keys and the values go to the same rows");
+    }
     for (size_t b = 0; b < batch; b++) {
         const int n = cu_seqlens[b + 1] - cu_seqlens[b];
         if (n == 0) continue;
@@ -316,7 +332,7 @@ extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *
 extern "C" llmtie_status llmtie_cache_rewind_q8(llmtie_gpu *g, void *const *caches, const int32_t *cap,
                                                 const int32_t *live, const int32_t *to, size_t batch, size_t kv_heads,
                                                 size_t head_dim)
-{
+try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!caches || !cap || !live || !to) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
     std::vector<std::pair<uintptr_t, size_t>> spans;
@@ -345,12 +361,13 @@ extern "C" llmtie_status llmtie_cache_rewind_q8(llmtie_gpu *g, void *const *cach
     }
     return LLMTIE_OK;
 }
+NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const *src, const int32_t *src_cap,
                                                void *const *dst, const int32_t *dst_cap, const int32_t *live,
                                                const int32_t *keep, size_t batch, size_t keep_first, size_t keep_recent,
                                                size_t kv_heads, size_t head_dim, int32_t *index, size_t index_len)
-{
+try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!src || !src_cap || !dst || !dst_cap || !live || !keep) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
     std::vector<std::pair<uintptr_t, size_t>> spans;
@@ -407,6 +424,7 @@ extern "C" llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const 
     }
     return LLMTIE_OK;
 }
+NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_cache_grow_q8(llmtie_gpu *g, const void *src, size_t src_len, void *dst, size_t dst_len,
                                               size_t kv_heads, size_t head_dim, size_t old_cap, size_t new_cap,
@@ -432,7 +450,7 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
                                                   size_t kv_heads, size_t head_dim, float scale, int32_t weigh,
                                                   llmtie_decode_scratch *scratch, void *out, size_t out_len,
                                                   int32_t out_f16)
-{
+try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!scratch) return llmtie_fail(LLMTIE_ERR_INVALID, "null decode scratch");
     if (!caches || !live || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
@@ -444,6 +462,7 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
     if (!q || !out) return llmtie_fail(LLMTIE_ERR_INVALID, "null query or output");
     if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
     if (((uintptr_t)out & 15u) != 0) return llmtie_misaligned("the output", out, 16);
+    if (meet(q, batch * n * 4, out, batch * n * (out_f16 ? 2 : 4))) return llmtie_fail(LLMTIE_ERR_INVALID, "the output overlaps the query");
     std::vector<std::pair<uintptr_t, size_t>> spans;
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(caches[b], cap[b], live[b]));
@@ -456,6 +475,7 @@ extern "C" llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q,
     }
     return run_jobs(g, jobs, q, out, out_f16, heads, kv_heads, head_dim, scale, 1, weigh, scratch);
 }
+NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads, size_t head_dim,
                                                int32_t sm_count, int32_t resident8, int32_t resident16, int32_t *grid,
@@ -483,7 +503,7 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
                                               size_t batch, const void *const *caches, const int32_t *past,
                                               const int32_t *cap, size_t heads, size_t kv_heads, size_t head_dim,
                                               float scale, int32_t causal, void *out, size_t out_len, int32_t out_f16)
-{
+try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!cu_seqlens || !caches || !past || !cap) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
     if (heads % kv_heads != 0 || heads == 0 || heads > 65535) return llmtie_unsupported(head_dim, heads, kv_heads);
@@ -495,6 +515,7 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
     if (total > (size_t)cu_seqlens[0] && (!q || !out)) return llmtie_fail(LLMTIE_ERR_INVALID, "null query or output");
     if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
     if (((uintptr_t)out & 15u) != 0) return llmtie_misaligned("the output", out, 16);
+    if (meet(q, total * n * 4, out, total * n * (out_f16 ? 2 : 4))) return llmtie_fail(LLMTIE_ERR_INVALID, "the output overlaps the query");
     for (size_t b = 0; b < batch; b++) {
         const int rows = cu_seqlens[b + 1] - cu_seqlens[b];
         if (rows == 0) continue;
@@ -627,3 +648,4 @@ extern "C" llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, siz
     }
     return LLMTIE_OK;
 }
+NO_MEMORY_IS_AN_ERROR
