@@ -362,15 +362,12 @@ struct PrefillParams {
 cudaError_t launch_prefill_mma(cudaStream_t st, const PrefillParams &p, int hd);
 
 // prefill_tc.cu: the tensor-memory kernel for aligned f16 caches at head_dim 64 or 128.
-#define LLMTIE_TC_MAX_SEQ 8
+#define LLMTIE_TC_MAX_SEQ 32
 struct PrefillTcSeq {
     int row0, tq, past, tk;   // tk: keys the sequence holds (past + tq when causal)
 };
-#define LLMTIE_TC_MAX_ORDER 1024
-struct PrefillTcParams {
-    alignas(64) CUtensorMap kmap[LLMTIE_TC_MAX_SEQ];
-    alignas(64) CUtensorMap vmap[LLMTIE_TC_MAX_SEQ];
-    PrefillTcSeq seq[LLMTIE_TC_MAX_SEQ];
+#define LLMTIE_TC_MAX_ORDER 2048
+struct PrefillTcCommon {
     int nseq;
     const float *q;
     long long q_stride;
@@ -396,8 +393,6 @@ struct PrefillTcParams {
     // blocks are cut so that a small launch still fills the device, one piece
     // of its key tiles. n_order == 0 means y is the row block, whole.
     int n_order;
-    uint32_t order[LLMTIE_TC_MAX_ORDER];   // pieces << 20 | piece << 14 | sequence << 8 | slot
-    uint16_t pslot[LLMTIE_TC_MAX_ORDER];   // where a piece's partial result goes
     // Partial results of the pieces, merged by prefill_merge_kernel:
     // part_o [pslot][gridDim.x][2 tiles][128 rows][hd] f32, un-normalised,
     // part_ml [..][128 rows] (reference maximum in log2 units, sum).
@@ -406,6 +401,18 @@ struct PrefillTcParams {
     // RoPE fused into the staging of q (or null: q arrives rotated): per packed
     // row, hd/2 cosines then hd/2 sines of the row's position.
     const float *rope_tab;
+};
+// With room for S sequences and O rows of the order: a launch takes the least of the
+// sizes that holds it (see launch_prefill_tc).
+template <int S, int O>
+struct PrefillTcParams : PrefillTcCommon {
+    static constexpr int kSeq = S, kOrder = O;
+    alignas(64) CUtensorMap kmap[S];
+    alignas(64) CUtensorMap vmap[S];
+    PrefillTcSeq seq[S];
+    static_assert(S <= 32 && O <= 2048, "what an entry of the order has room for");
+    uint32_t order[O];   // pieces << 24 | piece << 16 | sequence << 11 | slot
+    uint16_t pslot[O];   // where a piece's partial result goes
 };
 // One row block whose key tiles were cut into pieces: where its rows go.
 struct PrefillMergeGroup {

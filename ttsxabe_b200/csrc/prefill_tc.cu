@@ -350,9 +350,9 @@ struct Item {
     int head[2], r0[2], n[2];
 };
 
-template <int HD>
+template <int HD, typename Params>
 __global__ void __launch_bounds__(kThreads, 1)
-prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
+prefill_tc_kernel(const __grid_constant__ Params p)
 {
     using G = Geo<HD>;
     constexpr int TILE_QK = G::TILE_QK, TILE_V = G::TILE_V, SUBV = G::SUBV, KT = G::KT;
@@ -384,10 +384,10 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
         it.y -= z * p.items_y;
         // which sequence and which of its row-block slots (0 = the longest rows)
         const uint32_t item = p.n_order ? p.order[it.y] : 0u;
-        it.seq = p.n_order ? (int)((item >> 8) & 63u) : z;
-        const int slot = p.n_order ? (int)(item & 255u) : it.y;
-        it.pieces = p.n_order ? (int)(item >> 20) : 1;         // 1: the row block is whole
-        const int piece = (int)((item >> 14) & 63u);
+        it.seq = p.n_order ? (int)((item >> 11) & 31u) : z;
+        const int slot = p.n_order ? (int)(item & 2047u) : it.y;
+        it.pieces = p.n_order ? (int)(item >> 24) : 1;         // 1: the row block is whole
+        const int piece = (int)((item >> 16) & 255u);
         const PrefillTcSeq &sq = p.seq[it.seq];
         const int group = p.heads / p.kv_heads;
         const int row_blocks = (sq.tq + BM - 1) / BM;
@@ -758,7 +758,7 @@ prefill_tc_kernel(const __grid_constant__ PrefillTcParams p)
                 const bool part = pieces > 1;
                 const float inv = part ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
                 const long long ptile =
-                    ((long long)p.pslot[it.y] * p.items_x + it.x) * 2 + t;
+                    ((long long)(part ? p.pslot[it.y] : 0) * p.items_x + it.x) * 2 + t;
                 if (part) p.part_ml[ptile * BM + row] = make_float2(m_ref * sl2, l);
                 const bool out16 = p.out_f16 && !part;
                 const long long ostride = part ? HD : p.out_stride;      // elements
@@ -1182,8 +1182,35 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const __grid_constan
     }
 }
 
-const KernelReg reg_tc("flash_attn_h_tc", (const void *)prefill_tc_kernel<128>);
-const KernelReg reg_tc64("flash_attn_64_tc", (const void *)prefill_tc_kernel<64>);
+using Params1 = PrefillTcParams<1, 256>;
+using Params8 = PrefillTcParams<8, 1024>;
+using ParamsMost = PrefillTcParams<LLMTIE_TC_MAX_SEQ, LLMTIE_TC_MAX_ORDER>;
+
+const KernelReg reg_tc("flash_attn_h_tc", (const void *)prefill_tc_kernel<128, Params8>);
+const KernelReg reg_tc64("flash_attn_64_tc", (const void *)prefill_tc_kernel<64, Params8>);
+
+template <typename Params>
+void configure()
+{
+    cudaFuncSetAttribute(prefill_tc_kernel<128, Params>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<128>::SMEM);
+    cudaFuncSetAttribute(prefill_tc_kernel<64, Params>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<64>::SMEM);
+}
+
+// The launch with parameters of that size: what a launch costs grows with its
+// parameters' bytes (8 ragged prompts: 67.4 us with 8 KB of them, 69.5 with 21).
+template <typename Params>
+cudaError_t launch_with(const cudaLaunchConfig_t &cfg, int hd, const ParamsMost &all)
+{
+    Params p;
+    static_cast<PrefillTcCommon &>(p) = all;
+    memcpy(p.kmap, all.kmap, all.nseq * sizeof(p.kmap[0]));
+    memcpy(p.vmap, all.vmap, all.nseq * sizeof(p.vmap[0]));
+    memcpy(p.seq, all.seq, all.nseq * sizeof(p.seq[0]));
+    memcpy(p.order, all.order, all.n_order * sizeof(p.order[0]));
+    memcpy(p.pslot, all.pslot, all.n_order * sizeof(p.pslot[0]));
+    return hd == 128 ? cudaLaunchKernelEx(&cfg, prefill_tc_kernel<128, Params>, p)
+                     : cudaLaunchKernelEx(&cfg, prefill_tc_kernel<64, Params>, p);
+}
 const KernelReg reg_tcm("flash_attn_h_merge", (const void *)prefill_merge_kernel<128>);
 
 }  // namespace
@@ -1230,15 +1257,14 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !configured[dev]) {
-        cudaFuncSetAttribute(prefill_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Geo<128>::SMEM);
-        cudaFuncSetAttribute(prefill_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Geo<64>::SMEM);
+        configure<Params1>();
+        configure<Params8>();
+        configure<ParamsMost>();
         configured[dev] = true;
     }
     const uint64_t HD = (uint64_t)hd;
-    PrefillTcParams tp;
-    memset(&tp, 0, sizeof(tp));
+    ParamsMost tp;
+    static_cast<PrefillTcCommon &>(tp) = PrefillTcCommon{};
     int max_tq = 0;
     for (int b = 0; b < p.nseq; b++) {
         const PrefillSeq &s = p.seq[b];
@@ -1322,7 +1348,8 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         }
         const int sms = std::max(1, w.sm_count);
         const double share = (double)work * grid.x / sms;
-        if (!never && !tp.pair_rows && p.nseq <= 64 && longest >= 8 && longest > 1.25 * share) {
+        if (!never && !tp.pair_rows && longest >= 8 && longest > 1.25 * share) {
+            constexpr int kMostPieces = 255;     // (of a row block: what the order has room for)
             constexpr double kBlockCost = 4.0;   // an item's fixed costs, in tile steps
             constexpr double kMergeCost = 5.0;   // the merge kernel, in tile steps
             auto makespan = [&](int c) {
@@ -1364,7 +1391,7 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
             }
             if (!known) {
                 double best = makespan(0);
-                for (int c = (longest + 1) / 2; c >= 6; c -= (c > 24 ? 2 : 1)) {
+                for (int c = (longest + 1) / 2; c >= 6 && (longest + c - 1) / c <= kMostPieces; c -= (c > 24 ? 2 : 1)) {
                     const double t = makespan(c);
                     if (t < 0.95 * best && (cut == 0 || t < best)) {
                         best = t;
@@ -1387,10 +1414,12 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         // the SMs' last blocks are the short ones.
         struct Item { int tiles, seq, slot, piece, pieces, pslot; };
         std::vector<Item> items;
+        bool fits = true;
         for (int b = 0; b < p.nseq; b++) {
             for (int y = 0;; y++) {
                 const int n = tiles_of_slot(b, y);
                 if (n == 0) break;
+                fits = fits && y < 2048;
                 const int pieces = (cut > 0 && n > cut) ? (n + cut - 1) / cut : 1;
                 if (pieces > 1) groups.push_back({b, y, n_pslots, pieces});
                 for (int k = 0; k < pieces; k++) {
@@ -1400,13 +1429,13 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
                 if (pieces > 1) n_pslots += pieces;
             }
         }
-        if (!items.empty() && items.size() <= LLMTIE_TC_MAX_ORDER && n_pslots <= 65535) {
+        if (!items.empty() && fits && items.size() <= LLMTIE_TC_MAX_ORDER && n_pslots <= 65535) {
             std::stable_sort(items.begin(), items.end(),
                              [](const Item &a, const Item &b) { return a.tiles > b.tiles; });
             tp.n_order = (int)items.size();
             for (size_t i = 0; i < items.size(); i++) {
-                tp.order[i] = ((uint32_t)items[i].pieces << 20) | ((uint32_t)items[i].piece << 14) |
-                              ((uint32_t)items[i].seq << 8) | (uint32_t)items[i].slot;
+                tp.order[i] = ((uint32_t)items[i].pieces << 24) | ((uint32_t)items[i].piece << 16) |
+                              ((uint32_t)items[i].seq << 11) | (uint32_t)items[i].slot;
                 tp.pslot[i] = (uint16_t)items[i].pslot;
             }
             grid = dim3(grid.x, (unsigned)items.size(), 1);
@@ -1446,8 +1475,10 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = p.after_prepass ? 1 : 0;
-        err = hd == 128 ? cudaLaunchKernelEx(&cfg, prefill_tc_kernel<128>, tp)
-                        : cudaLaunchKernelEx(&cfg, prefill_tc_kernel<64>, tp);
+        auto holds = [&](int seq, int order) { return tp.nseq <= seq && tp.n_order <= order; };
+        err = holds(Params1::kSeq, Params1::kOrder)   ? launch_with<Params1>(cfg, hd, tp)
+              : holds(Params8::kSeq, Params8::kOrder) ? launch_with<Params8>(cfg, hd, tp)
+                                                      : launch_with<ParamsMost>(cfg, hd, tp);
     }
     if (part) {
         if (err == cudaSuccess) {
