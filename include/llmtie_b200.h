@@ -621,12 +621,13 @@ llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q, size_t q_l
  * no device): for contexts of live[0..batch) tokens, batch <= 32, on sm_count
  * SMs that hold resident8 / resident16 thread-block clusters of 8 and of 16 of
  * its blocks at once, the blocks of the grid, the cluster that takes each
- * (sequence, KV head) pair (0: the launch is cut by work) and about how long it
- * takes in nanoseconds. */
+ * (sequence, KV head) pair - several of them, where the grid has more blocks
+ * than that - (0: the launch is cut by work) and about how long it takes in
+ * nanoseconds. */
 llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads,
-                                    size_t head_dim, int32_t sm_count, int32_t resident8,
-                                    int32_t resident16, int32_t *grid, int32_t *cluster,
-                                    int64_t *ns);
+                                    size_t head_dim, int32_t weigh, int32_t sm_count,
+                                    int32_t resident8, int32_t resident16, int32_t *grid,
+                                    int32_t *cluster, int64_t *ns);
 
 /* llmtie_flash_attn_f16 over 8-bit caches, for a packed ragged batch: sequence
  * b's rows cu_seqlens[b] .. cu_seqlens[b+1] of q f32 [rows][heads*head_dim]
@@ -634,8 +635,8 @@ llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv
  * theirs and theirs (llmtie_rope_append_q8 puts them there): causal, or all to
  * all. out [rows][heads*head_dim], f16 or f32. Sequences of few rows go through
  * the decode kernel; of the others the live keys are unpacked to f16 once, into
- * memory that the handle keeps for the purpose, for at most eight sequences at
- * a time. */
+ * memory that the handle keeps for the purpose: for eight sequences at a time,
+ * or as many as take a gigabyte and are no more than 32. */
 llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len,
                                    const int32_t *cu_seqlens, size_t batch,
                                    const void *const *caches, const int32_t *past,

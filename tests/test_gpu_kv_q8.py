@@ -330,7 +330,7 @@ def test_decode_by_every_way_over_the_device(gpu, heads, kv, hd, batch, live, cl
     a block or two, and weights."""
     rng = np.random.default_rng(live)
     lives = [live - int(x) for x in rng.integers(0, min(live, 70), batch)]
-    assert decode_plan_q8(lives[:32], kv, hd)[1] == cluster
+    assert decode_plan_q8(lives[:32], kv, hd, weigh=True)[1] == cluster
     cap = [(n + 31) // 32 * 32 for n in lives]
     ms = []
     for c, n in zip(cap, lives):
@@ -352,6 +352,40 @@ def test_decode_by_every_way_over_the_device(gpu, heads, kv, hd, batch, live, cl
         w = got(gpu, ts[b], ms[b]).w
         assert np.abs(w[:, :n // 32] - (0.5 + share)).max(initial=0) <= 2e-4 * (1.5 + share.max(initial=0))
         assert (w[:, n // 32:] == 0.5).all()
+
+
+@pytest.mark.parametrize("heads,kv,hd,lives", [
+    (8, 1, 128, (20001,)), (4, 1, 128, (40000, 30)), (8, 2, 128, (31, 0, 33333)), (12, 4, 128, (12345,)),
+    (8, 1, 64, (25000, 7, 64, 1)), (3, 3, 64, (30007, 40000))])
+def test_decode_of_pairs_that_several_clusters_share(gpu, heads, kv, hd, lives):
+    """Long contexts of few KV heads, shorter ones among them that leave clusters
+    without a block; the same bits every time."""
+    rng = np.random.default_rng(sum(lives))
+    grid, cluster, _ = decode_plan_q8(lives, kv, hd)
+    assert cluster == 8 and grid > 8 * kv * len(lives)
+    cap = [(n + 31) // 32 * 32 or 32 for n in lives]
+    ms = []
+    for c, n in zip(cap, lives):
+        m = Q8Model(kv, hd, c, fill=0x7f)
+        full = n // 32
+        m.k[:, :full], m.v[:, :full] = (rng.integers(-127, 128, x.shape) for x in (m.k[:, :full], m.v[:, :full]))
+        m.ks[:], m.vs[:] = np.nan, np.nan
+        m.ks[:, :full], m.vs[:, :full] = rng.uniform(0.005, 0.02, (2, kv, full))
+        m.kt[:, :n % 32], m.vt[:, :n % 32] = rng.standard_normal((2, kv, n % 32, hd))
+        ms.append(m)
+    ts = [put(gpu, m) for m in ms]
+    q = rng.standard_normal((len(lives), heads, hd)).astype(np.float32)
+    scratch = DecodeScratch()
+    out = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch)).reshape(q.shape)
+    for b, n in enumerate(lives):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        want, _ = decode_want(q[b], ms[b], n, heads, hd ** -0.5)
+        assert rel_l2(want, out[b]) <= DECODE_REL, f"sequence {b} of {n}"
+    for _ in range(5):
+        again = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch))
+        assert np.array_equal(again.reshape(q.shape), out)
 
 
 def test_decode_sink_and_long_faint_context(gpu):
@@ -476,6 +510,49 @@ def test_flash_ragged_batch(gpu):
             want, _ = attend(q[rows].astype(np.float64), m.values("k", live[b]), m.values("v", live[b]), hd ** -0.5,
                              past[b] + np.arange(new[b]))
             assert_parity(f"sequence {b}", want, out[rows])
+
+
+@pytest.mark.parametrize("heads,kv,hd,batch", [(8, 1, 128, 33), (4, 4, 64, 70), (6, 2, 128, 32)])
+def test_flash_of_more_sequences_than_a_launch_takes(gpu, heads, kv, hd, batch):
+    rng = np.random.default_rng(batch)
+    past = [int(x) for x in rng.integers(0, 90, batch)]
+    new = [int(x) for x in rng.choice([0, 33, 66, 129, 140], batch)]
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(int).tolist()
+    live = [p + n for p, n in zip(past, new)]
+    cap = [max(32, (n + 31) // 32 * 32) for n in live]
+    ms = [filled(rng, kv, hd, c, n) for c, n in zip(cap, live)]
+    q = rng.standard_normal((cu[-1], heads, hd)).astype(np.float32)
+    out = gpu.download(gpu.flash_attn_q8(gpu.upload(q), cu, [put(gpu, m) for m in ms], cap, past, heads, kv, hd, hd ** -0.5, True))
+    out = out.reshape(q.shape)
+    for b, m in enumerate(ms):
+        rows = slice(cu[b], cu[b + 1])
+        if new[b]:
+            want, _ = attend(q[rows].astype(np.float64), m.values("k", live[b]), m.values("v", live[b]), hd ** -0.5,
+                             past[b] + np.arange(new[b]))
+            assert_parity(f"sequence {b}", want, out[rows])
+
+
+def test_flash_of_sequences_that_unpack_to_more_than_a_gigabyte(gpu):
+    """Twelve of them over one cache, 134 MB each: a launch ends with the eighth. The
+    rows are the same, so the results are, but for how a launch cuts its rows' keys."""
+    rng = np.random.default_rng(3)
+    heads, kv, hd, past, new, batch = 8, 4, 128, 65400, 40, 12
+    n = past + new
+    k, v = (gpu.upload(rng.standard_normal((n, kv * hd)).astype(np.float32)) for _ in range(2))
+    cap = (n + 31) // 32 * 32
+    t = gpu.kv_alloc_q8(kv, hd, cap)
+    gpu.rope_append_q8(None, k, v, [0, n], [t], [cap], [0], [0], None, heads, kv, hd)
+    q = rng.standard_normal((new, heads, hd)).astype(np.float32)
+    cu = [new * b for b in range(batch + 1)]
+    out = gpu.download(gpu.flash_attn_q8(gpu.upload(np.tile(q, (batch, 1, 1))), cu, [t] * batch, [cap] * batch, [past] * batch, heads, kv,
+                                         hd, hd ** -0.5, True)).reshape(batch, -1)
+    ko, vo = gpu.cache_read_q8([t], [cap], [n], [0], [0, n], kv, hd)
+    gpu.synchronize()
+    kk, vv = (x.double().cpu().numpy().reshape(n, kv, hd).transpose(1, 0, 2) for x in (ko, vo))
+    at = np.array([0, new - 1])
+    want, _ = attend(q[at].astype(np.float64), kk, vv, hd ** -0.5, past + at)
+    for b in (0, 7, 8, 11):
+        assert_parity(f"sequence {b}", want, out[b].reshape(q.shape)[at])
 
 
 def test_flash_of_a_prompt_longer_than_a_launch_takes(gpu):

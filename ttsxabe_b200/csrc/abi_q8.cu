@@ -95,14 +95,14 @@ llmtie_status check_rows(const int32_t *cu, size_t batch, size_t *total)
 
 // How the decode kernel would go over jobs [b0, b0 + LLMTIE_Q8_MAX_SEQ).
 llmtie_status plan_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, size_t b0, size_t kv_heads, size_t head_dim,
-                        DecodeQ8Plan &plan)
+                        bool weigh, DecodeQ8Plan &plan)
 {
     int per[LLMTIE_Q8_MAX_SEQ], clusters[2];
     const int n = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, jobs.size() - b0);
     for (int b = 0; b < n; b++) per[b] = (jobs[b0 + b].live + kQ8Block - 1) / kQ8Block;
     const cudaError_t e = decode_q8_clusters((int)head_dim, clusters);
     if (e != cudaSuccess) return llmtie_driver_fail("decode_q8", e);
-    plan_decode_q8(plan, per, n, (int)kv_heads, (int)head_dim, g->sm_count, clusters);
+    plan_decode_q8(plan, per, n, (int)kv_heads, (int)head_dim, g->sm_count, clusters, weigh);
     return LLMTIE_OK;
 }
 
@@ -136,21 +136,22 @@ llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, cons
         p.status = g->timeout_site;
         p.wait_cycles = g->wait_cycles;
         DecodeQ8Plan plan;
-        TRY(plan_jobs(g, jobs, b0, kv_heads, head_dim, plan));
+        TRY(plan_jobs(g, jobs, b0, kv_heads, head_dim, weigh != 0, plan));
         cudaError_t err;
         const int grid = plan.grid;
         p.cluster = plan.cluster;
+        p.parts = plan.parts;
         p.over = plan.over;
         const long long shares = units + (long long)p.over * p.nseq * (long long)kv_heads;
         p.each = grid ? (int)(shares / grid) : 0;
         p.more = grid ? (int)(shares % grid) : 0;
         const size_t pairs = (size_t)p.nseq * kv_heads;
-        const size_t slots = (size_t)std::max(p.cluster ? 1 : grid, 1) * 2 * 8;
+        const size_t slots = (size_t)(p.cluster ? std::max(grid / p.cluster, 1) : std::max(2 * grid, 1)) * 8;
         p.part_o = (float *)workspace_reserve(scratch->q8_part, slots * (head_dim + 2) * sizeof(float), g->stream, &err);
         if (!p.part_o) return llmtie_driver_fail("allocating", err);
         p.part_ml = (float2 *)(p.part_o + slots * head_dim);
         const size_t had = scratch->q8_ctr.bytes;
-        p.ctr = (unsigned *)workspace_reserve(scratch->q8_ctr, pairs * sizeof(unsigned), g->stream, &err);
+        p.ctr = (unsigned *)workspace_reserve(scratch->q8_ctr, pairs * 8 * sizeof(unsigned), g->stream, &err);
         if (!p.ctr) return llmtie_driver_fail("allocating", err);
         if (scratch->q8_ctr.bytes != had) {
             err = cudaMemsetAsync(p.ctr, 0, scratch->q8_ctr.bytes, g->stream);
@@ -478,8 +479,8 @@ try {
 NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads, size_t head_dim,
-                                               int32_t sm_count, int32_t resident8, int32_t resident16, int32_t *grid,
-                                               int32_t *cluster, int64_t *ns)
+                                               int32_t weigh, int32_t sm_count, int32_t resident8, int32_t resident16,
+                                               int32_t *grid, int32_t *cluster, int64_t *ns)
 {
     if ((head_dim != 64 && head_dim != 128) || kv_heads == 0 || kv_heads > 4096) return llmtie_unsupported(head_dim, kv_heads, kv_heads);
     if (!live || !grid || !cluster || !ns || batch > LLMTIE_Q8_MAX_SEQ || sm_count <= 0) {
@@ -492,7 +493,7 @@ extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch
     }
     const int clusters[2] = {resident8, resident16};
     DecodeQ8Plan plan;
-    plan_decode_q8(plan, units, (int)batch, (int)kv_heads, (int)head_dim, sm_count, clusters);
+    plan_decode_q8(plan, units, (int)batch, (int)kv_heads, (int)head_dim, sm_count, clusters, weigh != 0);
     *grid = plan.grid;
     *cluster = plan.cluster;
     *ns = (int64_t)(plan.us * 1000.0);
@@ -549,7 +550,7 @@ try {
     }
     for (size_t j = 0; j < jobs.size(); j += LLMTIE_Q8_MAX_SEQ) {
         DecodeQ8Plan plan;
-        TRY(plan_jobs(g, jobs, j, kv_heads, head_dim, plan));
+        TRY(plan_jobs(g, jobs, j, kv_heads, head_dim, false, plan));
         decoded += plan.us;
     }
     if (decoded > unpacked + (others ? 0.0 : 13.0)) {
@@ -564,6 +565,7 @@ try {
     // sequence of more than kRows rows is as many of them as it takes, over the
     // same keys.
     constexpr int kRows = 16384;
+    constexpr size_t kMostUnpacked = (size_t)1 << 30;   // for more than eight sequences
     for (size_t b = 0, done = 0; b < batch;) {
         Q8UnpackParams up;
         PrefillParams pp;
@@ -579,6 +581,7 @@ try {
             }
             const int live = past[b] + rows;
             const size_t cap16 = ((size_t)live + 7) / 8 * 8, half = (kv_heads * cap16 * head_dim * 2 + 255) / 256 * 256;
+            if (up.nseq >= 8 && bytes + 2 * half > kMostUnpacked) break;
             Q8UnpackSeq &u = up.seq[up.nseq++];
             u.base = (const unsigned char *)caches[b];
             u.nb = cap[b] / kQ8Block;

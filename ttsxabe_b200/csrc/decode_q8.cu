@@ -27,8 +27,9 @@
 // three the queue at the memory makes every other load wait: 344 against 301 us
 // for 8 x 131072 keys of 8 heads x 128, which is 6.9-7.1 TB/s). A pair
 // (sequence, KV head) is taken by a cluster of blocks of the grid that merge
-// through distributed shared memory, or the grid is cut by work and the last
-// block to arrive merges (see plan_decode_q8, and there what either costs). The
+// through distributed shared memory, or by several, whose results the last to
+// arrive merges row by row, or the grid is cut by work and the last block to
+// arrive merges (see plan_decode_q8, and there what each costs). The
 // tensor pipe is 20 % busy, so there is no more to gain from tcgen05 here.
 #include "kv_q8.cuh"
 
@@ -204,18 +205,18 @@ __device__ __forceinline__ void store_row(const DecodeQ8Params &p, long long at,
     }
 }
 
-// By cluster: pair blockIdx.x / p.cluster, cut evenly over the cluster's blocks.
+// By cluster: a pair is cut evenly over the blocks of its p.parts clusters.
 __device__ __forceinline__ Run run_of_rank(const DecodeQ8Params &p)
 {
-    const int pair = (int)blockIdx.x / p.cluster, rank = (int)blockIdx.x - pair * p.cluster;
+    const int over = p.parts * p.cluster, pair = (int)blockIdx.x / over, rank = (int)blockIdx.x - pair * over;
     Run r;
     r.seq = pair / p.kv_heads;
     r.head = pair - r.seq * p.kv_heads;
     const int full = p.seq[r.seq].full;
     r.units = (p.seq[r.seq].live + 31) >> 5;
     r.begin = 0;
-    r.first = (int)((long long)r.units * rank / p.cluster);
-    const int stop = (int)((long long)r.units * (rank + 1) / p.cluster);
+    r.first = (int)((long long)r.units * rank / over);
+    const int stop = (int)((long long)r.units * (rank + 1) / over);
     r.tail = stop > full && r.first < stop;
     r.last = min(stop, full);
     r.whole = p.cluster == 1;
@@ -269,6 +270,66 @@ __device__ __forceinline__ void weigh(const DecodeQ8Params &p, int seq0, int hea
             if (k < group) sum = fmaf(ex2(y[k].x - f[k].x) * f[k].y, y[k].y, sum);
         }
         *weight = before + sum;
+    }
+}
+
+// Row `row` of `count` partial results, slots first + skew, first + step, first + 2
+// step and so on: in that order, 32 at a time, 16 of their loads in flight.
+template <int HD>
+__device__ __forceinline__ void merge_parts(const DecodeQ8Params &p, int lane, int count, int first, int step, int skew, int row,
+                                            float &M, float &L, float (&o)[HD / 32])
+{
+    constexpr int V = HD / 32, U = 16;
+    M = -CUDART_INF_F;
+    L = 0.0f;
+#pragma unroll
+    for (int e = 0; e < V; e++) o[e] = 0.0f;
+    for (int at = 0; at < count; at += 32) {
+        const int n = min(32, count - at);
+        auto slot = [&](int i) { return first + step * (at + i) + (at + i == 0 ? skew : 0); };
+        float2 ml = make_float2(-CUDART_INF_F, 0.0f);
+        if (lane < n) ml = __ldcg(&p.part_ml[slot(lane) * kRows + row]);
+        float y[U][V];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if (i0 + i < n) {
+                    const float *src = p.part_o + ((long long)slot(i0 + i) * kRows + row) * HD + V * lane;
+                    if constexpr (V == 4) {
+                        const float4 z = __ldcg((const float4 *)src);
+                        y[i][0] = z.x; y[i][1] = z.y; y[i][2] = z.z; y[i][3] = z.w;
+                    } else {
+                        const float2 z = __ldcg((const float2 *)src);
+                        y[i][0] = z.x; y[i][1] = z.y;
+                    }
+                }
+            }
+        };
+        load(0);
+        float top = ml.x;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        top = fmaxf(top, M);
+        const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
+        const float f = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+        float sum = f * ml.y;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        L = fmaf(L, keep, sum);
+#pragma unroll
+        for (int e = 0; e < V; e++) o[e] *= keep;
+        for (int i0 = 0; i0 < n; i0 += U) {
+            if (i0) load(i0);
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+                if (i0 + i < n) {
+#pragma unroll
+                    for (int e = 0; e < V; e++) o[e] = fmaf(fi, y[i][e], o[e]);
+                }
+            }
+        }
+        M = top;
     }
 }
 
@@ -737,6 +798,28 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 }
                 M = top;
             }
+            if (p.parts > 1) {
+                // a row of a pair that several clusters share: the last to arrive merges
+                // them, in their order whoever came last
+                const int cluster = (int)blockIdx.x / p.cluster, pair = cluster / p.parts;
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    *(float2 *)(p.part_o + ((long long)cluster * kRows + row) * HD + V * lane + e) = make_float2(o[e], o[e + 1]);
+                }
+                if (lane == 0) p.part_ml[cluster * kRows + row] = make_float2(M, L);
+                __threadfence();
+                __syncwarp();
+                unsigned seen = 0;
+                if (lane == 0) {
+                    unsigned *ctr = &p.ctr[pair * kRows + row];
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(ctr) : "memory");
+                    if (seen == (unsigned)(p.parts - 1)) *ctr = 0u;
+                }
+                seen = __shfl_sync(0xffffffffu, seen, 0);
+                if (seen != (unsigned)(p.parts - 1)) continue;
+                __threadfence();
+                merge_parts<HD>(p, lane, p.parts, pair * p.parts, 1, 0, row, M, L, o);
+            }
             const float inv = 1.0f / L;
 #pragma unroll
             for (int e = 0; e < V; e++) o[e] *= inv;
@@ -791,58 +874,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         // The contributors in order, whoever came last: the same bits every time. A
         // block's first run has slot 0, and only b0 may hold the pair in its last.
         const int skew = first_unit(p, b0) >= now.begin ? 0 : 1;
-        float M = -CUDART_INF_F, L = 0.0f, o[V];
-#pragma unroll
-        for (int e = 0; e < V; e++) o[e] = 0.0f;
-        for (int bb = b0; bb <= b1; bb += 32) {
-            const int n = min(32, b1 + 1 - bb);
-            const int my_slot = 2 * (bb + lane) + (bb + lane == b0 ? skew : 0);
-            float2 ml = make_float2(-CUDART_INF_F, 0.0f);
-            if (lane < n) ml = __ldcg(&p.part_ml[my_slot * kRows + row]);
-            constexpr int U = 16;
-            float y[U][V];
-            auto load = [&](int i0) {
-#pragma unroll
-                for (int i = 0; i < U; i++) {
-                    if (i0 + i < n) {
-                        const int b = bb + i0 + i;
-                        const float *src = p.part_o + ((long long)(2 * b + (b == b0 ? skew : 0)) * kRows + row) * HD + V * lane;
-                        if constexpr (V == 4) {
-                            const float4 z = __ldcg((const float4 *)src);
-                            y[i][0] = z.x; y[i][1] = z.y; y[i][2] = z.z; y[i][3] = z.w;
-                        } else {
-                            const float2 z = __ldcg((const float2 *)src);
-                            y[i][0] = z.x; y[i][1] = z.y;
-                        }
-                    }
-                }
-            };
-            load(0);
-            float top = ml.x;
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-            top = fmaxf(top, M);
-            const float keep = M == -CUDART_INF_F ? 0.0f : ex2(M - top);
-            const float f = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
-            float sum = f * ml.y;
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-            L = fmaf(L, keep, sum);
-#pragma unroll
-            for (int e = 0; e < V; e++) o[e] *= keep;
-            for (int i0 = 0; i0 < n; i0 += U) {
-                if (i0) load(i0);
-#pragma unroll
-                for (int i = 0; i < U; i++) {
-                    const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
-                    if (i0 + i < n) {
-#pragma unroll
-                        for (int e = 0; e < V; e++) o[e] = fmaf(fi, y[i][e], o[e]);
-                    }
-                }
-            }
-            M = top;
-        }
+        float M, L, o[V];
+        merge_parts<HD>(p, lane, b1 + 1 - b0, 2 * b0, 2, skew, row, M, L, o);
         const float inv = 1.0f / L;
 #pragma unroll
         for (int e = 0; e < V; e++) o[e] *= inv;
@@ -932,16 +965,18 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
                      : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, p.cluster, decode_q8_kernel<64>, p);
 }
 
-void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters)
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters, bool weigh)
 {
     // Microseconds, as measured (148 SMs): cache blocks a microsecond that the memory
     // gives (6.9 TB/s), a warp's time for one when nothing but the warp itself bounds
     // it, and what a launch costs besides: by a cluster of 1, 2, 4, 8 or 16 blocks of
     // the grid (the last are packed onto half as many SMs), by the cut (whose merge
     // goes through memory, and is long where many blocks share a pair: short
-    // launches), and for a further wave of blocks of the grid.
+    // launches, and 0.1 us for each block beyond 32), by several clusters a pair, and
+    // for a further wave of blocks of the grid.
     const double all = (hd == 128 ? 842.0 : 1684.0) * sm_count / 148, one = hd == 128 ? 0.7 : 0.6;
-    constexpr double kCluster[5] = {4.0, 4.5, 5.0, 5.4, 6.3}, kPacked = 1.15, kCut = 7.0, kShort = 16.0, kWave = 3.5;
+    constexpr double kCluster[5] = {4.0, 4.5, 5.0, 5.4, 6.3}, kPacked = 1.15, kCut = 7.0, kShort = 16.0, kWave = 3.5,
+                     kJoin = 0.1, kParts = 8.3, kPart = 0.11;
     const int most = sm_count * (hd == 128 ? Geo<128>::RESIDENT : Geo<64>::RESIDENT);
     long long total = 0, longest = 0;
     for (int i = 0; i < n; i++) {
@@ -949,7 +984,7 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
         longest = std::max<long long>(longest, units[i]);
     }
     const long long pairs = (long long)n * kv_heads;
-    plan = DecodeQ8Plan{0, 0, 0, 0.0};
+    plan = DecodeQ8Plan{0, 0, 1, 0, 0.0};
     if (total == 0) return;
     // the cut by work: never fewer than four cache blocks, one a warp, for a block of
     // the grid; where a launch is short, as many that what the warps take in turn (0.5
@@ -971,7 +1006,8 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
         over = 0;
     }
     const long long share = (total + grid - 1) / grid;
-    plan = DecodeQ8Plan{(int)grid, 0, over, (over ? kCut : kShort) + std::max((double)total / all, one * (double)((share + 3) / 4))};
+    const double joined = kJoin * std::max(0.0, (double)grid / (double)pairs - 32.0);
+    plan = DecodeQ8Plan{(int)grid, 0, 1, over, (over ? kCut : kShort) + std::max((double)total / all, one * (double)((share + 3) / 4)) + joined};
     for (int i = 0, c = 1; i < 5; i++, c *= 2) {
         const long long blocks = pairs * c;
         if (c > 1 && blocks > most) break;
@@ -979,7 +1015,18 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
         const double waves = (double)((blocks + most - 1) / most), part = std::max(1.0, (double)blocks / most);
         const double own = one * (double)(((longest + c - 1) / c + 3) / 4) * (c == 16 ? kPacked : 1.0);
         const double cost = kCluster[i] + kWave * (waves - 1.0) + std::max((double)total / all * waves / part, own * waves);
-        if (cost < plan.us && blocks <= 0x7fffffff) plan = DecodeQ8Plan{(int)blocks, c, 0, cost};
+        if (cost < plan.us && blocks <= 0x7fffffff) plan = DecodeQ8Plan{(int)blocks, c, 1, 0, cost};
+    }
+    // Several clusters of eight for a pair, as many as the device holds at once, and
+    // none of them without a block. (Not where weights are taken: no cluster then knows
+    // the rows' sums.) 131072 tokens, one KV head x 128: 15 us by 32 clusters, 45 by the
+    // cut, whose last block has 296 results to merge; 8000 tokens: 12 us by 32 clusters,
+    // 9 by one of 16.
+    for (long long parts = 2; parts <= 32 && pairs * parts <= clusters[0] && parts * 8 <= longest && !weigh; parts++) {
+        const long long blocks = pairs * parts * 8;
+        const double own = one * (double)(((longest + 8 * parts - 1) / (8 * parts) + 3) / 4);
+        const double cost = kParts + kPart * (double)parts + std::max((double)total / all * std::max(1.0, 0.8 * most / (double)blocks), own);
+        if (cost < plan.us) plan = DecodeQ8Plan{(int)blocks, 8, (int)parts, 0, cost};
     }
 }
 

@@ -179,7 +179,7 @@ struct DecodeQ8Params {
     DecodeQ8Seq seq[LLMTIE_Q8_MAX_SEQ];
     int unit0[LLMTIE_Q8_MAX_SEQ + 1];                  // first 32-token unit of each sequence
     int each, more, over;                              // the cut over the grid: see first_unit in decode_q8.cu
-    int cluster;                                       // or: a cluster of so many blocks a pair, no cut (0: the cut)
+    int cluster, parts;                                // or: a pair to so many clusters of so many blocks, no cut (0: the cut)
     long long stat0[LLMTIE_Q8_MAX_SEQ];                // first block of each sequence in `stats`
     int nseq, heads, kv_heads;
     int causal;              // query i sees live - n + 1 + i tokens, else all
@@ -187,9 +187,9 @@ struct DecodeQ8Params {
     void *out;               // the same, f16 or f32
     int out_f16;
     float sl2;               // scale * log2(e)
-    float *part_o;           // [block][2][8][hd]
-    float2 *part_ml;         // [block][2][8]
-    unsigned *ctr;           // arrivals of each (sequence, KV head), zero at rest
+    float *part_o;           // [block][2][8][hd], or [cluster][8][hd]
+    float2 *part_ml;         // [block][2][8], or [cluster][8]
+    unsigned *ctr;           // arrivals of each (sequence, KV head), or of each of its rows; zero at rest
     float2 *stats;           // [block of a sequence][8] (maximum, sum), or null: no weights
     int *status;
     long long wait_cycles;
@@ -199,10 +199,12 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
 // kv_heads times, is laid over the device.
 struct DecodeQ8Plan {
     int grid;      // blocks of the grid (0: nothing to do)
-    int cluster;   // a cluster of so many a pair, or 0: cut by work
+    int cluster;   // clusters of so many, or 0: cut by work
+    int parts;     // that many of them a pair
     int over;      // what the cut charges a run
     double us;     // about what it takes
 };
-void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters);
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters,
+                    bool weigh);
 // How many clusters of 8 and of 16 blocks the current device holds at once.
 cudaError_t decode_q8_clusters(int hd, int (&clusters)[2]);
