@@ -532,6 +532,29 @@ def test_flash_of_more_sequences_than_a_launch_takes(gpu, heads, kv, hd, batch):
             assert_parity(f"sequence {b}", want, out[rows])
 
 
+@pytest.mark.parametrize("heads,kv,hd,batch", [(16, 4, 128, 20), (32, 8, 64, 11)])
+def test_flash_of_a_few_more_blocks_than_the_device_holds(gpu, heads, kv, hd, batch):
+    """Rows whose keys are cut because the last round of blocks would leave most of
+    the device idle; sequences of different lengths over one cache."""
+    rng = np.random.default_rng(batch)
+    new, longest = 40, 2500
+    m = filled(rng, kv, hd, 2560, longest + new)
+    t = put(gpu, m)
+    past = [longest - int(x) for x in rng.integers(0, 300, batch)]
+    past[0] = longest
+    cu = [new * b for b in range(batch + 1)]
+    q = rng.standard_normal((cu[-1], heads, hd)).astype(np.float32)
+    # (a shorter sequence's last tokens lie in complete blocks: it ends with one)
+    past = [p if p == longest else (p + new) // 32 * 32 - new for p in past]
+    out = gpu.download(gpu.flash_attn_q8(gpu.upload(q), cu, [t] * batch, [2560] * batch, past, heads, kv, hd, hd ** -0.5, True))
+    out = out.reshape(q.shape)
+    k, v = m.values("k", longest + new), m.values("v", longest + new)
+    for b in range(batch):
+        rows = slice(cu[b], cu[b + 1])
+        want, _ = attend(q[rows].astype(np.float64), k[:, :past[b] + new], v[:, :past[b] + new], hd ** -0.5, past[b] + np.arange(new))
+        assert_parity(f"sequence {b}", want, out[rows])
+
+
 def test_flash_of_sequences_that_unpack_to_more_than_a_gigabyte(gpu):
     """Twelve of them over one cache, 134 MB each: a launch ends with the eighth. The
     rows are the same, so the results are, but for how a launch cuts its rows' keys."""

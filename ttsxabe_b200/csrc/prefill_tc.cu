@@ -1348,7 +1348,11 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         }
         const int sms = std::max(1, w.sm_count);
         const double share = (double)work * grid.x / sms;
-        if (!never && !tp.pair_rows && longest >= 8 && longest > 1.25 * share) {
+        // Too few blocks; or so few to an SM that the last round leaves many idle (11
+        // sequences of 172 key tiles, 16 blocks each: two rounds for 1.2 rounds' work).
+        const long long blocks = (long long)lens.size() * grid.x;
+        const bool few = longest > 1.25 * share, uneven = !few && longest >= 16 && blocks <= 3ll * sms;
+        if (!never && !tp.pair_rows && longest >= 8 && (few || uneven)) {
             constexpr int kMostPieces = 255;     // (of a row block: what the order has room for)
             constexpr double kBlockCost = 4.0;   // an item's fixed costs, in tile steps
             constexpr double kMergeCost = 5.0;   // the merge kernel, in tile steps
@@ -1391,7 +1395,17 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
             }
             if (!known) {
                 double best = makespan(0);
-                for (int c = (longest + 1) / 2; c >= 6 && (longest + c - 1) / c <= kMostPieces; c -= (c > 24 ? 2 : 1)) {
+                if (uneven && best > 1.15 * (share + kBlockCost * (double)blocks / sms)) {
+                    for (int k : {2, 3, 4, 6}) {
+                        const int c = (longest + k - 1) / k;
+                        const double t = c >= 6 ? makespan(c) : best;
+                        if (t < 0.95 * best && (cut == 0 || t < best)) {
+                            best = t;
+                            cut = c;
+                        }
+                    }
+                }
+                for (int c = (longest + 1) / 2; few && c >= 6 && (longest + c - 1) / c <= kMostPieces; c -= (c > 24 ? 2 : 1)) {
                     const double t = makespan(c);
                     if (t < 0.95 * best && (cut == 0 || t < best)) {
                         best = t;
