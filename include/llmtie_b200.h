@@ -625,9 +625,9 @@ llmtie_status llmtie_decode_batched_q8(llmtie_gpu *g, const float *q, size_t q_l
  * than that - (0: the launch is cut by work) and about how long it takes in
  * nanoseconds. */
 llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads,
-                                    size_t head_dim, int32_t weigh, int32_t sm_count,
-                                    int32_t resident8, int32_t resident16, int32_t *grid,
-                                    int32_t *cluster, int64_t *ns);
+                                    size_t head_dim, int32_t sm_count, int32_t resident8,
+                                    int32_t resident16, int32_t *grid, int32_t *cluster,
+                                    int64_t *ns);
 
 /* llmtie_flash_attn_f16 over 8-bit caches, for a packed ragged batch: sequence
  * b's rows cu_seqlens[b] .. cu_seqlens[b+1] of q f32 [rows][heads*head_dim]

@@ -330,7 +330,7 @@ def test_decode_by_every_way_over_the_device(gpu, heads, kv, hd, batch, live, cl
     a block or two, and weights."""
     rng = np.random.default_rng(live)
     lives = [live - int(x) for x in rng.integers(0, min(live, 70), batch)]
-    assert decode_plan_q8(lives[:32], kv, hd, weigh=True)[1] == cluster
+    assert decode_plan_q8(lives[:32], kv, hd)[1] == cluster
     cap = [(n + 31) // 32 * 32 for n in lives]
     ms = []
     for c, n in zip(cap, lives):
@@ -372,17 +372,20 @@ def test_decode_of_pairs_that_several_clusters_share(gpu, heads, kv, hd, lives):
         m.ks[:], m.vs[:] = np.nan, np.nan
         m.ks[:, :full], m.vs[:, :full] = rng.uniform(0.005, 0.02, (2, kv, full))
         m.kt[:, :n % 32], m.vt[:, :n % 32] = rng.standard_normal((2, kv, n % 32, hd))
+        m.w[:] = 0
         ms.append(m)
     ts = [put(gpu, m) for m in ms]
     q = rng.standard_normal((len(lives), heads, hd)).astype(np.float32)
     scratch = DecodeScratch()
-    out = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch)).reshape(q.shape)
+    out = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch, weigh=True)).reshape(q.shape)
     for b, n in enumerate(lives):
         if n == 0:
             assert (out[b] == 0).all()
             continue
-        want, _ = decode_want(q[b], ms[b], n, heads, hd ** -0.5)
+        want, share = decode_want(q[b], ms[b], n, heads, hd ** -0.5)
         assert rel_l2(want, out[b]) <= DECODE_REL, f"sequence {b} of {n}"
+        w = got(gpu, ts[b], ms[b]).w
+        assert np.abs(w[:, :n // 32] - share).max(initial=0) <= 2e-4 * (1 + share.max(initial=0))
     for _ in range(5):
         again = gpu.download(gpu.decode_batched_q8(gpu.upload(q), ts, lives, cap, heads, kv, hd, hd ** -0.5, scratch))
         assert np.array_equal(again.reshape(q.shape), out)

@@ -83,15 +83,14 @@ def test_decode_plan(hd):
         kv = int(rng.choice([1, 2, 8, 20]))
         n = int(rng.integers(1, 33))
         live = [int(x) for x in np.exp(rng.uniform(0, np.log(40000), n))]
-        weigh = bool(rng.integers(0, 2))
-        grid, cluster, ns = decode_plan_q8(live, kv, hd, weigh=weigh)
+        grid, cluster, ns = decode_plan_q8(live, kv, hd)
         pairs, units = n * kv, kv * sum((t + 31) // 32 for t in live)
         seen.add(cluster)
         assert ns > 0
         if cluster:
             parts, rest = divmod(grid, pairs * cluster)
             assert rest == 0 and parts >= 1 and cluster in (1, 2, 4, 8, 16)
-            assert parts == 1 or (cluster == 8 and not weigh and parts <= 32 and pairs * parts <= 36)
+            assert parts == 1 or (cluster == 8 and parts <= 32 and pairs * parts <= 36)
             assert cluster == 1 or grid <= most
             assert cluster < 8 or pairs <= (36 if cluster == 8 else 16)
         else:
@@ -99,10 +98,9 @@ def test_decode_plan(hd):
     assert {0, 1, 2, 4} <= seen
     assert decode_plan_q8([2048], 8, hd)[1] in (8, 16)
     assert decode_plan_q8([131072] * 8, 8, hd)[0] <= most
-    # few pairs of many blocks: several clusters each, but one where weights are taken
+    # few pairs of many blocks: several clusters each
     grid, cluster, _ = decode_plan_q8([40000, 30000], 1, hd)
     assert cluster == 8 and grid >= 10 * 16
-    assert decode_plan_q8([12000], 1, hd, weigh=True)[:2] == (16, 16)
     # no clusters where the device holds none; nothing for no tokens
     assert decode_plan_q8([2048], 8, hd, resident=(0, 0))[1] <= 4
     assert decode_plan_q8([0, 0], 8, hd)[:2] == (0, 0)

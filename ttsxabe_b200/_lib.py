@@ -106,7 +106,7 @@ PROTOTYPES = {
     "llmtie_decode_batched_q8": (
         i32, [vp, vp, sz, pvp, pi32, pi32, sz, sz, sz, sz, f32, i32, vp, vp, sz, i32]),
     "llmtie_decode_plan_q8": (
-        i32, [pi32, sz, sz, sz, i32, i32, i32, i32, pi32, pi32, C.POINTER(C.c_int64)]),
+        i32, [pi32, sz, sz, sz, i32, i32, i32, pi32, pi32, C.POINTER(C.c_int64)]),
     "llmtie_flash_attn_q8": (
         i32, [vp, vp, sz, pi32, sz, pvp, pi32, pi32, sz, sz, sz, f32, i32, vp, sz, i32]),
     "llmtie_cache_evict_q8": (

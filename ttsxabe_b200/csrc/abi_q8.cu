@@ -95,14 +95,14 @@ llmtie_status check_rows(const int32_t *cu, size_t batch, size_t *total)
 
 // How the decode kernel would go over jobs [b0, b0 + LLMTIE_Q8_MAX_SEQ).
 llmtie_status plan_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, size_t b0, size_t kv_heads, size_t head_dim,
-                        bool weigh, DecodeQ8Plan &plan)
+                        DecodeQ8Plan &plan)
 {
     int per[LLMTIE_Q8_MAX_SEQ], clusters[2];
     const int n = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, jobs.size() - b0);
     for (int b = 0; b < n; b++) per[b] = (jobs[b0 + b].live + kQ8Block - 1) / kQ8Block;
     const cudaError_t e = decode_q8_clusters((int)head_dim, clusters);
     if (e != cudaSuccess) return llmtie_driver_fail("decode_q8", e);
-    plan_decode_q8(plan, per, n, (int)kv_heads, (int)head_dim, g->sm_count, clusters, weigh);
+    plan_decode_q8(plan, per, n, (int)kv_heads, (int)head_dim, g->sm_count, clusters);
     return LLMTIE_OK;
 }
 
@@ -136,7 +136,7 @@ llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, cons
         p.status = g->timeout_site;
         p.wait_cycles = g->wait_cycles;
         DecodeQ8Plan plan;
-        TRY(plan_jobs(g, jobs, b0, kv_heads, head_dim, weigh != 0, plan));
+        TRY(plan_jobs(g, jobs, b0, kv_heads, head_dim, plan));
         cudaError_t err;
         const int grid = plan.grid;
         p.cluster = plan.cluster;
@@ -158,12 +158,14 @@ llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, cons
             if (err != cudaSuccess) return llmtie_driver_fail("zeroing", err);
         }
         if (weigh && blocks > 0) {
-            p.stats = (float2 *)workspace_reserve(scratch->q8_stats, (size_t)blocks * 8 * sizeof(float2), g->stream, &err);
+            p.stats = (float2 *)workspace_reserve(scratch->q8_stats, ((size_t)blocks + pairs) * 8 * sizeof(float2), g->stream, &err);
             if (!p.stats) return llmtie_driver_fail("allocating", err);
+            p.fin = p.stats + blocks * 8;
         }
         LaunchScope ls(g, head_dim == 128 ? "decode_q8_128" : "decode_q8_64");
         err = launch_decode_q8(g->stream, p, (int)head_dim, grid);
         if (err != cudaSuccess) return llmtie_driver_fail("decode_q8", err);
+        if (p.stats) g->launches++;   // two kernels in that launcher then
         TRY(ls.done());
     }
     return LLMTIE_OK;
@@ -479,8 +481,8 @@ try {
 NO_MEMORY_IS_AN_ERROR
 
 extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv_heads, size_t head_dim,
-                                               int32_t weigh, int32_t sm_count, int32_t resident8, int32_t resident16,
-                                               int32_t *grid, int32_t *cluster, int64_t *ns)
+                                               int32_t sm_count, int32_t resident8, int32_t resident16, int32_t *grid,
+                                               int32_t *cluster, int64_t *ns)
 {
     if ((head_dim != 64 && head_dim != 128) || kv_heads == 0 || kv_heads > 4096) return llmtie_unsupported(head_dim, kv_heads, kv_heads);
     if (!live || !grid || !cluster || !ns || batch > LLMTIE_Q8_MAX_SEQ || sm_count <= 0) {
@@ -493,7 +495,7 @@ extern "C" llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch
     }
     const int clusters[2] = {resident8, resident16};
     DecodeQ8Plan plan;
-    plan_decode_q8(plan, units, (int)batch, (int)kv_heads, (int)head_dim, sm_count, clusters, weigh != 0);
+    plan_decode_q8(plan, units, (int)batch, (int)kv_heads, (int)head_dim, sm_count, clusters);
     *grid = plan.grid;
     *cluster = plan.cluster;
     *ns = (int64_t)(plan.us * 1000.0);
@@ -550,7 +552,7 @@ try {
     }
     for (size_t j = 0; j < jobs.size(); j += LLMTIE_Q8_MAX_SEQ) {
         DecodeQ8Plan plan;
-        TRY(plan_jobs(g, jobs, j, kv_heads, head_dim, false, plan));
+        TRY(plan_jobs(g, jobs, j, kv_heads, head_dim, plan));
         decoded += plan.us;
     }
     if (decoded > unpacked + (others ? 0.0 : 13.0)) {

@@ -243,36 +243,6 @@ __device__ __forceinline__ float2 peer_f2(uint32_t addr)
     return v;
 }
 
-// The weights of blocks [first, last) of one finished pair and of all of a second
-// (or of none: seq1 < 0), side by side, because what this costs is the latency of
-// its loads: what each complete block's tokens got, summed over
-// the group's heads; `fin` has each row's maximum and the inverse of its sum.
-template <int HD>
-__device__ __forceinline__ void weigh(const DecodeQ8Params &p, int seq0, int head0, int first, int last, int seq1, int head1,
-                                      const float2 *fin, int tid, int group)
-{
-    const int full0 = last - first, total = full0 + (seq1 >= 0 ? p.seq[seq1].full : 0);
-    for (int i = tid; i < total; i += kThreads) {
-        const bool second = i >= full0;
-        const int b = second ? i - full0 : first + i, seq = second ? seq1 : seq0, head = second ? head1 : head0;
-        const DecodeQ8Seq &sq = p.seq[seq];
-        const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
-        float *weight = (float *)(sq.base + at.w) + (long long)head * sq.nb + b;
-        const float2 *st = p.stats + (p.stat0[seq] + (long long)head * sq.full + b) * kRows;
-        const float2 *f = fin + (second ? kRows : 0);
-        float2 y[kRows];
-        const float before = *weight;
-#pragma unroll
-        for (int k = 0; k < kRows; k++) y[k] = k < group ? __ldcg(&st[k]) : make_float2(0.f, 0.f);
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kRows; k++) {
-            if (k < group) sum = fmaf(ex2(y[k].x - f[k].x) * f[k].y, y[k].y, sum);
-        }
-        *weight = before + sum;
-    }
-}
-
 // Row `row` of `count` partial results, slots first + skew, first + step, first + 2
 // step and so on: in that order, 32 at a time, 16 of their loads in flight.
 template <int HD>
@@ -343,7 +313,6 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[kWarps * G::STAGES];
     __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
-    __shared__ float2 final_s[2 * kRows];
     __shared__ int last_s[2];
     __shared__ float2 part_s[kRows];
 
@@ -723,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 #pragma unroll
                 for (int e = 0; e < V; e++) o[e] *= inv;
                 store_row<HD>(p, row_at(now.seq, now.head, row), lane, o);
-                if (lane == 0) final_s[row] = make_float2(M, inv);
+                if (p.stats && lane == 0) p.fin[((long long)now.seq * p.kv_heads + now.head) * kRows + row] = make_float2(M, inv);
             } else if (p.cluster) {
                 // (the ring is empty: there is no other run)
 #pragma unroll
@@ -739,19 +708,13 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 if (lane == 0) p.part_ml[slot * kRows + row] = make_float2(M, L);
             }
         }
-        if (now.whole) {
-            if (p.stats) {
-                __syncthreads();
-                weigh<HD>(p, now.seq, now.head, 0, sq.full, -1, 0, final_s, tid, rows);
-            }
-        } else if (is_first) {
-            shared0 = {now.seq, now.head, now.begin, now.units};
-        } else {
-            shared1 = {now.seq, now.head, now.begin, now.units};
+        if (!now.whole) {
+            if (is_first) shared0 = {now.seq, now.head, now.begin, now.units};
+            else shared1 = {now.seq, now.head, now.begin, now.units};
         }
         if (!more) break;
         is_first = false;
-        __syncthreads();   // merge, m_s and final_s are free again
+        __syncthreads();   // merge and m_s are free again
     }
 
     if (p.cluster > 1) {
@@ -824,20 +787,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 #pragma unroll
             for (int e = 0; e < V; e++) o[e] *= inv;
             store_row<HD>(p, row_at(run.seq, run.head, row), lane, o);
-        }
-        if (p.stats) {
-            // each block weighs its own cache blocks, and works the rows' sums out itself
-            if (tid < rows) {
-                float M = -CUDART_INF_F, L = 0.0f;
-                for (int k = 0; k < p.cluster; k++) M = fmaxf(M, peer_f2(peer(smem_u32(&part_s[tid]), k)).x);
-                for (int k = 0; k < p.cluster; k++) {
-                    const float2 ml = peer_f2(peer(smem_u32(&part_s[tid]), k));
-                    L = fmaf(ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - M), ml.y, L);
-                }
-                final_s[tid] = make_float2(M, 1.0f / L);
-            }
-            __syncthreads();
-            weigh<HD>(p, run.seq, run.head, run.first, run.last, -1, 0, final_s, tid, rows);
+            if (p.stats && lane == 0) p.fin[((long long)run.seq * p.kv_heads + run.head) * kRows + row] = make_float2(M, inv);
         }
         cluster_sync();   // no block leaves while another reads its results
         if (!ok) {
@@ -880,17 +830,48 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 #pragma unroll
         for (int e = 0; e < V; e++) o[e] *= inv;
         store_row<HD>(p, row_at(now.seq, now.head, row), lane, o);
-        if (lane == 0) final_s[item] = make_float2(M, inv);
-    }
-    if (p.stats && (last_s[0] || last_s[1])) {
-        __syncthreads();
-        const int seq = last_s[0] ? shared0.seq : shared1.seq;
-        weigh<HD>(p, seq, last_s[0] ? shared0.head : shared1.head, 0, p.seq[seq].full, last_s[0] && last_s[1] ? shared1.seq : -1, shared1.head, final_s + (last_s[0] ? 0 : kRows), tid, group);
+        if (p.stats && lane == 0) p.fin[(long long)pair * kRows + row] = make_float2(M, inv);
     }
     if (!ok) {
         // a wait gave up: leave the copies still in flight time to land
         for (int i = 0; i < 64; i++) __nanosleep(1000);
     }
+}
+
+// The weights, behind the decode kernel: what the tokens of each complete block got,
+// summed over the group's heads, from the block's maximum and sum of each row (in
+// `stats`) and the row's own (in `fin`). A thread a cache block, bound by the latency of
+// its 64 bytes: with this work in the decode kernel, done for a pair by whichever block
+// finished it, 4 x 131072 tokens of 4 KV heads x 128 took 134 us; they take 95, and 86
+// without weights. (The next kernel may start once the decode is over, no earlier: a
+// decode set up among these blocks is spread badly over the SMs, 66 us for 49 with 30 x
+// 15000 tokens of 4 KV heads x 64.)
+constexpr int kWeighThreads = 128;
+template <int HD>
+__global__ void __launch_bounds__(kWeighThreads) q8_weigh_kernel(const __grid_constant__ DecodeQ8Params p)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int pair = (int)blockIdx.x, seq = pair / p.kv_heads, head = pair - seq * p.kv_heads, group = p.heads / p.kv_heads;
+    const DecodeQ8Seq &sq = p.seq[seq];
+    const int b = (int)blockIdx.y * kWeighThreads + (int)threadIdx.x;
+    if (b >= sq.full) return;
+    const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
+    float *weight = (float *)(sq.base + at.w) + (long long)head * sq.nb + b;
+    const float2 *st = p.stats + (p.stat0[seq] + (long long)head * sq.full + b) * kRows, *f = p.fin + (long long)pair * kRows;
+    float2 y[kRows], z[kRows];
+    const float before = *weight;
+#pragma unroll
+    for (int k = 0; k < kRows; k++) {
+        y[k] = k < group ? st[k] : make_float2(0.f, 0.f);
+        z[k] = k < group ? f[k] : make_float2(0.f, 0.f);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kRows; k++) {
+        if (k < group) sum = fmaf(ex2(y[k].x - z[k].x) * z[k].y, y[k].y, sum);
+    }
+    *weight = before + sum;
 }
 
 // Sequences that hold no token: zeros.
@@ -961,11 +942,17 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
     }
     if (grid == 0) return cudaSuccess;
     const dim3 blocks((unsigned)grid);
-    return hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, p.cluster, decode_q8_kernel<128>, p)
-                     : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, p.cluster, decode_q8_kernel<64>, p);
+    const cudaError_t e = hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, p.cluster, decode_q8_kernel<128>, p)
+                                    : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, p.cluster, decode_q8_kernel<64>, p);
+    if (e != cudaSuccess || !p.stats) return e;
+    int most = 0;
+    for (int b = 0; b < p.nseq; b++) most = std::max(most, p.seq[b].full);
+    const dim3 all((unsigned)(p.nseq * p.kv_heads), (unsigned)((most + kWeighThreads - 1) / kWeighThreads));
+    return hd == 128 ? launch_dependent(st, all, kWeighThreads, 0, 1, q8_weigh_kernel<128>, p)
+                     : launch_dependent(st, all, kWeighThreads, 0, 1, q8_weigh_kernel<64>, p);
 }
 
-void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters, bool weigh)
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters)
 {
     // Microseconds, as measured (148 SMs): cache blocks a microsecond that the memory
     // gives (6.9 TB/s), a warp's time for one when nothing but the warp itself bounds
@@ -1018,11 +1005,10 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
         if (cost < plan.us && blocks <= 0x7fffffff) plan = DecodeQ8Plan{(int)blocks, c, 1, 0, cost};
     }
     // Several clusters of eight for a pair, as many as the device holds at once, and
-    // none of them without a block. (Not where weights are taken: no cluster then knows
-    // the rows' sums.) 131072 tokens, one KV head x 128: 15 us by 32 clusters, 45 by the
+    // none of them without a block. 131072 tokens, one KV head x 128: 15 us by 32 clusters, 45 by the
     // cut, whose last block has 296 results to merge; 8000 tokens: 12 us by 32 clusters,
     // 9 by one of 16.
-    for (long long parts = 2; parts <= 32 && pairs * parts <= clusters[0] && parts * 8 <= longest && !weigh; parts++) {
+    for (long long parts = 2; parts <= 32 && pairs * parts <= clusters[0] && parts * 8 <= longest; parts++) {
         const long long blocks = pairs * parts * 8;
         const double own = one * (double)(((longest + 8 * parts - 1) / (8 * parts) + 3) / 4);
         const double cost = kParts + kPart * (double)parts + std::max((double)total / all * std::max(1.0, 0.8 * most / (double)blocks), own);

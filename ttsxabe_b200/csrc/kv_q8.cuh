@@ -191,6 +191,7 @@ struct DecodeQ8Params {
     float2 *part_ml;         // [block][2][8], or [cluster][8]
     unsigned *ctr;           // arrivals of each (sequence, KV head), or of each of its rows; zero at rest
     float2 *stats;           // [block of a sequence][8] (maximum, sum), or null: no weights
+    float2 *fin;             // [sequence, KV head][8] (maximum, 1 / sum), with them
     int *status;
     long long wait_cycles;
 };
@@ -204,7 +205,6 @@ struct DecodeQ8Plan {
     int over;      // what the cut charges a run
     double us;     // about what it takes
 };
-void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters,
-                    bool weigh);
+void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, int hd, int sm_count, const int *clusters);
 // How many clusters of 8 and of 16 blocks the current device holds at once.
 cudaError_t decode_q8_clusters(int hd, int (&clusters)[2]);

@@ -176,14 +176,13 @@ def decode_plan(tk, kv_heads: int, rows: int, head_dim: int, sm_count: int = 148
     return mode.value, list(table[:grid.value + 1])
 
 
-def decode_plan_q8(live, kv_heads: int, head_dim: int, weigh: bool = False, sm_count: int = 148,
-                   resident=(36, 16)):
+def decode_plan_q8(live, kv_heads: int, head_dim: int, sm_count: int = 148, resident=(36, 16)):
     """How an 8-bit decode launch is laid over the device (host only): (blocks of
     the grid, size of the clusters that take a pair or 0 for the cut by work, about
     how many nanoseconds), for a device that holds `resident` clusters of 8 and 16 blocks."""
     grid, cluster, ns = C.c_int32(0), C.c_int32(0), C.c_int64(0)
     _check(_lib.load().llmtie_decode_plan_q8((C.c_int32 * len(live))(*live), len(live), kv_heads,
-                                             head_dim, int(weigh), sm_count, *resident,
+                                             head_dim, sm_count, *resident,
                                              C.byref(grid), C.byref(cluster), C.byref(ns)))
     return grid.value, cluster.value, ns.value
 
