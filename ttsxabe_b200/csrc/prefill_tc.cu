@@ -82,7 +82,8 @@ enum Bar {
     O_DONE = 14,   // +t
     S_FREE = 16,   // +t (head_dim 64 only)
     ITEM = 18,     // +slot
-    NBARS = 22
+    ITEM_FREE = 22,
+    NBARS = 26
 };
 
 // ---- PTX wrappers -----------------------------------------------------------------
@@ -373,9 +374,11 @@ prefill_tc_kernel(const __grid_constant__ Params p)
     // device has a block for each, at its coordinates (p.rounds == 0). Otherwise the
     // grid is a block an SM; a block's first item is its own number's, and the producer
     // takes each further one off the launch's counter when it has asked for the last
-    // tiles of the one before, and leaves it in a slot of `items`. (Four of them: the
-    // producer is never more than two steps ahead of the MMAs, and every item but the
-    // first has a step at least.)
+    // tiles of the one before, and leaves it in a slot of `items`. A slot is filled again
+    // when every warp that goes by the items has copied it (ITEM_FREE): the MMA issuer
+    // is never more than two steps behind, but a tile without rows in a run of short
+    // items, or the two warps that only prefetch, are tied to nothing else. (Four slots:
+    // none is waited for in practice.)
     auto unpack_item = [&](int x, int yz) {
         Item it;
         it.x = x;
@@ -466,7 +469,10 @@ prefill_tc_kernel(const __grid_constant__ Params p)
             mbar_init(BAR(O_DONE + s), 1);
             mbar_init(BAR(S_FREE + s), 4);
         }
-        for (int s = 0; s < 4; s++) mbar_init(BAR(ITEM + s), 1);
+        for (int s = 0; s < 4; s++) {
+            mbar_init(BAR(ITEM + s), 1);
+            mbar_init(BAR(ITEM_FREE + s), 11);   // the softmax's eight warps, the issuer, the two that prefetch
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid == 64) {
@@ -510,6 +516,8 @@ prefill_tc_kernel(const __grid_constant__ Params p)
         if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 50);
         if (!ok) break;
         const Item it = items[i & 3u];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(ITEM_FREE + (i & 3u)));
         if (it.seq < 0) break;
         const Item &sq = it;
         const int pieces = it.pieces, jbeg = it.jbeg, all_keys = it.all_keys;
@@ -877,6 +885,10 @@ prefill_tc_kernel(const __grid_constant__ Params p)
                         it.seq = -1;
                     }
                 }
+                if (i >= 4) {
+                    ok = mbar_wait(BAR(ITEM_FREE + (i & 3u)), ((i >> 2) & 1u) ^ 1u, wt, 32);
+                    if (!ok) break;
+                }
                 if (i > 0) items[i & 3u] = it;
                 mbar_arrive(BAR(ITEM + (i & 3u)));
                 if (it.seq < 0) break;
@@ -939,6 +951,7 @@ prefill_tc_kernel(const __grid_constant__ Params p)
                 if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 51);
                 if (!ok) break;
                 const Item it = items[i & 3u];
+                mbar_arrive(BAR(ITEM_FREE + (i & 3u)));
                 if (it.seq < 0) break;
                 const int n_a = it.n[0], n_b = it.n[1], n_max = max(n_a, n_b);
                 auto n_of = [n_a, n_b](int t) { return t ? n_b : n_a; };
@@ -1014,9 +1027,13 @@ prefill_tc_kernel(const __grid_constant__ Params p)
         }
     } else if (p.rounds) {
         // ============== the two other warps: the next item's queries into L2 ===================
+        // (every block's first item is taken at once: there is nothing to ask ahead for)
+        if (lane == 0) mbar_arrive(BAR(ITEM_FREE + 0));
         for (uint32_t i = 1;; i++) {
             if (!mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 52)) break;
             const Item it = items[i & 3u];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(ITEM_FREE + (i & 3u)));
             if (it.seq < 0) break;
             // (a warp a tile; the lanes of a line of 128 bytes are one row's)
             const int t = warp - 10, rows = min(BM, it.tq - (t ? it.r0[1] : it.r0[0]));
