@@ -90,3 +90,32 @@ def test_long_items_among_many_short_ones(gpu):
         again = b.run()
         gpu.synchronize()
         assert torch.equal(again, first)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(36, 4, 64), (27, 3, 128), (32, 8, 128)])
+def test_a_launch_whose_waits_run_out_ends_and_leaves_the_next_one_right(gpu, heads, kv, hd):
+    """With a limit of a cycle or a few thousand, waits give up anywhere in an item.
+    The launch ends, says so once, and what comes after it is whole."""
+    from ttsxabe_b200 import DeviceTimeout
+
+    past, new = [700] + [0] * 31, [300] + [1 + 9 * i for i in range(31)]
+    b = Batch(gpu, heads, kv, hd, past, new, seed=2)
+    want = b.run()
+    gpu.synchronize()
+    b.check(want)
+    for limit in (1, 500, 3000, 10000, 30000):
+        gpu.set_wait_limit_cycles(limit)
+        try:
+            b.run()
+            try:
+                gpu.synchronize()
+                reported = False
+            except DeviceTimeout:
+                reported = True
+            gpu.synchronize()
+        finally:
+            gpu.set_wait_limit_cycles(0)
+        assert reported or limit > 1
+        again = b.run()
+        gpu.synchronize()
+        assert torch.equal(again, want)

@@ -83,7 +83,8 @@ enum Bar {
     S_FREE = 16,   // +t (head_dim 64 only)
     ITEM = 18,     // +slot
     ITEM_FREE = 22,
-    NBARS = 26
+    Q_FREE = 26,   // +t
+    NBARS = 28
 };
 
 // ---- PTX wrappers -----------------------------------------------------------------
@@ -468,6 +469,7 @@ prefill_tc_kernel(const __grid_constant__ Params p)
             mbar_init(BAR(P_FULL + s), 4);
             mbar_init(BAR(O_DONE + s), 1);
             mbar_init(BAR(S_FREE + s), 4);
+            mbar_init(BAR(Q_FREE + s), 4);
         }
         for (int s = 0; s < 4; s++) {
             mbar_init(BAR(ITEM + s), 1);
@@ -529,8 +531,10 @@ prefill_tc_kernel(const __grid_constant__ Params p)
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         if (me.n > 0) {
             // The tile's four warps are past the item before: its epilogue may have gone
-            // through this memory.
-            if (i > 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+            // through this memory. (A barrier of the hardware's own would wait for good
+            // for a warp that has given up.)
+            if (done_items > 0) ok = mbar_wait(BAR(Q_FREE + t), (done_items - 1) & 1u, wt, 24 + t);
+            if (!ok) break;
             // -- stage Q: f32 rows -> f16, scaled, into the swizzled K-major layout ------
             {
                 const float *qh = p.q + (long long)sq.row0 * p.q_stride + me.head * HD;
@@ -863,6 +867,8 @@ prefill_tc_kernel(const __grid_constant__ Params p)
                 }
             }
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(Q_FREE + t));
             steps += (uint32_t)me.n;
             done_items++;
         }
