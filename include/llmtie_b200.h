@@ -80,7 +80,9 @@ int32_t llmtie_ordinal(llmtie_gpu *g);
 llmtie_status llmtie_synchronize(llmtie_gpu *g);
 /* How long a device-side wait (an mbarrier of the tensor-memory prefill, a
  * flag another GPU raises) may spin before it gives up, in SM cycles. The
- * default, also restored by cycles <= 0, is 2^31: about a second. No
+ * default, also restored by cycles <= 0, is 2^31: about a second. It is the
+ * limit for one step of a kernel's pipeline; a warp of the prefill that sits
+ * out an item of work waits up to that for each of the item's key tiles. No
  * counterpart in the reference, whose kernels never wait on one another. */
 llmtie_status llmtie_set_wait_limit_cycles(llmtie_gpu *g, int64_t cycles);
 

@@ -119,3 +119,24 @@ def test_a_launch_whose_waits_run_out_ends_and_leaves_the_next_one_right(gpu, he
         again = b.run()
         gpu.synchronize()
         assert torch.equal(again, want)
+
+
+def test_the_wait_limit_is_one_for_a_step_however_long_an_item_is(gpu):
+    """Items of 512 key tiles without a second row block: the warps that sit an item out
+    wait much longer than 200000 cycles (0.1 ms), none waits as long for a step."""
+    heads, kv, hd, rows, n = 156, 52, 128, 100, 65536
+    torch.manual_seed(4)
+    q = torch.randn(rows, heads, hd, device=gpu.device).half().float()
+    k = torch.randn(kv, n, hd, device=gpu.device, dtype=torch.float16)
+    v = torch.randn(kv, hd, n, device=gpu.device, dtype=torch.float16)
+    torch.cuda.synchronize()
+    gpu.set_wait_limit_cycles(200_000)
+    try:
+        out = gpu.flash_attn_f16(q, k, v, rows, n - rows, heads, kv, hd, n, hd ** -0.5, True).view(rows, heads, hd)
+        gpu.synchronize()
+    finally:
+        gpu.set_wait_limit_cycles(0)
+    for j in (0, 25, 51):
+        group = slice(3 * j, 3 * j + 3)
+        want, tol = attention(q[:, group].double(), k[j:j + 1].double(), v[j:j + 1].double().transpose(1, 2), hd ** -0.5, n - rows)
+        assert ((out[:, group].double() - want).abs() <= tol).all(), f"KV head {j}"

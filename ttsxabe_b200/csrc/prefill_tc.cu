@@ -145,7 +145,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 // pipeline step lasts). The bound is a deadline in
 // SM cycles, checked every 256 polls together with the block's abort flag.
 // Returns false once the deadline passed or another role gave up; the caller
-// then leaves its loop.
+// then leaves its loop. The limit is one for a step of the pipeline: a wait that
+// lasts as long as `spans` of them has so many.
 struct Waiter {
     volatile int *abort_flag;   // the block's own (shared memory)
     int *status;                // the handle's site word
@@ -153,7 +154,7 @@ struct Waiter {
     int epoch;
     long long cycles;
 };
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waiter &w, int site)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waiter &w, int site, int spans = 1)
 {
     if (mbar_try(bar, parity)) return true;
     const long long start = clock64();
@@ -161,7 +162,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 15u) == 0) {
             if (*w.abort_flag) return false;
-            if (clock64() - start > w.cycles) break;
+            if (clock64() - start > w.cycles * spans) break;
         }
     }
     *w.abort_flag = 1;
@@ -380,6 +381,9 @@ prefill_tc_kernel(const __grid_constant__ Params p)
     // is never more than two steps behind, but a tile without rows in a run of short
     // items, or the two warps that only prefetch, are tied to nothing else. (Four slots:
     // none is waited for in practice.)
+    // What a wait for the next item may last, in steps, besides those of the item in
+    // between: the two that the producer is ahead, a tile's staging and its epilogue.
+    constexpr int kBetween = 6;
     auto unpack_item = [&](int x, int yz) {
         Item it;
         it.x = x;
@@ -514,8 +518,9 @@ prefill_tc_kernel(const __grid_constant__ Params p)
         const int t = warp >> 2;
         bool ok = true;
         uint32_t steps = 0, done_items = 0;              // this tile's, over the items before
+        int spans = kBetween;                            // that the next item may be away
         for (uint32_t i = 0; ok; i++) {
-        if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 50);
+        if (i > 0) ok = mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 50, spans);
         if (!ok) break;
         const Item it = items[i & 3u];
         __syncwarp();
@@ -871,6 +876,9 @@ prefill_tc_kernel(const __grid_constant__ Params p)
             if (lane == 0) mbar_arrive(BAR(Q_FREE + t));
             steps += (uint32_t)me.n;
             done_items++;
+            spans = kBetween;
+        } else {
+            spans = it.n[0] + it.n[1] + kBetween;        // (the other tile's)
         }
         }
     } else if (warp == 8) {
@@ -1034,13 +1042,16 @@ prefill_tc_kernel(const __grid_constant__ Params p)
     } else if (p.rounds) {
         // ============== the two other warps: the next item's queries into L2 ===================
         // (every block's first item is taken at once: there is nothing to ask ahead for)
+        int spans = max(items[0].n[0], items[0].n[1]) + kBetween;    // that the next item is away
+        __syncwarp();
         if (lane == 0) mbar_arrive(BAR(ITEM_FREE + 0));
         for (uint32_t i = 1;; i++) {
-            if (!mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 52)) break;
+            if (!mbar_wait(BAR(ITEM + (i & 3u)), (i >> 2) & 1u, wt, 52, spans)) break;
             const Item it = items[i & 3u];
             __syncwarp();
             if (lane == 0) mbar_arrive(BAR(ITEM_FREE + (i & 3u)));
             if (it.seq < 0) break;
+            spans = max(it.n[0], it.n[1]) + kBetween;
             // (a warp a tile; the lanes of a line of 128 bytes are one row's)
             const int t = warp - 10, rows = min(BM, it.tq - (t ? it.r0[1] : it.r0[0]));
             if ((t ? it.n[1] : it.n[0]) == 0) continue;
