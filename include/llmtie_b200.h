@@ -74,7 +74,7 @@ int32_t llmtie_ordinal(llmtie_gpu *g);
 /* Gpu::synchronize (device.rs:1433-1440). Also surfaces LLMTIE_ERR_TIMEOUT if
  * a kernel's bounded wait gave up since the last report (llmtie_download
  * reports it as well). A timeout is reported once; reporting it clears the
- * arrival counters of every decode scratch of the handle, so the next call
+ * f16 arrival counters of every decode scratch of the handle, so the next call
  * starts clean. What the kernel that gave up should have written is
  * undefined. */
 llmtie_status llmtie_synchronize(llmtie_gpu *g);

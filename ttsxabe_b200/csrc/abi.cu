@@ -236,17 +236,19 @@ extern "C" int32_t llmtie_ordinal(llmtie_gpu *g) { return g ? g->ordinal : -1; }
 // After the stream has been waited for: whether a bounded device wait gave up
 // since the last report. The word is host memory the kernels write through a
 // mapping, so looking at it costs nothing. A timeout is reported once; the
-// words are cleared, and so are the arrival counters of every DecodeScratch
-// of this handle, which a launch that gave up may have left mid-count.
+// words are cleared, and so are the arrival counters of f16 decode in every
+// DecodeScratch of this handle, which a launch that gave up may have left
+// mid-count. The item counters of prefill and the arrivals of 8-bit decode are
+// left alone: a block that gives up counts itself there all the same, so they
+// come back to zero, and a graph on another stream may be counting in its own.
 static llmtie_status report_device_timeout(llmtie_gpu *g)
 {
     const int site = *(volatile int *)g->timeout_host;
     if (site == 0) return LLMTIE_OK;
     *(volatile int *)g->timeout_host = 0;
-    cudaMemsetAsync(g->abort_epoch, 0, kHandleWords * sizeof(int), g->stream);
+    cudaMemsetAsync(g->abort_epoch, 0, sizeof(int), g->stream);
     for (llmtie_decode_scratch *s : g->scratches) {
         if (s->ctr) cudaMemsetAsync(s->ctr, 0, s->ctr_words * sizeof(unsigned), g->stream);
-        if (s->q8_ctr.ptr) cudaMemsetAsync(s->q8_ctr.ptr, 0, s->q8_ctr.bytes, g->stream);
     }
     return llmtie_fail(LLMTIE_ERR_TIMEOUT, "a bounded device wait gave up (site %d)", site);
 }
