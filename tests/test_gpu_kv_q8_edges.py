@@ -1,0 +1,60 @@
+"""The 8-bit KV cache where it could go wrong: waits that run out, values that are not
+finite, caches that are forked, buffers in the wrong place."""
+import numpy as np
+import pytest
+import torch
+
+from ttsxabe_b200 import DecodeScratch, DeviceTimeout, decode_plan_q8
+
+pytestmark = pytest.mark.gpu
+
+
+def caches_of(gpu, kv, hd, lives, seed, cap=None):
+    """Caches of random tokens, and their capacities."""
+    torch.manual_seed(seed)
+    caps = [max(32, (n + 31) // 32 * 32) if cap is None else cap for n in lives]
+    ts = [gpu.kv_alloc_q8(kv, hd, c) for c in caps]
+    rows = np.concatenate([[0], np.cumsum(lives)]).tolist()
+    k, v = torch.randn(2, rows[-1], kv * hd, device=gpu.device)
+    torch.cuda.synchronize()
+    zeros = [0] * len(lives)
+    gpu.rope_append_q8(None, k, v, rows, ts, caps, zeros, zeros, None, kv, kv, hd)
+    gpu.synchronize()
+    return ts, caps
+
+
+# ---- waits that run out ----------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv,hd,batch,live,cluster", [
+    (32, 8, 128, 16, 600, 2), (32, 8, 128, 1, 1999, 8), (4, 1, 128, 1, 7000, 16), (32, 8, 128, 1, 33000, 0), (20, 20, 64, 8, 1500, 2),
+    (8, 1, 128, 1, 40000, 8)])
+def test_decode_under_a_limit_of_a_cycle_ends_and_leaves_the_next_one_right(gpu, heads, kv, hd, batch, live, cluster):
+    """A wait may give up or find its copy there in time; either way the launch ends,
+    and its counters are at zero for the next."""
+    lives = [live - 3 * b for b in range(batch)]
+    assert decode_plan_q8(lives, kv, hd)[1] == cluster
+    ts, caps = caches_of(gpu, kv, hd, lives, seed=live)
+    q = torch.randn(batch, heads * hd, device=gpu.device)
+    torch.cuda.synchronize()
+    scratch = DecodeScratch()
+
+    def run():
+        return gpu.decode_batched_q8(q, ts, lives, caps, heads, kv, hd, hd ** -0.5, scratch)
+
+    want = run()
+    gpu.synchronize()
+    for _ in range(5):
+        gpu.set_wait_limit_cycles(1)
+        try:
+            out = run()
+            try:
+                gpu.synchronize()
+                assert torch.equal(out, want)
+            except DeviceTimeout:
+                pass
+        finally:
+            gpu.set_wait_limit_cycles(0)
+        gpu.synchronize()
+        out = run()
+        gpu.synchronize()
+        assert torch.equal(out, want)

@@ -422,8 +422,11 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
         return ahead_blk < ahead.last;
     };
+    bool ok = true;
     auto fetch = [&] {
-        if (!skip_done()) return;
+        // (after a wait that gave up the stage's copy may still be in flight, and its
+        // barrier in the phase it was armed for: nothing more is asked for)
+        if (!ok || !skip_done()) return;
         if (lane == 0) {
             const int stage = issued % G::STAGES;
             const uint32_t dst = ring0 + (uint32_t)stage * G::STAGE, bar = bar0 + 8 * stage;
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     };
     for (int s = 0; s < G::STAGES; s++) fetch();
 
-    bool ok = true, is_first = true;
+    bool is_first = true;
     Shared shared0 = {0, 0, 0, 0}, shared1 = {0, 0, 0, 0};       // of the first run and the last
     for (;;) {
         const DecodeQ8Seq &sq = p.seq[run.seq];
