@@ -66,6 +66,17 @@ llmtie_status llmtie_open(int32_t ordinal, llmtie_gpu **out);
 /* The same, adopting a stream the caller owns (a cudaStream_t). */
 llmtie_status llmtie_open_on_stream(int32_t ordinal, void *stream, llmtie_gpu **out);
 void llmtie_close(llmtie_gpu *g);
+/* Calls may be captured into a CUDA graph once the same call has been made
+ * before the capture: a handle and a decode scratch keep workspaces, which grow
+ * on the first call that needs more of them, and growing under a capture is
+ * refused (LLMTIE_ERR_DRIVER). A workspace that a captured call uses is kept
+ * until the handle (or the decode scratch) is freed even where a later call
+ * outgrows it, so that the graph may be replayed. The calls of a handle or a
+ * scratch share those workspaces: graphs that hold such calls are replayed one
+ * after another, and not while another call of the same handle or scratch runs.
+ * (A prefill of more work than the device holds at once goes by counters, of
+ * which a handle has enough for 8192 captured launches in its life; captured
+ * after that it gives the same results, a few percent slower.) */
 /* Message of the last refused or failed call on this thread. */
 const char *llmtie_last_error(void);
 /* The handle's cudaStream_t. */
@@ -542,11 +553,7 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
  * query (but for rows that are rotated in place). A capacity that is not a multiple of
  * 32 is refused with LLMTIE_ERR_RAGGED_BLOCK.
  *
- * Calls may be captured into a CUDA graph once the same call has been made
- * before the capture: workspaces grow on the first call, which a capture
- * refuses, and a workspace that was outgrown is kept until the handle (or the
- * decode scratch) is freed, so that a captured call may be replayed. Graphs
- * that share a handle or a scratch must not be replayed at the same time. */
+ * Calls may be captured into a CUDA graph as others may (see llmtie_close). */
 
 /* Bytes of a cache; 0 for a shape that there is none of. Host only. */
 size_t llmtie_kv_q8_bytes(size_t kv_heads, size_t head_dim, size_t cap);

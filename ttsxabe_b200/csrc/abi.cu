@@ -59,24 +59,35 @@ llmtie_status llmtie_fail(llmtie_status code, const char *fmt, ...)
 
 extern "C" const char *llmtie_last_error(void) { return g_err; }
 
-void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t *err)
+void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t *err, size_t least)
 {
     *err = cudaSuccess;
-    if (bytes <= w.bytes) return w.ptr;
-    if (w.keep) {
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        *err = cudaStreamIsCapturing(st, &capture);
-        if (*err == cudaSuccess && capture != cudaStreamCaptureStatusNone) {
-            *err = cudaErrorStreamCaptureUnsupported;   // make the call once before capturing it
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    const cudaError_t asked = cudaStreamIsCapturing(st, &status);
+    if (asked != cudaSuccess) cudaGetLastError();
+    const bool capturing = asked != cudaSuccess || status != cudaStreamCaptureStatusNone;
+    if (bytes <= w.bytes) {
+        w.captured = w.captured || capturing;
+        return w.ptr;
+    }
+    if (capturing) {
+        *err = cudaErrorStreamCaptureUnsupported;   // make the call once before capturing it
+        return nullptr;
+    }
+    if (w.captured) {
+        try {
+            w.outgrown.push_back({w.ptr, w.bytes});
+        } catch (const std::bad_alloc &) {
+            *err = cudaErrorMemoryAllocation;
+            return nullptr;
         }
-        if (*err != cudaSuccess) return nullptr;
-        if (w.ptr) w.outgrown.push_back(w.ptr);
     } else if (w.ptr) {
         cudaFreeAsync(w.ptr, st);
     }
     w.ptr = nullptr;
     w.bytes = 0;
-    size_t want = 1 << 20;
+    w.captured = false;
+    size_t want = least;
     while (want < bytes) want <<= 1;
     *err = cudaMallocAsync(&w.ptr, want, st);
     if (*err != cudaSuccess) {
@@ -89,11 +100,12 @@ void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t
 
 void workspace_free(Workspace &w, cudaStream_t st)
 {
-    for (void *p : w.outgrown) cudaFreeAsync(p, st);
+    for (const Workspace::Buffer &b : w.outgrown) cudaFreeAsync(b.ptr, st);
     if (w.ptr) cudaFreeAsync(w.ptr, st);
     w.outgrown.clear();
     w.ptr = nullptr;
     w.bytes = 0;
+    w.captured = false;
 }
 
 LaunchScope::LaunchScope(llmtie_gpu *g_, const char *name_) : g(g_), name(name_)
@@ -215,9 +227,9 @@ extern "C" void llmtie_close(llmtie_gpu *g)
     if (!g) return;
     cudaSetDevice(g->ordinal);
     if (g->stream) cudaStreamSynchronize(g->stream);
-    if (g->ws_rope.ptr) cudaFreeAsync(g->ws_rope.ptr, g->stream);
-    if (g->ws_part.ptr) cudaFreeAsync(g->ws_part.ptr, g->stream);
-    if (g->ws_kv16.ptr) cudaFreeAsync(g->ws_kv16.ptr, g->stream);
+    workspace_free(g->ws_rope, g->stream);
+    workspace_free(g->ws_part, g->stream);
+    workspace_free(g->ws_kv16, g->stream);
     llmtie_decode_scratch_free(g, g->q8_scratch);
     workspace_free(g->ws_q8, g->stream);
     workspace_free(g->ws_q8_part, g->stream);
@@ -248,7 +260,8 @@ static llmtie_status report_device_timeout(llmtie_gpu *g)
     *(volatile int *)g->timeout_host = 0;
     cudaMemsetAsync(g->abort_epoch, 0, sizeof(int), g->stream);
     for (llmtie_decode_scratch *s : g->scratches) {
-        if (s->ctr) cudaMemsetAsync(s->ctr, 0, s->ctr_words * sizeof(unsigned), g->stream);
+        if (s->ctr.ptr) cudaMemsetAsync(s->ctr.ptr, 0, s->ctr.bytes, g->stream);
+        for (const Workspace::Buffer &b : s->ctr.outgrown) cudaMemsetAsync(b.ptr, 0, b.bytes, g->stream);
     }
     return llmtie_fail(LLMTIE_ERR_TIMEOUT, "a bounded device wait gave up (site %d)", site);
 }
@@ -271,8 +284,10 @@ extern "C" llmtie_status llmtie_set_wait_limit_cycles(llmtie_gpu *g, int64_t cyc
 // What a tensor-memory prefill launch is given for its bounded waits; every
 // launch gets a number of its own. The counters its blocks go by belong to the
 // handle for a launch on its stream, where one follows another; a captured launch has
-// its own, since graphs may be replayed beside each other on other streams. Once those
-// are used up a captured launch has none and takes a block for every item.
+// its own, so that a graph replayed on another stream takes no items from it. Once those
+// are used up a captured launch has none and takes a block for every item. (That is all
+// that is a launch's own: the pieces of cut rows, the ragged pre-pass's table and staged
+// caches lie in the handle's workspaces, which one call uses at a time.)
 static WaitCtl next_wait_ctl(llmtie_gpu *g)
 {
     g->epoch = g->epoch == 0x7fffffff ? 1 : g->epoch + 1;
@@ -1083,8 +1098,8 @@ extern "C" void llmtie_decode_scratch_free(llmtie_gpu *g, llmtie_decode_scratch 
 {
     if (!s) return;
     if (g) {
-        if (s->part) cudaFreeAsync(s->part, g->stream);
-        if (s->ctr) cudaFreeAsync(s->ctr, g->stream);
+        workspace_free(s->part, g->stream);
+        workspace_free(s->ctr, g->stream);
         workspace_free(s->q8_part, g->stream);
         workspace_free(s->q8_ctr, g->stream);
         workspace_free(s->q8_stats, g->stream);
@@ -1100,25 +1115,15 @@ extern "C" void llmtie_decode_scratch_free(llmtie_gpu *g, llmtie_decode_scratch 
 static llmtie_status scratch_reserve(llmtie_gpu *g, llmtie_decode_scratch *s, size_t pairs,
                                      size_t partials, size_t hd)
 {
-    const size_t floats = partials * 8 * (hd + 2);
-    if (floats > s->part_floats) {
-        if (s->part) cudaFreeAsync(s->part, g->stream);
-        s->part = nullptr;
-        s->part_floats = 0;
-        const size_t want = next_pow2(floats);
-        const cudaError_t e = cudaMallocAsync((void **)&s->part, want * sizeof(float), g->stream);
-        if (e != cudaSuccess) return driver_fail("allocating", e);
-        s->part_floats = want;
-    }
-    if (pairs > s->ctr_words) {
-        if (s->ctr) cudaFreeAsync(s->ctr, g->stream);
-        s->ctr = nullptr;
-        s->ctr_words = 0;
-        const size_t want = next_pow2(pairs);
-        cudaError_t e = cudaMallocAsync((void **)&s->ctr, want * sizeof(unsigned), g->stream);
-        if (e == cudaSuccess) e = cudaMemsetAsync(s->ctr, 0, want * sizeof(unsigned), g->stream);
-        if (e != cudaSuccess) return driver_fail("allocating", e);
-        s->ctr_words = want;
+    cudaError_t e;
+    workspace_reserve(s->part, partials * 8 * (hd + 2) * sizeof(float), g->stream, &e, 1024);
+    if (e != cudaSuccess) return driver_fail("allocating", e);
+    const size_t had = s->ctr.bytes;
+    workspace_reserve(s->ctr, pairs * sizeof(unsigned), g->stream, &e, 256);
+    if (e != cudaSuccess) return driver_fail("allocating", e);
+    if (s->ctr.bytes != had) {
+        e = cudaMemsetAsync(s->ctr.ptr, 0, s->ctr.bytes, g->stream);
+        if (e != cudaSuccess) return driver_fail("zeroing", e);
     }
     return LLMTIE_OK;
 }
@@ -1267,8 +1272,8 @@ static llmtie_status decode_launch(llmtie_gpu *g, const char *name, DecodeParams
         const llmtie_status s =
             scratch_reserve(g, scratch, pairs + 1, (size_t)grid * 2, (size_t)hd);
         if (s != LLMTIE_OK) return s;
-        sp.part = scratch->part;
-        sp.ctr = scratch->ctr;
+        sp.part = (float *)scratch->part.ptr;
+        sp.ctr = (unsigned *)scratch->ctr.ptr;
         if (xch) {
             sp.xch_world = xch->world;
             sp.xch_rank = xch->rank;
@@ -1277,7 +1282,7 @@ static llmtie_status decode_launch(llmtie_gpu *g, const char *name, DecodeParams
                 sp.xch_flags[r] = xch->flags[r];
             }
             sp.xch_step = xch->step;
-            sp.xch_done = scratch->ctr + pairs;   // one more counter after the pairs'
+            sp.xch_done = sp.ctr + pairs;   // one more counter after the pairs'
             sp.xch_pairs = (int)pairs;
             sp.xch_rank_stride = (long long)p.nseq * p.out_seq;
             if (fused) {
@@ -1298,8 +1303,8 @@ static llmtie_status decode_launch(llmtie_gpu *g, const char *name, DecodeParams
     const llmtie_status s =
         scratch_reserve(g, scratch, pairs, pairs * (size_t)p.max_splits, (size_t)hd);
     if (s != LLMTIE_OK) return s;
-    p.part = scratch->part;
-    p.ctr = scratch->ctr;
+    p.part = (float *)scratch->part.ptr;
+    p.ctr = (unsigned *)scratch->ctr.ptr;
     LaunchScope ls(g, name);
     const cudaError_t e = launch_decode_f16(g->stream, p, hd);
     if (e != cudaSuccess) return driver_fail(name, e);
@@ -1474,8 +1479,8 @@ extern "C" llmtie_status llmtie_attn_decode(llmtie_gpu *g, const float *q, size_
     LaunchScope ls(g, "attn_decode_f64");
     launch_decode_f32(g->stream, q, (long long)q_off, k, v, out, (long long)out_off, (int)heads,
                       (int)kv_heads, (int)head_dim, (int)tk, (int)cap, scale_q ? scale : 1.0f,
-                      scale_q ? 1.0f : scale, scratch ? scratch->part : nullptr,
-                      scratch ? scratch->ctr : nullptr);
+                      scale_q ? 1.0f : scale, scratch ? (float *)scratch->part.ptr : nullptr,
+                      scratch ? (unsigned *)scratch->ctr.ptr : nullptr);
     return ls.done();
 }
 

@@ -22,19 +22,22 @@ struct KprofEntry {
 // A device buffer the handle keeps between calls and only ever grows, so that
 // a call which needs scratch memory allocates nothing once it is warm. Work
 // on a handle is stream-ordered, so one call's use ends before the next's begins.
-// With `keep` set a buffer that was outgrown is kept until the handle closes,
-// because a captured graph may still replay work in it, and growing under a
-// capture is refused, because the memory would belong to the graph.
+// Growing under a capture is refused, because the memory would belong to the
+// graph; a buffer that a captured call was given is kept when it is outgrown,
+// until its owner is freed, because the graph may still replay work in it.
 struct Workspace {
     void *ptr = nullptr;
     size_t bytes = 0;
-    bool keep = false;
-    std::vector<void *> outgrown;
-    Workspace() = default;
-    explicit Workspace(bool keep_) : keep(keep_) {}
+    bool captured = false;           // a captured call was given `ptr`
+    struct Buffer {
+        void *ptr;
+        size_t bytes;
+    };
+    std::vector<Buffer> outgrown;    // those of captured calls
 };
-// Returns at least `bytes` of it (null and *err set if the allocation failed).
-void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t *err);
+// Returns at least `bytes` of it (null and *err set if the allocation failed),
+// allocated in powers of two from `least` on.
+void *workspace_reserve(Workspace &w, size_t bytes, cudaStream_t st, cudaError_t *err, size_t least = (size_t)1 << 20);
 
 struct llmtie_gpu {
     int ordinal = 0;
@@ -66,8 +69,8 @@ struct llmtie_gpu {
     Workspace ws_rope;   // the ragged prefill's table of cosines and sines (or its copy of q)
     Workspace ws_part;   // partial results of a prefill whose long row blocks were cut
     llmtie_decode_scratch *q8_scratch = nullptr;   // for prompts of few rows over the 8-bit cache
-    Workspace ws_q8{true};       // the 8-bit cache: its live keys as f16 for prefill, eviction's block lists
-    Workspace ws_q8_part{true};  // the pieces of cut row blocks of prefill over it
+    Workspace ws_q8;         // the 8-bit cache: its live keys as f16 for prefill, eviction's block lists
+    Workspace ws_q8_part;    // the pieces of cut row blocks of prefill over it
     Workspace ws_kv16;   // f16 copies of the live keys of caches the tensor-memory prefill cannot map
 };
 
@@ -81,12 +84,10 @@ struct DecodeMapKey {
 };
 
 struct llmtie_decode_scratch {
-    float *part = nullptr;     // [pairs][splits][8][hd + 2]
-    unsigned *ctr = nullptr;   // [pairs], zero at rest
-    size_t part_floats = 0;
-    size_t ctr_words = 0;
+    Workspace part;   // float [pairs][splits][8][hd + 2]
+    Workspace ctr;    // unsigned [pairs], zero at rest
     // the same for decode over the 8-bit cache, and its blocks' statistics
-    Workspace q8_part{true}, q8_ctr{true}, q8_stats{true};
+    Workspace q8_part, q8_ctr, q8_stats;
     // tensor maps of the caches this scratch was last used with, per sequence slot
     DecodeMapKey map_key[32];
     alignas(64) CUtensorMap kmap[32];
