@@ -422,11 +422,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
         return ahead_blk < ahead.last;
     };
-    bool ok = true;
     auto fetch = [&] {
-        // (after a wait that gave up the stage's copy may still be in flight, and its
-        // barrier in the phase it was armed for: nothing more is asked for)
-        if (!ok || !skip_done()) return;
+        if (!skip_done()) return;
         if (lane == 0) {
             const int stage = issued % G::STAGES;
             const uint32_t dst = ring0 + (uint32_t)stage * G::STAGE, bar = bar0 + 8 * stage;
@@ -440,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
     };
     for (int s = 0; s < G::STAGES; s++) fetch();
 
-    bool is_first = true;
+    bool ok = true, is_first = true;
     Shared shared0 = {0, 0, 0, 0}, shared1 = {0, 0, 0, 0};       // of the first run and the last
     for (;;) {
         const DecodeQ8Seq &sq = p.seq[run.seq];
@@ -555,10 +552,13 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         }
 
         // -- the warp's blocks
-        for (int blk = run.first + warp; blk < run.last; blk += kWarps) {
+        for (int blk = ok ? run.first + warp : run.last; blk < run.last; blk += kWarps) {
             const int stage = used % G::STAGES;
             const uint32_t kb = ring0 + (uint32_t)stage * G::STAGE, vb = kb + G::BLOCK;
-            if (ok) ok = ring_wait(bar0 + 8 * stage, (uint32_t)(used / G::STAGES) & 1u, p.status, p.wait_cycles);
+            // (given up, the stage's copy may still be in flight, and its barrier in the
+            // phase it was armed for: the warp takes and asks for no more blocks)
+            ok = ring_wait(bar0 + 8 * stage, (uint32_t)(used / G::STAGES) & 1u, p.status, p.wait_cycles);
+            if (!ok) break;
             used++;
             // scores: column n of tile t is token 8 (n / 2) + 2 t + n % 2
             float s[8];
