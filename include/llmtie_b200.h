@@ -534,7 +534,9 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
  * f16. The tokens of the last, incomplete block are f16 rows (the tail) until
  * the block is complete, so the codes do not depend on how the tokens arrived,
  * one by one or in prompts cut anywhere. A block that holds an infinity or a
- * NaN reads back as NaN throughout.
+ * NaN reads back as NaN throughout. A row that attends to a key or a value that
+ * is not finite may come out as NaN in every channel of the head; one that does
+ * not (a causal row before it) is not touched by it.
  *
  * A cache is ONE buffer of llmtie_kv_q8_bytes bytes, 16-byte aligned, for a
  * capacity of a multiple of 32 tokens. With nb = capacity / 32 it holds, each

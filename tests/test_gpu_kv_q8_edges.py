@@ -58,3 +58,55 @@ def test_decode_under_a_limit_of_a_cycle_ends_and_leaves_the_next_one_right(gpu,
         out = run()
         gpu.synchronize()
         assert torch.equal(out, want)
+
+
+# ---- values that are not finite ------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("heads,kv,hd,past,n", [
+    (8, 2, 128, 500, 8), (8, 1, 64, 61, 9), (4, 4, 64, 3, 20),           # few rows: the decode kernel
+    (32, 8, 128, 90, 200), (27, 3, 128, 500, 150), (36, 4, 64, 0, 140),  # the prefill kernel
+    (8, 2, 128, 4000, 250)])                                              # its keys cut into pieces
+def test_rows_before_a_value_that_is_not_finite(gpu, heads, kv, hd, past, n, which, bad):
+    """It lies in the tail or in a complete block of the first KV head, among the
+    prompt's own rows. Rows that may not see it are what they are without it, bit
+    for bit, and those that see it are not finite."""
+    live = past + n
+    cap = (live + 31) // 32 * 32
+    torch.manual_seed(live)
+    k, v = torch.randn(2, live, kv, hd, device=gpu.device)
+    q = torch.randn(n, heads, hd, device=gpu.device)
+    torch.cuda.synchronize()
+
+    def run(k, v):
+        t = gpu.kv_alloc_q8(kv, hd, cap)
+        gpu.rope_append_q8(None, k, v, [0, live], [t], [cap], [0], [0], None, heads, kv, hd)
+        out = gpu.flash_attn_q8(q, [0, n], [t], [cap], [past], heads, kv, hd, hd ** -0.5, True)
+        gpu.synchronize()
+        return out.view(n, heads, hd)
+
+    clean = run(k, v)
+    assert clean.isfinite().all()
+    spots = [live - 1, live - n // 3] + ([live // 32 * 32 - 7] if live // 32 * 32 - 7 > past else [])
+    for spot in spots:
+        rows = {"k": k, "v": v}
+        x = rows[which] = rows[which].clone()
+        x[spot, 0, 5] = bad
+        torch.cuda.synchronize()
+        out = run(rows["k"], rows["v"])
+        group = heads // kv
+        assert torch.equal(out[:, group:], clean[:, group:])
+        # a complete block is of NaN throughout
+        first = spot // 32 * 32 if spot < live // 32 * 32 else spot
+        before = max(first - past, 0)
+        assert torch.equal(out[:before, :group], clean[:before, :group])
+        seen = out[before:, :group]
+        if which == "k" and first == spot:
+            # (where the infinite key's score is minus infinity, nothing is added)
+            counts = torch.isnan(x[spot, 0, 5]) | (q[before:, :group, 5] > 0)
+            assert seen[counts].isnan().all()
+        elif first != spot:
+            assert seen.isnan().all()
+        else:
+            assert (~seen.isfinite()).any(-1).all()

@@ -303,7 +303,8 @@ __device__ __forceinline__ void merge_parts(const DecodeQ8Params &p, int lane, i
     }
 }
 
-template <int HD>
+// PROMPT: a job may hold several queries, the first of which see less than the last.
+template <int HD, bool PROMPT>
 __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(const __grid_constant__ DecodeQ8Params p)
 {
     using G = Geo<HD>;
@@ -489,6 +490,22 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
         float m = -CUDART_INF_F, l = 0.0f;       // reference maximum of row r; this lane's part of the sum
         float acc[NT][2];
         if (tail_n > 0) {
+            if constexpr (PROMPT) {
+                // 0 times a value that a row may not see would be NaN if the value is not
+                // finite: it becomes a zero behind a key of NaN, as in q8_unpack_kernel
+                uint32_t odd = 0;
+#pragma unroll
+                for (int t = 0; t < 8; t++) {
+                    if (__any_sync(0xffffffffu, not_finite(tv[t].x) || not_finite(tv[t].y))) {
+                        odd |= 1u << t;
+                        tv[t] = make_uint2(0u, 0u);
+                    }
+                }
+                if (odd >> r & 1u) {
+#pragma unroll
+                    for (int i = 0; i < 2 * PANELS; i++) tk[i / 2][i % 2] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                }
+            }
             const float unit = f_q * 32639.0f, over = f_q != 0.0f ? p.sl2 / unit : 0.0f;   // sl2 top, 1 / top
             float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -564,7 +581,8 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
             float s[8];
             float mb = -CUDART_INF_F;
             const int turn = (blk - run.first - warp) / kWarps & 31;
-            const float sk = __shfl_sync(0xffffffffu, k_scale, turn), sv = __shfl_sync(0xffffffffu, v_scale, turn);
+            const float sk = __shfl_sync(0xffffffffu, k_scale, turn);
+            float sv = __shfl_sync(0xffffffffu, v_scale, turn);
             if (turn == 15) load_scales(blk + 17 * kWarps, k_next, v_next);
             if (turn == 31) {
                 k_scale = k_next;
@@ -591,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
                 for (int i = 0; i < 8; i++) {
                     if (32 * blk + 8 * c + i > lim) s[i] = -CUDART_INF_F;
                 }
+                if (PROMPT && 32 * blk > lim) sv = 0.0f;     // (and the block may be of NaN)
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) mb = fmaxf(mb, s[i]);
@@ -888,8 +907,8 @@ __global__ void q8_zero_rows_kernel(const __grid_constant__ DecodeQ8Params p, in
     }
 }
 
-const KernelReg reg128("decode_q8_128", (const void *)decode_q8_kernel<128>);
-const KernelReg reg64("decode_q8_64", (const void *)decode_q8_kernel<64>);
+const KernelReg reg128("decode_q8_128", (const void *)decode_q8_kernel<128, false>);
+const KernelReg reg64("decode_q8_64", (const void *)decode_q8_kernel<64, false>);
 
 }  // namespace
 
@@ -901,13 +920,14 @@ static cudaError_t configure(int dev, int hd, int (**resident)[2])
     static int clusters[64][2][2];
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!done[dev]) {
-        const void *kernel[2] = {(const void *)decode_q8_kernel<128>, (const void *)decode_q8_kernel<64>};
-        const int smem[2] = {Geo<128>::SMEM, Geo<64>::SMEM};
-        for (int i = 0; i < 2; i++) {
+        const void *kernel[4] = {(const void *)decode_q8_kernel<128, false>, (const void *)decode_q8_kernel<64, false>,
+                                 (const void *)decode_q8_kernel<128, true>, (const void *)decode_q8_kernel<64, true>};
+        const int smem[4] = {Geo<128>::SMEM, Geo<64>::SMEM, Geo<128>::SMEM, Geo<64>::SMEM};
+        for (int i = 0; i < 4; i++) {
             cudaError_t e = cudaFuncSetAttribute(kernel[i], cudaFuncAttributeMaxDynamicSharedMemorySize, smem[i]);
             if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
-            for (int c = 0; c < 2; c++) {
+            for (int c = 0; c < 2 && i < 2; c++) {           // (the others take as much of an SM)
                 cudaLaunchConfig_t cfg = {};
                 cudaLaunchAttribute attr[1];
                 cfg.gridDim = dim3(c ? 16 : 8);
@@ -936,8 +956,11 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
     cudaGetDevice(&dev);
     const cudaError_t ce = configure(dev, hd, nullptr);
     if (ce != cudaSuccess) return ce;
-    bool empty = false;
-    for (int b = 0; b < p.nseq; b++) empty = empty || p.seq[b].live == 0;
+    bool empty = false, prompt = false;
+    for (int b = 0; b < p.nseq; b++) {
+        empty = empty || p.seq[b].live == 0;
+        prompt = prompt || (p.causal && p.seq[b].n > 1);
+    }
     if (empty) {
         q8_zero_rows_kernel<<<p.nseq, 256, 0, st>>>(p, p.heads * hd);
         const cudaError_t e = cudaGetLastError();
@@ -945,8 +968,9 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
     }
     if (grid == 0) return cudaSuccess;
     const dim3 blocks((unsigned)grid);
-    const cudaError_t e = hd == 128 ? launch_dependent(st, blocks, kThreads, Geo<128>::SMEM, p.cluster, decode_q8_kernel<128>, p)
-                                    : launch_dependent(st, blocks, kThreads, Geo<64>::SMEM, p.cluster, decode_q8_kernel<64>, p);
+    const auto kernel = hd == 128 ? (prompt ? decode_q8_kernel<128, true> : decode_q8_kernel<128, false>)
+                                  : (prompt ? decode_q8_kernel<64, true> : decode_q8_kernel<64, false>);
+    const cudaError_t e = launch_dependent(st, blocks, kThreads, hd == 128 ? Geo<128>::SMEM : Geo<64>::SMEM, p.cluster, kernel, p);
     if (e != cudaSuccess || !p.stats) return e;
     int most = 0;
     for (int b = 0; b < p.nseq; b++) most = std::max(most, p.seq[b].full);

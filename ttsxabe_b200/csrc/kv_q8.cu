@@ -362,7 +362,10 @@ __global__ void __launch_bounds__(kThreads) q8_read_kernel(const __grid_constant
 // laid over. blockIdx = (kUnpack cache blocks, KV head); a thread turns four times
 // eight codes of either into 16 bytes (so that the lanes of a store write whole
 // sectors), all eight loads in flight. Past the live tokens, up to the
-// capacity (the next multiple of eight), lie zeros. Bound by memory: 16896 tokens
+// capacity (the next multiple of eight), lie zeros. A value that is not finite would
+// make NaN of every row of a tile, those that may not see its token among them (0
+// times it): it becomes a zero behind a key of NaN, which does that to the rows that
+// see it and to no others. Bound by memory: 16896 tokens
 // of 8 heads x 128, 104 MB, in 16 us (23 with stores of half sectors).
 template <int HD>
 __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_constant__ Q8UnpackParams p)
@@ -396,6 +399,10 @@ __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_consta
         const int i = tid + u * kThreads, blk = blk0 + i / PER, e = i % PER;
         if (blk >= full) continue;
         const int panel = e / (kQ8Block * 8), t = e / 8 % kQ8Block, d = panel * 64 + e % 8 * 8;
+        if (vsc[u] != vsc[u]) {
+            ksc[u] = vsc[u];
+            vsc[u] = 0.0f;
+        }
         const uint2 k0 = dequant4(kc[u].x, ksc[u]), k1 = dequant4(kc[u].y, ksc[u]);
         *(uint4 *)(ko + (long long)(32 * blk + t) * HD + d) = make_uint4(k0.x, k0.y, k1.x, k1.y);
         const uint2 v0 = dequant4(vc[u].x, vsc[u]), v1 = dequant4(vc[u].y, vsc[u]);
@@ -410,7 +417,15 @@ __global__ void __launch_bounds__(kThreads) q8_unpack_kernel(const __grid_consta
         const int upto = sq.cap16 - 32 * full;
         for (int i = tid; i < PER; i += kThreads) {
             const int t = i / (HD / 8), d = i % (HD / 8);
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u), k = t < tail ? kt[i] : zero, v = t < tail ? vt[i] : zero;
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            uint4 k = t < tail ? kt[i] : zero, v = t < tail ? vt[i] : zero;
+            // (every lane is here; a row's are LANES neighbours)
+            constexpr uint32_t LANES = HD / 8;
+            const uint32_t odd = __ballot_sync(0xffffffffu, not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w));
+            if (odd >> (tid % 32 / LANES * LANES) & ((1u << LANES) - 1u)) {
+                k = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                v = zero;
+            }
             if (t < upto) ((uint4 *)(ko + (long long)32 * full * HD))[i] = k;
             rows[t][4 * d] = v.x;
             rows[t][4 * d + 1] = v.y;

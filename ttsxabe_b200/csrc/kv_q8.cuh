@@ -78,6 +78,12 @@ inline cudaError_t launch_dependent(cudaStream_t st, dim3 grid, int threads, siz
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Whether either f16 of a word is an infinity or NaN.
+__device__ __forceinline__ bool not_finite(uint32_t w)
+{
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+}
+
 // ---- kv_q8.cu ---------------------------------------------------------------
 
 struct Q8AppendSeq {
