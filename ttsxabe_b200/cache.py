@@ -115,6 +115,11 @@ class KvCacheQ8:
         self.newest = min(self.newest, 32 * keep_recent + self.len % 32)
         self.len = evicted_len(self.len, keep)
 
+    def can_truncate(self, length: int) -> bool:
+        """Whether the conversation can be cut to `length` positions: not where blocks
+        have been evicted among what would stay or go."""
+        return length == 0 or self.pos - length <= self.newest
+
     def truncate(self, length: int) -> None:
         """Forgets every position of the conversation from `length` on."""
         gone = self.pos - length
@@ -123,7 +128,7 @@ class KvCacheQ8:
         if length == 0:
             self.clear()
             return
-        if gone > self.newest:
+        if not self.can_truncate(length):
             raise InvalidArgument(f"cutting a conversation of {self.pos} positions to {length}: "
                                   f"blocks before the last {self.newest} have been evicted")
         self.gpu.cache_rewind_q8([self.data], [self.cap], [self.len], [self.len - gone],
@@ -153,7 +158,7 @@ class Prefix:
     the tokens from the first that differs are prefilled."""
 
     def __init__(self, caches) -> None:
-        self.caches = list(caches)          # one KvCache a layer
+        self.caches = list(caches)          # one KvCache or KvCacheQ8 a layer
         self.held: list[int] = []
 
     def __len__(self) -> int:
@@ -169,13 +174,23 @@ class Prefix:
 
     def keep(self, ids) -> int:
         """Cuts the caches back to what they share with the prompt `ids`
-        (generate.rs:139-141) and returns that length: the prompt is prefilled
-        from there, with `past` = the returned value."""
+        (generate.rs:139-141) and returns that length: the prompt is run from
+        there on, at the rotary positions from there on, behind what each cache
+        holds (`past`: the returned value, but for 8-bit caches that have evicted
+        blocks). Where the cut would fall among evicted blocks nothing is kept."""
         reused = shared_prefix(self.held, ids)
+        if any(isinstance(c, KvCacheQ8) and not c.can_truncate(reused) for c in self.caches):
+            reused = 0
         for c in self.caches:
             c.truncate(reused)
         del self.held[reused:]
         return reused
+
+    @property
+    def past(self) -> list[int]:
+        """How many tokens each layer's cache holds: what a call that appends to it or
+        attends over it is given as `past`."""
+        return [c.len for c in self.caches]
 
     def extend(self, ids) -> None:
         """Records tokens the caches now hold (after a prefill or a decoded step)."""
