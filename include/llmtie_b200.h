@@ -415,6 +415,14 @@ llmtie_status llmtie_decode_batched_push(llmtie_gpu *g, const float *q, size_t q
                                          const llmtie_exchange *xch);
 llmtie_status llmtie_lse_merge_wait(llmtie_gpu *g, const llmtie_exchange *xch, size_t rows,
                                     size_t head_dim, float *out, size_t out_len);
+/* Into pieces of how many 128-key tiles a prefill launch cuts its row blocks (0:
+ * none is cut; host only, no device needed; no counterpart in the reference):
+ * tiles[0..n) are the key tiles of its blocks of 128 query rows, over all
+ * sequences, of which each pair of a group's heads (`columns` of them) takes
+ * every one. It depends on nothing else. Groups of an odd number of heads, which
+ * pair row blocks instead, are not cut. */
+llmtie_status llmtie_prefill_cut(const int32_t *tiles, size_t n, int32_t columns, int32_t sm_count,
+                                 int32_t *cut);
 /* How a batched decode launch over contexts tk[0..batch) would be cut over
  * the grid (host only, no device needed; no counterpart in the reference):
  * grid_out = blocks launched on a device of sm_count SMs, ustart[c] = the

@@ -28,5 +28,6 @@ from .gpu import (  # noqa: F401
     decode_plan_q8,
     evicted_len,
     kv_q8_bytes,
+    prefill_cut,
 )
 from .cache import KvCache, KvCacheQ8, Prefix, shared_prefix, want_capacity  # noqa: F401

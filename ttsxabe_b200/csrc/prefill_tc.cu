@@ -1247,6 +1247,96 @@ cudaError_t launch_with(const cudaLaunchConfig_t &cfg, int hd, const ParamsMost 
 }
 const KernelReg reg_tcm("flash_attn_h_merge", (const void *)prefill_merge_kernel<128>);
 
+// Whether to cut long row blocks into pieces of their key range, and into pieces of
+// how many tiles (0: no cut). `lens` are the row blocks' key tiles, each taken
+// `columns` times. A causal launch is a set of blocks of very unequal length (1 to
+// tq/128 key tiles); when there are too few of them for the SMs - a short sequence, or
+// one KV head's share of a long one - the longest block is the launch; and where there
+// are so few to an SM that the last round leaves many idle (11 sequences of 172 key
+// tiles, 16 blocks each: two rounds for 1.2 rounds' work), pieces even it out. Pieces of
+// at most `cut` tiles write partial results that a second kernel merges. A piece is a
+// block with a block's fixed costs (its query tiles staged, first scores, epilogue: some
+// four tile steps), so the cut is chosen by playing the launch through: blocks go to the
+// SMs in grid order, longest first, each to the SM that is free first.
+int prefill_cut(std::vector<int> lens, int columns, int sms)
+{
+    long long work = 0;
+    std::sort(lens.begin(), lens.end(), std::greater<int>());
+    const int longest = lens.empty() ? 0 : lens[0];
+    for (int n : lens) work += n;
+    const double share = (double)work * columns / sms;
+    const long long blocks = (long long)lens.size() * columns;
+    const bool few = longest > 1.25 * share, uneven = !few && longest >= 16 && blocks <= 3ll * sms;
+    if (longest < 8 || !(few || uneven)) return 0;
+    constexpr int kMostPieces = 255;     // (of a row block: what the order has room for)
+    constexpr double kBlockCost = 4.0;   // an item's fixed costs, in tile steps
+    constexpr double kMergeCost = 5.0;   // the merge kernel, in tile steps
+    auto pieces_of = [](int n, int c) { return c > 0 && n > c ? (n + c - 1) / c : 1; };
+    auto makespan = [&](int c) {
+        std::vector<int> items;
+        for (int n : lens) {
+            const int pieces = pieces_of(n, c);
+            for (int k = 0; k < pieces; k++) items.push_back(((k + 1) * n) / pieces - (k * n) / pieces);
+        }
+        if (items.size() > LLMTIE_TC_MAX_ORDER) return 1e30;
+        std::sort(items.begin(), items.end(), std::greater<int>());
+        std::vector<double> free_at(sms, 0.0);   // a heap of the SMs' finishing times
+        auto later = std::greater<double>();
+        for (int len : items) {
+            for (int x = 0; x < columns; x++) {
+                std::pop_heap(free_at.begin(), free_at.end(), later);
+                free_at.back() += len + kBlockCost;
+                std::push_heap(free_at.begin(), free_at.end(), later);
+            }
+        }
+        return *std::max_element(free_at.begin(), free_at.end()) + (c > 0 ? kMergeCost : 0.0);
+    };
+    // No cut into pieces of c tiles takes less than this; it grows as c shrinks.
+    auto at_least = [&](int c) {
+        long long items = 0;
+        for (int n : lens) items += pieces_of(n, c);
+        return share + kBlockCost * (double)(items * columns) / sms + kMergeCost;
+    };
+    // The search takes 0.05 to 0.2 ms of host time (512 rows on 131072 keys; 2.4 without
+    // at_least and by steps of two), a millisecond for 75 row blocks of up to 3300 tiles,
+    // and a caller repeats the same shapes: the last answers are kept, by all that they
+    // depend on.
+    struct Memo { std::vector<int> lens; int columns, sms, cut; };
+    static std::mutex memo_lock;
+    static std::vector<Memo> memo;
+    {
+        std::lock_guard<std::mutex> hold(memo_lock);
+        for (const Memo &m : memo) {
+            if (m.columns == columns && m.sms == sms && m.lens == lens) return m.cut;
+        }
+    }
+    int cut = 0;
+    double best = makespan(0);
+    if (uneven && best > 1.15 * (share + kBlockCost * (double)blocks / sms)) {
+        for (int k : {2, 3, 4, 6}) {
+            const int c = (longest + k - 1) / k;
+            const double t = c >= 6 ? makespan(c) : best;
+            if (t < 0.95 * best && (cut == 0 || t < best)) {
+                best = t;
+                cut = c;
+            }
+        }
+    }
+    // (in steps of a sixteenth where pieces are long)
+    for (int c = (longest + 1) / 2; few && c >= 6 && (longest + c - 1) / c <= kMostPieces; c -= std::max(c > 24 ? 2 : 1, c / 16)) {
+        if (at_least(c) >= 0.95 * best) break;
+        const double t = makespan(c);
+        if (t < 0.95 * best && (cut == 0 || t < best)) {
+            best = t;
+            cut = c;
+        }
+    }
+    std::lock_guard<std::mutex> hold(memo_lock);
+    if (memo.size() >= 64) memo.erase(memo.begin());
+    memo.push_back({std::move(lens), columns, sms, cut});
+    return cut;
+}
+
 }  // namespace
 
 bool llmtie_encode_tiled_f16(CUtensorMap *map, int rank, const void *base, const uint64_t *dims,
@@ -1283,6 +1373,20 @@ bool prefill_tc_eligible(const PrefillParams &p, int hd)
         if (((uintptr_t)p.seq[b].k & 15u) != 0 || ((uintptr_t)p.seq[b].v & 15u) != 0) return false;
     }
     return encode_fn() != nullptr;
+}
+
+extern "C" llmtie_status llmtie_prefill_cut(const int32_t *tiles, size_t n, int32_t columns, int32_t sm_count, int32_t *cut)
+try {
+    if ((n > 0 && !tiles) || !cut || columns <= 0 || sm_count <= 0 || n > 1u << 20) {
+        return llmtie_fail(LLMTIE_ERR_INVALID, "a malformed cut request");
+    }
+    for (size_t i = 0; i < n; i++) {
+        if (tiles[i] <= 0 || tiles[i] > 1 << 22) return llmtie_fail(LLMTIE_ERR_INVALID, "a row block of %d key tiles", tiles[i]);
+    }
+    *cut = prefill_cut(std::vector<int>(tiles, tiles + n), columns, sm_count);
+    return LLMTIE_OK;
+} catch (const std::bad_alloc &) {
+    return llmtie_fail(LLMTIE_ERR_DRIVER, "no host memory for the tables of the call");
 }
 
 cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, const WaitCtl &w)
@@ -1356,101 +1460,18 @@ cudaError_t launch_prefill_tc(cudaStream_t st, const PrefillParams &p, int hd, c
         const int keys = p.causal ? s.past + std::min(s.tq, top * BM) : s.tk;
         return (keys + BN - 1) / BN;
     };
-    // Whether to cut long row blocks into pieces of their key range. A causal
-    // launch is a set of blocks of very unequal length (1 to tq/128 key
-    // tiles); when there are too few of them for the SMs - a short sequence,
-    // or one KV head's share of a long one - the longest block is the launch.
-    // Pieces of at most `cut` tiles write partial results that a second
-    // kernel merges. A piece is a block with a block's fixed costs (its
-    // query tiles staged, first scores, epilogue: some five tile steps), so
-    // the cut is chosen by playing the launch through: blocks go to the SMs
-    // in grid order, longest first, each to the SM that is free first.
     int cut = 0;
     {
         static const bool never = getenv("LLMTIE_B200_NO_SPLIT") != nullptr;
         std::vector<int> lens;
-        long long work = 0;
-        int longest = 0;
-        for (int b = 0; b < p.nseq; b++) {
+        for (int b = 0; b < p.nseq && !never && !tp.pair_rows; b++) {
             for (int y = 0;; y++) {
                 const int n = tiles_of_slot(b, y);
                 if (n == 0) break;
                 lens.push_back(n);
-                work += n;
-                longest = std::max(longest, n);
             }
         }
-        const int sms = std::max(1, w.sm_count);
-        const double share = (double)work * grid.x / sms;
-        // Too few blocks; or so few to an SM that the last round leaves many idle (11
-        // sequences of 172 key tiles, 16 blocks each: two rounds for 1.2 rounds' work).
-        const long long blocks = (long long)lens.size() * grid.x;
-        const bool few = longest > 1.25 * share, uneven = !few && longest >= 16 && blocks <= 3ll * sms;
-        if (!never && !tp.pair_rows && longest >= 8 && (few || uneven)) {
-            constexpr int kMostPieces = 255;     // (of a row block: what the order has room for)
-            constexpr double kBlockCost = 4.0;   // an item's fixed costs, in tile steps
-            constexpr double kMergeCost = 5.0;   // the merge kernel, in tile steps
-            auto makespan = [&](int c) {
-                std::vector<int> items;
-                for (int n : lens) {
-                    const int pieces = (c > 0 && n > c) ? (n + c - 1) / c : 1;
-                    for (int k = 0; k < pieces; k++) {
-                        items.push_back(((k + 1) * n) / pieces - (k * n) / pieces);
-                    }
-                }
-                if (items.size() > LLMTIE_TC_MAX_ORDER) return 1e30;
-                std::sort(items.begin(), items.end(), std::greater<int>());
-                std::vector<double> free_at(sms, 0.0);   // a heap of the SMs' finishing times
-                auto later = std::greater<double>();
-                for (int len : items) {
-                    for (unsigned x = 0; x < grid.x; x++) {
-                        std::pop_heap(free_at.begin(), free_at.end(), later);
-                        free_at.back() += len + kBlockCost;
-                        std::push_heap(free_at.begin(), free_at.end(), later);
-                    }
-                }
-                return *std::max_element(free_at.begin(), free_at.end()) + (c > 0 ? kMergeCost : 0.0);
-            };
-            // The search costs a fraction of a millisecond of host time, and a
-            // caller repeats the same shapes: the last answers are kept.
-            struct Memo { long long work; int longest, gx, n, sms, cut; };
-            static std::mutex memo_lock;
-            static std::vector<Memo> memo;
-            bool known = false;
-            {
-                std::lock_guard<std::mutex> hold(memo_lock);
-                for (const Memo &m : memo) {
-                    if (m.work == work && m.longest == longest && m.gx == (int)grid.x &&
-                        m.n == (int)lens.size() && m.sms == sms) {
-                        cut = m.cut;
-                        known = true;
-                    }
-                }
-            }
-            if (!known) {
-                double best = makespan(0);
-                if (uneven && best > 1.15 * (share + kBlockCost * (double)blocks / sms)) {
-                    for (int k : {2, 3, 4, 6}) {
-                        const int c = (longest + k - 1) / k;
-                        const double t = c >= 6 ? makespan(c) : best;
-                        if (t < 0.95 * best && (cut == 0 || t < best)) {
-                            best = t;
-                            cut = c;
-                        }
-                    }
-                }
-                for (int c = (longest + 1) / 2; few && c >= 6 && (longest + c - 1) / c <= kMostPieces; c -= (c > 24 ? 2 : 1)) {
-                    const double t = makespan(c);
-                    if (t < 0.95 * best && (cut == 0 || t < best)) {
-                        best = t;
-                        cut = c;
-                    }
-                }
-                std::lock_guard<std::mutex> hold(memo_lock);
-                if (memo.size() >= 64) memo.erase(memo.begin());
-                memo.push_back({work, longest, (int)grid.x, (int)lens.size(), sms, cut});
-            }
-        }
+        cut = prefill_cut(std::move(lens), (int)grid.x, std::max(1, w.sm_count));
     }
     static const bool tell = getenv("LLMTIE_B200_TELL_CUT") != nullptr;
     if (tell) fprintf(stderr, "prefill: row blocks cut at %d tiles\n", cut);

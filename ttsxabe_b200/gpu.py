@@ -158,6 +158,16 @@ def decode_cut(tk, kv_heads: int, head_dim: int, sm_count: int = 148) -> list[in
     return list(table[:grid.value + 1])
 
 
+def prefill_cut(tiles, columns: int, sm_count: int = 148) -> int:
+    """Into pieces of how many 128-key tiles a prefill launch whose blocks of 128 rows
+    have `tiles` of them, for each of `columns` pairs of heads, cuts its row blocks
+    (host only); 0 for none."""
+    cut = C.c_int32(0)
+    _check(_lib.load().llmtie_prefill_cut((C.c_int32 * len(tiles))(*tiles), len(tiles), columns, sm_count,
+                                          C.byref(cut)))
+    return cut.value
+
+
 def decode_plan(tk, kv_heads: int, rows: int, head_dim: int, sm_count: int = 148,
                 resident=None):
     """The whole choice a decode launch makes (host only): returns
