@@ -558,9 +558,9 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
  *   value tail   f16  [kv_heads][32][head_dim]
  * How many tokens it holds is the caller's to know (its `live` or `past`).
  * head_dim is 64 or 128. The entries take HOST tables with a cache, a capacity
- * and lengths for each sequence, up to 65536 sequences a call; caches that one
- * call writes must not share memory, nor may an output share any with the
- * query (but for rows that are rotated in place). A capacity that is not a multiple of
+ * and lengths for each sequence, up to 65536 sequences a call; a cache that a
+ * call writes must not share memory with another of that call, nor may an
+ * output share any with the query (but for rows that are rotated in place). A capacity that is not a multiple of
  * 32 is refused with LLMTIE_ERR_RAGGED_BLOCK.
  *
  * Calls may be captured into a CUDA graph as others may (see llmtie_close). */
@@ -669,7 +669,8 @@ llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len,
  * others those of the largest weight, the lower block where two weigh the same
  * (a weight that is negative or NaN counts as zero). They keep their order,
  * codes, scales and weights, and go to dst[b], which may be src[b] (with its
- * capacity) or a cache of its own; the tail follows them. Afterwards the cache
+ * capacity) or a cache of its own; the tail follows them. Several sequences may
+ * have the same source, which forks it. Afterwards the cache
  * holds min(live / 32, keep) * 32 + live % 32 tokens; the keys keep the
  * rotation of the positions they were appended at. `index` (or NULL) gets the
  * number in src of each block kept, int32 [batch][kv_heads][K], K the most that

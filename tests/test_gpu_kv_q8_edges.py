@@ -110,3 +110,50 @@ def test_rows_before_a_value_that_is_not_finite(gpu, heads, kv, hd, past, n, whi
             assert seen.isnan().all()
         else:
             assert (~seen.isfinite()).any(-1).all()
+
+
+# ---- caches that are forked --------------------------------------------------------------
+
+@pytest.mark.parametrize("kv,hd", [(8, 128), (3, 64)])
+def test_a_cache_evicted_into_several_others(gpu, kv, hd):
+    """One call that forks a cache gives what a call for each gives; so does growing it
+    behind them. The source is left as it was."""
+    live, cap = 900, 928
+    (src,), _ = caches_of(gpu, kv, hd, [live], seed=hd, cap=cap)
+    q = torch.randn(kv * hd, device=gpu.device)
+    torch.cuda.synchronize()
+    gpu.decode_batched_q8(q, [src], [live], [cap], kv, kv, hd, hd ** -0.5, DecodeScratch(), weigh=True)
+    gpu.synchronize()
+    before = src.clone()
+    caps, keep = [320, 608, 928, 64], [9, 18, 28, 0]
+    alone, forked = ([gpu.kv_alloc_q8(kv, hd, c) for c in caps] for _ in range(2))
+    for d, c, k in zip(alone, caps, keep):
+        gpu.cache_evict_q8([src], [cap], [d], [c], [live], [k], 0, 0, kv, hd)
+    gpu.cache_evict_q8([src] * 4, [cap] * 4, forked, caps, [live] * 4, keep, 0, 0, kv, hd)
+    gpu.synchronize()
+    assert torch.equal(src, before)
+    for a, b in zip(alone, forked):
+        assert torch.equal(a, b)
+
+
+def test_evictions_that_would_race_are_refused(gpu):
+    from ttsxabe_b200 import InvalidArgument
+
+    kv, hd, cap, live = 2, 64, 128, 100
+    (a, b, c), _ = caches_of(gpu, kv, hd, [live] * 3, seed=1, cap=cap)
+    both = gpu.kv_alloc_q8(kv, hd, 2 * cap)
+    size = a.numel()
+    before = gpu.launch_count()
+    for src, dst in [((a, a), (b, b)),          # one destination twice
+                     ((a, b), (b, c)),          # a destination that is another's source
+                     ((a, a), (a, c)),          # cut in place and read
+                     ((a, a), (c, a)),
+                     ((both[:size],), (both[16:size + 16],)),
+                     ((both[256:size + 256],), (both[:size],))]:
+        n = len(src)
+        with pytest.raises(InvalidArgument, match="share memory"):
+            gpu.cache_evict_q8(list(src), [cap] * n, list(dst), [cap] * n, [live] * n, [2] * n, 0, 0, kv, hd)
+    assert gpu.launch_count() == before
+    # in place beside a copy of another
+    gpu.cache_evict_q8([a, b], [cap] * 2, [a, c], [cap] * 2, [live] * 2, [2] * 2, 0, 0, kv, hd)
+    gpu.synchronize()

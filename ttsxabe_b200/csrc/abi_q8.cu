@@ -47,15 +47,21 @@ llmtie_status check_cache(const void *base, int32_t cap, long long live)
     return LLMTIE_OK;
 }
 
-// Caches that one call writes must not share memory: their writes would race.
-llmtie_status check_apart(std::vector<std::pair<uintptr_t, size_t>> &spans)
+// Caches that one call writes must not share memory, nor one that it writes with one
+// that it reads: they would race. (Those that it only reads may be the same.)
+typedef std::vector<std::pair<uintptr_t, size_t>> Spans;
+llmtie_status check_apart(Spans &writes, const Spans &reads = Spans())
 {
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); i++) {
-        if (spans[i].first < spans[i - 1].first + spans[i - 1].second) {
-            return llmtie_fail(LLMTIE_ERR_INVALID, "two caches of one call share memory");
-        }
+    std::sort(writes.begin(), writes.end());
+    bool meet = false;
+    for (size_t i = 1; i < writes.size(); i++) meet = meet || writes[i].first < writes[i - 1].first + writes[i - 1].second;
+    for (const auto &r : reads) {
+        // the first that starts at or behind it, and the one before
+        const auto w = std::lower_bound(writes.begin(), writes.end(), std::make_pair(r.first, (size_t)0));
+        meet = meet || (w != writes.end() && w->first < r.first + r.second);
+        meet = meet || (w != writes.begin() && r.first < (w - 1)->first + (w - 1)->second);
     }
+    if (meet) return llmtie_fail(LLMTIE_ERR_INVALID, "two caches of one call share memory");
     return LLMTIE_OK;
 }
 
@@ -239,7 +245,7 @@ try {
             return llmtie_fail(LLMTIE_ERR_INVALID, "the rotated query overlaps the rows the call reads");
         }
     }
-    std::vector<std::pair<uintptr_t, size_t>> spans;
+    Spans spans;
     for (size_t b = 0; b < batch; b++) {
         const int n = cu_seqlens[b + 1] - cu_seqlens[b];
         if (n == 0) continue;
@@ -338,7 +344,7 @@ extern "C" llmtie_status llmtie_cache_rewind_q8(llmtie_gpu *g, void *const *cach
 try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!caches || !cap || !live || !to) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
-    std::vector<std::pair<uintptr_t, size_t>> spans;
+    Spans spans;
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(caches[b], cap[b], live[b]));
         if (to[b] < 0 || to[b] > live[b]) {
@@ -373,7 +379,7 @@ extern "C" llmtie_status llmtie_cache_evict_q8(llmtie_gpu *g, const void *const 
 try {
     TRY(check_geometry(g, batch, kv_heads, head_dim));
     if (!src || !src_cap || !dst || !dst_cap || !live || !keep) return llmtie_fail(LLMTIE_ERR_INVALID, "null sequence table");
-    std::vector<std::pair<uintptr_t, size_t>> spans;
+    Spans writes, reads;
     int most = 0;
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(src[b], src_cap[b], live[b]));
@@ -385,15 +391,15 @@ try {
         const int kept = std::min(full, keep[b]);
         most = std::max(most, kept);
         TRY(check_cache(dst[b], dst_cap[b], (long long)kept * kQ8Block + live[b] % kQ8Block));
-        spans.emplace_back((uintptr_t)src[b], cache_bytes(kv_heads, head_dim, (size_t)src_cap[b]));
+        writes.emplace_back((uintptr_t)dst[b], cache_bytes(kv_heads, head_dim, (size_t)dst_cap[b]));
         if (dst[b] != src[b]) {
-            spans.emplace_back((uintptr_t)dst[b], cache_bytes(kv_heads, head_dim, (size_t)dst_cap[b]));
+            reads.emplace_back((uintptr_t)src[b], cache_bytes(kv_heads, head_dim, (size_t)src_cap[b]));
         } else if (dst_cap[b] != src_cap[b]) {
             return llmtie_fail(LLMTIE_ERR_INVALID, "a cache shortened in place keeps its capacity of %d, not %d", src_cap[b],
                                dst_cap[b]);
         }
     }
-    TRY(check_apart(spans));
+    TRY(check_apart(writes, reads));
     if (index && index_len < batch * kv_heads * (size_t)most) return overrun(batch * kv_heads * (size_t)most, index_len);
     for (size_t b0 = 0; b0 < batch; b0 += LLMTIE_Q8_MAX_SEQ) {
         Q8EvictParams p;
@@ -466,7 +472,7 @@ try {
     if (((uintptr_t)q & 15u) != 0) return llmtie_misaligned("the query", q, 16);
     if (((uintptr_t)out & 15u) != 0) return llmtie_misaligned("the output", out, 16);
     if (meet(q, batch * n * 4, out, batch * n * (out_f16 ? 2 : 4))) return llmtie_fail(LLMTIE_ERR_INVALID, "the output overlaps the query");
-    std::vector<std::pair<uintptr_t, size_t>> spans;
+    Spans spans;
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(caches[b], cap[b], live[b]));
         if (weigh) spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
