@@ -157,3 +157,21 @@ def test_evictions_that_would_race_are_refused(gpu):
     # in place beside a copy of another
     gpu.cache_evict_q8([a, b], [cap] * 2, [a, c], [cap] * 2, [live] * 2, [2] * 2, 0, 0, kv, hd)
     gpu.synchronize()
+
+
+# ---- what a call launches ------------------------------------------------------------------
+
+def test_decode_counts_every_kernel(gpu):
+    """One, another for the weights of complete blocks, another for the zeros of
+    sequences without a token."""
+    kv, hd = 2, 64
+    ts, caps = caches_of(gpu, kv, hd, [70, 5], seed=1)
+    q = torch.randn(2, kv * hd, device=gpu.device)
+    torch.cuda.synchronize()
+    for lives, weigh, want in [([70, 5], False, 1), ([70, 5], True, 2), ([0, 5], False, 2), ([0, 5], True, 2), ([70, 0], True, 3), ([0, 0], True, 1)]:
+        before = gpu.launch_count()
+        out = gpu.decode_batched_q8(q, ts, lives, caps, kv, kv, hd, 0.1, DecodeScratch(), weigh=weigh).view(2, -1)
+        gpu.synchronize()
+        assert gpu.launch_count() - before == want, (lives, weigh)
+        for b in range(2):
+            assert (out[b] == 0).all() == (lives[b] == 0)

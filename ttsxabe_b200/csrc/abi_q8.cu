@@ -122,9 +122,11 @@ llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, cons
         memset(&p, 0, sizeof(p));
         p.nseq = (int)std::min<size_t>(LLMTIE_Q8_MAX_SEQ, jobs.size() - b0);
         long long units = 0, blocks = 0;
+        bool empty = false;
         for (int b = 0; b < p.nseq; b++) {
             p.seq[b] = jobs[b0 + b];
             const int t = p.seq[b].live;
+            empty = empty || t == 0;
             p.unit0[b] = (int)units;
             p.stat0[b] = blocks;
             units += (long long)((t + kQ8Block - 1) / kQ8Block) * (long long)kv_heads;
@@ -171,7 +173,8 @@ llmtie_status run_jobs(llmtie_gpu *g, const std::vector<DecodeQ8Seq> &jobs, cons
         LaunchScope ls(g, head_dim == 128 ? "decode_q8_128" : "decode_q8_64");
         err = launch_decode_q8(g->stream, p, (int)head_dim, grid);
         if (err != cudaSuccess) return llmtie_driver_fail("decode_q8", err);
-        if (p.stats) g->launches++;   // two kernels in that launcher then
+        if (p.stats) g->launches++;            // two kernels in that launcher then
+        if (empty && grid > 0) g->launches++;  // and another that writes the zeros
         TRY(ls.done());
     }
     return LLMTIE_OK;
