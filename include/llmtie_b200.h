@@ -560,7 +560,8 @@ llmtie_status llmtie_prefill_varlen(llmtie_gpu *g, const float *q, size_t q_len,
  * head_dim is 64 or 128. The entries take HOST tables with a cache, a capacity
  * and lengths for each sequence, up to 65536 sequences a call; a cache that a
  * call writes must not share memory with another of that call, nor may an
- * output share any with the query (but for rows that are rotated in place). A capacity that is not a multiple of
+ * output share any with a cache or with the query (but for rows that are
+ * rotated in place). A capacity that is not a multiple of
  * 32 is refused with LLMTIE_ERR_RAGGED_BLOCK.
  *
  * Calls may be captured into a CUDA graph as others may (see llmtie_close). */

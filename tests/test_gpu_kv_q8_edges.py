@@ -175,3 +175,53 @@ def test_decode_counts_every_kernel(gpu):
         assert gpu.launch_count() - before == want, (lives, weigh)
         for b in range(2):
             assert (out[b] == 0).all() == (lives[b] == 0)
+
+
+# ---- buffers in the wrong place -----------------------------------------------------------
+
+def test_buffers_in_a_caches_memory_are_refused(gpu):
+    from ttsxabe_b200 import InvalidArgument
+
+    heads, kv, hd, cap, live = 4, 2, 64, 64, 40
+    (t, u), _ = caches_of(gpu, kv, hd, [live] * 2, seed=1, cap=cap)
+    f32, f16, i32 = (t.view(x) for x in (torch.float32, torch.float16, torch.int32))
+    q, k = gpu.zeros(heads * hd), gpu.zeros(kv * hd)
+    f = gpu.rope_inv_freq(10000.0, hd)
+    rows = torch.empty(live * kv * hd, dtype=torch.float16, device=gpu.device)
+    torch.cuda.synchronize()
+    before, held = gpu.launch_count(), t.clone()
+    a, w = [t], [cap]
+
+    def append(q=q, k=k, v=k, f=f, q_out=None):
+        gpu.rope_append_q8(q, k, v, [0, 1], a, w, [live], [live], f, heads, kv, hd, q_out=q_out)
+
+    wide, narrow = heads * hd, kv * hd
+    for call in [lambda: append(q=f32[:wide]), lambda: append(q_out=f32[16:wide + 16]), lambda: append(k=f32[:narrow]),
+                 lambda: append(v=f32[-narrow:]), lambda: append(f=f32[:hd // 2]), lambda: append(k=f32[4:narrow + 4]),
+                 lambda: gpu.decode_batched_q8(q, a, [live], w, heads, kv, hd, 0.1, DecodeScratch(), out=f32[:wide]),
+                 lambda: gpu.decode_batched_q8(q, a, [live], w, heads, kv, hd, 0.1, DecodeScratch(), out=f16[-wide:]),
+                 lambda: gpu.decode_batched_q8(f32[:wide], a, [live], w, heads, kv, hd, 0.1, DecodeScratch(), weigh=True),
+                 lambda: gpu.flash_attn_q8(q, [0, 1], a, w, [live - 1], heads, kv, hd, 0.1, True, out=f32[:wide]),
+                 lambda: gpu.cache_read_q8(a, w, [live], [0], [0, live], kv, hd, k_out=f16[:rows.numel()], v_out=rows),
+                 lambda: gpu.cache_read_q8(a, w, [live], [0], [0, live], kv, hd, k_out=rows, v_out=f16[:rows.numel()]),
+                 lambda: gpu.cache_evict_q8(a, w, [u], w, [live], [1], 0, 0, kv, hd, index=i32[:8]),
+                 lambda: gpu.cache_evict_q8([u], w, a, w, [live], [1], 0, 0, kv, hd, index=i32[:8])]:
+        with pytest.raises(InvalidArgument, match="memory of an 8-bit cache"):
+            call()
+    assert gpu.launch_count() == before
+    # a query that is only read may lie anywhere
+    gpu.decode_batched_q8(f32[:wide], a, [live], w, heads, kv, hd, 0.1, DecodeScratch())
+    gpu.synchronize()
+    assert torch.equal(t, held)
+
+
+def test_rotated_queries_over_the_frequencies_are_refused(gpu):
+    from ttsxabe_b200 import InvalidArgument
+
+    heads, kv, hd, cap = 4, 2, 64, 64
+    t = gpu.kv_alloc_q8(kv, hd, cap)
+    k, both = gpu.zeros(kv * hd), gpu.zeros(heads * hd + hd)
+    torch.cuda.synchronize()
+    with pytest.raises(InvalidArgument, match="overlaps"):
+        gpu.rope_append_q8(gpu.zeros(heads * hd), k, k, [0, 1], [t], [cap], [0], [0], both[heads * hd - 8:heads * hd + hd // 2 - 8],
+                           heads, kv, hd, q_out=both[:heads * hd])

@@ -70,6 +70,15 @@ bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
     return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
 }
 
+// A buffer that the call writes, or reads while it writes the cache, in a cache's memory.
+llmtie_status check_clear(const char *what, const void *p, size_t bytes, const void *cache, size_t cache_size)
+{
+    if (p && bytes && meet(p, bytes, cache, cache_size)) {
+        return llmtie_fail(LLMTIE_ERR_INVALID, "%s: memory of an 8-bit cache of the same call", what);
+    }
+    return LLMTIE_OK;
+}
+
 llmtie_status overrun(size_t need, size_t have)
 {
     return llmtie_fail(LLMTIE_ERR_SLICE_OVERRUN, "reading to %zu in a buffer of %zu", need, have);
@@ -244,7 +253,8 @@ try {
         if (((uintptr_t)q_out & 15u) != 0) return llmtie_misaligned("the rotated query", q_out, 16);
         // in place, or clear of everything the call reads
         const size_t kv_bytes = total * kv_heads * head_dim * 4;
-        if ((q_out != q && meet(q_out, need * 4, q, need * 4)) || meet(q_out, need * 4, k, kv_bytes) || meet(q_out, need * 4, v, kv_bytes)) {
+        if ((q_out != q && meet(q_out, need * 4, q, need * 4)) || meet(q_out, need * 4, k, kv_bytes) || meet(q_out, need * 4, v, kv_bytes) ||
+            meet(q_out, need * 4, inv_freq, head_dim / 2 * 4)) {
             return llmtie_fail(LLMTIE_ERR_INVALID, "the rotated query overlaps the rows the call reads");
         }
     }
@@ -256,7 +266,15 @@ try {
         if (pos[b] < 0 || (long long)pos[b] + n > 0x7fffffffll) {
             return llmtie_fail(LLMTIE_ERR_INVALID, "rows at position %d", pos[b]);
         }
-        spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
+        const size_t size = cache_bytes(kv_heads, head_dim, (size_t)cap[b]), kv_bytes = total * kv_heads * head_dim * 4;
+        TRY(check_clear("the key rows", k, kv_bytes, caches[b], size));
+        TRY(check_clear("the value rows", v, kv_bytes, caches[b], size));
+        if (inv_freq) TRY(check_clear("the inverse frequencies", inv_freq, head_dim / 2 * 4, caches[b], size));
+        if (turn_q) {
+            TRY(check_clear("the queries", q, total * heads * head_dim * 4, caches[b], size));
+            TRY(check_clear("the rotated queries", q_out, total * heads * head_dim * 4, caches[b], size));
+        }
+        spans.emplace_back((uintptr_t)caches[b], size);
     }
     TRY(check_apart(spans));
     for (size_t b0 = 0; b0 < batch;) {
@@ -319,6 +337,9 @@ extern "C" llmtie_status llmtie_cache_read_q8(llmtie_gpu *g, const void *const *
         if (first[b] < 0 || (long long)first[b] + n > live[b]) {
             return llmtie_fail(LLMTIE_ERR_CACHE_OVERRUN, "reading to %lld of a cache that holds %d", (long long)first[b] + n, live[b]);
         }
+        const size_t size = cache_bytes(kv_heads, head_dim, (size_t)cap[b]), bytes = total * kv_heads * head_dim * 2;
+        TRY(check_clear("the keys read", k_out, bytes, caches[b], size));
+        TRY(check_clear("the values read", v_out, bytes, caches[b], size));
     }
     for (size_t b0 = 0; b0 < batch;) {
         Q8ReadParams p;
@@ -403,7 +424,11 @@ try {
         }
     }
     TRY(check_apart(writes, reads));
-    if (index && index_len < batch * kv_heads * (size_t)most) return overrun(batch * kv_heads * (size_t)most, index_len);
+    const size_t numbers = batch * kv_heads * (size_t)most;
+    if (index && index_len < numbers) return overrun(numbers, index_len);
+    for (const Spans *spans : {&writes, &reads}) {
+        for (const auto &s : *spans) TRY(check_clear("the blocks' numbers", index, numbers * 4, (const void *)s.first, s.second));
+    }
     for (size_t b0 = 0; b0 < batch; b0 += LLMTIE_Q8_MAX_SEQ) {
         Q8EvictParams p;
         memset(&p, 0, sizeof(p));
@@ -478,7 +503,12 @@ try {
     Spans spans;
     for (size_t b = 0; b < batch; b++) {
         TRY(check_cache(caches[b], cap[b], live[b]));
-        if (weigh) spans.emplace_back((uintptr_t)caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b]));
+        const size_t size = cache_bytes(kv_heads, head_dim, (size_t)cap[b]);
+        TRY(check_clear("the output", out, batch * n * (out_f16 ? 2 : 4), caches[b], size));
+        if (weigh) {
+            TRY(check_clear("the query", q, batch * n * 4, caches[b], size));
+            spans.emplace_back((uintptr_t)caches[b], size);
+        }
     }
     TRY(check_apart(spans));
     std::vector<DecodeQ8Seq> jobs(batch);
@@ -532,6 +562,7 @@ try {
         const int rows = cu_seqlens[b + 1] - cu_seqlens[b];
         if (rows == 0) continue;
         TRY(check_cache(caches[b], cap[b], past[b] < 0 ? -1 : (long long)past[b] + rows));
+        TRY(check_clear("the output", out, total * n * (out_f16 ? 2 : 4), caches[b], cache_bytes(kv_heads, head_dim, (size_t)cap[b])));
     }
     // Sequences of few rows may go through the decode kernel, which reads their codes
     // as they lie, as a job for every eight rows of a group: where that is estimated to
