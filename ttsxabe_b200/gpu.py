@@ -644,6 +644,12 @@ class Gpu:
     # the layout). Where a list of them is given, each is checked against its
     # capacity; a table made by `ptr_table` is taken as it is.
 
+    def _here(self, *tensors) -> None:
+        """Every tensor of a call lies on the handle's device (None is passed over)."""
+        for t in tensors:
+            if t is not None and t.get_device() != self.ordinal:
+                raise InvalidArgument(f"a tensor on {t.device}, not cuda:{self.ordinal}")
+
     def _q8_table(self, caches, cap, kv_heads, head_dim) -> C.Array:
         if isinstance(caches, C.Array):
             return caches
@@ -681,6 +687,11 @@ class Gpu:
     def rope_inv_freq(self, theta, head_dim, freq_div=None) -> torch.Tensor:
         """The inverse frequencies that `rope_scaled` goes by, to be kept for
         `rope_append_q8`."""
+        self._here(freq_div)
+        if freq_div is not None and (freq_div.dtype != torch.float32 or not freq_div.is_contiguous()
+                                     or freq_div.numel() < head_dim // 2):
+            raise InvalidArgument(f"divisors want {head_dim // 2} contiguous float32, got "
+                                  f"{freq_div.numel()} of {freq_div.dtype}")
         out = self.uninit(head_dim // 2)
         _check(self._lib.llmtie_rope_inv_freq(self._h, _ptr(freq_div), head_dim, theta,
                                               out.data_ptr(), out.numel()))
@@ -701,18 +712,32 @@ class Gpu:
         f32 = torch.float32
         if (k.dtype is not f32 or v.dtype is not f32 or not k.is_contiguous()
                 or not v.is_contiguous()
-                or (inv_freq is not None and inv_freq.dtype is not f32)
+                or (inv_freq is not None and (inv_freq.dtype is not f32 or not inv_freq.is_contiguous()))
                 or (q is not None and (q.dtype is not f32 or not q.is_contiguous()))
                 or (q_out is not None and (q_out.dtype is not f32 or not q_out.is_contiguous()))):
             raise self._not_rows(q, k, v, inv_freq, q_out)
+        here = self.ordinal
+        if (k.get_device() != here or v.get_device() != here
+                or (q is not None and q.get_device() != here)
+                or (q_out is not None and q_out.get_device() != here)
+                or (inv_freq is not None and inv_freq.get_device() != here)):
+            self._here(q, k, v, inv_freq, q_out)
         if q_out is None:
             q_out = q
-        _check(self._lib.llmtie_rope_append_q8(
-            self._h, _ptr(q), 0 if q is None else q.numel(), _ptr(q_out),
-            0 if q_out is None else q_out.numel(), k.data_ptr(), k.numel(), v.data_ptr(),
-            v.numel(), self._i32_table(cu_seqlens), n, table, self._i32_table(past),
-            self._i32_table(pos), self._i32_table(cap), _ptr(inv_freq),
-            0 if inv_freq is None else inv_freq.numel(), heads, kv_heads, head_dim))
+        # (a decode step is bound by the host: tables that are made are passed straight on)
+        made = C.Array
+        status = self._lib.llmtie_rope_append_q8(
+            self._h, None if q is None else q.data_ptr(), 0 if q is None else q.numel(),
+            None if q_out is None else q_out.data_ptr(), 0 if q_out is None else q_out.numel(),
+            k.data_ptr(), k.numel(), v.data_ptr(), v.numel(),
+            cu_seqlens if isinstance(cu_seqlens, made) else self._i32_table(cu_seqlens), n, table,
+            past if isinstance(past, made) else self._i32_table(past),
+            pos if isinstance(pos, made) else self._i32_table(pos),
+            cap if isinstance(cap, made) else self._i32_table(cap),
+            None if inv_freq is None else inv_freq.data_ptr(),
+            0 if inv_freq is None else inv_freq.numel(), heads, kv_heads, head_dim)
+        if status:
+            _check(status)
 
     def cache_read_q8(self, caches, cap, live, first, cu_seqlens, kv_heads, head_dim, k_out=None,
                       v_out=None):
@@ -733,10 +758,17 @@ class Gpu:
         if k_out.dtype is not f16 or v_out.dtype is not f16 or not (k_out.is_contiguous()
                                                                      and v_out.is_contiguous()):
             raise InvalidArgument(f"reading into {k_out.dtype} and {v_out.dtype}")
-        _check(self._lib.llmtie_cache_read_q8(
-            self._h, table, self._i32_table(cap), self._i32_table(live), self._i32_table(first),
-            self._i32_table(cu_seqlens), n, kv_heads, head_dim, k_out.data_ptr(), k_out.numel(),
-            v_out.data_ptr(), v_out.numel()))
+        if k_out.get_device() != self.ordinal or v_out.get_device() != self.ordinal:
+            self._here(k_out, v_out)
+        made = C.Array
+        status = self._lib.llmtie_cache_read_q8(
+            self._h, table, cap if isinstance(cap, made) else self._i32_table(cap),
+            live if isinstance(live, made) else self._i32_table(live),
+            first if isinstance(first, made) else self._i32_table(first),
+            cu_seqlens if isinstance(cu_seqlens, made) else self._i32_table(cu_seqlens), n,
+            kv_heads, head_dim, k_out.data_ptr(), k_out.numel(), v_out.data_ptr(), v_out.numel())
+        if status:
+            _check(status)
         return k_out, v_out
 
     def cache_rewind_q8(self, caches, cap, live, to, kv_heads, head_dim) -> None:
@@ -748,9 +780,12 @@ class Gpu:
             len(table), kv_heads, head_dim))
 
     def cache_grow_q8(self, src, dst, kv_heads, head_dim, old_cap, new_cap, live) -> None:
+        self._here(src, dst)
+        if not (src.is_contiguous() and dst.is_contiguous()):
+            raise InvalidArgument(f"8-bit caches with strides {src.stride()} and {dst.stride()}")
         _check(self._lib.llmtie_cache_grow_q8(
-            self._h, src.data_ptr(), src.numel(), dst.data_ptr(), dst.numel(), kv_heads, head_dim,
-            old_cap, new_cap, live))
+            self._h, src.data_ptr(), src.numel() * src.element_size(), dst.data_ptr(),
+            dst.numel() * dst.element_size(), kv_heads, head_dim, old_cap, new_cap, live))
 
     def decode_batched_q8(self, q, caches, live, cap, heads, kv_heads, head_dim, scale,
                           scratch: DecodeScratch, out=None, weigh=False) -> torch.Tensor:
@@ -765,6 +800,8 @@ class Gpu:
             out = self.uninit(n * heads * head_dim)
         if q.dtype is not torch.float32 or not q.is_contiguous():
             raise self._not_rows(q)
+        if q.get_device() != self.ordinal or out.get_device() != self.ordinal:
+            self._here(q, out)
         _check(self._lib.llmtie_decode_batched_q8(
             self._h, q.data_ptr(), q.numel(), table, self._i32_table(live), self._i32_table(cap),
             n, heads, kv_heads, head_dim, scale, int(bool(weigh)), scratch._bind(self),
@@ -784,6 +821,7 @@ class Gpu:
             out = self.uninit(int(cu_seqlens[n]) * heads * head_dim)
         if q.dtype is not torch.float32 or not q.is_contiguous():
             raise self._not_rows(q)
+        self._here(q, out)
         _check(self._lib.llmtie_flash_attn_q8(
             self._h, q.data_ptr(), q.numel(), self._i32_table(cu_seqlens), n, table,
             self._i32_table(past), self._i32_table(cap), heads, kv_heads, head_dim, scale,
@@ -807,6 +845,7 @@ class Gpu:
         self._tables_of(len(s), d, src_cap, dst_cap, live, keep)
         if index is not None and (index.dtype != torch.int32 or not index.is_contiguous()):
             raise InvalidArgument(f"an index of {index.dtype} with strides {index.stride()}")
+        self._here(index)
         _check(self._lib.llmtie_cache_evict_q8(
             self._h, s, self._i32_table(src_cap), d, self._i32_table(dst_cap),
             self._i32_table(live), self._i32_table(keep), len(s), keep_first, keep_recent,
