@@ -225,3 +225,33 @@ def test_rotated_queries_over_the_frequencies_are_refused(gpu):
     with pytest.raises(InvalidArgument, match="overlaps"):
         gpu.rope_append_q8(gpu.zeros(heads * hd), k, k, [0, 1], [t], [cap], [0], [0], both[heads * hd - 8:heads * hd + hd // 2 - 8],
                            heads, kv, hd, q_out=both[:heads * hd])
+
+
+# ---- a kernel set up while the one that writes its input still runs ---------------------------
+
+@pytest.mark.parametrize("heads,kv,hd,n,past", [(32, 8, 128, 512, 3000), (32, 8, 128, 64, 200), (20, 20, 64, 300, 0)])
+def test_a_prompt_right_behind_the_kernel_that_rotates_its_queries(gpu, heads, kv, hd, n, past):
+    """The queries are rotated in place; the same bits as with a pause in between, over
+    buffers that hold other queries from one round to the next."""
+    live = past + n
+    cap = (live + 31) // 32 * 32
+    (t,), _ = caches_of(gpu, kv, hd, [past], seed=n, cap=cap) if past else ([gpu.kv_alloc_q8(kv, hd, cap)], None)
+    f = gpu.rope_inv_freq(10000.0, hd)
+    rows = [torch.randn(n, w * hd, device=gpu.device) for w in (heads, heads, kv, kv)]
+    x, held = torch.empty_like(rows[0]), t.clone()
+    torch.cuda.synchronize()
+
+    def step(source, pause):
+        with torch.cuda.stream(gpu.stream):
+            x.copy_(source)
+            t.copy_(held)                  # (the rows of its tail gave way to the prompt's)
+        gpu.rope_append_q8(x, rows[2], rows[3], [0, n], [t], [cap], [past], [past], f, heads, kv, hd)
+        if pause:
+            gpu.synchronize()
+        out = gpu.flash_attn_q8(x, [0, n], [t], [cap], [past], heads, kv, hd, hd ** -0.5, True)
+        gpu.synchronize()
+        return out
+
+    want = [step(q, True) for q in rows[:2]]
+    for i in range(60):
+        assert torch.equal(step(rows[i % 2], False), want[i % 2])

@@ -541,6 +541,8 @@ prefill_tc_kernel(const __grid_constant__ Params p)
             if (done_items > 0) ok = mbar_wait(BAR(Q_FREE + t), (done_items - 1) & 1u, wt, 24 + t);
             if (!ok) break;
             // -- stage Q: f32 rows -> f16, scaled, into the swizzled K-major layout ------
+            // (by ld.global.cg: the kernels that write q and the table may have been running
+            // when this one was set up, so they are not constant for its life)
             {
                 const float *qh = p.q + (long long)sq.row0 * p.q_stride + me.head * HD;
                 const int w = warp & 3;
@@ -568,10 +570,10 @@ prefill_tc_kernel(const __grid_constant__ Params p)
                             if (me.r0 + r < sq.tq) {
                                 const float *src = qh + (long long)(me.r0 + r) * p.q_stride + 4 * c;
                                 const float *tr = tab + (long long)(me.r0 + r) * HD + 4 * c;
-                                a[u] = __ldg((const float4 *)src);
-                                b[u] = __ldg((const float4 *)(src + HD / 2));
-                                cs[u] = __ldg((const float4 *)tr);
-                                sn[u] = __ldg((const float4 *)(tr + HD / 2));
+                                a[u] = __ldcg((const float4 *)src);
+                                b[u] = __ldcg((const float4 *)(src + HD / 2));
+                                cs[u] = __ldcg((const float4 *)tr);
+                                sn[u] = __ldcg((const float4 *)(tr + HD / 2));
                             }
                         }
 #pragma unroll
@@ -610,7 +612,7 @@ prefill_tc_kernel(const __grid_constant__ Params p)
                         const int r = 32 * w + rr0 + u * RPI + sub_row;
                         x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (me.r0 + r < sq.tq) {
-                            x[u] = __ldg((const float4 *)(qh + (long long)(me.r0 + r) * p.q_stride +
+                            x[u] = __ldcg((const float4 *)(qh + (long long)(me.r0 + r) * p.q_stride +
                                                           4 * col4));
                         }
                     }
@@ -1151,7 +1153,7 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const __grid_constan
     constexpr int V = HD / 32;                 // channels a lane carries
     constexpr int kBatch = 8;
     // (launched as the attention kernel's programmatic dependent: nothing of
-    // that kernel's may be read before it has ended)
+    // that kernel's may be read before it has ended, nor as if it were constant)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PrefillMergeGroup g = p.group[blockIdx.x];
     const int x = blockIdx.y >> 1, t = blockIdx.y & 1;
@@ -1172,13 +1174,13 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const __grid_constan
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
             const long long tile = tile0 + (long long)min(k0 + k, g.pieces - 1) * tile_step;
-            ml[k] = __ldg(&p.part_ml[tile * BM + row]);
+            ml[k] = __ldcg(&p.part_ml[tile * BM + row]);
             const float *src = p.part_o + (tile * BM + row) * HD + V * lane;
             if constexpr (V == 4) {
-                const float4 v = __ldg((const float4 *)src);
+                const float4 v = __ldcg((const float4 *)src);
                 o[k][0] = v.x; o[k][1] = v.y; o[k][2] = v.z; o[k][3] = v.w;
             } else {
-                const float2 v = __ldg((const float2 *)src);
+                const float2 v = __ldcg((const float2 *)src);
                 o[k][0] = v.x; o[k][1] = v.y;
             }
         }
