@@ -653,10 +653,14 @@ llmtie_status llmtie_decode_plan_q8(const int32_t *live, size_t batch, size_t kv
  * b's rows cu_seqlens[b] .. cu_seqlens[b+1] of q f32 [rows][heads*head_dim]
  * (already rotated) attend to its cache, which holds past[b] tokens before
  * theirs and theirs (llmtie_rope_append_q8 puts them there): causal, or all to
- * all. out [rows][heads*head_dim], f16 or f32. Sequences of few rows go through
+ * all. out [rows][heads*head_dim], f16 or f32. As in the other prefills the
+ * queries, the keys and values and the probabilities are f16 operands with f32
+ * sums (about 5e-4 of a row, relative, where the cache's own rounding is 2e-4),
+ * but for prompts of few rows, which are held as a decode's. Sequences of few rows go through
  * the decode kernel; of the others the live keys are unpacked to f16 once, into
- * memory that the handle keeps for the purpose: for eight sequences at a time,
- * or as many as take a gigabyte and are no more than 32. */
+ * memory that the handle keeps for the purpose (twice the bytes of the caches):
+ * for eight sequences at a time, or as many as take a gigabyte and are no more
+ * than 32. */
 llmtie_status llmtie_flash_attn_q8(llmtie_gpu *g, const float *q, size_t q_len,
                                    const int32_t *cu_seqlens, size_t batch,
                                    const void *const *caches, const int32_t *past,

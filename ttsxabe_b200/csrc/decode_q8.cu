@@ -25,7 +25,7 @@
 // The kernel is bound by reading the cache: each warp keeps a ring of its own
 // blocks in flight (cp.async.bulk, an mbarrier a stage; two stages, since with
 // three the queue at the memory makes every other load wait: 344 against 301 us
-// for 8 x 131072 keys of 8 heads x 128, which is 6.9-7.1 TB/s). A pair
+// for 8 x 131072 keys of 8 heads x 128, which is 7.1 TB/s; up to 320 on other B200s). A pair
 // (sequence, KV head) is taken by a cluster of blocks of the grid that merge
 // through distributed shared memory, or by several, whose results the last to
 // arrive merges row by row, or the grid is cut by work and the last block to
@@ -1032,8 +1032,8 @@ void plan_decode_q8(DecodeQ8Plan &plan, const int *units, int n, int kv_heads, i
         if (cost < plan.us && blocks <= 0x7fffffff) plan = DecodeQ8Plan{(int)blocks, c, 1, 0, cost};
     }
     // Several clusters of eight for a pair, as many as the device holds at once, and
-    // none of them without a block. 131072 tokens, one KV head x 128: 15 us by 32 clusters, 45 by the
-    // cut, whose last block has 296 results to merge; 8000 tokens: 12 us by 32 clusters,
+    // none of them without a block. 131072 tokens, one KV head x 128: 16 us by 29 clusters, 45 by the
+    // cut, whose last block has 296 results to merge; 8000 tokens: 12 us by all of them,
     // 9 by one of 16.
     for (long long parts = 2; parts <= 32 && pairs * parts <= clusters[0] && parts * 8 <= longest; parts++) {
         const long long blocks = pairs * parts * 8;
