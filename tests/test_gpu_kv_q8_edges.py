@@ -255,3 +255,36 @@ def test_a_prompt_right_behind_the_kernel_that_rotates_its_queries(gpu, heads, k
     want = [step(q, True) for q in rows[:2]]
     for i in range(60):
         assert torch.equal(step(rows[i % 2], False), want[i % 2])
+
+
+# ---- scales --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.5])
+@pytest.mark.parametrize("heads,kv,hd,past,n", [(8, 2, 128, 300, 1), (8, 2, 128, 300, 6), (32, 8, 128, 90, 200), (27, 3, 64, 70, 140),
+                                                (8, 2, 128, 4000, 250)])
+def test_any_scale(gpu, heads, kv, hd, past, n, scale):
+    """Of either sign and none, in the decode kernel and in the prefill kernel. A query
+    rounded to f16, half a step of 2^-10 a channel, moves a score by no more than d =
+    |scale| sum |q k| 2^-11, so the probabilities by a factor within e^(2 d) either way
+    and the result by (e^(2 d) - 1) sum p |v|; the rest is what the prefill of such
+    queries may be off by."""
+    from tests.test_gpu_prefill_items import attention
+
+    live = past + n
+    (t,), (cap,) = caches_of(gpu, kv, hd, [live], seed=live)
+    q = 0.1 * torch.randn(n, heads, hd, device=gpu.device)
+    torch.cuda.synchronize()
+    out = gpu.flash_attn_q8(q, [0, n], [t], [cap], [past], heads, kv, hd, scale, True)
+    ko, vo = gpu.cache_read_q8([t], [cap], [live], [0], [0, live], kv, hd)
+    gpu.synchronize()
+    k, v = (x.view(-1, kv, hd).double().transpose(0, 1) for x in (ko, vo))
+    want, tol = attention(q.double(), k, v, scale, past)
+    most, _ = attention(q.double(), k, v.abs(), scale, past)                 # sum p |v|
+    for h in range(heads):
+        d = abs(scale) * (q[:, h].double().abs() @ k[h // (heads // kv)].abs().T).max(-1, keepdim=True).values * 2.0 ** -11
+        tol[:, h] += torch.expm1(2 * d) * most[:, h]
+    assert ((out.view_as(want).double() - want).abs() <= tol).all()
+    if n == 1:
+        one = gpu.decode_batched_q8(q, [t], [live], [cap], heads, kv, hd, scale, DecodeScratch())
+        gpu.synchronize()
+        assert ((one.view_as(want).double() - want).abs() <= tol).all()

@@ -2,6 +2,7 @@
 // abi.cu every range is checked here, before anything is launched.
 #include "kv_q8.cuh"
 
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -679,8 +680,9 @@ try {
         pp.heads = (int)heads;
         pp.kv_heads = (int)kv_heads;
         pp.causal = causal ? 1 : 0;
-        pp.q_scale = 1.0f;
-        pp.sl2 = scale * kLog2e;
+        // (the kernel takes its maxima before it scales: a scale that is not positive goes into q)
+        pp.q_scale = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
+        pp.sl2 = scale == 0.0f ? kLog2e : fabsf(scale) * kLog2e;
         const bool tc = llmtie_use_tc(pp, (int)head_dim);
         static const bool no_pdl = getenv("LLMTIE_B200_NO_PDL") != nullptr;
         pp.after_prepass = (tc && !no_pdl && !g->kprof) ? 1 : 0;
