@@ -288,3 +288,29 @@ def test_any_scale(gpu, heads, kv, hd, past, n, scale):
         one = gpu.decode_batched_q8(q, [t], [live], [cap], heads, kv, hd, scale, DecodeScratch())
         gpu.synchronize()
         assert ((one.view_as(want).double() - want).abs() <= tol).all()
+
+
+# ---- the longest caches ----------------------------------------------------------------------
+
+def test_weights_past_the_rows_of_a_grid(gpu):
+    """More than 2^28 tokens (34 GB of codes): 2^23 + 1 complete blocks, each of which
+    gets its share of an even attention."""
+    from ttsxabe_b200 import kv_q8_bytes
+
+    kv, hd = 1, 64
+    at = (1 << 28) + 32
+    live, cap = at + 8, at + 32
+    t = torch.zeros(kv_q8_bytes(kv, hd, cap), dtype=torch.uint8, device=gpu.device)
+    k, v = torch.zeros(8, hd, device=gpu.device), torch.ones(8, hd, device=gpu.device)
+    q = torch.randn(hd, device=gpu.device)
+    torch.cuda.synchronize()
+    gpu.rope_append_q8(None, k, v, [0, 8], [t], [cap], [at], [0], None, 1, kv, hd)
+    out = gpu.decode_batched_q8(q, [t], [live], [cap], 1, kv, hd, 0.125, DecodeScratch(), weigh=True)
+    gpu.synchronize()
+    nb = cap // 32
+    first = 2 * cap * hd + 2 * ((4 * nb + 127) // 128 * 128)      # behind the codes and two sections of scales
+    w = t[first:first + 4 * nb].view(torch.float32)[:at // 32].double()
+    # (sums in f32: two roundings for each doubling of the number of terms, and the exponentials')
+    off = 64 * 2.0 ** -24
+    assert ((w * live / 32 - 1).abs() <= off).all()
+    assert ((out.double() * live / 8 - 1).abs() <= off).all()

@@ -869,6 +869,7 @@ __global__ void __launch_bounds__(kThreads, Geo<HD>::RESIDENT) decode_q8_kernel(
 // decode set up among these blocks is spread badly over the SMs, 66 us for 49 with 30 x
 // 15000 tokens of 4 KV heads x 64.)
 constexpr int kWeighThreads = 128;
+constexpr int kGridRows = 65535;     // a grid has no more (and as many layers): reached at 2^28 tokens
 template <int HD>
 __global__ void __launch_bounds__(kWeighThreads) q8_weigh_kernel(const __grid_constant__ DecodeQ8Params p)
 {
@@ -876,7 +877,7 @@ __global__ void __launch_bounds__(kWeighThreads) q8_weigh_kernel(const __grid_co
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int pair = (int)blockIdx.x, seq = pair / p.kv_heads, head = pair - seq * p.kv_heads, group = p.heads / p.kv_heads;
     const DecodeQ8Seq &sq = p.seq[seq];
-    const int b = (int)blockIdx.y * kWeighThreads + (int)threadIdx.x;
+    const int b = (int)(blockIdx.z * kGridRows + blockIdx.y) * kWeighThreads + (int)threadIdx.x;
     if (b >= sq.full) return;
     const Q8Layout at = q8_layout(p.kv_heads, HD, sq.nb);
     float *weight = (float *)(sq.base + at.w) + (long long)head * sq.nb + b;
@@ -974,7 +975,8 @@ cudaError_t launch_decode_q8(cudaStream_t st, const DecodeQ8Params &p, int hd, i
     if (e != cudaSuccess || !p.stats) return e;
     int most = 0;
     for (int b = 0; b < p.nseq; b++) most = std::max(most, p.seq[b].full);
-    const dim3 all((unsigned)(p.nseq * p.kv_heads), (unsigned)((most + kWeighThreads - 1) / kWeighThreads));
+    const int rows = (most + kWeighThreads - 1) / kWeighThreads;
+    const dim3 all((unsigned)(p.nseq * p.kv_heads), (unsigned)std::min(rows, kGridRows), (unsigned)((rows + kGridRows - 1) / kGridRows));
     return hd == 128 ? launch_dependent(st, all, kWeighThreads, 0, 1, q8_weigh_kernel<128>, p)
                      : launch_dependent(st, all, kWeighThreads, 0, 1, q8_weigh_kernel<64>, p);
 }
